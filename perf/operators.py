@@ -298,7 +298,7 @@ def _plain_append(s):
             mantissa, exponent = torch.frexp(f.abs().amax(dim=-1))
             # the smallest power of two that leaves no value of the row above 448 = 0.875 * 2^9
             k = torch.where(mantissa > 0.875, exponent - 8, exponent - 9).clamp(min=-126)
-            k = torch.where(mantissa == 0, 0, k)
+            k = torch.where(mantissa == 0, -126, k)
             codes = torch.ldexp(f, -k[:, None]).to(torch.float8_e4m3fn)
             pages.view(torch.uint8).view(-1, head)[at] = codes.view(torch.uint8)
             scales.view(-1)[at] = (k + 127).to(torch.uint8)
@@ -408,7 +408,7 @@ def _exact_append(s):
                 rows = x[n + c["n_batch"] * hd, :count].double()
                 if scales is not None:
                     ratio = rows.abs().amax(dim=-1).cpu().numpy() / 448.0
-                    k = np.array([0 if r == 0 else max(-126, math.ceil(math.log2(r))) for r in ratio], np.int64)
+                    k = np.array([-126 if r == 0 else max(-126, math.ceil(math.log2(r))) for r in ratio], np.int64)
                     k = torch.from_numpy(k).cuda()
                     rows = rows * torch.pow(2.0, -k.double())[:, None]
                     size[page, hd, slot] = (k + 127).to(torch.uint8)
