@@ -641,6 +641,130 @@ int nntile_hip_mask_tile_class_fp32(void *stream, int64_t k_rows, int64_t q_cols
 int nntile_hip_mask_tile_class_bool(void *stream, int64_t k_rows, int64_t q_cols,
         const uint8_t *mask, int64_t offset, int32_t *workspace, int32_t *class_out);
 
+/* ---- 11. key/value cache in pages -----------------------------------------------
+ * No counterpart in the reference, whose KVCache (wrappers/python/nntile/layer/
+ * cache_utils.py:117-225) gives every batch the same length.  Sequences of
+ * different lengths share a pool of pages: row p of sequence n lies in page
+ * table[p / page_rows + max_pages*n], row p % page_rows of it.
+ *   k_pages, v_pages   [head, page_rows, n_head_kv, n_pages], `page_stride`
+ *                      elements from one page to the next (>= head * page_rows *
+ *                      n_head_kv; larger where K and V share one pool)
+ *   k_scales, v_scales [page_rows, n_head_kv, n_pages] bytes, scale_stride apart; both null: the
+ *                      pages hold the tile type.  Else they hold e4m3 codes (bf16 and
+ *                      fp16 tiles; fp32: NNTILE_HIP_EUNSUPPORTED) and row r of a page
+ *                      stands for code * 2^(scale - 127).
+ *   table              [max_pages, n_batch], lens [n_batch]: int32, on the device and
+ *                      read when the kernel runs, so a captured call follows them.
+ *                      lens counts the rows of a sequence INCLUDING those that the
+ *                      step appends; less than 0 stands for 0, more than max_pages *
+ *                      page_rows for that.  A table entry outside [0, n_pages) is no
+ *                      page: its rows are not written, read back as zeros, and are
+ *                      hidden from every query.  Entries behind the last row of a
+ *                      sequence are not looked at.
+ *   new_rows           [n_batch] int32 or null: how many of the call's new tokens the
+ *                      sequence has (padded batches); null: all of them.  Taken into
+ *                      [0, the call's number].
+ * page_rows is a power of two from 16 to 65536, head 64 or 128 (other head sizes and
+ * page sizes: NNTILE_HIP_EUNSUPPORTED).  Pages, scales, and tiles start at
+ * multiples of 16 bytes; page_stride bytes and scale_stride are multiples of 16.
+ * max_pages * page_rows and n_batch * n_head_kv * kv_group * rows are below 2^31. */
+typedef struct nntile_hip_paged_cache
+{
+    void *k_pages, *v_pages;
+    uint8_t *k_scales, *v_scales;
+    const int32_t *table, *lens, *new_rows;
+    int64_t head, page_rows, n_head_kv, n_pages, max_pages, n_batch;
+    int64_t page_stride, scale_stride;
+} nntile_hip_paged_cache;
+
+/* k_new, v_new [head, rows, n_batch, n_head_kv] to rows [lens - new_rows, lens) of
+ * the sequences (token r < new_rows to row lens - new_rows + r; rows before 0 are
+ * dropped), both tensors in one launch.  8-bit pages: a row's scale is the smallest
+ * power of two, from 2^-126 on, that leaves no value above 448; codes are rounded
+ * to nearest even.  A row with a NaN or an infinity is stored as NaN.  rows == 0
+ * is a no-op.  The new rows of different sequences must be different rows of the
+ * pool. */
+int nntile_hip_paged_kv_append_bf16(void *stream, const nntile_hip_paged_cache *cache,
+        int64_t rows, const uint16_t *k_new, const uint16_t *v_new);
+int nntile_hip_paged_kv_append_fp16(void *stream, const nntile_hip_paged_cache *cache,
+        int64_t rows, const uint16_t *k_new, const uint16_t *v_new);
+int nntile_hip_paged_kv_append_fp32(void *stream, const nntile_hip_paged_cache *cache,
+        int64_t rows, const float *k_new, const float *v_new);
+
+/* Rows [first, first + rows) of every sequence into dense tiles k_out, v_out
+ * [head, rows, n_batch, n_head_kv], which the tile and grid entry points read; rows
+ * at or behind lens are zeros.  From 8-bit pages to fp16, what lies past the type's
+ * range becomes its largest value.  new_rows is not looked at. */
+int nntile_hip_paged_kv_read_bf16(void *stream, const nntile_hip_paged_cache *cache,
+        int64_t first, int64_t rows, uint16_t *k_out, uint16_t *v_out);
+int nntile_hip_paged_kv_read_fp16(void *stream, const nntile_hip_paged_cache *cache,
+        int64_t first, int64_t rows, uint16_t *k_out, uint16_t *v_out);
+int nntile_hip_paged_kv_read_fp32(void *stream, const nntile_hip_paged_cache *cache,
+        int64_t first, int64_t rows, float *k_out, float *v_out);
+
+/* Attention of the q_seq newest tokens of every sequence over its pages: Q, A
+ * [head, q_seq, n_batch, kv_group, n_head_kv], lse [q_seq, n_batch, kv_group,
+ * n_head_kv].  Query j < new_rows is the token at row lens - new_rows + j;
+ * NNTILE_HIP_MASK_CAUSAL lets it see the rows up to its own,
+ * NNTILE_HIP_MASK_NONE all rows below lens.  Queries j >= new_rows and those of
+ * sequences without rows see nothing.  flags: 0 or NNTILE_HIP_SDPA_OVERWRITE, with
+ * the meaning they have for the decode entry points (rows that see nothing, rows
+ * with a NaN among their scores).  What lies in rows that a query does not see -
+ * NaN, infinities - does not reach it.
+ * The keys of all sequences are shared out evenly over the chip's workgroups,
+ * whatever the lengths; shares of one sequence are joined in fp32 in the order of
+ * the keys.  The same call gives the same bits every time.
+ * workspace: nntile_hip_sdpa_fwd_paged_workspace_bytes of device memory, 16-byte
+ * aligned, private to the call until the stream has passed it; its contents do not
+ * matter, and the size does not depend on lens. */
+typedef struct nntile_hip_sdpa_paged_args
+{
+    nntile_hip_paged_cache cache;
+    int64_t q_seq, kv_group;
+    int32_t mask_mode, flags;
+    const void *Q;
+    float *lse;
+    void *A;
+} nntile_hip_sdpa_paged_args;
+
+size_t nntile_hip_sdpa_fwd_paged_workspace_bytes(const nntile_hip_sdpa_paged_args *args);
+int nntile_hip_sdpa_fwd_paged_bf16(void *stream, const nntile_hip_sdpa_paged_args *args,
+        void *workspace, size_t workspace_bytes);
+int nntile_hip_sdpa_fwd_paged_fp16(void *stream, const nntile_hip_sdpa_paged_args *args,
+        void *workspace, size_t workspace_bytes);
+int nntile_hip_sdpa_fwd_paged_fp32(void *stream, const nntile_hip_sdpa_paged_args *args,
+        void *workspace, size_t workspace_bytes);
+
+/* ---- 12. rotary embedding with positions of several axes --------------------------
+ * nntile_hip_rope_* takes tables of sines and cosines; here they follow from the
+ * positions, of one axis (text) or several (time, rows and columns of video
+ * patches): pair i of a row is turned by
+ *   angle = positions[axes[i]] * freqs[i]
+ * (forward and backward as in section 7, written and not added; the arithmetic in fp32, one
+ * rounding to the tile type; the angle's product and its whole turns in 64 bits).
+ *   positions  [seq, n_batch, n_axes] int64; pos_batch_stride is seq, or 0 where
+ *              all sequences share the positions ([seq, 1, n_axes])
+ *   freqs      [head/2] double, radians; 0 leaves a pair as it is
+ *   axes       [head/2] int32; an entry outside [0, n_axes) stands for position 0
+ *   q, q_out   [head, seq, n_batch, heads_q], k, k_out [head, seq, n_batch, heads_k]:
+ *              both in one launch; heads_k may be 0 and k, k_out null
+ * Any even head; src and dst may be the same buffer. */
+typedef struct nntile_hip_rope_axes_args
+{
+    int64_t head, seq, n_batch, heads_q, heads_k, n_axes;
+    int64_t pos_batch_stride;
+    int32_t backward, reserved;
+    const int64_t *positions;
+    const double *freqs;
+    const int32_t *axes;
+    const void *q, *k;
+    void *q_out, *k_out;
+} nntile_hip_rope_axes_args;
+
+int nntile_hip_rope_axes_bf16(void *stream, const nntile_hip_rope_axes_args *args);
+int nntile_hip_rope_axes_fp16(void *stream, const nntile_hip_rope_axes_args *args);
+int nntile_hip_rope_axes_fp32(void *stream, const nntile_hip_rope_axes_args *args);
+
 /* Library version and the ISA it was built for ("gfx950"). */
 const char *nntile_hip_sdpa_version(void);
 

@@ -624,6 +624,300 @@ PyObject *rope(PyObject *, PyObject *const *v, Py_ssize_t n_args)
     });
 }
 
+// ---- paged cache, rotary positions of several axes ------------------------------
+
+// All tensors of a call lie on the current device: that is where the call's
+// stream is and where the kernels run.
+struct SameDevice
+{
+    const c10::Device here = c10::Device(c10::kCUDA, c10::hip::current_device());
+    void check(const at::Tensor &t) const
+    {
+        if(!t.is_cuda())
+        {
+            PyErr_SetString(PyExc_ValueError, "tiles must be contiguous device tensors");
+            throw Bad();
+        }
+        if(t.device() != here)
+        {
+            PyErr_SetString(PyExc_ValueError, "all tensors of a call must be on the current device");
+            throw Bad();
+        }
+    }
+    const at::Tensor &dense(PyObject *o) const
+    {
+        const at::Tensor &t = tile(o);
+        check(t);
+        return t;
+    }
+};
+
+void wants(const at::Tensor &t, at::ScalarType type, int64_t dims, const char *what)
+{
+    if(t.scalar_type() != type || t.dim() != dims)
+    {
+        PyErr_Format(PyExc_ValueError, "%s", what);
+        throw Bad();
+    }
+}
+
+// Elements from one page to the next of a pool whose pages are contiguous.
+int64_t pool_stride(const at::Tensor &t)
+{
+    int64_t inner = 1;
+    for(int64_t d = t.dim() - 1; d >= 1; --d)
+    {
+        if(t.size(d) != 1 && t.stride(d) != inner)
+        {
+            PyErr_SetString(PyExc_ValueError, "the pages of a pool must be contiguous");
+            throw Bad();
+        }
+        inner *= t.size(d);
+    }
+    return t.size(0) > 1 ? t.stride(0) : inner;
+}
+
+// Pools, table, lengths, scales and new rows into the argument block; false: they
+// do not fit each other.  `ty`: the type of the tiles.
+bool fill_paged(nntile_hip_paged_cache &c, const SameDevice &dev, Type ty, PyObject *k_pages_,
+        PyObject *v_pages_, PyObject *table_, PyObject *lens_, PyObject *k_scales_,
+        PyObject *v_scales_, PyObject *new_rows_)
+{
+    const at::Tensor &k_pages = tensor(k_pages_), &v_pages = tensor(v_pages_);
+    const at::Tensor &table = dev.dense(table_), &lens = dev.dense(lens_);
+    dev.check(k_pages);
+    dev.check(v_pages);
+    wants(table, at::kInt, 2, "the page table is an int32 tensor [n_batch, max_pages]");
+    wants(lens, at::kInt, 1, "the lengths are an int32 tensor [n_batch]");
+    c = {};
+    const bool packed = k_scales_ != Py_None;
+    if(packed != (v_scales_ != Py_None))
+    {
+        return false;
+    }
+    const at::ScalarType held = packed ? at::kFloat8_e4m3fn
+        : ty == BF16 ? at::kBFloat16 : ty == FP16 ? at::kHalf : at::kFloat;
+    const char *text = "pages are tensors [n_pages, n_head_kv, page_rows, head] of the tiles' type, "
+        "or torch.float8_e4m3fn with scales";
+    wants(k_pages, held, 4, text);
+    wants(v_pages, held, 4, text);
+    c.page_stride = pool_stride(k_pages);
+    if(k_pages.sizes() != v_pages.sizes() || pool_stride(v_pages) != c.page_stride
+            || lens.size(0) != table.size(0))
+    {
+        return false;
+    }
+    c.k_pages = k_pages.data_ptr();
+    c.v_pages = v_pages.data_ptr();
+    c.n_pages = k_pages.size(0);
+    c.n_head_kv = k_pages.size(1);
+    c.page_rows = k_pages.size(2);
+    c.head = k_pages.size(3);
+    if(packed)
+    {
+        const at::Tensor &ks = tensor(k_scales_), &vs = tensor(v_scales_);
+        dev.check(ks);
+        dev.check(vs);
+        const char *scales = "scales are uint8 tensors [n_pages, n_head_kv, page_rows]";
+        wants(ks, at::kByte, 3, scales);
+        wants(vs, at::kByte, 3, scales);
+        c.scale_stride = pool_stride(ks);
+        if(ks.sizes() != vs.sizes() || pool_stride(vs) != c.scale_stride
+                || ks.sizes() != k_pages.sizes().slice(0, 3))
+        {
+            return false;
+        }
+        c.k_scales = static_cast<uint8_t *>(ks.data_ptr());
+        c.v_scales = static_cast<uint8_t *>(vs.data_ptr());
+    }
+    c.table = static_cast<const int32_t *>(table.data_ptr());
+    c.lens = static_cast<const int32_t *>(lens.data_ptr());
+    c.n_batch = table.size(0);
+    c.max_pages = table.size(1);
+    if(new_rows_ != Py_None)
+    {
+        const at::Tensor &new_rows = dev.dense(new_rows_);
+        wants(new_rows, at::kInt, 1, "new_rows is an int32 tensor [n_batch]");
+        if(new_rows.size(0) != c.n_batch)
+        {
+            return false;
+        }
+        c.new_rows = static_cast<const int32_t *>(new_rows.data_ptr());
+    }
+    return true;
+}
+
+// Two tiles [n_head_kv * n_batch, rows, head] of one type beside a cache.
+bool tiles_fit(const nntile_hip_paged_cache &c, const at::Tensor &k, const at::Tensor &v)
+{
+    return k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type()
+        && k.size(0) == c.n_head_kv * c.n_batch && k.size(2) == c.head;
+}
+
+// (k_new, v_new, k_pages, v_pages, table, lens, k_scales, v_scales, new_rows, stream)
+PyObject *paged_append(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+    return guarded(n, 10, [&]() -> int
+    {
+        const at::Tensor &k = tile(v[0]), &w = tile(v[1]);
+        const SameDevice dev;
+        dev.check(k);
+        dev.check(w);
+        rank3(k);
+        rank3(w);
+        const Type ty = type_of(v[0], k);
+        nntile_hip_paged_cache c;
+        if(!fill_paged(c, dev, ty, v[2], v[3], v[4], v[5], v[6], v[7], v[8]) || !tiles_fit(c, k, w))
+        {
+            return NNTILE_HIP_EINVAL;
+        }
+        void *s = stream_of(v[9]);
+        const int64_t rows = k.size(1);
+        if(ty == FP32)
+        {
+            return unlocked(nntile_hip_paged_kv_append_fp32, s, &c, rows,
+                    static_cast<const float *>(k.data_ptr()), static_cast<const float *>(w.data_ptr()));
+        }
+        return unlocked(ty == BF16 ? nntile_hip_paged_kv_append_bf16 : nntile_hip_paged_kv_append_fp16,
+                s, &c, rows, static_cast<const uint16_t *>(k.data_ptr()),
+                static_cast<const uint16_t *>(w.data_ptr()));
+    });
+}
+
+// (k_pages, v_pages, table, lens, k_out, v_out, first, k_scales, v_scales, stream)
+PyObject *paged_read(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+    return guarded(n, 10, [&]() -> int
+    {
+        const at::Tensor &k = tile(v[4]), &w = tile(v[5]);
+        const SameDevice dev;
+        dev.check(k);
+        dev.check(w);
+        rank3(k);
+        rank3(w);
+        const Type ty = type_of(v[4], k);
+        nntile_hip_paged_cache c;
+        if(!fill_paged(c, dev, ty, v[0], v[1], v[2], v[3], v[7], v[8], Py_None) || !tiles_fit(c, k, w))
+        {
+            return NNTILE_HIP_EINVAL;
+        }
+        const int64_t first = integer(v[6]), rows = k.size(1);
+        void *s = stream_of(v[9]);
+        if(ty == FP32)
+        {
+            return unlocked(nntile_hip_paged_kv_read_fp32, s, &c, first, rows,
+                    static_cast<float *>(k.data_ptr()), static_cast<float *>(w.data_ptr()));
+        }
+        return unlocked(ty == BF16 ? nntile_hip_paged_kv_read_bf16 : nntile_hip_paged_kv_read_fp16,
+                s, &c, first, rows, static_cast<uint16_t *>(k.data_ptr()),
+                static_cast<uint16_t *>(w.data_ptr()));
+    });
+}
+
+// (k_pages, v_pages, table, lens, Q, lse, A, mask_mode, kv_group, workspace, k_scales, v_scales,
+// new_rows, flags, stream)
+PyObject *fwd_paged(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+    return guarded(n, 15, [&]() -> int
+    {
+        const at::Tensor &Q = tile(v[4]), &lse = tile(v[5]), &A = tile(v[6]), &ws = tile(v[9]);
+        const SameDevice dev;
+        for(const at::Tensor *t : {&Q, &lse, &A, &ws})
+        {
+            dev.check(*t);
+        }
+        rank3(Q);
+        const Type ty = type_of(v[4], Q);
+        wants(lse, at::kFloat, 2, "lse is an fp32 tensor [batch, q_seq]");
+        nntile_hip_sdpa_paged_args a = {};
+        if(!fill_paged(a.cache, dev, ty, v[0], v[1], v[2], v[3], v[10], v[11], v[12])
+                || A.sizes() != Q.sizes() || A.scalar_type() != Q.scalar_type())
+        {
+            return NNTILE_HIP_EINVAL;
+        }
+        a.q_seq = Q.size(1);
+        a.kv_group = integer(v[8]);
+        a.mask_mode = (int32_t)integer(v[7]);
+        a.flags = (int32_t)integer(v[13]);
+        const int64_t entries = a.cache.n_head_kv * a.cache.n_batch;
+        if(a.kv_group < 1 || a.kv_group > Q.size(0) || Q.size(0) != entries * a.kv_group
+                || Q.size(2) != a.cache.head || lse.size(0) != Q.size(0) || lse.size(1) != Q.size(1))
+        {
+            return NNTILE_HIP_EINVAL;
+        }
+        a.Q = Q.data_ptr();
+        a.lse = static_cast<float *>(lse.data_ptr());
+        a.A = A.data_ptr();
+        return unlocked(ty == BF16 ? nntile_hip_sdpa_fwd_paged_bf16
+                : ty == FP16 ? nntile_hip_sdpa_fwd_paged_fp16 : nntile_hip_sdpa_fwd_paged_fp32,
+                stream_of(v[14]), &a, ws.data_ptr(), nbytes(&ws));
+    });
+}
+
+// (positions, freqs, axes, q, q_out, k, k_out, backward, stream)
+PyObject *rope_axes(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+    return guarded(n, 9, [&]() -> int
+    {
+        const at::Tensor &pos = tile(v[0]), &freqs = tile(v[1]), &axes = tile(v[2]), &q = tile(v[3]),
+              &q_out = tile(v[4]);
+        const at::Tensor *k = maybe_tile(v[5]), *k_out = maybe_tile(v[6]);
+        const SameDevice dev;
+        for(const at::Tensor *t : {&pos, &freqs, &axes, &q, &q_out, k, k_out})
+        {
+            if(t != nullptr)
+            {
+                dev.check(*t);
+            }
+        }
+        wants(pos, at::kLong, 3, "positions are an int64 tensor [n_axes, n_batch, seq]");
+        wants(freqs, at::kDouble, 1, "freqs is a float64 tensor [head/2]");
+        wants(axes, at::kInt, 1, "axes is an int32 tensor [head/2]");
+        rank3(q);
+        const int backward = PyObject_IsTrue(v[7]);
+        if(backward < 0)
+        {
+            throw Bad();
+        }
+        const Type ty = type_of(v[3], q);
+        nntile_hip_rope_axes_args a = {};
+        a.n_axes = pos.size(0);
+        a.n_batch = pos.size(1);
+        a.seq = q.size(1);
+        a.head = q.size(2);
+        if(a.n_batch < 1 || a.n_axes < 1 || pos.size(2) != a.seq || a.head % 2 != 0
+                || freqs.size(0) != a.head / 2
+                || axes.size(0) != a.head / 2 || q.size(0) % a.n_batch != 0 || q_out.sizes() != q.sizes()
+                || q_out.scalar_type() != q.scalar_type() || (k == nullptr) != (k_out == nullptr))
+        {
+            return NNTILE_HIP_EINVAL;
+        }
+        a.pos_batch_stride = a.n_batch == 1 ? 0 : a.seq;
+        a.heads_q = q.size(0) / a.n_batch;
+        if(k != nullptr)
+        {
+            if(k->dim() != 3 || k->size(1) != a.seq || k->size(2) != a.head || k->size(0) % a.n_batch != 0
+                    || k_out->sizes() != k->sizes() || k->scalar_type() != q.scalar_type()
+                    || k_out->scalar_type() != q.scalar_type())
+            {
+                return NNTILE_HIP_EINVAL;
+            }
+            a.heads_k = k->size(0) / a.n_batch;
+            a.k = k->data_ptr();
+            a.k_out = k_out->data_ptr();
+        }
+        a.backward = backward;
+        a.positions = static_cast<const int64_t *>(pos.data_ptr());
+        a.freqs = static_cast<const double *>(freqs.data_ptr());
+        a.axes = static_cast<const int32_t *>(axes.data_ptr());
+        a.q = q.data_ptr();
+        a.q_out = q_out.data_ptr();
+        return unlocked(ty == BF16 ? nntile_hip_rope_axes_bf16
+                : ty == FP16 ? nntile_hip_rope_axes_fp16 : nntile_hip_rope_axes_fp32,
+                stream_of(v[8]), &a);
+    });
+}
+
 // (alpha, src, dst, m, n, stream)
 PyObject *transpose(PyObject *, PyObject *const *v, Py_ssize_t n_args)
 {
@@ -731,6 +1025,7 @@ PyMethodDef methods[] = {
     FAST(fwd_tile), FAST(fwd_tile_cache), FAST(fwd_tile_cache_ws), FAST(tile_cache_workspace), FAST(fwd_decode), FAST(fwd_decode_cache),
     FAST(fwd_decode_append_cache), FAST(cache_step), FAST(kv_append), FAST(flash_fwd),
     FAST(flash_bwd), FAST(bwd_tile), FAST(accumulate), FAST(rope), FAST(transpose),
+    FAST(paged_append), FAST(paged_read), FAST(fwd_paged), FAST(rope_axes),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_front", nullptr, -1, methods, nullptr, nullptr,

@@ -21,29 +21,10 @@
 // bf16, one and two columns a thread: 2 x 65536 x 64 (33.6 MB) 7.3 and 6.9 us =
 // 4.9 TB/s, 2 x 65536 x 256 24.0 and 22.3 = 6.0 TB/s; fp32 2 x 65536 x 256 55.1 and
 // 52.6.
-#include "sdpa_common.hpp"
+#include "rope_common.hpp"
 
 namespace nntile_hip
 {
-
-struct RopeF32
-{
-    typedef float storage;
-    static __device__ __forceinline__ float to_float(float v) { return v; }
-    static __device__ __forceinline__ float from_float(float v) { return v; }
-};
-struct RopeBf16
-{
-    typedef uint16_t storage;
-    static __device__ __forceinline__ float to_float(uint16_t v) { return Bf16::to_float(v); }
-    static __device__ __forceinline__ uint16_t from_float(float v) { return Bf16::from_float(v); }
-};
-struct RopeFp16
-{
-    typedef uint16_t storage;
-    static __device__ __forceinline__ float to_float(uint16_t v) { return Fp16::to_float(v); }
-    static __device__ __forceinline__ uint16_t from_float(float v) { return Fp16::from_float(v); }
-};
 
 // Quotients of numbers below 2^31 by a fixed divisor: a multiplication by
 // 2^32 (2^shift - by) / by + 1, rounded down, an addition and a shift, exact
@@ -64,21 +45,6 @@ struct RopeDivide
         return (__umulhi(t, factor) + t) >> shift;
     }
 };
-
-template<bool BACKWARD>
-__device__ __forceinline__ void rotate(float c, float s, float a, float b, float &x, float &y)
-{
-    if(BACKWARD)
-    {
-        x = fmaf(c, a, s * b);
-        y = fmaf(c, b, -(s * a));
-    }
-    else
-    {
-        x = fmaf(c, a, -(s * b));
-        y = fmaf(s, a, c * b);
-    }
-}
 
 template<typename S, bool BACKWARD, int COLS>
 __global__ __launch_bounds__(256)

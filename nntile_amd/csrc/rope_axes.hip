@@ -1,0 +1,181 @@
+// Rotary embedding, forward and backward, with angles that follow from positions of one
+// or several axes (time, rows, columns):
+//
+//   angle[i] = positions[axes[i]] * freqs[i],  i = 0 .. head/2 - 1
+//
+// and the pair (2i, 2i+1) of every head of the token is turned by it (rope_common.hpp).
+// The queries and the keys of a layer go through one launch.
+//
+// The angle is taken in 64 bits and reduced there to less than half a turn: at position
+// 100000 its fp32 product would be off by 0.004 radians.  What is left of it, up to one turn,
+// loses 2^-25 of a turn in fp32 at most; sine and cosine of it are those of the device
+// library.  A thread takes
+// four pairs of a token (16 bytes of a 16-bit tensor, 32 of an fp32 one) of HEADS heads and
+// computes their sines and cosines once.
+#include "paged.hpp"
+#include "rope_common.hpp"
+
+namespace nntile_hip
+{
+
+// Sine and cosine of 2 pi times the broken part of position * freq / (2 pi).
+__device__ __forceinline__ void turn_of(int64_t position, double freq, float &s, float &c)
+{
+    const double turns = (double)position * (freq * 0.15915494309189533577);
+    const float half = (float)(2.0 * (turns - rint(turns)));        // in half turns, [-1, 1]
+    sincospif(half, &s, &c);
+}
+
+__device__ __forceinline__ int64_t position_on(const RopeAxesParams &p, int axis, int64_t at)
+{
+    return axis >= 0 && axis < p.n_axes ? p.positions[axis * p.pos_axis_stride + at] : 0;
+}
+
+// Four pairs a thread.  Threads go along the tokens of a sequence (contiguous for a given
+// head), blockIdx.y over sequences and groups of HEADS heads.
+template<typename S, bool BACKWARD, int HEADS>
+__global__ __launch_bounds__(256)
+void rope_axes_vec_kernel(const RopeAxesParams p)
+{
+    typedef typename S::storage E;
+    constexpr int NV = (int)sizeof(E) / 2;      // 16-byte pieces of four pairs
+    const int per_row = (int)(p.head / 8);
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if(t >= p.seq * per_row)
+    {
+        return;
+    }
+    const int64_t token = t / per_row;
+    const int i = 4 * (int)(t - token * per_row);
+    const int n = (int)(blockIdx.y % p.n_batch);
+    const int h0 = (int)(blockIdx.y / p.n_batch) * HEADS;
+    const int heads = (int)(p.heads_q + p.heads_k);
+    const int64_t entry = p.seq * p.head;
+    const int64_t in_row = token * p.head + 2 * i;
+    u32x4 raw[HEADS][NV];
+#pragma unroll
+    for(int j = 0; j < HEADS; ++j)
+    {
+        // (heads past the last re-read it)
+        const int h = min(h0 + j, heads - 1);
+        const bool key = h >= p.heads_q;
+        const E *from = static_cast<const E *>(key ? p.k : p.q)
+            + ((key ? h - p.heads_q : h) * p.n_batch + n) * entry + in_row;
+#pragma unroll
+        for(int v = 0; v < NV; ++v)
+        {
+            raw[j][v] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(from) + v);
+        }
+    }
+    float s[4], c[4];
+#pragma unroll
+    for(int k = 0; k < 4; ++k)
+    {
+        turn_of(position_on(p, p.axes[i + k], n * p.pos_batch_stride + token), p.freqs[i + k], s[k],
+                c[k]);
+    }
+#pragma unroll
+    for(int j = 0; j < HEADS; ++j)
+    {
+        __attribute__((aligned(16))) E in[8];
+        __attribute__((aligned(16))) E out[8];
+#pragma unroll
+        for(int v = 0; v < NV; ++v)
+        {
+            reinterpret_cast<u32x4 *>(in)[v] = raw[j][v];
+        }
+#pragma unroll
+        for(int k = 0; k < 4; ++k)
+        {
+            float x, y;
+            rotate<BACKWARD>(c[k], s[k], S::to_float(in[2 * k]), S::to_float(in[2 * k + 1]), x, y);
+            out[2 * k] = S::from_float(x);
+            out[2 * k + 1] = S::from_float(y);
+        }
+        const int h = h0 + j;
+        if(h < heads)
+        {
+            const bool key = h >= p.heads_q;
+            E *to = static_cast<E *>(key ? p.k_out : p.q_out)
+                + ((key ? h - p.heads_q : h) * p.n_batch + n) * entry + in_row;
+#pragma unroll
+            for(int v = 0; v < NV; ++v)
+            {
+                __builtin_nontemporal_store(reinterpret_cast<const u32x4 *>(out)[v],
+                        reinterpret_cast<u32x4 *>(to) + v);
+            }
+        }
+    }
+}
+
+// One pair a thread: heads that are no multiple of 8, addresses that are not aligned.
+template<typename S, bool BACKWARD>
+__global__ __launch_bounds__(256)
+void rope_axes_pair_kernel(const RopeAxesParams p, int64_t pairs)
+{
+    typedef typename S::storage E;
+    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if(t >= pairs)
+    {
+        return;
+    }
+    const int64_t half = p.head / 2;
+    const int64_t row = t / half;
+    const int i = (int)(t - row * half);
+    const int64_t entry = row / p.seq;
+    const int64_t token = row - entry * p.seq;
+    const int64_t n = entry % p.n_batch;
+    const int64_t q_entries = p.heads_q * p.n_batch;
+    const bool key = entry >= q_entries;
+    const int64_t at = (row - (key ? q_entries * p.seq : 0)) * p.head + 2 * i;
+    const E *from = static_cast<const E *>(key ? p.k : p.q) + at;
+    E *to = static_cast<E *>(key ? p.k_out : p.q_out) + at;
+    float s, c, x, y;
+    turn_of(position_on(p, p.axes[i], n * p.pos_batch_stride + token), p.freqs[i], s, c);
+    rotate<BACKWARD>(c, s, S::to_float(from[0]), S::to_float(from[1]), x, y);
+    to[0] = S::from_float(x);
+    to[1] = S::from_float(y);
+}
+
+template<typename S, bool BACKWARD>
+static int launch_typed(hipStream_t stream, const RopeAxesParams &p)
+{
+    auto aligned = [](const void *x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+    const int64_t heads = p.heads_q + p.heads_k;
+    const int64_t blocks_x = (p.seq * (p.head / 8) + 255) / 256;
+    constexpr int HEADS = 4;
+    const int64_t blocks_y = p.n_batch * ((heads + HEADS - 1) / HEADS);
+    if(p.head % 8 == 0 && aligned(p.q) && aligned(p.q_out) && aligned(p.k) && aligned(p.k_out)
+            && blocks_x <= 0x7fffffff && blocks_y <= 65535)
+    {
+        hipLaunchKernelGGL((rope_axes_vec_kernel<S, BACKWARD, HEADS>),
+                dim3((unsigned)blocks_x, (unsigned)blocks_y), dim3(256), 0, stream, p);
+    }
+    else
+    {
+        const int64_t pairs = heads * p.n_batch * p.seq * (p.head / 2);
+        if((pairs + 255) / 256 > 0x7fffffff)
+        {
+            return NNTILE_HIP_EINVAL;
+        }
+        hipLaunchKernelGGL((rope_axes_pair_kernel<S, BACKWARD>), dim3((unsigned)((pairs + 255) / 256)),
+                dim3(256), 0, stream, p, pairs);
+    }
+    return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;
+}
+
+int launch_rope_axes(hipStream_t stream, int dtype, bool backward, const RopeAxesParams &p)
+{
+    switch(dtype * 2 + (backward ? 1 : 0))
+    {
+        case 0: return launch_typed<RopeBf16, false>(stream, p);
+        case 1: return launch_typed<RopeBf16, true>(stream, p);
+        case 2: return launch_typed<RopeFp16, false>(stream, p);
+        case 3: return launch_typed<RopeFp16, true>(stream, p);
+        case 4: return launch_typed<RopeF32, false>(stream, p);
+        case 5: return launch_typed<RopeF32, true>(stream, p);
+        default: return NNTILE_HIP_EINVAL;
+    }
+}
+
+} // namespace nntile_hip

@@ -1,0 +1,1092 @@
+// Attention of a few new tokens per sequence over a key/value cache in pages, for sequences of
+// any lengths, gfx950.  With s = q.k / sqrt(head) over the keys a query sees:
+//
+//   lse = log sum exp(s),   A = sum exp(s - lse) v
+//
+// merged into the running pair (lse, A) or written over it.  Bound by the one pass over
+// the keys and values in HBM.
+//
+//  * The kv_group query heads of a key/value head are taken together, rows = kv_group * q_seq in
+//    blocks of 16 (NR of them a workgroup; more rows: several workgroups read the keys).
+//  * The keys of a sequence are cut into blocks of 4 * KEYS, the blocks of all (sequence,
+//    head, row group) units are numbered through, and every workgroup takes an equal
+//    run of them, whatever the lengths: it finds its first unit by a scan of the lengths (they
+//    live on the device, so a captured launch follows them).  Units that lie within
+//    one workgroup are finished there; the others leave partial results (unnormalised
+//    output, maximum, sum, all fp32) that a second launch joins in the order of the keys.
+//  * A wavefront streams KEYS keys at a time, its own ones, through its own two slots of LDS
+//    (global_load_lds, 16 bytes a lane): no barrier within a unit, 8 KB in flight
+//    per wavefront while 8 KB are worked on, eight wavefronts a CU.  The pages of the next
+//    keys are looked up by scalar loads meanwhile.
+//  * S^T = K Q^T and O^T += V^T P^T with matrix instructions of 16 x 16; P^T is the
+//    accumulator of S^T as it stands (the keys of an instruction are numbered so), V^T
+//    comes through the transposing LDS reads (fp32: single values).  A lane has one query row.
+//  * 8-bit pages: codes become bf16 / fp16 exactly in front of the matrix
+//    instructions; the power of two of a key row goes into the score.  That of a value row goes into the
+//    probability, which has a running maximum of its own (of score + exponent), so that what
+//    is rounded to fp16 is at most 1 and its largest is 1, however small the values are.
+//
+// Probabilities are rounded to the tile type (8-bit pages: to fp16) for the matrix instruction, as in
+// the other attention kernels; the sum of the softmax takes them unrounded.
+#include <type_traits>
+
+#include "paged.hpp"
+
+namespace nntile_hip
+{
+
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(2))) int i32x2;
+typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
+typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
+
+constexpr int kPagedWaves = 4;
+constexpr int kPagedThreads = 64 * kPagedWaves;
+constexpr int kPagedCUs = 256;
+// Workgroups that the keys are shared out to at most: two a CU
+constexpr int kPagedShares = 2 * kPagedCUs;
+
+enum PagedKind { kPaged16, kPaged8, kPaged32 };
+
+template<int KIND, int HEAD>
+struct PagedShape
+{
+    static constexpr int RB = KIND == kPaged32 ? HEAD * 4 : KIND == kPaged8 ? HEAD : HEAD * 2;   // bytes of a row
+    static constexpr int CPR = RB / 16;                     // 16-byte chunks of a row
+    static constexpr int RPL = RB >= 256 ? 1 : 256 / RB;    // rows per 256-byte line of LDS banks
+    static constexpr int KEYS = 4096 / RB > 16 ? 4096 / RB : 16;    // of a wavefront's step
+    static constexpr int BLOCK = kPagedWaves * KEYS;        // keys of a workgroup's step
+    static constexpr int GROUPS = KEYS / 16;
+    static constexpr int K_BYTES = KEYS * RB;
+    static constexpr int STAGE = 2 * K_BYTES;
+    static constexpr int LOADS = K_BYTES / 1024;            // load instructions of a step's K
+    static constexpr int ROWS_PER_LOAD = 1024 / RB;
+    static constexpr int RING = kPagedWaves * 2 * STAGE;
+    static constexpr int WGS_PER_CU = RING > 72 * 1024 ? 1 : 2;
+
+    // Where chunk c of row r lies: chunk position c ^ swizzle(r) of the row, so that the
+    // rows one LDS instruction reads fall on different banks.
+    static __host__ __device__ constexpr int k_swizzle(int r) { return (r / RPL) % CPR; }
+    static __host__ __device__ constexpr int v_swizzle(int r)
+    {
+        return KIND == kPaged16 ? 2 * ((r / RPL) % (CPR / 2))
+            : KIND == kPaged8 ? k_swizzle(r) : 4 * ((r >> 2) & 3);
+    }
+};
+
+// A load that is the same for the whole wavefront, through the scalar cache.
+template<typename W>
+__device__ __forceinline__ W scalar_load(const void *base, int64_t byte)
+{
+    typedef const __attribute__((address_space(4))) W *ptr;
+    return *reinterpret_cast<ptr>(reinterpret_cast<uintptr_t>(base) + byte);
+}
+
+__device__ __forceinline__ int uniform(int x)
+{
+    return __builtin_amdgcn_readfirstlane(x);
+}
+
+template<int N> __device__ __forceinline__ void paged_wait_loads()
+{
+    static_assert(N >= 0 && N < 64, "vmcnt is a 6-bit counter");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+    asm volatile("" ::: "memory");
+}
+
+__device__ __forceinline__ void paged_wait_lds()
+{
+    // lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));
+    asm volatile("" ::: "memory");
+}
+
+// Over the four lanes that share a query row: lane, lane ^ 16, lane ^ 32, lane ^ 48.
+__device__ __forceinline__ float quad_max(float x)
+{
+    typedef __attribute__((ext_vector_type(2))) uint32_t pair;
+    const uint32_t u = __float_as_uint(x);
+    const pair r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return max_across_halves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+
+__device__ __forceinline__ float quad_sum(float x)
+{
+    typedef __attribute__((ext_vector_type(2))) uint32_t pair;
+    const uint32_t u = __float_as_uint(x);
+    const pair r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return sum_across_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// exponent of a scale byte
+__device__ __forceinline__ float scale_of(uint32_t bytes, int i)
+{
+    return __uint_as_float(((bytes >> (8 * i)) & 255u) << 23);
+}
+
+// Matrix instructions and operands of the three kinds.
+template<typename T> __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c)
+{
+    if constexpr(__is_same(T, Bf16))
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    else
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+}
+
+template<typename T> __device__ __forceinline__ f32x4 mfma16(u32x2 a, u32x2 b, f32x4 c)
+{
+    if constexpr(__is_same(T, Bf16))
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a),
+                __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+    }
+    else
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a),
+                __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+    }
+}
+
+// Four e4m3 codes as four values of T
+template<typename T> __device__ __forceinline__ u32x2 widen4(uint32_t codes)
+{
+    if constexpr(__is_same(T, Bf16))
+    {
+        return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, false)),
+            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, true))};
+    }
+    else
+    {
+        return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, false)),
+            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, true))};
+    }
+}
+
+// Whether a word of two 16-bit values holds a NaN or an infinity
+template<typename T> __device__ __forceinline__ bool not_finite2(uint32_t w)
+{
+    constexpr uint32_t E = __is_same(T, Bf16) ? 0x7f80u : 0x7c00u;
+    return (w & E) == E || ((w >> 16) & E) == E;
+}
+
+// What a workgroup works on at a time: key blocks [step, step + steps) of unit u (head and row
+// group) of sequence n.
+struct PagedSegment
+{
+    int n, len, blocks;     // sequence, its rows, their key blocks
+    int u, step, steps;
+};
+
+// The folded row of a unit: (m, l) in log2 units, o unnormalised; into the running pair.
+// Eight (head 128) or four (head 64) values from d0 on.  The threads of a row run in one wavefront,
+// in lock step: every one has read lse before the first writes it.
+template<typename T, int VALUES>
+__device__ __forceinline__ void paged_finish_row(const PagedAttendParams &p, int head, int64_t row,
+        int d0, float m, float l, const float (&o)[VALUES])
+{
+    const bool none = m == neg_inf() && l == 0.0f;
+    float lse_out = neg_inf(), w_old = 0.0f, sc = 0.0f;
+    if(none)
+    {
+        if(!p.overwrite)
+        {
+            return;
+        }
+    }
+    else
+    {
+        const float lse_new = (m == neg_inf() ? 0.0f : m) * kLn2 + __builtin_amdgcn_logf(l) * kLn2;
+        float w_new;
+        merge_weights(p.overwrite ? neg_inf() : p.lse[row], lse_new, w_old, w_new, lse_out);
+        sc = w_new / l;
+    }
+    float v[VALUES];
+#pragma unroll
+    for(int i = 0; i < VALUES; ++i)
+    {
+        v[i] = none ? 0.0f : o[i] * sc;
+    }
+    if constexpr(__is_same(T, float))
+    {
+        float *dst = static_cast<float *>(p.A) + row * head + d0;
+#pragma unroll
+        for(int i = 0; i < VALUES; i += 4)
+        {
+            f32x4 *at = reinterpret_cast<f32x4 *>(dst + i);
+            f32x4 out = {v[i], v[i + 1], v[i + 2], v[i + 3]};
+            if(w_old != 0.0f)
+            {
+                out += w_old * *at;
+            }
+            *at = out;
+        }
+    }
+    else
+    {
+        uint16_t *dst = static_cast<uint16_t *>(p.A) + row * head + d0;
+#pragma unroll
+        for(int i = 0; i < VALUES; i += 4)
+        {
+            u32x2 *at = reinterpret_cast<u32x2 *>(dst + i);
+            if(w_old != 0.0f)
+            {
+                const u32x2 old = *at;
+                v[i] += w_old * T::to_float((uint16_t)(old[0] & 0xffffu));
+                v[i + 1] += w_old * T::to_float((uint16_t)(old[0] >> 16));
+                v[i + 2] += w_old * T::to_float((uint16_t)(old[1] & 0xffffu));
+                v[i + 3] += w_old * T::to_float((uint16_t)(old[1] >> 16));
+            }
+            *at = u32x2{T::pack2(v[i], v[i + 1]), T::pack2(v[i + 2], v[i + 3])};
+        }
+    }
+    if(d0 == 0)
+    {
+        p.lse[row] = lse_out;
+    }
+}
+
+// Row of lse (times head: of Q and A) of query row rr of key/value head h of sequence n
+__device__ __forceinline__ int64_t paged_query_row(const PagedAttendParams &p, int n, int h, int rr)
+{
+    const int g = rr / p.q_seq, tok = rr % p.q_seq;
+    return (n + (int64_t)p.c.n_batch * (g + (int64_t)p.kv_group * h)) * p.q_seq + tok;
+}
+
+template<typename T, int KIND, int HEAD, int NR>
+__global__ __launch_bounds__(kPagedThreads, (PagedShape<KIND, HEAD>::WGS_PER_CU))
+void sdpa_paged_kernel(const PagedAttendParams p)
+{
+    typedef PagedShape<KIND, HEAD> Shape;
+    constexpr int RB = Shape::RB, CPR = Shape::CPR, KEYS = Shape::KEYS, GROUPS = Shape::GROUPS;
+    constexpr int LOADS = Shape::LOADS, K_BYTES = Shape::K_BYTES, STAGE = Shape::STAGE;
+    constexpr int DBLOCKS = HEAD / 16;
+    // registers of a row block's query operand: 16 bytes each
+    constexpr int QREGS = KIND == kPaged32 ? HEAD / 16 : HEAD / 32;
+    // the tile type of the probabilities and values as the matrix instruction takes them
+    constexpr bool PV_BF16 = KIND == kPaged16 && __is_same(T, Bf16);
+
+    constexpr int MERGE_LD = HEAD + 4;
+    constexpr int MERGE_BYTES = kPagedWaves * 16 * (MERGE_LD + 2) * 4;
+    static_assert(MERGE_BYTES <= Shape::RING, "the wavefronts' results of a row block share the ring");
+    __shared__ __attribute__((aligned(1024))) char ring[Shape::RING];
+    __shared__ int scan_of[kPagedThreads], wave_sum[kPagedWaves], found;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int col = lane & 15, quad = lane >> 4;
+
+    // ---- the workgroup's run of key blocks ----------------------------------------
+    // Every thread adds up the blocks of a few neighbouring sequences, then a scan.
+    const int chunk = (p.c.n_batch + kPagedThreads - 1) / kPagedThreads;
+    auto blocks_of = [&](int n) { return (paged_len(p.c, n) + Shape::BLOCK - 1) / Shape::BLOCK; };
+    int mine = 0;
+    for(int n = tid * chunk; n < min((tid + 1) * chunk, p.c.n_batch); ++n)
+    {
+        mine += blocks_of(n);
+    }
+    int upto = mine;
+#pragma unroll
+    for(int o = 1; o < 64; o <<= 1)
+    {
+        const int other = __shfl_up(upto, o);
+        upto += lane >= o ? other : 0;
+    }
+    if(lane == 63)
+    {
+        wave_sum[wave] = upto;
+    }
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for(int w = 0; w < kPagedWaves; ++w)
+    {
+        upto += w < wave ? wave_sum[w] : 0;
+        total += wave_sum[w];
+    }
+    total = uniform(total);
+    scan_of[tid] = upto - mine;
+    if(blockIdx.x == 0)
+    {
+        // for the launch that joins the shares
+        int at = upto - mine;
+        for(int n = tid * chunk; n < min((tid + 1) * chunk, p.c.n_batch); ++n)
+        {
+            p.before[n] = at;
+            at += blocks_of(n);
+        }
+        if(tid == 0)
+        {
+            p.before[p.c.n_batch] = total;
+        }
+    }
+    const int64_t all = (int64_t)total * p.units;
+    int64_t at = all * blockIdx.x / p.shares;
+    const int64_t end = all * (blockIdx.x + 1) / p.shares;
+    if(at >= end)
+    {
+        return;
+    }
+    PagedSegment seg;
+    {
+        // the last thread whose sequences begin at or before the block, then sequence by sequence
+        const int block = (int)(at / p.units);
+        if(tid == 0)
+        {
+            found = 0;
+        }
+        __syncthreads();
+        const bool here = tid * chunk < p.c.n_batch && scan_of[tid] <= block
+            && (tid == kPagedThreads - 1 || (tid + 1) * chunk >= p.c.n_batch || scan_of[tid + 1] > block);
+        if(here)
+        {
+            found = tid;
+        }
+        __syncthreads();
+        const int t = uniform(found);
+        int before = uniform(scan_of[t]);
+        seg.n = t * chunk;
+        for(;;)
+        {
+            seg.len = uniform(paged_len(p.c, seg.n));
+            seg.blocks = (seg.len + Shape::BLOCK - 1) / Shape::BLOCK;
+            if(before + seg.blocks > block || seg.n + 1 >= p.c.n_batch)
+            {
+                break;
+            }
+            before += seg.blocks;
+            ++seg.n;
+        }
+        const int rest = (int)(at - (int64_t)before * p.units);
+        seg.u = uniform(rest / seg.blocks);
+        seg.step = uniform(rest % seg.blocks);
+    }
+
+    char *const slots = ring + wave * 2 * STAGE;
+    // lane's place in every load instruction: row of the 16-row group, chunk
+    uint32_t k_off[LOADS], v_off[LOADS];
+#pragma unroll
+    for(int i = 0; i < LOADS; ++i)
+    {
+        const int r = i * Shape::ROWS_PER_LOAD + lane / CPR;
+        k_off[i] = (uint32_t)((r & 15) * RB + ((lane % CPR) ^ Shape::k_swizzle(r)) * 16);
+        v_off[i] = (uint32_t)((r & 15) * RB + ((lane % CPR) ^ Shape::v_swizzle(r)) * 16);
+    }
+    // lane's addresses of the operands in a slot; the 16-key groups lie 16 * RB apart
+    // (the swizzles have a period of 16 rows)
+    constexpr int KREADS = RB / 64;         // 16-byte reads of a key row by its four lanes
+    uint32_t k_at[KREADS];
+#pragma unroll
+    for(int i = 0; i < KREADS; ++i)
+    {
+        k_at[i] = (uint32_t)(col * RB + ((4 * i + quad) ^ Shape::k_swizzle(col)) * 16);
+    }
+    uint32_t v_at[DBLOCKS];
+#pragma unroll
+    for(int db = 0; db < DBLOCKS; ++db)
+    {
+        if constexpr(KIND == kPaged16)
+        {
+            // transposing read: lane i of a quad gives the address of row i / 4, four values
+            // from 4 * (i % 4) on
+            const int r = 4 * quad + (col >> 2), c = 2 * db + ((col >> 1) & 1);
+            v_at[db] = (uint32_t)(K_BYTES + r * RB + (c ^ Shape::v_swizzle(r)) * 16 + 8 * (col & 1));
+        }
+        else if constexpr(KIND == kPaged8)
+        {
+            // ... of row i / 2, eight values from 8 * (i % 2) on; rows 4 .. 7 are the
+            // next 16-key group's
+            const int j = col >> 1, r = 4 * quad + (j & 3) + 16 * (j >> 2);
+            v_at[db] = (uint32_t)(K_BYTES + r * RB + (db ^ Shape::v_swizzle(r)) * 16 + 8 * (col & 1));
+        }
+        else
+        {
+            // single values of row 4 * quad (+ i: the swizzle is the same for the four)
+            const int r = 4 * quad, d = 16 * db + col;
+            v_at[db] = (uint32_t)(K_BYTES + r * RB + ((d >> 2) ^ Shape::v_swizzle(r)) * 16 + 4 * (d & 3));
+        }
+    }
+    const float c_log2 = p.scale * kLog2e;
+
+    for(;;)
+    {
+        seg.steps = (int)min((int64_t)(seg.blocks - seg.step), end - at);
+        const int h = seg.u / p.row_groups, rg = seg.u - h * p.row_groups;
+        const int given = uniform(paged_new(p.c, seg.n, p.q_seq));
+        const int key_lo = seg.step * Shape::BLOCK;
+        const int key_hi = min(key_lo + seg.steps * Shape::BLOCK, seg.len);
+        const int my_first = key_lo + wave * KEYS;
+        const int n_mine = my_first < key_hi ? (key_hi - my_first + Shape::BLOCK - 1) / Shape::BLOCK : 0;
+
+        // ---- the lane's query rows ---------------------------------------------------
+        u32x4 qf[NR][QREGS];
+        int last[NR];           // the last key the row sees
+        bool row_ok[NR];
+#pragma unroll
+        for(int nr = 0; nr < NR; ++nr)
+        {
+            const int rr = (rg * NR + nr) * 16 + col;
+            const int tok = rr % p.q_seq;
+            row_ok[nr] = rr < p.rows && tok < given;
+            last[nr] = p.causal ? seg.len - given + tok : seg.len - 1;
+            constexpr int E = KIND == kPaged32 ? 4 : 2;
+            const char *src = static_cast<const char *>(p.Q)
+                + paged_query_row(p, seg.n, h, rr < p.rows ? rr : 0) * HEAD * E;
+#pragma unroll
+            for(int i = 0; i < QREGS; ++i)
+            {
+                // 16-bit: head values 32i + 8*quad ..; 8-bit pages, whose 16-byte reads hold 16 values:
+                // 64(i/2) + 16*quad + 8(i%2) ..; fp32: 16i + 4*quad ..
+                const int d = KIND == kPaged16 ? 32 * i + 8 * quad
+                    : KIND == kPaged8 ? 64 * (i / 2) + 16 * quad + 8 * (i % 2) : 16 * i + 4 * quad;
+                qf[nr][i] = row_ok[nr] ? *reinterpret_cast<const u32x4 *>(src + d * E) : u32x4{0, 0, 0, 0};
+            }
+        }
+        // below it every row sees every key
+        const int all_see = p.causal ? seg.len - given : seg.len - 1;
+
+        f32x4 o[NR][DBLOCKS];
+        float m_run[NR], l_run[NR], t_run[NR];      // t_run: of score + exponent of the value row
+#pragma unroll
+        for(int nr = 0; nr < NR; ++nr)
+        {
+            m_run[nr] = t_run[nr] = neg_inf();
+            l_run[nr] = 0.0f;
+#pragma unroll
+            for(int db = 0; db < DBLOCKS; ++db)
+            {
+                o[nr][db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        }
+
+        // ---- pages and loads ------------------------------------------------------------
+        const int64_t table_row = (int64_t)seg.n * p.c.max_pages;
+        auto look_up = [&](int i, int (&page)[GROUPS])
+        {
+#pragma unroll
+            for(int g = 0; g < GROUPS; ++g)
+            {
+                // (groups behind the last row take the page of the last)
+                const int row = min(my_first + i * Shape::BLOCK + 16 * g, seg.len - 1);
+                page[g] = scalar_load<int>(p.c.table, 4 * (table_row + (row >> p.c.page_shift)));
+            }
+        };
+        auto in_page = [&](int i, int g)
+        {
+            const int row = min(my_first + i * Shape::BLOCK + 16 * g, seg.len - 1) & ~15;
+            return ((int64_t)h << p.c.page_shift) + (row & ((1 << p.c.page_shift) - 1));
+        };
+        // (a page that is none is read as page 0 and hidden)
+        auto real_page = [&](int page) { return (unsigned)page < (unsigned)p.c.n_pages ? page : 0; };
+        auto fetch = [&](int i, const int (&page)[GROUPS], char *slot)
+        {
+#pragma unroll
+            for(int ld = 0; ld < LOADS; ++ld)
+            {
+                const int g = ld * Shape::ROWS_PER_LOAD / 16;
+                const int64_t from = real_page(page[g]) * p.c.page_stride + in_page(i, g) * RB;
+                load_to_lds16<0, true>(p.c.k_pages + from, k_off[ld], slot + ld * 1024);
+            }
+#pragma unroll
+            for(int ld = 0; ld < LOADS; ++ld)
+            {
+                const int g = ld * Shape::ROWS_PER_LOAD / 16;
+                const int64_t from = real_page(page[g]) * p.c.page_stride + in_page(i, g) * RB;
+                load_to_lds16<0, true>(p.c.v_pages + from, v_off[ld], slot + K_BYTES + ld * 1024);
+            }
+        };
+        // the scale bytes of keys 16g + 4*quad .. + 3
+        auto scales = [&](const uint8_t *of, int i, const int (&page)[GROUPS], uint32_t (&out)[GROUPS])
+        {
+#pragma unroll
+            for(int g = 0; g < GROUPS; ++g)
+            {
+                const u32x4 w = scalar_load<u32x4>(of, real_page(page[g]) * p.c.scale_stride + in_page(i, g));
+                out[g] = quad == 0 ? w[0] : quad == 1 ? w[1] : quad == 2 ? w[2] : w[3];
+            }
+        };
+
+        int page[GROUPS], page_next[GROUPS];
+        if(n_mine > 0)
+        {
+            look_up(0, page);
+            fetch(0, page, slots);
+            look_up(min(1, n_mine - 1), page_next);
+        }
+        for(int i = 0; i < n_mine; ++i)
+        {
+            char *const slot = slots + (i & 1) * STAGE;
+            uint32_t ks[GROUPS], vs[GROUPS];
+            if constexpr(KIND == kPaged8)
+            {
+                scales(p.c.k_scales, i, page, ks);
+                scales(p.c.v_scales, i, page, vs);
+            }
+            uint32_t hidden = 0;        // groups without a page
+#pragma unroll
+            for(int g = 0; g < GROUPS; ++g)
+            {
+                hidden |= (unsigned)page[g] < (unsigned)p.c.n_pages ? 0u : 1u << g;
+            }
+            // the reads of the slot that is filled next have returned
+            paged_wait_lds();
+            if(i + 1 < n_mine)
+            {
+                fetch(i + 1, page_next, slots + ((i + 1) & 1) * STAGE);
+#pragma unroll
+                for(int g = 0; g < GROUPS; ++g)
+                {
+                    page[g] = page_next[g];
+                }
+                look_up(min(i + 2, n_mine - 1), page_next);
+                paged_wait_loads<2 * LOADS>();
+            }
+            else
+            {
+                paged_wait_loads<0>();
+            }
+            const int key0 = my_first + i * Shape::BLOCK;
+            if(key0 + KEYS > seg.len || hidden != 0)
+            {
+                // values of rows that are none: zeros, so that what lies there does not
+                // get into the products (their probabilities are exactly 0)
+#pragma unroll
+                for(int g = 0; g < GROUPS; ++g)
+                {
+                    const int rows_there = (hidden >> g) & 1 ? 0 : min(max(seg.len - key0 - 16 * g, 0), 16);
+                    for(int b = rows_there * RB + lane * 16; b < 16 * RB; b += 64 * 16)
+                    {
+                        *reinterpret_cast<u32x4 *>(slot + K_BYTES + g * 16 * RB + b) = u32x4{0, 0, 0, 0};
+                    }
+                }
+                paged_wait_lds();
+            }
+
+            // ---- scores --------------------------------------------------------------
+            f32x4 s[NR][GROUPS];
+#pragma unroll
+            for(int g = 0; g < GROUPS; ++g)
+            {
+#pragma unroll
+                for(int nr = 0; nr < NR; ++nr)
+                {
+                    s[nr][g] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+#pragma unroll
+                for(int r = 0; r < KREADS; ++r)
+                {
+                    const u32x4 kf = *reinterpret_cast<const u32x4 *>(slot + k_at[r] + g * 16 * RB);
+                    if constexpr(KIND == kPaged16)
+                    {
+#pragma unroll
+                        for(int nr = 0; nr < NR; ++nr)
+                        {
+                            s[nr][g] = mfma32<T>(kf, qf[nr][r], s[nr][g]);
+                        }
+                    }
+                    else if constexpr(KIND == kPaged8)
+                    {
+#pragma unroll
+                        for(int half = 0; half < 2; ++half)
+                        {
+                            const u32x2 a = widen4<T>(kf[2 * half]), b = widen4<T>(kf[2 * half + 1]);
+                            const u32x4 wide = {a[0], a[1], b[0], b[1]};
+#pragma unroll
+                            for(int nr = 0; nr < NR; ++nr)
+                            {
+                                s[nr][g] = mfma32<T>(wide, qf[nr][2 * r + half], s[nr][g]);
+                            }
+                        }
+                    }
+                    else
+                    {
+#pragma unroll
+                        for(int e = 0; e < 4; ++e)
+                        {
+#pragma unroll
+                            for(int nr = 0; nr < NR; ++nr)
+                            {
+                                s[nr][g] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[e]),
+                                        __uint_as_float(qf[nr][r][e]), s[nr][g], 0, 0, 0);
+                            }
+                        }
+                    }
+                }
+            }
+
+            // ---- probabilities -------------------------------------------------------
+            const bool partly = key0 + KEYS - 1 > all_see || hidden != 0;
+            uint32_t pw[NR][GROUPS][2];                 // 16-bit pairs
+            f32x4 pf[NR][GROUPS];                       // fp32
+#pragma unroll
+            for(int nr = 0; nr < NR; ++nr)
+            {
+                float top = neg_inf(), top_t = neg_inf();
+#pragma unroll
+                for(int g = 0; g < GROUPS; ++g)
+                {
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
+                    {
+                        float x = s[nr][g][e] * c_log2;
+                        if constexpr(KIND == kPaged8)
+                        {
+                            x *= scale_of(ks[g], e);
+                        }
+                        if(partly)
+                        {
+                            const int key = key0 + 16 * g + 4 * quad + e;
+                            x = key > last[nr] || key >= seg.len || ((hidden >> g) & 1) ? neg_inf() : x;
+                        }
+                        s[nr][g][e] = x;
+                        top = fmaxf(top, x);
+                        if constexpr(KIND == kPaged8)
+                        {
+                            top_t = fmaxf(top_t, x + (float)((int)((vs[g] >> (8 * e)) & 255u) - 127));
+                        }
+                    }
+                }
+                const float m_new = fmaxf(m_run[nr], quad_max(top));
+                const float m_safe = m_new == neg_inf() ? 0.0f : m_new;
+                const float fade = fast_exp2(m_run[nr] - m_safe);
+                float t_safe = m_safe, fade_o = fade;
+                if constexpr(KIND == kPaged8)
+                {
+                    const float t_new = fmaxf(t_run[nr], quad_max(top_t));
+                    t_safe = t_new == neg_inf() ? 0.0f : t_new;
+                    fade_o = fast_exp2(t_run[nr] - t_safe);
+                    t_run[nr] = t_new;
+                }
+                float sum = 0.0f;
+#pragma unroll
+                for(int g = 0; g < GROUPS; ++g)
+                {
+                    f32x4 x;
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
+                    {
+                        x[e] = fast_exp2(s[nr][g][e] - m_safe);
+                        sum += x[e];
+                    }
+                    if constexpr(KIND == kPaged8)
+                    {
+#pragma unroll
+                        for(int e = 0; e < 4; ++e)
+                        {
+                            x[e] = fast_exp2(s[nr][g][e] + (float)((int)((vs[g] >> (8 * e)) & 255u) - 127) - t_safe);
+                        }
+                    }
+                    if constexpr(KIND == kPaged32)
+                    {
+                        pf[nr][g] = x;
+                    }
+                    else if constexpr(PV_BF16)
+                    {
+                        pw[nr][g][0] = Bf16::pack2(x[0], x[1]);
+                        pw[nr][g][1] = Bf16::pack2(x[2], x[3]);
+                    }
+                    else
+                    {
+                        pw[nr][g][0] = Fp16::pack2(x[0], x[1]);
+                        pw[nr][g][1] = Fp16::pack2(x[2], x[3]);
+                    }
+                }
+                l_run[nr] = l_run[nr] * fade + sum;
+                m_run[nr] = m_new;
+                if(__any(fade_o != 1.0f))
+                {
+#pragma unroll
+                    for(int db = 0; db < DBLOCKS; ++db)
+                    {
+                        o[nr][db] *= fade_o;
+                    }
+                }
+            }
+
+            // ---- output ----------------------------------------------------------------
+            // Product of the slot's values with the probabilities, without the values of keys
+            // behind `upto` where MASKED; row block nr, sum c.
+            auto value_words = [&](int db, int t, u32x4 &w)
+            {
+                typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+                typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+                // keys 32t + {4*quad + 0..3, 16 + 4*quad + 0..3}
+                if constexpr(KIND == kPaged16)
+                {
+                    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (lds_s16x4 *)(slot + v_at[db] + 32 * t * RB)));
+                    const u32x2 b = GROUPS == 1 ? u32x2{0, 0}
+                        : __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                    (lds_s16x4 *)(slot + v_at[db] + (32 * t + 16) * RB)));
+                    w = u32x4{a[0], a[1], b[0], b[1]};
+                }
+                else if constexpr(KIND == kPaged8)
+                {
+                    const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                (lds_i32x2 *)(slot + v_at[db] + 32 * t * RB)));
+                    const u32x2 a = widen4<Fp16>(v[0]), b = widen4<Fp16>(v[1]);
+                    w = u32x4{a[0], a[1], b[0], b[1]};
+                }
+                else
+                {
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
+                    {
+                        // key 16t + 4*quad + e
+                        w[e] = *reinterpret_cast<const uint32_t *>(slot + v_at[db] + (16 * t + e) * RB);
+                    }
+                }
+            };
+            // products of the value words of step t (32 keys, fp32: 16)
+            auto multiply = [&](const u32x4 &w, int t, int nr, f32x4 c) -> f32x4
+            {
+                if constexpr(KIND == kPaged32)
+                {
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
+                    {
+                        c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[e]), pf[nr][t][e], c, 0, 0, 0);
+                    }
+                    return c;
+                }
+                else if constexpr(GROUPS == 1)
+                {
+                    typedef typename std::conditional<PV_BF16, Bf16, Fp16>::type P;
+                    return mfma16<P>(u32x2{w[0], w[1]}, u32x2{pw[nr][0][0], pw[nr][0][1]}, c);
+                }
+                else
+                {
+                    typedef typename std::conditional<PV_BF16, Bf16, Fp16>::type P;
+                    return mfma32<P>(w, u32x4{pw[nr][2 * t][0], pw[nr][2 * t][1], pw[nr][2 * t + 1][0],
+                            pw[nr][2 * t + 1][1]}, c);
+                }
+            };
+            constexpr int TSTEPS = KIND == kPaged32 ? GROUPS : (GROUPS + 1) / 2;
+            bool odd = false;           // values that are no numbers among keys that not every row sees
+            if(partly && p.causal && p.q_seq > 1)
+            {
+                uint32_t any = 0;
+#pragma unroll
+                for(int db = 0; db < DBLOCKS; ++db)
+                {
+#pragma unroll
+                    for(int t = 0; t < TSTEPS; ++t)
+                    {
+                        u32x4 w;
+                        value_words(db, t, w);
+#pragma unroll
+                        for(int e = 0; e < 4; ++e)
+                        {
+                            any |= KIND == kPaged32 ? (w[e] & 0x7f800000u) == 0x7f800000u
+                                : PV_BF16 ? not_finite2<Bf16>(w[e]) : not_finite2<Fp16>(w[e]);
+                        }
+                    }
+                }
+                odd = __any(any != 0);
+            }
+            if(!odd)
+            {
+#pragma unroll
+                for(int db = 0; db < DBLOCKS; ++db)
+                {
+#pragma unroll
+                    for(int t = 0; t < TSTEPS; ++t)
+                    {
+                        u32x4 w;
+                        value_words(db, t, w);
+#pragma unroll
+                        for(int nr = 0; nr < NR; ++nr)
+                        {
+                            o[nr][db] = multiply(w, t, nr, o[nr][db]);
+                        }
+                    }
+                }
+            }
+            else
+            {
+                // A probability of 0 does not hide such a value (0 * NaN): token by token, with the
+                // values behind what the token sees taken out, the rows of the token taken over.
+                for(int tok = 0; tok < given; ++tok)
+                {
+                    const int upto = all_see + (p.causal ? tok : 0);
+#pragma unroll
+                    for(int db = 0; db < DBLOCKS; ++db)
+                    {
+                        f32x4 fresh[NR];
+#pragma unroll
+                        for(int nr = 0; nr < NR; ++nr)
+                        {
+                            fresh[nr] = o[nr][db];
+                        }
+#pragma unroll
+                        for(int t = 0; t < TSTEPS; ++t)
+                        {
+                            u32x4 w;
+                            value_words(db, t, w);
+#pragma unroll
+                            for(int e = 0; e < 4; ++e)
+                            {
+                                if constexpr(KIND == kPaged32)
+                                {
+                                    w[e] = key0 + 16 * t + 4 * quad + e > upto ? 0u : w[e];
+                                }
+                                else
+                                {
+                                    const int key = key0 + 32 * t + 16 * (e >> 1) + 4 * quad + 2 * (e & 1);
+                                    w[e] &= (key > upto ? 0u : 0xffffu) | (key + 1 > upto ? 0u : 0xffff0000u);
+                                }
+                            }
+#pragma unroll
+                            for(int nr = 0; nr < NR; ++nr)
+                            {
+                                fresh[nr] = multiply(w, t, nr, fresh[nr]);
+                            }
+                        }
+#pragma unroll
+                        for(int nr = 0; nr < NR; ++nr)
+                        {
+                            const bool mine_too = ((rg * NR + nr) * 16 + col) % p.q_seq == tok;
+#pragma unroll
+                            for(int e = 0; e < 4; ++e)
+                            {
+                                o[nr][db][e] = mine_too ? fresh[nr][e] : o[nr][db][e];
+                            }
+                        }
+                    }
+                }
+            }
+        }
+
+        // ---- the four wavefronts' results, then the unit's or the share's ----------------
+        const bool begins = seg.step == 0, ends = seg.step + seg.steps == seg.blocks;
+        float *const merge_o = reinterpret_cast<float *>(ring);
+        float *const merge_ml = merge_o + kPagedWaves * 16 * MERGE_LD;
+#pragma unroll
+        for(int nr = 0; nr < NR; ++nr)
+        {
+            __syncthreads();        // every wavefront is done with the ring, or with the last row block
+            float m = m_run[nr], l = quad_sum(l_run[nr]), to_m = 1.0f;
+            if constexpr(KIND == kPaged8)
+            {
+                to_m = m == neg_inf() ? 0.0f : fast_exp2(t_run[nr] - m);
+            }
+            if(!row_ok[nr])
+            {
+                m = neg_inf();
+                l = 0.0f;
+            }
+#pragma unroll
+            for(int db = 0; db < DBLOCKS; ++db)
+            {
+                f32x4 x = o[nr][db];
+                if constexpr(KIND == kPaged8)
+                {
+                    x *= to_m;
+                }
+                *reinterpret_cast<f32x4 *>(merge_o + (wave * 16 + col) * MERGE_LD + 16 * db + 4 * quad)
+                    = row_ok[nr] ? x : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+            if(quad == 0)
+            {
+                merge_ml[2 * (wave * 16 + col)] = m;
+                merge_ml[2 * (wave * 16 + col) + 1] = l;
+            }
+            __syncthreads();
+            constexpr int VALUES = HEAD / 16;       // a thread's, of 16 threads a row
+            const int row = tid / 16, d0 = (tid % 16) * VALUES;
+            float top = neg_inf(), sum = 0.0f, v[VALUES];
+#pragma unroll
+            for(int w = 0; w < kPagedWaves; ++w)
+            {
+                top = fmaxf(top, merge_ml[2 * (w * 16 + row)]);
+            }
+            const float safe = top == neg_inf() ? 0.0f : top;
+#pragma unroll
+            for(int j = 0; j < VALUES; ++j)
+            {
+                v[j] = 0.0f;
+            }
+#pragma unroll
+            for(int w = 0; w < kPagedWaves; ++w)
+            {
+                const float f = fast_exp2(merge_ml[2 * (w * 16 + row)] - safe);
+                sum += f * merge_ml[2 * (w * 16 + row) + 1];
+#pragma unroll
+                for(int j = 0; j < VALUES; ++j)
+                {
+                    v[j] += f * merge_o[(w * 16 + row) * MERGE_LD + d0 + j];
+                }
+            }
+            const int rr = (rg * NR + nr) * 16 + row;
+            if(begins && ends)
+            {
+                if(rr < p.rows)
+                {
+                    paged_finish_row<T>(p, HEAD, paged_query_row(p, seg.n, h, rr), d0, top, sum, v);
+                }
+            }
+            else
+            {
+                const int64_t place = ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * (NR * 16) + nr * 16 + row;
+#pragma unroll
+                for(int j = 0; j < VALUES; j += 4)
+                {
+                    *reinterpret_cast<f32x4 *>(p.part_o + place * HEAD + d0 + j)
+                        = f32x4{v[j], v[j + 1], v[j + 2], v[j + 3]};
+                }
+                if(d0 == 0)
+                {
+                    p.part_ml[2 * place] = top;
+                    p.part_ml[2 * place + 1] = sum;
+                }
+            }
+        }
+        at += seg.steps;
+        if(at >= end)
+        {
+            return;
+        }
+        // the next unit, of this sequence or of the next that has rows
+        __syncthreads();
+        seg.step = 0;
+        if(++seg.u == p.units)
+        {
+            seg.u = 0;
+            do
+            {
+                ++seg.n;
+                seg.len = uniform(paged_len(p.c, seg.n));
+                seg.blocks = (seg.len + Shape::BLOCK - 1) / Shape::BLOCK;
+            } while(seg.blocks == 0);       // (`end` lies behind a block that exists)
+        }
+    }
+}
+
+// Joins the shares of the units that more than one workgroup worked on, and writes the
+// rows of sequences without keys.  HEAD/4 threads a row.
+template<typename T, int HEAD>
+__global__ __launch_bounds__(256)
+void sdpa_paged_join_kernel(const PagedAttendParams p, int rows_of_share)
+{
+    constexpr int TPR = HEAD / 4;
+    const int64_t t = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const int d0 = (threadIdx.x % TPR) * 4;
+    // t = (n * n_head_kv + h) * rows + rr
+    const int64_t all_rows = (int64_t)p.c.n_batch * p.c.n_head_kv * p.rows;
+    if(t >= all_rows)
+    {
+        return;
+    }
+    const int rr = (int)(t % p.rows);
+    const int64_t unit = t / p.rows;
+    const int n = (int)(unit / p.c.n_head_kv), h = (int)(unit % p.c.n_head_kv);
+    const int64_t row = paged_query_row(p, n, h, rr);
+    const int before = p.before[n], blocks = p.before[n + 1] - before;
+    float top = neg_inf(), sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if(blocks > 0)
+    {
+        const int64_t all = (int64_t)p.before[p.c.n_batch] * p.units;
+        const int rg = rr / rows_of_share, in_share = rr - rg * rows_of_share;
+        const int64_t first_block = (int64_t)before * p.units + (int64_t)(h * p.row_groups + rg) * blocks;
+        // share w takes blocks [w * all / shares, (w + 1) * all / shares)
+        const int w0 = (int)(((first_block + 1) * p.shares - 1) / all);
+        const int w1 = (int)(((first_block + blocks) * p.shares - 1) / all);
+        if(w0 == w1)
+        {
+            return;         // finished there
+        }
+        for(int w = w0; w <= w1; ++w)
+        {
+            if(all * w / p.shares == all * (w + 1) / p.shares)
+            {
+                continue;   // (more shares than blocks: this one has none)
+            }
+            const int64_t place = ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * rows_of_share + in_share;
+            const float m = p.part_ml[2 * place], l = p.part_ml[2 * place + 1];
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(p.part_o + place * HEAD + d0);
+            const float next = fmaxf(top, m);
+            const float safe = next == neg_inf() ? 0.0f : next;
+            const float old = fast_exp2(top - safe), f = fast_exp2(m - safe);
+            sum = sum * old + l * f;
+#pragma unroll
+            for(int j = 0; j < 4; ++j)
+            {
+                v[j] = v[j] * old + x[j] * f;
+            }
+            top = next;
+        }
+    }
+    paged_finish_row<T>(p, HEAD, row, d0, top, sum, v);
+}
+
+static int row_blocks(int64_t rows)
+{
+    return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+}
+
+static size_t align16(size_t x)
+{
+    return (x + 15) & ~(size_t)15;
+}
+
+size_t paged_attend_workspace_bytes(int64_t n_batch, int64_t rows, int64_t head)
+{
+    const size_t places = (size_t)kPagedShares * 2 * 16 * row_blocks(rows);
+    return align16(4 * ((size_t)n_batch + 1)) + places * (size_t)(head + 2) * 4;
+}
+
+template<typename T, int KIND, int HEAD, int NR>
+static int launch_form(hipStream_t stream, PagedAttendParams &p)
+{
+    typedef PagedShape<KIND, HEAD> Shape;
+    p.row_groups = (p.rows + 16 * NR - 1) / (16 * NR);
+    p.units = p.c.n_head_kv * p.row_groups;
+    // at most as many shares as there can be blocks
+    const int64_t most = (int64_t)p.c.n_batch * p.units * (p.c.max_rows / Shape::BLOCK + 1);
+    const int64_t places = kPagedCUs * Shape::WGS_PER_CU;
+    p.shares = (int32_t)(most < places ? most : places);
+    hipLaunchKernelGGL((sdpa_paged_kernel<T, KIND, HEAD, NR>), dim3((unsigned)p.shares),
+            dim3(kPagedThreads), 0, stream, p);
+    const int64_t all_rows = (int64_t)p.c.n_batch * p.c.n_head_kv * p.rows;
+    const int per_wg = 256 / (HEAD / 4);
+    hipLaunchKernelGGL((sdpa_paged_join_kernel<T, HEAD>), dim3((unsigned)((all_rows + per_wg - 1) / per_wg)),
+            dim3(256), 0, stream, p, 16 * NR);
+    return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;
+}
+
+template<typename T, int KIND>
+static int launch_kind(hipStream_t stream, PagedAttendParams &p, int head)
+{
+    switch(row_blocks(p.rows) * 256 + head)
+    {
+        case 256 + 64: return launch_form<T, KIND, 64, 1>(stream, p);
+        case 256 + 128: return launch_form<T, KIND, 128, 1>(stream, p);
+        case 512 + 64: return launch_form<T, KIND, 64, 2>(stream, p);
+        case 512 + 128: return launch_form<T, KIND, 128, 2>(stream, p);
+        case 1024 + 64: return launch_form<T, KIND, 64, 4>(stream, p);
+        case 1024 + 128: return launch_form<T, KIND, 128, 4>(stream, p);
+        default: return NNTILE_HIP_EUNSUPPORTED;
+    }
+}
+
+int launch_paged_attend(hipStream_t stream, int dtype, PagedAttendParams &p, int head, void *workspace)
+{
+    const size_t places = (size_t)kPagedShares * 2 * 16 * row_blocks(p.rows);
+    p.before = static_cast<int32_t *>(workspace);
+    p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + align16(4 * ((size_t)p.c.n_batch + 1)));
+    p.part_ml = p.part_o + places * (size_t)head;
+    if(p.c.k_scales != nullptr)
+    {
+        return dtype == 0 ? launch_kind<Bf16, kPaged8>(stream, p, head)
+            : dtype == 1 ? launch_kind<Fp16, kPaged8>(stream, p, head) : NNTILE_HIP_EUNSUPPORTED;
+    }
+    return dtype == 0 ? launch_kind<Bf16, kPaged16>(stream, p, head)
+        : dtype == 1 ? launch_kind<Fp16, kPaged16>(stream, p, head)
+        : launch_kind<float, kPaged32>(stream, p, head);
+}
+
+} // namespace nntile_hip

@@ -89,6 +89,30 @@ class BwdGridArgs(ctypes.Structure):
                 ("workspace_bytes", ctypes.c_size_t)]
 
 
+class PagedCacheArgs(ctypes.Structure):
+    """nntile_hip_paged_cache."""
+    _fields_ = [("k_pages", _vp), ("v_pages", _vp), ("k_scales", _vp), ("v_scales", _vp),
+                ("table", _vp), ("lens", _vp), ("new_rows", _vp),
+                ("head", _i64), ("page_rows", _i64), ("n_head_kv", _i64), ("n_pages", _i64),
+                ("max_pages", _i64), ("n_batch", _i64), ("page_stride", _i64), ("scale_stride", _i64)]
+
+
+class PagedArgs(ctypes.Structure):
+    """nntile_hip_sdpa_paged_args."""
+    _fields_ = [("cache", PagedCacheArgs), ("q_seq", _i64), ("kv_group", _i64),
+                ("mask_mode", ctypes.c_int32), ("flags", ctypes.c_int32),
+                ("Q", _vp), ("lse", _vp), ("A", _vp)]
+
+
+class RopeAxesArgs(ctypes.Structure):
+    """nntile_hip_rope_axes_args."""
+    _fields_ = [("head", _i64), ("seq", _i64), ("n_batch", _i64), ("heads_q", _i64),
+                ("heads_k", _i64), ("n_axes", _i64), ("pos_batch_stride", _i64),
+                ("backward", ctypes.c_int32), ("reserved", ctypes.c_int32),
+                ("positions", _vp), ("freqs", _vp), ("axes", _vp),
+                ("q", _vp), ("k", _vp), ("q_out", _vp), ("k_out", _vp)]
+
+
 class VariableInterface(ctypes.Structure):
     _fields_ = [("id", ctypes.c_int), ("ptr", ctypes.c_size_t),
                 ("dev_handle", ctypes.c_size_t), ("offset", ctypes.c_size_t),
@@ -137,6 +161,11 @@ EXPORTS = (
     + ["nntile_hip_sdpa_fwd_tile_cache_" + t for t in ("bf16", "fp16", "fp32")]
     + ["nntile_hip_sdpa_fwd_tile_cache_ws_" + t for t in ("bf16", "fp16", "fp32")]
     + ["nntile_hip_sdpa_fwd_tile_cache_workspace_bytes" + t for t in ("", "_fp32")]
+    + ["nntile_hip_paged_kv_append_" + t for t in ("bf16", "fp16", "fp32")]
+    + ["nntile_hip_paged_kv_read_" + t for t in ("bf16", "fp16", "fp32")]
+    + ["nntile_hip_sdpa_fwd_paged_" + t for t in ("bf16", "fp16", "fp32")]
+    + ["nntile_hip_sdpa_fwd_paged_workspace_bytes"]
+    + ["nntile_hip_rope_axes_" + t for t in ("bf16", "fp16", "fp32")]
     + ["nntile_hip_mask_tile_class_" + t for t in ("bf16", "fp16", "fp32", "bool")]
     + ["nntile_hip_sdpa_fwd_grid_codelet_" + t for t in ("bf16", "fp16", "fp32")]
     + ["nntile_hip_sdpa_bwd_grid_codelet_" + t for t in ("bf16", "fp16")]
@@ -213,6 +242,20 @@ def lib():
             f = getattr(L, "nntile_hip_kv_cache_append_" + t)
             f.argtypes = [_vp] + [_i64] * 5 + [_vp] * 4
             f.restype = ctypes.c_int
+            f = getattr(L, "nntile_hip_paged_kv_append_" + t)
+            f.argtypes = [_vp, ctypes.POINTER(PagedCacheArgs), _i64, _vp, _vp]
+            f.restype = ctypes.c_int
+            f = getattr(L, "nntile_hip_paged_kv_read_" + t)
+            f.argtypes = [_vp, ctypes.POINTER(PagedCacheArgs), _i64, _i64, _vp, _vp]
+            f.restype = ctypes.c_int
+            f = getattr(L, "nntile_hip_sdpa_fwd_paged_" + t)
+            f.argtypes = [_vp, ctypes.POINTER(PagedArgs), _vp, ctypes.c_size_t]
+            f.restype = ctypes.c_int
+            f = getattr(L, "nntile_hip_rope_axes_" + t)
+            f.argtypes = [_vp, ctypes.POINTER(RopeAxesArgs)]
+            f.restype = ctypes.c_int
+        L.nntile_hip_sdpa_fwd_paged_workspace_bytes.argtypes = [ctypes.POINTER(PagedArgs)]
+        L.nntile_hip_sdpa_fwd_paged_workspace_bytes.restype = ctypes.c_size_t
         for t in ("bf16", "fp16", "fp32", "bool"):
             f = getattr(L, "nntile_hip_mask_tile_class_" + t)
             f.argtypes = [_vp, _i64, _i64, _vp, _i64, _vp, ctypes.POINTER(ctypes.c_int32)]
@@ -740,6 +783,81 @@ def transpose(alpha, src, dst, m, n, stream=None):
     """dst = alpha * src^T; src is m x n in Fortran order (memory order of a
     C-ordered [n, m] tensor), dst n x m in Fortran order."""
     _check(_native().transpose(alpha, src, dst, m, n, stream), "transpose")
+
+
+def paged_kv_append(k_new, v_new, k_pages, v_pages, table, lens, k_scales=None, v_scales=None,
+                    new_rows=None, stream=None):
+    """Write k_new, v_new ([n_head_kv*n_batch, rows, head]) into the pages of a
+    cache: k_pages, v_pages [n_pages, n_head_kv, page_rows, head] in the type of
+    the tiles, or torch.float8_e4m3fn with k_scales, v_scales [n_pages,
+    n_head_kv, page_rows] (uint8, the exponent of a row's power of two + 127);
+    only their first axis may be strided.  table: [n_batch, max_pages] int32 page
+    numbers; lens: [n_batch] int32 rows of each sequence, the new ones included;
+    new_rows: [n_batch] int32, how many of `rows` each sequence brings (None: all).
+    Tables and lengths are read on the device when the call runs."""
+    _check(_native().paged_append(k_new, v_new, k_pages, v_pages, table, lens, k_scales, v_scales,
+                                  new_rows, stream), "paged_kv_append")
+
+
+def paged_kv_read(k_pages, v_pages, table, lens, k_out, v_out, first=0, k_scales=None,
+                  v_scales=None, stream=None):
+    """Rows [first, first + rows) of every sequence of a paged cache (see
+    paged_kv_append) into k_out, v_out ([n_head_kv*n_batch, rows, head]); rows at
+    or behind lens are zeros."""
+    _check(_native().paged_read(k_pages, v_pages, table, lens, k_out, v_out, first, k_scales,
+                                v_scales, stream), "paged_kv_read")
+
+
+def paged_workspace_bytes(Q, n_batch, kv_group):
+    """Bytes of workspace sdpa_fwd_paged needs for queries like Q over any
+    cache of n_batch sequences."""
+    if n_batch < 1 or kv_group < 1 or Q.dim() != 3 or Q.shape[0] % (n_batch * kv_group):
+        raise SdpaError(EINVAL, "paged_workspace_bytes")
+    a = PagedArgs()
+    a.q_seq, a.kv_group = Q.shape[1], kv_group
+    a.cache.head, a.cache.n_batch = Q.shape[2], n_batch
+    a.cache.n_head_kv = Q.shape[0] // (n_batch * kv_group)
+    return int(lib().nntile_hip_sdpa_fwd_paged_workspace_bytes(ctypes.byref(a)))
+
+
+def sdpa_fwd_paged(k_pages, v_pages, table, lens, Q, lse, A, mask_mode, kv_group, workspace,
+                   k_scales=None, v_scales=None, new_rows=None, flags=0, stream=None):
+    """Attention of the newest tokens over a paged cache (see paged_kv_append):
+    Q, A [n_head_kv*kv_group*n_batch, q_seq, head], lse [.., q_seq].  Query j of
+    a sequence is its row lens - new_rows + j (new_rows None: q_seq);
+    MASK_CAUSAL lets it see the rows up to its own, MASK_NONE all.  workspace: a
+    device byte tensor of at least paged_workspace_bytes()."""
+    _check(_native().fwd_paged(k_pages, v_pages, table, lens, Q, lse, A, mask_mode, kv_group,
+                               workspace, k_scales, v_scales, new_rows, flags, stream),
+           "sdpa_fwd_paged")
+
+
+def rope_axes_freqs(head, sections, base=10000.0, own=False, device="cuda"):
+    """freqs and axes of rope_axes for `sections` pairs on each axis, one after
+    the other (together head/2): pair i turns by base^(-2i/head) radians per
+    position of its axis; own=True counts i, and head, within the axis."""
+    if head < 2 or head % 2 or not sections or min(sections) < 0 or sum(sections) != head // 2:
+        raise ValueError("sections are numbers of pairs that add up to half of the head")
+    pair = torch.arange(head // 2, dtype=torch.float64)
+    axes = torch.repeat_interleave(torch.arange(len(sections)), torch.tensor(sections))
+    if own:
+        start = torch.tensor([sum(sections[:a]) for a in range(len(sections))])
+        size = torch.tensor([float(max(1, n)) for n in sections], dtype=torch.float64)
+        power = (pair - start[axes]) / size[axes]
+    else:
+        power = 2.0 * pair / head
+    freqs = torch.pow(torch.tensor(float(base), dtype=torch.float64), -power)
+    return freqs.to(device), axes.to(torch.int32).to(device)
+
+
+def rope_axes(positions, freqs, axes, q, q_out, k=None, k_out=None, backward=False, stream=None):
+    """Rotary embedding of q (and k) ([heads*n_batch, seq, head]) with angles
+    positions[axes[i]] * freqs[i] for pair i; positions [n_axes, n_batch, seq]
+    int64 ([n_axes, 1, seq]: the same for every entry of q and k), freqs [head/2]
+    float64, axes [head/2] int32.  backward=True applies the transposed rotation
+    (dy -> dx).  q_out may be q."""
+    _check(_native().rope_axes(positions, freqs, axes, q, q_out, k, k_out, backward, stream),
+           "rope_axes")
 
 
 def flash_sdpa_fwd_codelet(K, Q, mask, lse, V, A, scratch_lse=None, scratch_A=None,
