@@ -40,29 +40,43 @@ typedef __attribute__((ext_vector_type(2))) int i32x2;
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
 typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
 
-constexpr int kPagedWaves = 4;
-constexpr int kPagedThreads = 64 * kPagedWaves;
 constexpr int kPagedCUs = 256;
 // Workgroups that the keys are shared out to at most: two a CU
 constexpr int kPagedShares = 2 * kPagedCUs;
+// What a unit costs beside its key blocks, in blocks
+constexpr int kPagedUnitCost = 1;
+// A count of shares and the tag above it
+constexpr unsigned long long kPagedTagUnit = 4096;
+static_assert(kPagedShares < (int)kPagedTagUnit, "counts stay below the tag");
+// A value no earlier call of this process has used; its low four bits are clear.
+unsigned long long next_decode_tag();
 
 enum PagedKind { kPaged16, kPaged8, kPaged32 };
 
-template<int KIND, int HEAD>
+template<int KIND, int HEAD, int NR, int HALVES>
 struct PagedShape
 {
+    static constexpr int STREAMS = 4;                       // wavefronts that take different keys
+    static constexpr int WAVES = STREAMS * HALVES;
+    static constexpr int THREADS = 64 * WAVES;
+    static constexpr int QROWS = 16 * NR * HALVES;          // query rows of a workgroup
     static constexpr int RB = KIND == kPaged32 ? HEAD * 4 : KIND == kPaged8 ? HEAD : HEAD * 2;   // bytes of a row
     static constexpr int CPR = RB / 16;                     // 16-byte chunks of a row
     static constexpr int RPL = RB >= 256 ? 1 : 256 / RB;    // rows per 256-byte line of LDS banks
     static constexpr int KEYS = 4096 / RB > 16 ? 4096 / RB : 16;    // of a wavefront's step
-    static constexpr int BLOCK = kPagedWaves * KEYS;        // keys of a workgroup's step
+    static constexpr int BLOCK = STREAMS * KEYS;        // keys of a workgroup's step
     static constexpr int GROUPS = KEYS / 16;
     static constexpr int K_BYTES = KEYS * RB;
     static constexpr int STAGE = 2 * K_BYTES;
     static constexpr int LOADS = K_BYTES / 1024;            // load instructions of a step's K
     static constexpr int ROWS_PER_LOAD = 1024 / RB;
-    static constexpr int RING = kPagedWaves * 2 * STAGE;
+    static constexpr int RING = WAVES * 2 * STAGE;
     static constexpr int WGS_PER_CU = RING > 72 * 1024 ? 1 : 2;
+    static constexpr int MIN_WAVES = WAVES * WGS_PER_CU / 4;        // of a SIMD
+    // the query rows: the operands of one block of 16 stay in registers, those of two in LDS
+    static constexpr int QB = HEAD * (KIND == kPaged32 ? 4 : 2);
+    static constexpr int Q_BYTES = NR > 1 ? QROWS * QB : 16;
+    static __host__ __device__ constexpr int q_swizzle(int r) { return r % (QB / 16 < 16 ? QB / 16 : 16); }
 
     // Where chunk c of row r lies: chunk position c ^ swizzle(r) of the row, so that the
     // rows one LDS instruction reads fall on different banks.
@@ -183,6 +197,38 @@ struct PagedSegment
     int u, step, steps;
 };
 
+// Share w of `all` blocks: [begin(w), begin(w + 1)); the share that has a block.
+struct PagedSplit
+{
+    uint32_t base, rest;    // the first `rest` shares take one block more
+    __device__ __forceinline__ PagedSplit(uint32_t all, uint32_t shares) : base(all / shares), rest(all % shares) {}
+    __device__ __forceinline__ uint32_t begin(uint32_t w) const { return w * base + min(w, rest); }
+    __device__ __forceinline__ uint32_t of(uint32_t block) const
+    {
+        const uint32_t longer = rest * (base + 1);
+        return block < longer ? block / (base + 1) : rest + (block - longer) / base;
+    }
+};
+
+// Partial results go from one workgroup to another of the same launch, on any XCD: stores and
+// loads that the device serves, not a CU's or an XCD's own cache.
+__device__ __forceinline__ void put2(float *to, float a, float b)
+{
+    typedef __attribute__((ext_vector_type(2))) float f32x2;
+    __hip_atomic_store(reinterpret_cast<unsigned long long *>(to),
+            __builtin_bit_cast(unsigned long long, f32x2{a, b}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+__device__ __forceinline__ void get2(const float *from, float &a, float &b)
+{
+    typedef __attribute__((ext_vector_type(2))) float f32x2;
+    const f32x2 v = __builtin_bit_cast(f32x2, __hip_atomic_load(
+                reinterpret_cast<unsigned long long *>(const_cast<float *>(from)), __ATOMIC_RELAXED,
+                __HIP_MEMORY_SCOPE_AGENT));
+    a = v[0];
+    b = v[1];
+}
+
 // The folded row of a unit: (m, l) in log2 units, o unnormalised; into the running pair.
 // Eight (head 128) or four (head 64) values from d0 on.  The threads of a row run in one wavefront,
 // in lock step: every one has read lse before the first writes it.
@@ -258,36 +304,157 @@ __device__ __forceinline__ int64_t paged_query_row(const PagedAttendParams &p, i
     return (n + (int64_t)p.c.n_batch * (g + (int64_t)p.kv_group * h)) * p.q_seq + tok;
 }
 
-template<typename T, int KIND, int HEAD, int NR>
-__global__ __launch_bounds__(kPagedThreads, (PagedShape<KIND, HEAD>::WGS_PER_CU))
+// Joins the shares w0 .. w0 + parts - 1 of a unit, in this order, and finishes its rows.  HEAD/4 threads a
+// row; where the rows leave threads over, they take turns at the shares and the sums
+// are added up through LDS.
+template<typename T, int HEAD, int THREADS, int QROWS>
+__device__ __forceinline__ void paged_join(const PagedAttendParams &p, int n, int h, int rg, int rows_here,
+        int w0, int parts, float *lds)
+{
+    constexpr int TPR = HEAD / 4, ROWS = THREADS / TPR;
+    constexpr int AT_ONCE = 8;
+    int turns = 1;
+    while(2 * turns * rows_here <= ROWS && 2 * turns <= parts)
+    {
+        turns *= 2;
+    }
+    const int d0 = (threadIdx.x % TPR) * 4, slot = threadIdx.x / TPR;
+    const int turn = slot % turns;
+    for(int r0 = 0; r0 < rows_here; r0 += ROWS / turns)
+    {
+        const int r = r0 + slot / turns;
+        float top = neg_inf(), sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if(r < rows_here)
+        {
+            for(int i0 = turn; i0 < parts; i0 += AT_ONCE * turns)
+            {
+                float m[AT_ONCE], l[AT_ONCE], x[AT_ONCE][4];
+#pragma unroll
+                for(int j = 0; j < AT_ONCE; ++j)
+                {
+                    // (behind the last share: it again, with no weight)
+                    const int i = min(i0 + j * turns, parts - 1);
+                    const int64_t place = ((int64_t)(w0 + i) * 2 + (i == 0 ? 1 : 0)) * QROWS + r;
+                    get2(p.part_ml + 2 * place, m[j], l[j]);
+                    get2(p.part_o + place * HEAD + d0, x[j][0], x[j][1]);
+                    get2(p.part_o + place * HEAD + d0 + 2, x[j][2], x[j][3]);
+                }
+                float next = top;
+#pragma unroll
+                for(int j = 0; j < AT_ONCE; ++j)
+                {
+                    next = i0 + j * turns < parts ? fmaxf(next, m[j]) : next;
+                }
+                const float safe = next == neg_inf() ? 0.0f : next;
+                const float old = fast_exp2(top - safe);
+                sum *= old;
+#pragma unroll
+                for(int e = 0; e < 4; ++e)
+                {
+                    v[e] *= old;
+                }
+#pragma unroll
+                for(int j = 0; j < AT_ONCE; ++j)
+                {
+                    if(i0 + j * turns < parts)
+                    {
+                        const float f = fast_exp2(m[j] - safe);
+                        sum += l[j] * f;
+#pragma unroll
+                        for(int e = 0; e < 4; ++e)
+                        {
+                            v[e] += x[j][e] * f;
+                        }
+                    }
+                }
+                top = next;
+            }
+        }
+        if(turns > 1)
+        {
+            // (r0 takes one value only: the rows fit beside each other)
+            float *const at = lds + slot * (HEAD + 4);
+            *reinterpret_cast<f32x4 *>(at + d0) = f32x4{v[0], v[1], v[2], v[3]};
+            if(d0 == 0)
+            {
+                at[HEAD] = top;
+                at[HEAD + 1] = sum;
+            }
+            __syncthreads();
+            if(turn == 0 && r < rows_here)
+            {
+                float next = neg_inf();
+                for(int j = 0; j < turns; ++j)
+                {
+                    next = fmaxf(next, at[j * (HEAD + 4) + HEAD]);
+                }
+                const float safe = next == neg_inf() ? 0.0f : next;
+                sum = 0.0f;
+                f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+                for(int j = 0; j < turns; ++j)
+                {
+                    const float f = fast_exp2(at[j * (HEAD + 4) + HEAD] - safe);
+                    sum += f * at[j * (HEAD + 4) + HEAD + 1];
+                    o += f * *reinterpret_cast<const f32x4 *>(at + j * (HEAD + 4) + d0);
+                }
+                top = next;
+#pragma unroll
+                for(int e = 0; e < 4; ++e)
+                {
+                    v[e] = o[e];
+                }
+            }
+        }
+        if(turn == 0 && r < rows_here)
+        {
+            paged_finish_row<T>(p, HEAD, paged_query_row(p, n, h, rg * QROWS + r), d0, top, sum, v);
+        }
+    }
+}
+
+template<typename T, int KIND, int HEAD, int NR, int HALVES>
+__global__ __launch_bounds__((PagedShape<KIND, HEAD, NR, HALVES>::THREADS), (PagedShape<KIND, HEAD, NR, HALVES>::MIN_WAVES))
 void sdpa_paged_kernel(const PagedAttendParams p)
 {
-    typedef PagedShape<KIND, HEAD> Shape;
+    typedef PagedShape<KIND, HEAD, NR, HALVES> Shape;
     constexpr int RB = Shape::RB, CPR = Shape::CPR, KEYS = Shape::KEYS, GROUPS = Shape::GROUPS;
     constexpr int LOADS = Shape::LOADS, K_BYTES = Shape::K_BYTES, STAGE = Shape::STAGE;
+    constexpr int WAVES = Shape::WAVES, STREAMS = Shape::STREAMS, THREADS = Shape::THREADS;
     constexpr int DBLOCKS = HEAD / 16;
     // registers of a row block's query operand: 16 bytes each
     constexpr int QREGS = KIND == kPaged32 ? HEAD / 16 : HEAD / 32;
-    // the tile type of the probabilities and values as the matrix instruction takes them
+    constexpr int QROWS = Shape::QROWS;
+    constexpr bool Q_IN_LDS = NR > 1;
+    // the type of the probabilities and values as the matrix instruction takes them
     constexpr bool PV_BF16 = KIND == kPaged16 && __is_same(T, Bf16);
+    typedef typename std::conditional<PV_BF16, Bf16, Fp16>::type PV;
 
     constexpr int MERGE_LD = HEAD + 4;
-    constexpr int MERGE_BYTES = kPagedWaves * 16 * (MERGE_LD + 2) * 4;
+    constexpr int MERGE_BYTES = STREAMS * 16 * HALVES * (MERGE_LD + 2) * 4;
     static_assert(MERGE_BYTES <= Shape::RING, "the wavefronts' results of a row block share the ring");
+    static_assert(STREAMS * 64 == 256, "the merge takes 16 threads a row");
+    constexpr int JOIN_ROWS = THREADS / (HEAD / 4);     // rows that are joined at a time
+    static_assert(JOIN_ROWS * (HEAD + 4) * 4 <= Shape::RING, "... and so do the shares' sums");
     __shared__ __attribute__((aligned(1024))) char ring[Shape::RING];
-    __shared__ int scan_of[kPagedThreads], wave_sum[kPagedWaves], found;
+    __shared__ __attribute__((aligned(16))) char q_rows[Shape::Q_BYTES];
+    __shared__ int scan_of[THREADS], wave_sum[WAVES], found;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int col = lane & 15, quad = lane >> 4;
+    // Up to 64 rows: two wavefronts read the same keys at about the same time, the second
+    // through the L2, for 32 rows each (one with all 64 has too few registers).
+    const int stream = wave % STREAMS, half = wave / STREAMS;
 
     // ---- the workgroup's run of key blocks ----------------------------------------
-    // Every thread adds up the blocks of a few neighbouring sequences, then a scan.
-    const int chunk = (p.c.n_batch + kPagedThreads - 1) / kPagedThreads;
+    // Every thread adds up the blocks of a few neighbouring sequences, then a scan.  A unit counts
+    // as a block more than it has: its begin and end cost about as much.
+    const int chunk = (p.c.n_batch + THREADS - 1) / THREADS;
     auto blocks_of = [&](int n) { return (paged_len(p.c, n) + Shape::BLOCK - 1) / Shape::BLOCK; };
+    auto cost_of = [](int blocks) { return blocks == 0 ? 0 : blocks + kPagedUnitCost; };
     int mine = 0;
     for(int n = tid * chunk; n < min((tid + 1) * chunk, p.c.n_batch); ++n)
     {
-        mine += blocks_of(n);
+        mine += cost_of(blocks_of(n));
     }
     int upto = mine;
 #pragma unroll
@@ -303,45 +470,47 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     __syncthreads();
     int total = 0;
 #pragma unroll
-    for(int w = 0; w < kPagedWaves; ++w)
+    for(int w = 0; w < WAVES; ++w)
     {
         upto += w < wave ? wave_sum[w] : 0;
         total += wave_sum[w];
     }
-    total = uniform(total);
     scan_of[tid] = upto - mine;
-    if(blockIdx.x == 0)
+    // sequences without rows: shared out, too, for the rows of their queries
+    for(int n = blockIdx.x; n < p.c.n_batch; n += gridDim.x)
     {
-        // for the launch that joins the shares
-        int at = upto - mine;
-        for(int n = tid * chunk; n < min((tid + 1) * chunk, p.c.n_batch); ++n)
+        if(uniform(paged_len(p.c, n)) == 0 && p.overwrite)
         {
-            p.before[n] = at;
-            at += blocks_of(n);
-        }
-        if(tid == 0)
-        {
-            p.before[p.c.n_batch] = total;
+            const int rows = p.c.n_head_kv * p.rows;
+            for(int t = tid; t < rows * (HEAD / 4); t += THREADS)
+            {
+                const int r = t / (HEAD / 4);
+                const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                paged_finish_row<T>(p, HEAD, paged_query_row(p, n, r / p.rows, r % p.rows),
+                        4 * (t % (HEAD / 4)), neg_inf(), 0.0f, zero);
+            }
         }
     }
-    const int64_t all = (int64_t)total * p.units;
-    int64_t at = all * blockIdx.x / p.shares;
-    const int64_t end = all * (blockIdx.x + 1) / p.shares;
-    if(at >= end)
+    const uint32_t all = (uint32_t)uniform(total) * (uint32_t)p.units;
+    const uint32_t shares = min((uint32_t)p.shares, all);
+    if(blockIdx.x >= shares)
     {
         return;
     }
+    const PagedSplit split(all, shares);
+    uint32_t at = split.begin(blockIdx.x);
+    const uint32_t end = split.begin(blockIdx.x + 1);
     PagedSegment seg;
     {
         // the last thread whose sequences begin at or before the block, then sequence by sequence
-        const int block = (int)(at / p.units);
+        const int block = (int)(at / (uint32_t)p.units);
         if(tid == 0)
         {
             found = 0;
         }
         __syncthreads();
         const bool here = tid * chunk < p.c.n_batch && scan_of[tid] <= block
-            && (tid == kPagedThreads - 1 || (tid + 1) * chunk >= p.c.n_batch || scan_of[tid + 1] > block);
+            && (tid == THREADS - 1 || (tid + 1) * chunk >= p.c.n_batch || scan_of[tid + 1] > block);
         if(here)
         {
             found = tid;
@@ -354,17 +523,18 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         {
             seg.len = uniform(paged_len(p.c, seg.n));
             seg.blocks = (seg.len + Shape::BLOCK - 1) / Shape::BLOCK;
-            if(before + seg.blocks > block || seg.n + 1 >= p.c.n_batch)
+            if(before + cost_of(seg.blocks) > block || seg.n + 1 >= p.c.n_batch)
             {
                 break;
             }
-            before += seg.blocks;
+            before += cost_of(seg.blocks);
             ++seg.n;
         }
-        const int rest = (int)(at - (int64_t)before * p.units);
-        seg.u = uniform(rest / seg.blocks);
-        seg.step = uniform(rest % seg.blocks);
+        const uint32_t rest = at - (uint32_t)before * (uint32_t)p.units;
+        seg.u = uniform((int)(rest / (uint32_t)cost_of(seg.blocks)));
+        seg.step = uniform((int)(rest % (uint32_t)cost_of(seg.blocks)));
     }
+    uint32_t unit_begin = at - (uint32_t)seg.step;      // of the unit's first block among all
 
     char *const slots = ring + wave * 2 * STAGE;
     // lane's place in every load instruction: row of the 16-row group, chunk
@@ -414,38 +584,77 @@ void sdpa_paged_kernel(const PagedAttendParams p)
 
     for(;;)
     {
-        seg.steps = (int)min((int64_t)(seg.blocks - seg.step), end - at);
+        // (the last place of a unit has no block: seg.steps may be 0)
+        seg.steps = (int)min((uint32_t)max(seg.blocks - seg.step, 0), end - at);
+        const uint32_t taken = min((uint32_t)(cost_of(seg.blocks) - seg.step), end - at);
+        if(seg.steps > 0)
+        {
         const int h = seg.u / p.row_groups, rg = seg.u - h * p.row_groups;
         const int given = uniform(paged_new(p.c, seg.n, p.q_seq));
         const int key_lo = seg.step * Shape::BLOCK;
         const int key_hi = min(key_lo + seg.steps * Shape::BLOCK, seg.len);
-        const int my_first = key_lo + wave * KEYS;
+        const int my_first = key_lo + stream * KEYS;
         const int n_mine = my_first < key_hi ? (key_hi - my_first + Shape::BLOCK - 1) / Shape::BLOCK : 0;
 
         // ---- the lane's query rows ---------------------------------------------------
-        u32x4 qf[NR][QREGS];
+        // 16-byte pieces of an operand begin at head values: 16-bit 32i + 8*quad; 8-bit pages, whose
+        // 16-byte reads hold 16 values, 64(i/2) + 16*quad + 8(i%2); fp32 16i + 4*quad
+        constexpr int E = KIND == kPaged32 ? 4 : 2;
+        auto q_piece = [&](int i)
+        {
+            return (KIND == kPaged16 ? 32 * i + 8 * quad : KIND == kPaged8 ? 64 * (i / 2) + 16 * quad + 8 * (i % 2)
+                    : 16 * i + 4 * quad) * E / 16;
+        };
+        u32x4 qf[Q_IN_LDS ? 1 : QREGS];
         int last[NR];           // the last key the row sees
+        int token[NR];
         bool row_ok[NR];
 #pragma unroll
         for(int nr = 0; nr < NR; ++nr)
         {
-            const int rr = (rg * NR + nr) * 16 + col;
-            const int tok = rr % p.q_seq;
-            row_ok[nr] = rr < p.rows && tok < given;
-            last[nr] = p.causal ? seg.len - given + tok : seg.len - 1;
-            constexpr int E = KIND == kPaged32 ? 4 : 2;
+            const int rr = rg * QROWS + (half * NR + nr) * 16 + col;
+            token[nr] = rr % p.q_seq;
+            row_ok[nr] = rr < p.rows && token[nr] < given;
+            last[nr] = p.causal ? seg.len - given + token[nr] : seg.len - 1;
+        }
+        if constexpr(Q_IN_LDS)
+        {
+            constexpr int PIECES = Shape::QB / 16;
+            for(int t = tid; t < QROWS * PIECES; t += THREADS)
+            {
+                const int r = t / PIECES, piece = t % PIECES, rr = rg * QROWS + r;
+                u32x4 x = {0, 0, 0, 0};
+                if(rr < p.rows && rr % p.q_seq < given)
+                {
+                    x = *reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.Q)
+                            + paged_query_row(p, seg.n, h, rr) * Shape::QB + piece * 16);
+                }
+                *reinterpret_cast<u32x4 *>(q_rows + r * Shape::QB + (piece ^ Shape::q_swizzle(r)) * 16) = x;
+            }
+            __syncthreads();
+        }
+        else
+        {
             const char *src = static_cast<const char *>(p.Q)
-                + paged_query_row(p, seg.n, h, rr < p.rows ? rr : 0) * HEAD * E;
+                + paged_query_row(p, seg.n, h, row_ok[0] ? rg * 16 + col : 0) * Shape::QB;
 #pragma unroll
             for(int i = 0; i < QREGS; ++i)
             {
-                // 16-bit: head values 32i + 8*quad ..; 8-bit pages, whose 16-byte reads hold 16 values:
-                // 64(i/2) + 16*quad + 8(i%2) ..; fp32: 16i + 4*quad ..
-                const int d = KIND == kPaged16 ? 32 * i + 8 * quad
-                    : KIND == kPaged8 ? 64 * (i / 2) + 16 * quad + 8 * (i % 2) : 16 * i + 4 * quad;
-                qf[nr][i] = row_ok[nr] ? *reinterpret_cast<const u32x4 *>(src + d * E) : u32x4{0, 0, 0, 0};
+                qf[i] = row_ok[0] ? *reinterpret_cast<const u32x4 *>(src + q_piece(i) * 16) : u32x4{0, 0, 0, 0};
             }
         }
+        auto q_operand = [&](int nr, int i) -> u32x4
+        {
+            if constexpr(Q_IN_LDS)
+            {
+                return *reinterpret_cast<const u32x4 *>(q_rows + ((half * NR + nr) * 16 + col) * Shape::QB
+                        + (q_piece(i) ^ Shape::q_swizzle(col)) * 16);
+            }
+            else
+            {
+                return qf[i];
+            }
+        };
         // below it every row sees every key
         const int all_see = p.causal ? seg.len - given : seg.len - 1;
 
@@ -489,14 +698,14 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             {
                 const int g = ld * Shape::ROWS_PER_LOAD / 16;
                 const int64_t from = real_page(page[g]) * p.c.page_stride + in_page(i, g) * RB;
-                load_to_lds16<0, true>(p.c.k_pages + from, k_off[ld], slot + ld * 1024);
+                load_to_lds16<0, HALVES == 1>(p.c.k_pages + from, k_off[ld], slot + ld * 1024);
             }
 #pragma unroll
             for(int ld = 0; ld < LOADS; ++ld)
             {
                 const int g = ld * Shape::ROWS_PER_LOAD / 16;
                 const int64_t from = real_page(page[g]) * p.c.page_stride + in_page(i, g) * RB;
-                load_to_lds16<0, true>(p.c.v_pages + from, v_off[ld], slot + K_BYTES + ld * 1024);
+                load_to_lds16<0, HALVES == 1>(p.c.v_pages + from, v_off[ld], slot + K_BYTES + ld * 1024);
             }
         };
         // the scale bytes of keys 16g + 4*quad .. + 3
@@ -516,6 +725,18 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             look_up(0, page);
             fetch(0, page, slots);
             look_up(min(1, n_mine - 1), page_next);
+        }
+        if(tid == 0 && (seg.step > 0 || seg.steps < seg.blocks))
+        {
+            // The unit's count of shares that are done starts with this call's tag, whatever the
+            // workspace holds: the first share that finds something else puts it there.
+            unsigned long long *const count = p.counts + ((int64_t)seg.n * p.units + seg.u);
+            unsigned long long seen = __hip_atomic_load(count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if((seen & ~(kPagedTagUnit - 1)) != p.tag)
+            {
+                __hip_atomic_compare_exchange_strong(count, &seen, p.tag, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                        __HIP_MEMORY_SCOPE_AGENT);
+            }
         }
         for(int i = 0; i < n_mine; ++i)
         {
@@ -566,309 +787,304 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                 paged_wait_lds();
             }
 
-            // ---- scores --------------------------------------------------------------
-            f32x4 s[NR][GROUPS];
-#pragma unroll
-            for(int g = 0; g < GROUPS; ++g)
+            // PARTLY: some of the keys are hidden from some row
+            auto attend = [&](auto partly)
             {
-#pragma unroll
-                for(int nr = 0; nr < NR; ++nr)
-                {
-                    s[nr][g] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                }
-#pragma unroll
-                for(int r = 0; r < KREADS; ++r)
-                {
-                    const u32x4 kf = *reinterpret_cast<const u32x4 *>(slot + k_at[r] + g * 16 * RB);
-                    if constexpr(KIND == kPaged16)
-                    {
-#pragma unroll
-                        for(int nr = 0; nr < NR; ++nr)
-                        {
-                            s[nr][g] = mfma32<T>(kf, qf[nr][r], s[nr][g]);
-                        }
-                    }
-                    else if constexpr(KIND == kPaged8)
-                    {
-#pragma unroll
-                        for(int half = 0; half < 2; ++half)
-                        {
-                            const u32x2 a = widen4<T>(kf[2 * half]), b = widen4<T>(kf[2 * half + 1]);
-                            const u32x4 wide = {a[0], a[1], b[0], b[1]};
-#pragma unroll
-                            for(int nr = 0; nr < NR; ++nr)
-                            {
-                                s[nr][g] = mfma32<T>(wide, qf[nr][2 * r + half], s[nr][g]);
-                            }
-                        }
-                    }
-                    else
-                    {
-#pragma unroll
-                        for(int e = 0; e < 4; ++e)
-                        {
-#pragma unroll
-                            for(int nr = 0; nr < NR; ++nr)
-                            {
-                                s[nr][g] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[e]),
-                                        __uint_as_float(qf[nr][r][e]), s[nr][g], 0, 0, 0);
-                            }
-                        }
-                    }
-                }
-            }
-
-            // ---- probabilities -------------------------------------------------------
-            const bool partly = key0 + KEYS - 1 > all_see || hidden != 0;
-            uint32_t pw[NR][GROUPS][2];                 // 16-bit pairs
-            f32x4 pf[NR][GROUPS];                       // fp32
-#pragma unroll
-            for(int nr = 0; nr < NR; ++nr)
-            {
-                float top = neg_inf(), top_t = neg_inf();
+                constexpr bool PARTLY = decltype(partly)::value;
+                // ---- scores --------------------------------------------------------------
+                f32x4 s[NR][GROUPS];
 #pragma unroll
                 for(int g = 0; g < GROUPS; ++g)
                 {
+                    u32x4 kf[KREADS];
 #pragma unroll
-                    for(int e = 0; e < 4; ++e)
+                    for(int r = 0; r < KREADS; ++r)
                     {
-                        float x = s[nr][g][e] * c_log2;
-                        if constexpr(KIND == kPaged8)
-                        {
-                            x *= scale_of(ks[g], e);
-                        }
-                        if(partly)
-                        {
-                            const int key = key0 + 16 * g + 4 * quad + e;
-                            x = key > last[nr] || key >= seg.len || ((hidden >> g) & 1) ? neg_inf() : x;
-                        }
-                        s[nr][g][e] = x;
-                        top = fmaxf(top, x);
-                        if constexpr(KIND == kPaged8)
-                        {
-                            top_t = fmaxf(top_t, x + (float)((int)((vs[g] >> (8 * e)) & 255u) - 127));
-                        }
+                        kf[r] = *reinterpret_cast<const u32x4 *>(slot + k_at[r] + g * 16 * RB);
                     }
-                }
-                const float m_new = fmaxf(m_run[nr], quad_max(top));
-                const float m_safe = m_new == neg_inf() ? 0.0f : m_new;
-                const float fade = fast_exp2(m_run[nr] - m_safe);
-                float t_safe = m_safe, fade_o = fade;
-                if constexpr(KIND == kPaged8)
-                {
-                    const float t_new = fmaxf(t_run[nr], quad_max(top_t));
-                    t_safe = t_new == neg_inf() ? 0.0f : t_new;
-                    fade_o = fast_exp2(t_run[nr] - t_safe);
-                    t_run[nr] = t_new;
-                }
-                float sum = 0.0f;
-#pragma unroll
-                for(int g = 0; g < GROUPS; ++g)
-                {
-                    f32x4 x;
-#pragma unroll
-                    for(int e = 0; e < 4; ++e)
-                    {
-                        x[e] = fast_exp2(s[nr][g][e] - m_safe);
-                        sum += x[e];
-                    }
+                    u32x4 wide[KIND == kPaged8 ? 2 * KREADS : 1];
                     if constexpr(KIND == kPaged8)
                     {
 #pragma unroll
-                        for(int e = 0; e < 4; ++e)
+                        for(int r = 0; r < 2 * KREADS; ++r)
                         {
-                            x[e] = fast_exp2(s[nr][g][e] + (float)((int)((vs[g] >> (8 * e)) & 255u) - 127) - t_safe);
+                            const u32x2 a = widen4<T>(kf[r / 2][2 * (r % 2)]), b = widen4<T>(kf[r / 2][2 * (r % 2) + 1]);
+                            wide[r] = u32x4{a[0], a[1], b[0], b[1]};
                         }
                     }
-                    if constexpr(KIND == kPaged32)
+#pragma unroll
+                    for(int nr = 0; nr < NR; ++nr)
                     {
-                        pf[nr][g] = x;
+                        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for(int i = 0; i < QREGS; ++i)
+                        {
+                            const u32x4 q = q_operand(nr, i);
+                            if constexpr(KIND == kPaged32)
+                            {
+#pragma unroll
+                                for(int e = 0; e < 4; ++e)
+                                {
+                                    x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[i][e]),
+                                            __uint_as_float(q[e]), x, 0, 0, 0);
+                                }
+                            }
+                            else
+                            {
+                                x = mfma32<T>(KIND == kPaged8 ? wide[i % (2 * KREADS)] : kf[i % KREADS], q, x);
+                            }
+                        }
+                        s[nr][g] = x;
+                            }
+                }
+
+                // ---- probabilities -------------------------------------------------------
+                uint32_t pw[NR][GROUPS][2];                 // 16-bit pairs
+                f32x4 pf[NR][GROUPS];                       // fp32
+#pragma unroll
+                for(int nr = 0; nr < NR; ++nr)
+                {
+                    float top = neg_inf(), top_t = neg_inf();
+#pragma unroll
+                    for(int g = 0; g < GROUPS; ++g)
+                    {
+#pragma unroll
+                        for(int e = 0; e < 4; ++e)
+                        {
+                            float x = s[nr][g][e] * c_log2;
+                            if constexpr(KIND == kPaged8)
+                            {
+                                x *= scale_of(ks[g], e);
+                            }
+                            if constexpr(PARTLY)
+                            {
+                                const int key = key0 + 16 * g + 4 * quad + e;
+                                x = key > last[nr] || key >= seg.len || ((hidden >> g) & 1) ? neg_inf() : x;
+                            }
+                            s[nr][g][e] = x;
+                            top = fmaxf(top, x);
+                            if constexpr(KIND == kPaged8)
+                            {
+                                top_t = fmaxf(top_t, x + (float)((int)((vs[g] >> (8 * e)) & 255u) - 127));
+                            }
+                        }
                     }
-                    else if constexpr(PV_BF16)
+                    const float m_new = fmaxf(m_run[nr], quad_max(top));
+                    const float m_safe = m_new == neg_inf() ? 0.0f : m_new;
+                    const float fade = fast_exp2(m_run[nr] - m_safe);
+                    float t_safe = m_safe, fade_o = fade;
+                    if constexpr(KIND == kPaged8)
                     {
-                        pw[nr][g][0] = Bf16::pack2(x[0], x[1]);
-                        pw[nr][g][1] = Bf16::pack2(x[2], x[3]);
+                        const float t_new = fmaxf(t_run[nr], quad_max(top_t));
+                        t_safe = t_new == neg_inf() ? 0.0f : t_new;
+                        fade_o = fast_exp2(t_run[nr] - t_safe);
+                        t_run[nr] = t_new;
+                    }
+                    float sum = 0.0f;
+#pragma unroll
+                    for(int g = 0; g < GROUPS; ++g)
+                    {
+                        f32x4 x;
+#pragma unroll
+                        for(int e = 0; e < 4; ++e)
+                        {
+                            x[e] = fast_exp2(s[nr][g][e] - m_safe);
+                            sum += x[e];
+                        }
+                        if constexpr(KIND == kPaged8)
+                        {
+#pragma unroll
+                            for(int e = 0; e < 4; ++e)
+                            {
+                                x[e] = fast_exp2(s[nr][g][e] + (float)((int)((vs[g] >> (8 * e)) & 255u) - 127) - t_safe);
+                            }
+                        }
+                        if constexpr(KIND == kPaged32)
+                        {
+                            pf[nr][g] = x;
+                        }
+                        else
+                        {
+                            pw[nr][g][0] = PV::pack2(x[0], x[1]);
+                            pw[nr][g][1] = PV::pack2(x[2], x[3]);
+                        }
+                    }
+                    l_run[nr] = l_run[nr] * fade + sum;
+                    m_run[nr] = m_new;
+                    if(__any(fade_o != 1.0f))
+                    {
+#pragma unroll
+                        for(int db = 0; db < DBLOCKS; ++db)
+                        {
+                            o[nr][db] *= fade_o;
+                        }
+                    }
+                    }
+
+                // ---- output ----------------------------------------------------------------
+                auto value_words = [&](int db, int t, u32x4 &w)
+                {
+                    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+                    typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+                    // keys 32t + {4*quad + 0..3, 16 + 4*quad + 0..3}
+                    if constexpr(KIND == kPaged16)
+                    {
+                        const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                    (lds_s16x4 *)(slot + v_at[db] + 32 * t * RB)));
+                        const u32x2 b = GROUPS == 1 ? u32x2{0, 0}
+                            : __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                        (lds_s16x4 *)(slot + v_at[db] + (32 * t + 16) * RB)));
+                        w = u32x4{a[0], a[1], b[0], b[1]};
+                    }
+                    else if constexpr(KIND == kPaged8)
+                    {
+                        const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                    (lds_i32x2 *)(slot + v_at[db] + 32 * t * RB)));
+                        const u32x2 a = widen4<Fp16>(v[0]), b = widen4<Fp16>(v[1]);
+                        w = u32x4{a[0], a[1], b[0], b[1]};
                     }
                     else
                     {
-                        pw[nr][g][0] = Fp16::pack2(x[0], x[1]);
-                        pw[nr][g][1] = Fp16::pack2(x[2], x[3]);
-                    }
-                }
-                l_run[nr] = l_run[nr] * fade + sum;
-                m_run[nr] = m_new;
-                if(__any(fade_o != 1.0f))
-                {
-#pragma unroll
-                    for(int db = 0; db < DBLOCKS; ++db)
-                    {
-                        o[nr][db] *= fade_o;
-                    }
-                }
-            }
-
-            // ---- output ----------------------------------------------------------------
-            // Product of the slot's values with the probabilities, without the values of keys
-            // behind `upto` where MASKED; row block nr, sum c.
-            auto value_words = [&](int db, int t, u32x4 &w)
-            {
-                typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-                typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-                // keys 32t + {4*quad + 0..3, 16 + 4*quad + 0..3}
-                if constexpr(KIND == kPaged16)
-                {
-                    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                (lds_s16x4 *)(slot + v_at[db] + 32 * t * RB)));
-                    const u32x2 b = GROUPS == 1 ? u32x2{0, 0}
-                        : __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                    (lds_s16x4 *)(slot + v_at[db] + (32 * t + 16) * RB)));
-                    w = u32x4{a[0], a[1], b[0], b[1]};
-                }
-                else if constexpr(KIND == kPaged8)
-                {
-                    const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                                (lds_i32x2 *)(slot + v_at[db] + 32 * t * RB)));
-                    const u32x2 a = widen4<Fp16>(v[0]), b = widen4<Fp16>(v[1]);
-                    w = u32x4{a[0], a[1], b[0], b[1]};
-                }
-                else
-                {
-#pragma unroll
-                    for(int e = 0; e < 4; ++e)
-                    {
-                        // key 16t + 4*quad + e
-                        w[e] = *reinterpret_cast<const uint32_t *>(slot + v_at[db] + (16 * t + e) * RB);
-                    }
-                }
-            };
-            // products of the value words of step t (32 keys, fp32: 16)
-            auto multiply = [&](const u32x4 &w, int t, int nr, f32x4 c) -> f32x4
-            {
-                if constexpr(KIND == kPaged32)
-                {
-#pragma unroll
-                    for(int e = 0; e < 4; ++e)
-                    {
-                        c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[e]), pf[nr][t][e], c, 0, 0, 0);
-                    }
-                    return c;
-                }
-                else if constexpr(GROUPS == 1)
-                {
-                    typedef typename std::conditional<PV_BF16, Bf16, Fp16>::type P;
-                    return mfma16<P>(u32x2{w[0], w[1]}, u32x2{pw[nr][0][0], pw[nr][0][1]}, c);
-                }
-                else
-                {
-                    typedef typename std::conditional<PV_BF16, Bf16, Fp16>::type P;
-                    return mfma32<P>(w, u32x4{pw[nr][2 * t][0], pw[nr][2 * t][1], pw[nr][2 * t + 1][0],
-                            pw[nr][2 * t + 1][1]}, c);
-                }
-            };
-            constexpr int TSTEPS = KIND == kPaged32 ? GROUPS : (GROUPS + 1) / 2;
-            bool odd = false;           // values that are no numbers among keys that not every row sees
-            if(partly && p.causal && p.q_seq > 1)
-            {
-                uint32_t any = 0;
-#pragma unroll
-                for(int db = 0; db < DBLOCKS; ++db)
-                {
-#pragma unroll
-                    for(int t = 0; t < TSTEPS; ++t)
-                    {
-                        u32x4 w;
-                        value_words(db, t, w);
 #pragma unroll
                         for(int e = 0; e < 4; ++e)
                         {
-                            any |= KIND == kPaged32 ? (w[e] & 0x7f800000u) == 0x7f800000u
-                                : PV_BF16 ? not_finite2<Bf16>(w[e]) : not_finite2<Fp16>(w[e]);
+                            // key 16t + 4*quad + e
+                            w[e] = *reinterpret_cast<const uint32_t *>(slot + v_at[db] + (16 * t + e) * RB);
                         }
                     }
-                }
-                odd = __any(any != 0);
-            }
-            if(!odd)
-            {
-#pragma unroll
-                for(int db = 0; db < DBLOCKS; ++db)
+                };
+                // products of the value words of step t (32 keys, fp32: 16)
+                auto multiply = [&](const u32x4 &w, int t, int nr, f32x4 c) -> f32x4
                 {
-#pragma unroll
-                    for(int t = 0; t < TSTEPS; ++t)
+                    if constexpr(KIND == kPaged32)
                     {
-                        u32x4 w;
-                        value_words(db, t, w);
 #pragma unroll
-                        for(int nr = 0; nr < NR; ++nr)
+                        for(int e = 0; e < 4; ++e)
                         {
-                            o[nr][db] = multiply(w, t, nr, o[nr][db]);
+                            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[e]), pf[nr][t][e], c, 0, 0, 0);
                         }
+                        return c;
                     }
-                }
-            }
-            else
-            {
-                // A probability of 0 does not hide such a value (0 * NaN): token by token, with the
-                // values behind what the token sees taken out, the rows of the token taken over.
-                for(int tok = 0; tok < given; ++tok)
+                    else if constexpr(GROUPS == 1)
+                    {
+                        return mfma16<PV>(u32x2{w[0], w[1]}, u32x2{pw[nr][0][0], pw[nr][0][1]}, c);
+                    }
+                    else
+                    {
+                        return mfma32<PV>(w, u32x4{pw[nr][2 * t][0], pw[nr][2 * t][1], pw[nr][2 * t + 1][0],
+                                pw[nr][2 * t + 1][1]}, c);
+                    }
+                };
+                constexpr int TSTEPS = KIND == kPaged32 ? GROUPS : (GROUPS + 1) / 2;
+                if constexpr(!PARTLY)
                 {
-                    const int upto = all_see + (p.causal ? tok : 0);
 #pragma unroll
                     for(int db = 0; db < DBLOCKS; ++db)
                     {
-                        f32x4 fresh[NR];
-#pragma unroll
-                        for(int nr = 0; nr < NR; ++nr)
-                        {
-                            fresh[nr] = o[nr][db];
-                        }
 #pragma unroll
                         for(int t = 0; t < TSTEPS; ++t)
                         {
                             u32x4 w;
                             value_words(db, t, w);
 #pragma unroll
-                            for(int e = 0; e < 4; ++e)
-                            {
-                                if constexpr(KIND == kPaged32)
-                                {
-                                    w[e] = key0 + 16 * t + 4 * quad + e > upto ? 0u : w[e];
-                                }
-                                else
-                                {
-                                    const int key = key0 + 32 * t + 16 * (e >> 1) + 4 * quad + 2 * (e & 1);
-                                    w[e] &= (key > upto ? 0u : 0xffffu) | (key + 1 > upto ? 0u : 0xffff0000u);
-                                }
-                            }
-#pragma unroll
                             for(int nr = 0; nr < NR; ++nr)
                             {
-                                fresh[nr] = multiply(w, t, nr, fresh[nr]);
-                            }
-                        }
-#pragma unroll
-                        for(int nr = 0; nr < NR; ++nr)
-                        {
-                            const bool mine_too = ((rg * NR + nr) * 16 + col) % p.q_seq == tok;
-#pragma unroll
-                            for(int e = 0; e < 4; ++e)
-                            {
-                                o[nr][db][e] = mine_too ? fresh[nr][e] : o[nr][db][e];
+                                o[nr][db] = multiply(w, t, nr, o[nr][db]);
                             }
                         }
                     }
                 }
+                else
+                {
+                    // Where a value is no number, a probability of 0 does not hide it (0 * NaN): then
+                    // token by token, with the values behind what the token sees taken out and only
+                    // the rows of the token taken over.
+                    bool odd = false;
+                    if(p.causal && p.q_seq > 1)
+                    {
+                        uint32_t any = 0;
+#pragma unroll
+                        for(int db = 0; db < DBLOCKS; ++db)
+                        {
+#pragma unroll
+                            for(int t = 0; t < TSTEPS; ++t)
+                            {
+                                u32x4 w;
+                                value_words(db, t, w);
+#pragma unroll
+                                for(int e = 0; e < 4; ++e)
+                                {
+                                    any |= KIND == kPaged32 ? (w[e] & 0x7f800000u) == 0x7f800000u
+                                        : not_finite2<PV>(w[e]);
+                                }
+                            }
+                        }
+                        odd = __any(any != 0);
+                    }
+                    const int rounds = odd ? given : 1;
+                    for(int tok = 0; tok < rounds; ++tok)
+                    {
+                        // (nothing is read ahead of the loop: the registers are the other step's)
+                        asm volatile("" ::: "memory");
+                        const int sees = odd ? all_see + tok : 0x7ffffffe;
+#pragma unroll
+                        for(int db = 0; db < DBLOCKS; ++db)
+                        {
+#pragma unroll
+                            for(int nr = 0; nr < NR; ++nr)
+                            {
+                                f32x4 fresh = o[nr][db];
+#pragma unroll
+                                for(int t = 0; t < TSTEPS; ++t)
+                                {
+                                    u32x4 w;
+                                    value_words(db, t, w);
+#pragma unroll
+                                    for(int e = 0; e < 4; ++e)
+                                    {
+                                        if constexpr(KIND == kPaged32)
+                                        {
+                                            w[e] = key0 + 16 * t + 4 * quad + e > sees ? 0u : w[e];
+                                        }
+                                        else
+                                        {
+                                            const int key = key0 + 32 * t + 16 * (e >> 1) + 4 * quad + 2 * (e & 1);
+                                            w[e] &= (key > sees ? 0u : 0xffffu) | (key + 1 > sees ? 0u : 0xffff0000u);
+                                        }
+                                    }
+                                    fresh = multiply(w, t, nr, fresh);
+                                }
+                                const bool take = !odd || token[nr] == tok;
+#pragma unroll
+                                for(int e = 0; e < 4; ++e)
+                                {
+                                    o[nr][db][e] = take ? fresh[e] : o[nr][db][e];
+                                }
+                            }
+                        }
+                    }
+                }
+            };
+            if(key0 + KEYS - 1 > all_see || hidden != 0)
+            {
+                attend(std::true_type());
+            }
+            else
+            {
+                attend(std::false_type());
             }
         }
 
-        // ---- the four wavefronts' results, then the unit's or the share's ----------------
-        const bool begins = seg.step == 0, ends = seg.step + seg.steps == seg.blocks;
+        // ---- the wavefronts' results, then the unit's or the share's ---------------------
+        const bool begins = seg.step == 0, whole = begins && seg.steps == seg.blocks;
+        const int rows_here = min(p.rows - rg * QROWS, QROWS);
         float *const merge_o = reinterpret_cast<float *>(ring);
-        float *const merge_ml = merge_o + kPagedWaves * 16 * MERGE_LD;
+        float *const merge_ml = merge_o + STREAMS * 16 * HALVES * MERGE_LD;
 #pragma unroll
         for(int nr = 0; nr < NR; ++nr)
         {
             __syncthreads();        // every wavefront is done with the ring, or with the last row block
+            const int mine = wave * 16 + col;
             float m = m_run[nr], l = quad_sum(l_run[nr]), to_m = 1.0f;
             if constexpr(KIND == kPaged8)
             {
@@ -887,65 +1103,93 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                 {
                     x *= to_m;
                 }
-                *reinterpret_cast<f32x4 *>(merge_o + (wave * 16 + col) * MERGE_LD + 16 * db + 4 * quad)
+                *reinterpret_cast<f32x4 *>(merge_o + mine * MERGE_LD + 16 * db + 4 * quad)
                     = row_ok[nr] ? x : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
             if(quad == 0)
             {
-                merge_ml[2 * (wave * 16 + col)] = m;
-                merge_ml[2 * (wave * 16 + col) + 1] = l;
+                merge_ml[2 * mine] = m;
+                merge_ml[2 * mine + 1] = l;
             }
             __syncthreads();
-            constexpr int VALUES = HEAD / 16;       // a thread's, of 16 threads a row
-            const int row = tid / 16, d0 = (tid % 16) * VALUES;
-            float top = neg_inf(), sum = 0.0f, v[VALUES];
-#pragma unroll
-            for(int w = 0; w < kPagedWaves; ++w)
+            // 16 threads a row; the row of stream w lies at (w + STREAMS * half) * 16 + row
+            constexpr int VALUES = HEAD / 16;
+            const int row = (tid / 16) % 16, its_half = tid / 256, d0 = (tid % 16) * VALUES;
+            const int in_group = (its_half * NR + nr) * 16 + row, rr = rg * QROWS + in_group;
+            if(rr < p.rows)
             {
-                top = fmaxf(top, merge_ml[2 * (w * 16 + row)]);
-            }
-            const float safe = top == neg_inf() ? 0.0f : top;
+                const int from = its_half * STREAMS * 16 + row;
+                float top = neg_inf(), sum = 0.0f, v[VALUES];
 #pragma unroll
-            for(int j = 0; j < VALUES; ++j)
-            {
-                v[j] = 0.0f;
-            }
-#pragma unroll
-            for(int w = 0; w < kPagedWaves; ++w)
-            {
-                const float f = fast_exp2(merge_ml[2 * (w * 16 + row)] - safe);
-                sum += f * merge_ml[2 * (w * 16 + row) + 1];
+                for(int w = 0; w < STREAMS; ++w)
+                {
+                    top = fmaxf(top, merge_ml[2 * (from + w * 16)]);
+                }
+                const float safe = top == neg_inf() ? 0.0f : top;
 #pragma unroll
                 for(int j = 0; j < VALUES; ++j)
                 {
-                    v[j] += f * merge_o[(w * 16 + row) * MERGE_LD + d0 + j];
+                    v[j] = 0.0f;
                 }
-            }
-            const int rr = (rg * NR + nr) * 16 + row;
-            if(begins && ends)
-            {
-                if(rr < p.rows)
+#pragma unroll
+                for(int w = 0; w < STREAMS; ++w)
+                {
+                    const float f = fast_exp2(merge_ml[2 * (from + w * 16)] - safe);
+                    sum += f * merge_ml[2 * (from + w * 16) + 1];
+#pragma unroll
+                    for(int j = 0; j < VALUES; ++j)
+                    {
+                        v[j] += f * merge_o[(from + w * 16) * MERGE_LD + d0 + j];
+                    }
+                }
+                if(whole)
                 {
                     paged_finish_row<T>(p, HEAD, paged_query_row(p, seg.n, h, rr), d0, top, sum, v);
                 }
-            }
-            else
-            {
-                const int64_t place = ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * (NR * 16) + nr * 16 + row;
+                else
+                {
+                    const int64_t place = ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * QROWS + in_group;
 #pragma unroll
-                for(int j = 0; j < VALUES; j += 4)
-                {
-                    *reinterpret_cast<f32x4 *>(p.part_o + place * HEAD + d0 + j)
-                        = f32x4{v[j], v[j + 1], v[j + 2], v[j + 3]};
-                }
-                if(d0 == 0)
-                {
-                    p.part_ml[2 * place] = top;
-                    p.part_ml[2 * place + 1] = sum;
+                    for(int j = 0; j < VALUES; j += 2)
+                    {
+                        put2(p.part_o + place * HEAD + d0 + j, v[j], v[j + 1]);
+                    }
+                    if(d0 == 0)
+                    {
+                        put2(p.part_ml + 2 * place, top, sum);
+                    }
                 }
             }
         }
-        at += seg.steps;
+        if(!whole)
+        {
+            // The share's results are with the device once its stores are acknowledged, every
+            // wavefront's in front of the barrier.  The workgroup that counts last joins.
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            const uint32_t w0 = split.of(unit_begin);
+            const uint32_t parts = split.of(unit_begin + (uint32_t)seg.blocks - 1) - w0 + 1;
+            unsigned long long *const count = p.counts + ((int64_t)seg.n * p.units + seg.u);
+            if(tid == 0)
+            {
+                const unsigned long long old = __hip_atomic_fetch_add(count, 1ull, __ATOMIC_RELAXED,
+                        __HIP_MEMORY_SCOPE_AGENT);
+                found = (uint32_t)(old & (kPagedTagUnit - 1)) == parts - 1;
+            }
+            __syncthreads();
+            if(uniform(found) != 0)
+            {
+                if(tid == 0)
+                {
+                    // (a replay of a captured call has this tag again)
+                    __hip_atomic_store(count, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                paged_join<T, HEAD, THREADS, QROWS>(p, seg.n, h, rg, rows_here, (int)w0, (int)parts,
+                        reinterpret_cast<float *>(ring));
+            }
+        }
+        }
+        at += taken;
         if(at >= end)
         {
             return;
@@ -953,6 +1197,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         // the next unit, of this sequence or of the next that has rows
         __syncthreads();
         seg.step = 0;
+        unit_begin = at;
         if(++seg.u == p.units)
         {
             seg.u = 0;
@@ -966,66 +1211,10 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     }
 }
 
-// Joins the shares of the units that more than one workgroup worked on, and writes the
-// rows of sequences without keys.  HEAD/4 threads a row.
-template<typename T, int HEAD>
-__global__ __launch_bounds__(256)
-void sdpa_paged_join_kernel(const PagedAttendParams p, int rows_of_share)
+// Blocks of 16 rows that a workgroup takes: 1, 2, or 4 by two wavefronts a key
+static int row_blocks(bool fp32, int64_t rows)
 {
-    constexpr int TPR = HEAD / 4;
-    const int64_t t = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-    const int d0 = (threadIdx.x % TPR) * 4;
-    // t = (n * n_head_kv + h) * rows + rr
-    const int64_t all_rows = (int64_t)p.c.n_batch * p.c.n_head_kv * p.rows;
-    if(t >= all_rows)
-    {
-        return;
-    }
-    const int rr = (int)(t % p.rows);
-    const int64_t unit = t / p.rows;
-    const int n = (int)(unit / p.c.n_head_kv), h = (int)(unit % p.c.n_head_kv);
-    const int64_t row = paged_query_row(p, n, h, rr);
-    const int before = p.before[n], blocks = p.before[n + 1] - before;
-    float top = neg_inf(), sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if(blocks > 0)
-    {
-        const int64_t all = (int64_t)p.before[p.c.n_batch] * p.units;
-        const int rg = rr / rows_of_share, in_share = rr - rg * rows_of_share;
-        const int64_t first_block = (int64_t)before * p.units + (int64_t)(h * p.row_groups + rg) * blocks;
-        // share w takes blocks [w * all / shares, (w + 1) * all / shares)
-        const int w0 = (int)(((first_block + 1) * p.shares - 1) / all);
-        const int w1 = (int)(((first_block + blocks) * p.shares - 1) / all);
-        if(w0 == w1)
-        {
-            return;         // finished there
-        }
-        for(int w = w0; w <= w1; ++w)
-        {
-            if(all * w / p.shares == all * (w + 1) / p.shares)
-            {
-                continue;   // (more shares than blocks: this one has none)
-            }
-            const int64_t place = ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * rows_of_share + in_share;
-            const float m = p.part_ml[2 * place], l = p.part_ml[2 * place + 1];
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(p.part_o + place * HEAD + d0);
-            const float next = fmaxf(top, m);
-            const float safe = next == neg_inf() ? 0.0f : next;
-            const float old = fast_exp2(top - safe), f = fast_exp2(m - safe);
-            sum = sum * old + l * f;
-#pragma unroll
-            for(int j = 0; j < 4; ++j)
-            {
-                v[j] = v[j] * old + x[j] * f;
-            }
-            top = next;
-        }
-    }
-    paged_finish_row<T>(p, HEAD, row, d0, top, sum, v);
-}
-
-static int row_blocks(int64_t rows)
-{
-    return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    return rows <= 16 ? 1 : rows <= 32 || fp32 ? 2 : 4;
 }
 
 static size_t align16(size_t x)
@@ -1033,52 +1222,70 @@ static size_t align16(size_t x)
     return (x + 15) & ~(size_t)15;
 }
 
-size_t paged_attend_workspace_bytes(int64_t n_batch, int64_t rows, int64_t head)
+// The workspace: a count per unit, then the shares' results.  (The larger of the types' sizes,
+// which differ in the rows of a workgroup.)
+static size_t count_bytes(int64_t n_batch, int64_t n_head_kv, int64_t rows)
 {
-    const size_t places = (size_t)kPagedShares * 2 * 16 * row_blocks(rows);
-    return align16(4 * ((size_t)n_batch + 1)) + places * (size_t)(head + 2) * 4;
+    const int64_t of_16bit = 16 * row_blocks(false, rows), of_fp32 = 16 * row_blocks(true, rows);
+    const int64_t groups = (rows + (of_16bit < of_fp32 ? of_16bit : of_fp32) - 1)
+        / (of_16bit < of_fp32 ? of_16bit : of_fp32);
+    return align16(8 * (size_t)(n_batch * n_head_kv) * (size_t)groups);
 }
 
-template<typename T, int KIND, int HEAD, int NR>
+static size_t share_rows(int64_t rows)
+{
+    return (size_t)kPagedShares * 2 * 16 * (size_t)row_blocks(false, rows);
+}
+
+size_t paged_attend_workspace_bytes(int64_t n_batch, int64_t n_head_kv, int64_t rows, int64_t head)
+{
+    return count_bytes(n_batch, n_head_kv, rows) + share_rows(rows) * (size_t)(head + 2) * 4;
+}
+
+template<typename T, int KIND, int HEAD, int NR, int HALVES>
 static int launch_form(hipStream_t stream, PagedAttendParams &p)
 {
-    typedef PagedShape<KIND, HEAD> Shape;
-    p.row_groups = (p.rows + 16 * NR - 1) / (16 * NR);
+    typedef PagedShape<KIND, HEAD, NR, HALVES> Shape;
+    p.row_groups = (p.rows + Shape::QROWS - 1) / Shape::QROWS;
     p.units = p.c.n_head_kv * p.row_groups;
     // at most as many shares as there can be blocks
-    const int64_t most = (int64_t)p.c.n_batch * p.units * (p.c.max_rows / Shape::BLOCK + 1);
+    const int64_t most = (int64_t)p.c.n_batch * p.units * (p.c.max_rows / Shape::BLOCK + 1 + kPagedUnitCost);
+    if(most > 0xffffffffll)
+    {
+        return NNTILE_HIP_EINVAL;
+    }
     const int64_t places = kPagedCUs * Shape::WGS_PER_CU;
     p.shares = (int32_t)(most < places ? most : places);
-    hipLaunchKernelGGL((sdpa_paged_kernel<T, KIND, HEAD, NR>), dim3((unsigned)p.shares),
-            dim3(kPagedThreads), 0, stream, p);
-    const int64_t all_rows = (int64_t)p.c.n_batch * p.c.n_head_kv * p.rows;
-    const int per_wg = 256 / (HEAD / 4);
-    hipLaunchKernelGGL((sdpa_paged_join_kernel<T, HEAD>), dim3((unsigned)((all_rows + per_wg - 1) / per_wg)),
-            dim3(256), 0, stream, p, 16 * NR);
+    p.tag = next_decode_tag() * (kPagedTagUnit / 16);
+    hipLaunchKernelGGL((sdpa_paged_kernel<T, KIND, HEAD, NR, HALVES>), dim3((unsigned)p.shares),
+            dim3(Shape::THREADS), 0, stream, p);
     return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;
 }
 
 template<typename T, int KIND>
 static int launch_kind(hipStream_t stream, PagedAttendParams &p, int head)
 {
-    switch(row_blocks(p.rows) * 256 + head)
+    switch(row_blocks(KIND == kPaged32, p.rows) * 256 + head)
     {
-        case 256 + 64: return launch_form<T, KIND, 64, 1>(stream, p);
-        case 256 + 128: return launch_form<T, KIND, 128, 1>(stream, p);
-        case 512 + 64: return launch_form<T, KIND, 64, 2>(stream, p);
-        case 512 + 128: return launch_form<T, KIND, 128, 2>(stream, p);
-        case 1024 + 64: return launch_form<T, KIND, 64, 4>(stream, p);
-        case 1024 + 128: return launch_form<T, KIND, 128, 4>(stream, p);
-        default: return NNTILE_HIP_EUNSUPPORTED;
+        case 256 + 64: return launch_form<T, KIND, 64, 1, 1>(stream, p);
+        case 256 + 128: return launch_form<T, KIND, 128, 1, 1>(stream, p);
+        case 512 + 64: return launch_form<T, KIND, 64, 2, 1>(stream, p);
+        case 512 + 128: return launch_form<T, KIND, 128, 2, 1>(stream, p);
+        default: break;
     }
+    if constexpr(KIND != kPaged32)
+    {
+        return head == 64 ? launch_form<T, KIND, 64, 2, 2>(stream, p) : launch_form<T, KIND, 128, 2, 2>(stream, p);
+    }
+    return NNTILE_HIP_EUNSUPPORTED;
 }
 
 int launch_paged_attend(hipStream_t stream, int dtype, PagedAttendParams &p, int head, void *workspace)
 {
-    const size_t places = (size_t)kPagedShares * 2 * 16 * row_blocks(p.rows);
-    p.before = static_cast<int32_t *>(workspace);
-    p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + align16(4 * ((size_t)p.c.n_batch + 1)));
-    p.part_ml = p.part_o + places * (size_t)head;
+    const size_t counts = count_bytes(p.c.n_batch, p.c.n_head_kv, p.rows);
+    p.counts = static_cast<unsigned long long *>(workspace);
+    p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + counts);
+    p.part_ml = p.part_o + share_rows(p.rows) * (size_t)head;
     if(p.c.k_scales != nullptr)
     {
         return dtype == 0 ? launch_kind<Bf16, kPaged8>(stream, p, head)
