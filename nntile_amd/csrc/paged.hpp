@@ -44,6 +44,9 @@ struct PagedAttendParams
     int32_t shares;                     // workgroups that the key blocks are shared out to
     unsigned long long *counts;         // workspace: shares that are done, of every unit, above them `tag`
     unsigned long long tag;             // unique to the call
+    int32_t join_behind;                // the shares are joined by a launch of its own
+    int32_t *before;                    // workspace, for that: cost of the sequences in front of each, n_batch + 1,
+                                        // and what a unit costs beside its blocks
     float *part_o;                      // workspace: [share][2][rows of a workgroup][head]
     float *part_ml;                     // workspace: [share][2][rows of a workgroup][2]
 };

@@ -21,13 +21,12 @@
 //  * S^T = K Q^T and O^T += V^T P^T with matrix instructions of 16 x 16; P^T is the
 //    accumulator of S^T as it stands (the keys of an instruction are numbered so), V^T
 //    comes through the transposing LDS reads (fp32: single values).  A lane has one query row.
-//  * 8-bit pages: codes become bf16 / fp16 exactly in front of the matrix
-//    instructions; the power of two of a key row goes into the score.  That of a value row goes into the
-//    probability, which has a running maximum of its own (of score + exponent), so that what
-//    is rounded to fp16 is at most 1 and its largest is 1, however small the values are.
+//  * 8-bit pages: codes become values of the tile type exactly in front of the matrix
+//    instructions.  The power of two of a key row goes into its codes (bf16) or into the score (fp16),
+//    that of a value row into the probability.
 //
-// Probabilities are rounded to the tile type (8-bit pages: to fp16) for the matrix instruction, as in
-// the other attention kernels; the sum of the softmax takes them unrounded.
+// Probabilities are rounded to the tile type for the matrix instruction, as in the other attention
+// kernels; the sum of the softmax takes them unrounded.
 #include <type_traits>
 
 #include "paged.hpp"
@@ -45,6 +44,8 @@ constexpr int kPagedCUs = 256;
 constexpr int kPagedShares = 2 * kPagedCUs;
 // What a unit costs beside its key blocks, in blocks
 constexpr int kPagedUnitCost = 1;
+// fp16 probabilities are kept times 2^14: 2^-28 of the largest still has all of its bits
+constexpr float kPagedLift = 14.0f;
 // A count of shares and the tag above it
 constexpr unsigned long long kPagedTagUnit = 4096;
 static_assert(kPagedShares < (int)kPagedTagUnit, "counts stay below the tag");
@@ -63,15 +64,17 @@ struct PagedShape
     static constexpr int RB = KIND == kPaged32 ? HEAD * 4 : KIND == kPaged8 ? HEAD : HEAD * 2;   // bytes of a row
     static constexpr int CPR = RB / 16;                     // 16-byte chunks of a row
     static constexpr int RPL = RB >= 256 ? 1 : 256 / RB;    // rows per 256-byte line of LDS banks
-    static constexpr int KEYS = 4096 / RB > 16 ? 4096 / RB : 16;    // of a wavefront's step
+    // keys of a wavefront's step: 8 KB of K and V; twice that, up to 64, where two wavefronts share them
+    static constexpr int ALONE = 4096 / RB > 16 ? 4096 / RB : 16;
+    static constexpr int KEYS = HALVES * ALONE < 64 ? HALVES * ALONE : 64;
     static constexpr int BLOCK = STREAMS * KEYS;        // keys of a workgroup's step
     static constexpr int GROUPS = KEYS / 16;
     static constexpr int K_BYTES = KEYS * RB;
     static constexpr int STAGE = 2 * K_BYTES;
     static constexpr int LOADS = K_BYTES / 1024;            // load instructions of a step's K
     static constexpr int ROWS_PER_LOAD = 1024 / RB;
-    static constexpr int RING = WAVES * 2 * STAGE;
-    static constexpr int WGS_PER_CU = RING > 72 * 1024 ? 1 : 2;
+    static constexpr int RING = STREAMS * 2 * STAGE;
+    static constexpr int WGS_PER_CU = RING > 72 * 1024 || WAVES > 4 ? 1 : 2;
     static constexpr int MIN_WAVES = WAVES * WGS_PER_CU / 4;        // of a SIMD
     // the query rows: the operands of one block of 16 stay in registers, those of two in LDS
     static constexpr int QB = HEAD * (KIND == kPaged32 ? 4 : 2);
@@ -167,18 +170,18 @@ template<typename T> __device__ __forceinline__ f32x4 mfma16(u32x2 a, u32x2 b, f
     }
 }
 
-// Four e4m3 codes as four values of T
-template<typename T> __device__ __forceinline__ u32x2 widen4(uint32_t codes)
+// Four e4m3 codes times a power of two as four values of T
+template<typename T> __device__ __forceinline__ u32x2 widen4(uint32_t codes, float scale)
 {
     if constexpr(__is_same(T, Bf16))
     {
-        return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, false)),
-            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, true))};
+        return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false)),
+            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true))};
     }
     else
     {
-        return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, false)),
-            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, true))};
+        return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, false)),
+            __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, scale, true))};
     }
 }
 
@@ -304,12 +307,13 @@ __device__ __forceinline__ int64_t paged_query_row(const PagedAttendParams &p, i
     return (n + (int64_t)p.c.n_batch * (g + (int64_t)p.kv_group * h)) * p.q_seq + tok;
 }
 
-// Joins the shares w0 .. w0 + parts - 1 of a unit, in this order, and finishes its rows.  HEAD/4 threads a
+// Joins the shares w0 .. w0 + parts - 1 of a unit, in this order, and finishes rows first_row .. +
+// rows_here - 1 of it.  HEAD/4 threads a
 // row; where the rows leave threads over, they take turns at the shares and the sums
 // are added up through LDS.
 template<typename T, int HEAD, int THREADS, int QROWS>
-__device__ __forceinline__ void paged_join(const PagedAttendParams &p, int n, int h, int rg, int rows_here,
-        int w0, int parts, float *lds)
+__device__ __forceinline__ void paged_join(const PagedAttendParams &p, int n, int h, int rg, int first_row,
+        int rows_here, int w0, int parts, float *lds)
 {
     constexpr int TPR = HEAD / 4, ROWS = THREADS / TPR;
     constexpr int AT_ONCE = 8;
@@ -334,7 +338,7 @@ __device__ __forceinline__ void paged_join(const PagedAttendParams &p, int n, in
                 {
                     // (behind the last share: it again, with no weight)
                     const int i = min(i0 + j * turns, parts - 1);
-                    const int64_t place = ((int64_t)(w0 + i) * 2 + (i == 0 ? 1 : 0)) * QROWS + r;
+                    const int64_t place = ((int64_t)(w0 + i) * 2 + (i == 0 ? 1 : 0)) * QROWS + first_row + r;
                     get2(p.part_ml + 2 * place, m[j], l[j]);
                     get2(p.part_o + place * HEAD + d0, x[j][0], x[j][1]);
                     get2(p.part_o + place * HEAD + d0 + 2, x[j][2], x[j][3]);
@@ -407,7 +411,7 @@ __device__ __forceinline__ void paged_join(const PagedAttendParams &p, int n, in
         }
         if(turn == 0 && r < rows_here)
         {
-            paged_finish_row<T>(p, HEAD, paged_query_row(p, n, h, rg * QROWS + r), d0, top, sum, v);
+            paged_finish_row<T>(p, HEAD, paged_query_row(p, n, h, rg * QROWS + first_row + r), d0, top, sum, v);
         }
     }
 }
@@ -426,8 +430,14 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     constexpr int QROWS = Shape::QROWS;
     constexpr bool Q_IN_LDS = NR > 1;
     // the type of the probabilities and values as the matrix instruction takes them
-    constexpr bool PV_BF16 = KIND == kPaged16 && __is_same(T, Bf16);
-    typedef typename std::conditional<PV_BF16, Bf16, Fp16>::type PV;
+    typedef typename std::conditional<__is_same(T, float), Fp16, T>::type PV;
+    // 8-bit pages, bf16: the scale of a key row goes into its codes (exact in bf16), that of a value row
+    // into its probabilities.  fp16 has not the range for either: its key scales go into
+    // the scores, and its probabilities take 2^(scale - largest scale so far + kPagedLift).
+    constexpr bool KSCALE_IN_CODES = KIND == kPaged8 && __is_same(T, Bf16);
+    constexpr bool RANGED = __is_same(PV, Fp16) && KIND != kPaged32;
+    // the power of two that the probabilities, and so their sum, carry
+    constexpr float kLift = RANGED && KIND == kPaged16 ? kPagedLift : 0.0f;
 
     constexpr int MERGE_LD = HEAD + 4;
     constexpr int MERGE_BYTES = STREAMS * 16 * HALVES * (MERGE_LD + 2) * 4;
@@ -447,15 +457,22 @@ void sdpa_paged_kernel(const PagedAttendParams p)
 
     // ---- the workgroup's run of key blocks ----------------------------------------
     // Every thread adds up the blocks of a few neighbouring sequences, then a scan.  A unit counts
-    // as a block more than it has: its begin and end cost about as much.
+    // as a block more than it has: its begin and end cost about as much.  (64 sequences of 17 to 16384
+    // 8-bit rows 82 -> 73 us.)  Where all sequences have as many blocks it does not, so that
+    // shares and units more often end together.
     const int chunk = (p.c.n_batch + THREADS - 1) / THREADS;
     auto blocks_of = [&](int n) { return (paged_len(p.c, n) + Shape::BLOCK - 1) / Shape::BLOCK; };
-    auto cost_of = [](int blocks) { return blocks == 0 ? 0 : blocks + kPagedUnitCost; };
+    int unit_cost = kPagedUnitCost;
+    auto cost_of = [&](int blocks) { return blocks == 0 ? 0 : blocks + unit_cost; };
+    const int blocks_0 = blocks_of(0);
     int mine = 0;
+    bool same = true;
     for(int n = tid * chunk; n < min((tid + 1) * chunk, p.c.n_batch); ++n)
     {
         mine += cost_of(blocks_of(n));
+        same = same && blocks_of(n) == blocks_0;
     }
+    same = __all(same);
     int upto = mine;
 #pragma unroll
     for(int o = 1; o < 64; o <<= 1)
@@ -465,17 +482,39 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     }
     if(lane == 63)
     {
-        wave_sum[wave] = upto;
+        wave_sum[wave] = same ? upto : ~upto;
     }
     __syncthreads();
     int total = 0;
 #pragma unroll
     for(int w = 0; w < WAVES; ++w)
     {
-        upto += w < wave ? wave_sum[w] : 0;
-        total += wave_sum[w];
+        const int sum = wave_sum[w];
+        same = same && sum >= 0;
+        upto += w < wave ? (sum < 0 ? ~sum : sum) : 0;
+        total += sum < 0 ? ~sum : sum;
     }
-    scan_of[tid] = upto - mine;
+    if(same)
+    {
+        unit_cost = 0;
+        total = p.c.n_batch * blocks_0;
+    }
+    scan_of[tid] = same ? min(tid * chunk, p.c.n_batch) * blocks_0 : upto - mine;
+    if(p.join_behind && blockIdx.x == 0)
+    {
+        // for the launch that joins the shares
+        int sum = scan_of[tid];
+        for(int n = tid * chunk; n < min((tid + 1) * chunk, p.c.n_batch); ++n)
+        {
+            p.before[n] = sum;
+            sum += cost_of(blocks_of(n));
+        }
+        if(tid == 0)
+        {
+            p.before[p.c.n_batch] = total;
+            p.before[p.c.n_batch + 1] = unit_cost;
+        }
+    }
     // sequences without rows: shared out, too, for the rows of their queries
     for(int n = blockIdx.x; n < p.c.n_batch; n += gridDim.x)
     {
@@ -491,6 +530,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             }
         }
     }
+    unit_cost = uniform(unit_cost);
     const uint32_t all = (uint32_t)uniform(total) * (uint32_t)p.units;
     const uint32_t shares = min((uint32_t)p.shares, all);
     if(blockIdx.x >= shares)
@@ -536,15 +576,21 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     }
     uint32_t unit_begin = at - (uint32_t)seg.step;      // of the unit's first block among all
 
-    char *const slots = ring + wave * 2 * STAGE;
-    // lane's place in every load instruction: row of the 16-row group, chunk
-    uint32_t k_off[LOADS], v_off[LOADS];
+    char *const slots = ring + stream * 2 * STAGE;
+    // lane's place in every load instruction: row of the 16-row group, chunk.  Of two wavefronts that
+    // share their keys, one loads K and one V.
+    constexpr bool PAIRED = HALVES == 2;
+    uint32_t k_off[LOADS], v_off[PAIRED ? 1 : LOADS];
 #pragma unroll
     for(int i = 0; i < LOADS; ++i)
     {
         const int r = i * Shape::ROWS_PER_LOAD + lane / CPR;
-        k_off[i] = (uint32_t)((r & 15) * RB + ((lane % CPR) ^ Shape::k_swizzle(r)) * 16);
-        v_off[i] = (uint32_t)((r & 15) * RB + ((lane % CPR) ^ Shape::v_swizzle(r)) * 16);
+        const int k_swizzle = PAIRED && half == 1 ? Shape::v_swizzle(r) : Shape::k_swizzle(r);
+        k_off[i] = (uint32_t)((r & 15) * RB + ((lane % CPR) ^ k_swizzle) * 16);
+        if constexpr(!PAIRED)
+        {
+            v_off[i] = (uint32_t)((r & 15) * RB + ((lane % CPR) ^ Shape::v_swizzle(r)) * 16);
+        }
     }
     // lane's addresses of the operands in a slot; the 16-key groups lie 16 * RB apart
     // (the swizzles have a period of 16 rows)
@@ -659,11 +705,12 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         const int all_see = p.causal ? seg.len - given : seg.len - 1;
 
         f32x4 o[NR][DBLOCKS];
-        float m_run[NR], l_run[NR], t_run[NR];      // t_run: of score + exponent of the value row
+        float m_run[NR], l_run[NR];
+        float top_scale = 0.0f;         // the largest scale byte of the value rows so far
 #pragma unroll
         for(int nr = 0; nr < NR; ++nr)
         {
-            m_run[nr] = t_run[nr] = neg_inf();
+            m_run[nr] = neg_inf();
             l_run[nr] = 0.0f;
 #pragma unroll
             for(int db = 0; db < DBLOCKS; ++db)
@@ -693,29 +740,37 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         auto real_page = [&](int page) { return (unsigned)page < (unsigned)p.c.n_pages ? page : 0; };
         auto fetch = [&](int i, const int (&page)[GROUPS], char *slot)
         {
+            int64_t from[GROUPS];
 #pragma unroll
-            for(int ld = 0; ld < LOADS; ++ld)
+            for(int g = 0; g < GROUPS; ++g)
             {
-                const int g = ld * Shape::ROWS_PER_LOAD / 16;
-                const int64_t from = real_page(page[g]) * p.c.page_stride + in_page(i, g) * RB;
-                load_to_lds16<0, HALVES == 1>(p.c.k_pages + from, k_off[ld], slot + ld * 1024);
+                from[g] = real_page(page[g]) * p.c.page_stride + in_page(i, g) * RB;
             }
+            const char *const first = PAIRED && half == 1 ? p.c.v_pages : p.c.k_pages;
+            char *const to = PAIRED && half == 1 ? slot + K_BYTES : slot;
 #pragma unroll
             for(int ld = 0; ld < LOADS; ++ld)
             {
-                const int g = ld * Shape::ROWS_PER_LOAD / 16;
-                const int64_t from = real_page(page[g]) * p.c.page_stride + in_page(i, g) * RB;
-                load_to_lds16<0, HALVES == 1>(p.c.v_pages + from, v_off[ld], slot + K_BYTES + ld * 1024);
+                load_to_lds16<0, true>(first + from[ld * Shape::ROWS_PER_LOAD / 16], k_off[ld], to + ld * 1024);
+            }
+            if constexpr(!PAIRED)
+            {
+#pragma unroll
+                for(int ld = 0; ld < LOADS; ++ld)
+                {
+                    load_to_lds16<0, true>(p.c.v_pages + from[ld * Shape::ROWS_PER_LOAD / 16], v_off[ld],
+                            slot + K_BYTES + ld * 1024);
+                }
             }
         };
-        // the scale bytes of keys 16g + 4*quad .. + 3
-        auto scales = [&](const uint8_t *of, int i, const int (&page)[GROUPS], uint32_t (&out)[GROUPS])
+        // the scale bytes of keys 16g + 4 * which .. + 3
+        auto scales = [&](const uint8_t *of, int which, int i, const int (&page)[GROUPS], uint32_t (&out)[GROUPS])
         {
 #pragma unroll
             for(int g = 0; g < GROUPS; ++g)
             {
                 const u32x4 w = scalar_load<u32x4>(of, real_page(page[g]) * p.c.scale_stride + in_page(i, g));
-                out[g] = quad == 0 ? w[0] : quad == 1 ? w[1] : quad == 2 ? w[2] : w[3];
+                out[g] = which == 0 ? w[0] : which == 1 ? w[1] : which == 2 ? w[2] : w[3];
             }
         };
 
@@ -726,7 +781,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             fetch(0, page, slots);
             look_up(min(1, n_mine - 1), page_next);
         }
-        if(tid == 0 && (seg.step > 0 || seg.steps < seg.blocks))
+        if(tid == 0 && !p.join_behind && (seg.step > 0 || seg.steps < seg.blocks))
         {
             // The unit's count of shares that are done starts with this call's tag, whatever the
             // workspace holds: the first share that finds something else puts it there.
@@ -738,23 +793,44 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                         __HIP_MEMORY_SCOPE_AGENT);
             }
         }
-        for(int i = 0; i < n_mine; ++i)
+        const int n_steps = PAIRED ? seg.steps : n_mine;
+        auto without_page = [&]()       // groups of the step
         {
-            char *const slot = slots + (i & 1) * STAGE;
-            uint32_t ks[GROUPS], vs[GROUPS];
-            if constexpr(KIND == kPaged8)
-            {
-                scales(p.c.k_scales, i, page, ks);
-                scales(p.c.v_scales, i, page, vs);
-            }
-            uint32_t hidden = 0;        // groups without a page
+            uint32_t hidden = 0;
 #pragma unroll
             for(int g = 0; g < GROUPS; ++g)
             {
                 hidden |= (unsigned)page[g] < (unsigned)p.c.n_pages ? 0u : 1u << g;
             }
-            // the reads of the slot that is filled next have returned
-            paged_wait_lds();
+            return hidden;
+        };
+        // One step; PARTLY: some of its keys may be hidden from some row.
+        auto take_step = [&](int i, auto partly)
+        {
+            constexpr bool PARTLY = decltype(partly)::value;
+            char *const slot = slots + (i & 1) * STAGE;
+            uint32_t ks[GROUPS], vs[GROUPS];
+            uint32_t hidden = 0;
+            if(!PARTLY || !PAIRED || i < n_mine)
+            {
+                if constexpr(KIND == kPaged8)
+                {
+                    scales(p.c.k_scales, KSCALE_IN_CODES ? col >> 2 : quad, i, page, ks);
+                    scales(p.c.v_scales, quad, i, page, vs);
+                }
+                hidden = PARTLY ? without_page() : 0;
+            }
+            if constexpr(PAIRED)
+            {
+                // both have loaded their half of this step, and are done with the slot filled next
+                paged_wait_loads<0>();
+                __syncthreads();
+            }
+            else
+            {
+                // the reads of the slot that is filled next have returned
+                paged_wait_lds();
+            }
             if(i + 1 < n_mine)
             {
                 fetch(i + 1, page_next, slots + ((i + 1) & 1) * STAGE);
@@ -764,14 +840,21 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                     page[g] = page_next[g];
                 }
                 look_up(min(i + 2, n_mine - 1), page_next);
-                paged_wait_loads<2 * LOADS>();
+                if constexpr(!PAIRED)
+                {
+                    paged_wait_loads<2 * LOADS>();
+                }
             }
-            else
+            else if constexpr(!PAIRED)
             {
                 paged_wait_loads<0>();
             }
+            if(PARTLY && PAIRED && i >= n_mine)
+            {
+                return;
+            }
             const int key0 = my_first + i * Shape::BLOCK;
-            if(key0 + KEYS > seg.len || hidden != 0)
+            if(PARTLY && (key0 + KEYS > seg.len || hidden != 0))
             {
                 // values of rows that are none: zeros, so that what lies there does not
                 // get into the products (their probabilities are exactly 0)
@@ -787,197 +870,247 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                 paged_wait_lds();
             }
 
-            // PARTLY: some of the keys are hidden from some row
-            auto attend = [&](auto partly)
+            // ---- scores --------------------------------------------------------------
+            f32x4 s[NR][GROUPS];
+#pragma unroll
+            for(int g = 0; g < GROUPS; ++g)
             {
-                constexpr bool PARTLY = decltype(partly)::value;
-                // ---- scores --------------------------------------------------------------
-                f32x4 s[NR][GROUPS];
+                u32x4 kf[KREADS];
 #pragma unroll
-                for(int g = 0; g < GROUPS; ++g)
+                for(int r = 0; r < KREADS; ++r)
                 {
-                    u32x4 kf[KREADS];
-#pragma unroll
-                    for(int r = 0; r < KREADS; ++r)
-                    {
-                        kf[r] = *reinterpret_cast<const u32x4 *>(slot + k_at[r] + g * 16 * RB);
-                    }
-                    u32x4 wide[KIND == kPaged8 ? 2 * KREADS : 1];
-                    if constexpr(KIND == kPaged8)
-                    {
-#pragma unroll
-                        for(int r = 0; r < 2 * KREADS; ++r)
-                        {
-                            const u32x2 a = widen4<T>(kf[r / 2][2 * (r % 2)]), b = widen4<T>(kf[r / 2][2 * (r % 2) + 1]);
-                            wide[r] = u32x4{a[0], a[1], b[0], b[1]};
-                        }
-                    }
-#pragma unroll
-                    for(int nr = 0; nr < NR; ++nr)
-                    {
-                        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for(int i = 0; i < QREGS; ++i)
-                        {
-                            const u32x4 q = q_operand(nr, i);
-                            if constexpr(KIND == kPaged32)
-                            {
-#pragma unroll
-                                for(int e = 0; e < 4; ++e)
-                                {
-                                    x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[i][e]),
-                                            __uint_as_float(q[e]), x, 0, 0, 0);
-                                }
-                            }
-                            else
-                            {
-                                x = mfma32<T>(KIND == kPaged8 ? wide[i % (2 * KREADS)] : kf[i % KREADS], q, x);
-                            }
-                        }
-                        s[nr][g] = x;
-                            }
+                    kf[r] = *reinterpret_cast<const u32x4 *>(slot + k_at[r] + g * 16 * RB);
                 }
-
-                // ---- probabilities -------------------------------------------------------
-                uint32_t pw[NR][GROUPS][2];                 // 16-bit pairs
-                f32x4 pf[NR][GROUPS];                       // fp32
+                u32x4 wide[KIND == kPaged8 ? 2 * KREADS : 1];
+                // (of the lane's key row)
+                const float k_scale = KSCALE_IN_CODES ? scale_of(ks[g], col & 3) : 1.0f;
+                if constexpr(KIND == kPaged8)
+                {
+#pragma unroll
+                    for(int r = 0; r < 2 * KREADS; ++r)
+                    {
+                        const u32x2 a = widen4<T>(kf[r / 2][2 * (r % 2)], k_scale),
+                        b = widen4<T>(kf[r / 2][2 * (r % 2) + 1], k_scale);
+                        wide[r] = u32x4{a[0], a[1], b[0], b[1]};
+                    }
+                }
 #pragma unroll
                 for(int nr = 0; nr < NR; ++nr)
                 {
-                    float top = neg_inf(), top_t = neg_inf();
+                    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for(int g = 0; g < GROUPS; ++g)
+                    for(int i = 0; i < QREGS; ++i)
                     {
-#pragma unroll
-                        for(int e = 0; e < 4; ++e)
-                        {
-                            float x = s[nr][g][e] * c_log2;
-                            if constexpr(KIND == kPaged8)
-                            {
-                                x *= scale_of(ks[g], e);
-                            }
-                            if constexpr(PARTLY)
-                            {
-                                const int key = key0 + 16 * g + 4 * quad + e;
-                                x = key > last[nr] || key >= seg.len || ((hidden >> g) & 1) ? neg_inf() : x;
-                            }
-                            s[nr][g][e] = x;
-                            top = fmaxf(top, x);
-                            if constexpr(KIND == kPaged8)
-                            {
-                                top_t = fmaxf(top_t, x + (float)((int)((vs[g] >> (8 * e)) & 255u) - 127));
-                            }
-                        }
-                    }
-                    const float m_new = fmaxf(m_run[nr], quad_max(top));
-                    const float m_safe = m_new == neg_inf() ? 0.0f : m_new;
-                    const float fade = fast_exp2(m_run[nr] - m_safe);
-                    float t_safe = m_safe, fade_o = fade;
-                    if constexpr(KIND == kPaged8)
-                    {
-                        const float t_new = fmaxf(t_run[nr], quad_max(top_t));
-                        t_safe = t_new == neg_inf() ? 0.0f : t_new;
-                        fade_o = fast_exp2(t_run[nr] - t_safe);
-                        t_run[nr] = t_new;
-                    }
-                    float sum = 0.0f;
-#pragma unroll
-                    for(int g = 0; g < GROUPS; ++g)
-                    {
-                        f32x4 x;
-#pragma unroll
-                        for(int e = 0; e < 4; ++e)
-                        {
-                            x[e] = fast_exp2(s[nr][g][e] - m_safe);
-                            sum += x[e];
-                        }
-                        if constexpr(KIND == kPaged8)
+                        const u32x4 q = q_operand(nr, i);
+                        if constexpr(KIND == kPaged32)
                         {
 #pragma unroll
                             for(int e = 0; e < 4; ++e)
                             {
-                                x[e] = fast_exp2(s[nr][g][e] + (float)((int)((vs[g] >> (8 * e)) & 255u) - 127) - t_safe);
+                                x = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[i][e]),
+                                        __uint_as_float(q[e]), x, 0, 0, 0);
                             }
-                        }
-                        if constexpr(KIND == kPaged32)
-                        {
-                            pf[nr][g] = x;
                         }
                         else
                         {
-                            pw[nr][g][0] = PV::pack2(x[0], x[1]);
-                            pw[nr][g][1] = PV::pack2(x[2], x[3]);
+                            x = mfma32<T>(KIND == kPaged8 ? wide[i % (2 * KREADS)] : kf[i % KREADS], q, x);
                         }
                     }
-                    l_run[nr] = l_run[nr] * fade + sum;
-                    m_run[nr] = m_new;
-                    if(__any(fade_o != 1.0f))
-                    {
-#pragma unroll
-                        for(int db = 0; db < DBLOCKS; ++db)
-                        {
-                            o[nr][db] *= fade_o;
-                        }
-                    }
-                    }
+                    s[nr][g] = x;
+                }
+            }
 
-                // ---- output ----------------------------------------------------------------
-                auto value_words = [&](int db, int t, u32x4 &w)
+            // ---- probabilities -------------------------------------------------------
+            // 8-bit pages: what a probability is multiplied by for its value row's power of two
+            f32x4 of_scale[GROUPS];
+            float fade_scale = 1.0f;
+            if constexpr(KIND == kPaged8)
+            {
+                float most = top_scale;
+#pragma unroll
+                for(int g = 0; g < GROUPS; ++g)
                 {
-                    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-                    typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-                    // keys 32t + {4*quad + 0..3, 16 + 4*quad + 0..3}
-                    if constexpr(KIND == kPaged16)
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
                     {
-                        const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                    (lds_s16x4 *)(slot + v_at[db] + 32 * t * RB)));
-                        const u32x2 b = GROUPS == 1 ? u32x2{0, 0}
-                            : __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                        (lds_s16x4 *)(slot + v_at[db] + (32 * t + 16) * RB)));
-                        w = u32x4{a[0], a[1], b[0], b[1]};
+                        const bool there = !PARTLY || (key0 + 16 * g + 4 * quad + e < seg.len && !((hidden >> g) & 1));
+                        const uint32_t byte = there ? (vs[g] >> (8 * e)) & 255u : 0u;
+                        of_scale[g][e] = RANGED ? (float)byte : __uint_as_float(byte << 23);
+                        most = RANGED ? fmaxf(most, of_scale[g][e]) : most;
                     }
-                    else if constexpr(KIND == kPaged8)
-                    {
-                        const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                                    (lds_i32x2 *)(slot + v_at[db] + 32 * t * RB)));
-                        const u32x2 a = widen4<Fp16>(v[0]), b = widen4<Fp16>(v[1]);
-                        w = u32x4{a[0], a[1], b[0], b[1]};
-                    }
-                    else
+                }
+                if constexpr(RANGED)
+                {
+                    most = quad_max(most);
+                    fade_scale = fast_exp2(top_scale - most);
+                    top_scale = most;
+#pragma unroll
+                    for(int g = 0; g < GROUPS; ++g)
                     {
 #pragma unroll
                         for(int e = 0; e < 4; ++e)
                         {
-                            // key 16t + 4*quad + e
-                            w[e] = *reinterpret_cast<const uint32_t *>(slot + v_at[db] + (16 * t + e) * RB);
+                            of_scale[g][e] = fast_exp2(of_scale[g][e] - (most - kPagedLift));
                         }
                     }
-                };
-                // products of the value words of step t (32 keys, fp32: 16)
-                auto multiply = [&](const u32x4 &w, int t, int nr, f32x4 c) -> f32x4
+                }
+            }
+            uint32_t pw[NR][GROUPS][2];                 // 16-bit pairs
+            f32x4 pf[NR][GROUPS];                       // fp32
+#pragma unroll
+            for(int nr = 0; nr < NR; ++nr)
+            {
+                float top = m_run[nr];
+#pragma unroll
+                for(int g = 0; g < GROUPS; ++g)
                 {
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
+                    {
+                        float x = s[nr][g][e];
+                        if constexpr(KIND == kPaged8 && !KSCALE_IN_CODES)
+                        {
+                            x *= scale_of(ks[g], e);
+                        }
+                        if constexpr(PARTLY)
+                        {
+                            const int key = key0 + 16 * g + 4 * quad + e;
+                            x = key > last[nr] || key >= seg.len || ((hidden >> g) & 1) ? neg_inf() : x;
+                        }
+                        s[nr][g][e] = x;
+                        top = fmaxf(top, x);
+                    }
+                }
+                // p = 2^(c * score - c * maximum): c is positive, and the product with the
+                // maximum is rounded the same way wherever it is taken
+                const float m_new = quad_max(top);
+                const float mc = m_new == neg_inf() ? 0.0f : m_new * c_log2;
+                const float fade = fast_exp2(m_run[nr] * c_log2 - mc);
+                const float off = kLift - mc;
+                float sum = 0.0f;
+#pragma unroll
+                for(int g = 0; g < GROUPS; ++g)
+                {
+                    f32x4 x;
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
+                    {
+                        x[e] = fast_exp2(fmaf(s[nr][g][e], c_log2, off));
+                        sum += x[e];
+                    }
+                    if constexpr(KIND == kPaged8)
+                    {
+#pragma unroll
+                        for(int e = 0; e < 4; ++e)
+                        {
+                            x[e] *= of_scale[g][e];
+                        }
+                    }
                     if constexpr(KIND == kPaged32)
                     {
-#pragma unroll
-                        for(int e = 0; e < 4; ++e)
-                        {
-                            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[e]), pf[nr][t][e], c, 0, 0, 0);
-                        }
-                        return c;
-                    }
-                    else if constexpr(GROUPS == 1)
-                    {
-                        return mfma16<PV>(u32x2{w[0], w[1]}, u32x2{pw[nr][0][0], pw[nr][0][1]}, c);
+                        pf[nr][g] = x;
                     }
                     else
                     {
-                        return mfma32<PV>(w, u32x4{pw[nr][2 * t][0], pw[nr][2 * t][1], pw[nr][2 * t + 1][0],
-                                pw[nr][2 * t + 1][1]}, c);
+                        pw[nr][g][0] = PV::pack2(x[0], x[1]);
+                        pw[nr][g][1] = PV::pack2(x[2], x[3]);
                     }
-                };
-                constexpr int TSTEPS = KIND == kPaged32 ? GROUPS : (GROUPS + 1) / 2;
-                if constexpr(!PARTLY)
+                }
+                l_run[nr] = l_run[nr] * fade + sum;
+                m_run[nr] = m_new;
+                const float fade_o = fade * fade_scale;
+                if(__any(fade_o != 1.0f))
                 {
+#pragma unroll
+                    for(int db = 0; db < DBLOCKS; ++db)
+                    {
+                        o[nr][db] *= fade_o;
+                    }
+                }
+            }
+
+            // ---- output ----------------------------------------------------------------
+            auto value_words = [&](int db, int t, u32x4 &w)
+            {
+                typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+                typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+                // keys 32t + {4*quad + 0..3, 16 + 4*quad + 0..3}
+                if constexpr(KIND == kPaged16)
+                {
+                    const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (lds_s16x4 *)(slot + v_at[db] + 32 * t * RB)));
+                    const u32x2 b = GROUPS == 1 ? u32x2{0, 0}
+                        : __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                    (lds_s16x4 *)(slot + v_at[db] + (32 * t + 16) * RB)));
+                    w = u32x4{a[0], a[1], b[0], b[1]};
+                }
+                else if constexpr(KIND == kPaged8)
+                {
+                    const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                (lds_i32x2 *)(slot + v_at[db] + 32 * t * RB)));
+                    const u32x2 a = widen4<PV>(v[0], 1.0f), b = widen4<PV>(v[1], 1.0f);
+                    w = u32x4{a[0], a[1], b[0], b[1]};
+                }
+                else
+                {
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
+                    {
+                        // key 16t + 4*quad + e
+                        w[e] = *reinterpret_cast<const uint32_t *>(slot + v_at[db] + (16 * t + e) * RB);
+                    }
+                }
+            };
+            // products of the value words of step t (32 keys, fp32: 16)
+            auto multiply = [&](const u32x4 &w, int t, int nr, f32x4 c) -> f32x4
+            {
+                if constexpr(KIND == kPaged32)
+                {
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
+                    {
+                        c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[e]), pf[nr][t][e], c, 0, 0, 0);
+                    }
+                    return c;
+                }
+                else if constexpr(GROUPS == 1)
+                {
+                    return mfma16<PV>(u32x2{w[0], w[1]}, u32x2{pw[nr][0][0], pw[nr][0][1]}, c);
+                }
+                else
+                {
+                    return mfma32<PV>(w, u32x4{pw[nr][2 * t][0], pw[nr][2 * t][1], pw[nr][2 * t + 1][0],
+                            pw[nr][2 * t + 1][1]}, c);
+                }
+            };
+            constexpr int TSTEPS = KIND == kPaged32 ? GROUPS : (GROUPS + 1) / 2;
+            if constexpr(!PARTLY)
+            {
+#pragma unroll
+                for(int db = 0; db < DBLOCKS; ++db)
+                {
+#pragma unroll
+                    for(int t = 0; t < TSTEPS; ++t)
+                    {
+                        u32x4 w;
+                        value_words(db, t, w);
+#pragma unroll
+                        for(int nr = 0; nr < NR; ++nr)
+                        {
+                            o[nr][db] = multiply(w, t, nr, o[nr][db]);
+                        }
+                    }
+                }
+            }
+            else
+            {
+                // Where a value is no number, a probability of 0 does not hide it (0 * NaN): then
+                // token by token, with the values behind what the token sees taken out and only
+                // the rows of the token taken over.
+                bool odd = false;
+                if(p.causal && p.q_seq > 1)
+                {
+                    uint32_t any = 0;
 #pragma unroll
                     for(int db = 0; db < DBLOCKS; ++db)
                     {
@@ -987,25 +1120,28 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                             u32x4 w;
                             value_words(db, t, w);
 #pragma unroll
-                            for(int nr = 0; nr < NR; ++nr)
+                            for(int e = 0; e < 4; ++e)
                             {
-                                o[nr][db] = multiply(w, t, nr, o[nr][db]);
+                                any |= KIND == kPaged32 ? (w[e] & 0x7f800000u) == 0x7f800000u
+                                    : not_finite2<PV>(w[e]);
                             }
                         }
                     }
+                    odd = __any(any != 0);
                 }
-                else
+                const int rounds = odd ? given : 1;
+                for(int tok = 0; tok < rounds; ++tok)
                 {
-                    // Where a value is no number, a probability of 0 does not hide it (0 * NaN): then
-                    // token by token, with the values behind what the token sees taken out and only
-                    // the rows of the token taken over.
-                    bool odd = false;
-                    if(p.causal && p.q_seq > 1)
-                    {
-                        uint32_t any = 0;
+                    // (nothing is read ahead of the loop: the registers are the other step's)
+                    asm volatile("" ::: "memory");
+                    const int sees = odd ? all_see + tok : 0x7ffffffe;
 #pragma unroll
-                        for(int db = 0; db < DBLOCKS; ++db)
+                    for(int db = 0; db < DBLOCKS; ++db)
+                    {
+#pragma unroll
+                        for(int nr = 0; nr < NR; ++nr)
                         {
+                            f32x4 fresh = o[nr][db];
 #pragma unroll
                             for(int t = 0; t < TSTEPS; ++t)
                             {
@@ -1014,65 +1150,39 @@ void sdpa_paged_kernel(const PagedAttendParams p)
 #pragma unroll
                                 for(int e = 0; e < 4; ++e)
                                 {
-                                    any |= KIND == kPaged32 ? (w[e] & 0x7f800000u) == 0x7f800000u
-                                        : not_finite2<PV>(w[e]);
-                                }
-                            }
-                        }
-                        odd = __any(any != 0);
-                    }
-                    const int rounds = odd ? given : 1;
-                    for(int tok = 0; tok < rounds; ++tok)
-                    {
-                        // (nothing is read ahead of the loop: the registers are the other step's)
-                        asm volatile("" ::: "memory");
-                        const int sees = odd ? all_see + tok : 0x7ffffffe;
-#pragma unroll
-                        for(int db = 0; db < DBLOCKS; ++db)
-                        {
-#pragma unroll
-                            for(int nr = 0; nr < NR; ++nr)
-                            {
-                                f32x4 fresh = o[nr][db];
-#pragma unroll
-                                for(int t = 0; t < TSTEPS; ++t)
-                                {
-                                    u32x4 w;
-                                    value_words(db, t, w);
-#pragma unroll
-                                    for(int e = 0; e < 4; ++e)
+                                    if constexpr(KIND == kPaged32)
                                     {
-                                        if constexpr(KIND == kPaged32)
-                                        {
-                                            w[e] = key0 + 16 * t + 4 * quad + e > sees ? 0u : w[e];
-                                        }
-                                        else
-                                        {
-                                            const int key = key0 + 32 * t + 16 * (e >> 1) + 4 * quad + 2 * (e & 1);
-                                            w[e] &= (key > sees ? 0u : 0xffffu) | (key + 1 > sees ? 0u : 0xffff0000u);
-                                        }
+                                        w[e] = key0 + 16 * t + 4 * quad + e > sees ? 0u : w[e];
                                     }
-                                    fresh = multiply(w, t, nr, fresh);
+                                    else
+                                    {
+                                        const int key = key0 + 32 * t + 16 * (e >> 1) + 4 * quad + 2 * (e & 1);
+                                        w[e] &= (key > sees ? 0u : 0xffffu) | (key + 1 > sees ? 0u : 0xffff0000u);
+                                    }
                                 }
-                                const bool take = !odd || token[nr] == tok;
+                                fresh = multiply(w, t, nr, fresh);
+                            }
+                            const bool take = !odd || token[nr] == tok;
 #pragma unroll
-                                for(int e = 0; e < 4; ++e)
-                                {
-                                    o[nr][db][e] = take ? fresh[e] : o[nr][db][e];
-                                }
+                            for(int e = 0; e < 4; ++e)
+                            {
+                                o[nr][db][e] = take ? fresh[e] : o[nr][db][e];
                             }
                         }
                     }
                 }
-            };
-            if(key0 + KEYS - 1 > all_see || hidden != 0)
-            {
-                attend(std::true_type());
             }
-            else
-            {
-                attend(std::false_type());
-            }
+        };
+        // (the steps without hidden keys on their own: two forms behind each other cost fewer
+        // registers than one or the other)
+        int i = 0;
+        for(; i < n_mine && my_first + i * Shape::BLOCK + KEYS - 1 <= all_see && without_page() == 0; ++i)
+        {
+            take_step(i, std::false_type());
+        }
+        for(; i < n_steps; ++i)
+        {
+            take_step(i, std::true_type());
         }
 
         // ---- the wavefronts' results, then the unit's or the share's ---------------------
@@ -1085,11 +1195,9 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         {
             __syncthreads();        // every wavefront is done with the ring, or with the last row block
             const int mine = wave * 16 + col;
-            float m = m_run[nr], l = quad_sum(l_run[nr]), to_m = 1.0f;
-            if constexpr(KIND == kPaged8)
-            {
-                to_m = m == neg_inf() ? 0.0f : fast_exp2(t_run[nr] - m);
-            }
+            float m = m_run[nr] * c_log2 - kLift, l = quad_sum(l_run[nr]);
+            // what the products of this wavefront are times
+            const float to_m = KIND == kPaged8 && RANGED ? fast_exp2(top_scale - (127.0f + kPagedLift)) : 1.0f;
             if(!row_ok[nr])
             {
                 m = neg_inf();
@@ -1099,7 +1207,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             for(int db = 0; db < DBLOCKS; ++db)
             {
                 f32x4 x = o[nr][db];
-                if constexpr(KIND == kPaged8)
+                if constexpr(KIND == kPaged8 && RANGED)
                 {
                     x *= to_m;
                 }
@@ -1161,7 +1269,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                 }
             }
         }
-        if(!whole)
+        if(!whole && !p.join_behind)
         {
             // The share's results are with the device once its stores are acknowledged, every
             // wavefront's in front of the barrier.  The workgroup that counts last joins.
@@ -1184,7 +1292,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                     // (a replay of a captured call has this tag again)
                     __hip_atomic_store(count, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
-                paged_join<T, HEAD, THREADS, QROWS>(p, seg.n, h, rg, rows_here, (int)w0, (int)parts,
+                paged_join<T, HEAD, THREADS, QROWS>(p, seg.n, h, rg, 0, rows_here, (int)w0, (int)parts,
                         reinterpret_cast<float *>(ring));
             }
         }
@@ -1211,6 +1319,34 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     }
 }
 
+// The join as a launch of its own, for units of more rows than one workgroup joins quickly: a
+// workgroup takes kJoinRows rows of a unit.
+constexpr int kJoinRows = 4;
+template<typename T, int HEAD, int QROWS>
+__global__ __launch_bounds__(256)
+void sdpa_paged_join_kernel(const PagedAttendParams p)
+{
+    __shared__ __attribute__((aligned(16))) float lds[256 / (HEAD / 4) * (HEAD + 4)];
+    const int first_row = (int)(blockIdx.x % (QROWS / kJoinRows)) * kJoinRows;
+    const int unit = (int)(blockIdx.x / (QROWS / kJoinRows));
+    const int n = unit / p.units, u = unit - n * p.units;
+    const int h = u / p.row_groups, rg = u - h * p.row_groups;
+    const int rows_here = min(p.rows - rg * QROWS - first_row, kJoinRows);
+    const uint32_t before = (uint32_t)p.before[n], cost = (uint32_t)p.before[n + 1] - before;
+    if(rows_here <= 0 || cost == 0)
+    {
+        return;
+    }
+    const uint32_t all = (uint32_t)p.before[p.c.n_batch] * (uint32_t)p.units;
+    const PagedSplit split(all, min((uint32_t)p.shares, all));
+    const uint32_t begin = before * (uint32_t)p.units + (uint32_t)u * cost;
+    const uint32_t w0 = split.of(begin), w1 = split.of(begin + cost - (uint32_t)p.before[p.c.n_batch + 1] - 1);
+    if(w0 != w1)
+    {
+        paged_join<T, HEAD, 256, QROWS>(p, n, h, rg, first_row, rows_here, (int)w0, (int)(w1 - w0 + 1), lds);
+    }
+}
+
 // Blocks of 16 rows that a workgroup takes: 1, 2, or 4 by two wavefronts a key
 static int row_blocks(bool fp32, int64_t rows)
 {
@@ -1222,7 +1358,7 @@ static size_t align16(size_t x)
     return (x + 15) & ~(size_t)15;
 }
 
-// The workspace: a count per unit, then the shares' results.  (The larger of the types' sizes,
+// The workspace: a count per unit, the sequences' blocks, the shares' results.  (The larger of the types' sizes,
 // which differ in the rows of a workgroup.)
 static size_t count_bytes(int64_t n_batch, int64_t n_head_kv, int64_t rows)
 {
@@ -1232,6 +1368,11 @@ static size_t count_bytes(int64_t n_batch, int64_t n_head_kv, int64_t rows)
     return align16(8 * (size_t)(n_batch * n_head_kv) * (size_t)groups);
 }
 
+static size_t before_bytes(int64_t n_batch)
+{
+    return align16(4 * ((size_t)n_batch + 2));
+}
+
 static size_t share_rows(int64_t rows)
 {
     return (size_t)kPagedShares * 2 * 16 * (size_t)row_blocks(false, rows);
@@ -1239,7 +1380,7 @@ static size_t share_rows(int64_t rows)
 
 size_t paged_attend_workspace_bytes(int64_t n_batch, int64_t n_head_kv, int64_t rows, int64_t head)
 {
-    return count_bytes(n_batch, n_head_kv, rows) + share_rows(rows) * (size_t)(head + 2) * 4;
+    return count_bytes(n_batch, n_head_kv, rows) + before_bytes(n_batch) + share_rows(rows) * (size_t)(head + 2) * 4;
 }
 
 template<typename T, int KIND, int HEAD, int NR, int HALVES>
@@ -1250,15 +1391,22 @@ static int launch_form(hipStream_t stream, PagedAttendParams &p)
     p.units = p.c.n_head_kv * p.row_groups;
     // at most as many shares as there can be blocks
     const int64_t most = (int64_t)p.c.n_batch * p.units * (p.c.max_rows / Shape::BLOCK + 1 + kPagedUnitCost);
-    if(most > 0xffffffffll)
+    if(most > 0x7fffffffll / (Shape::QROWS / kJoinRows))
     {
         return NNTILE_HIP_EINVAL;
     }
     const int64_t places = kPagedCUs * Shape::WGS_PER_CU;
     p.shares = (int32_t)(most < places ? most : places);
+    // (one workgroup would read the shares of 32 or 64 rows for as long as a launch takes, or longer)
+    p.join_behind = Shape::QROWS > 16;
     p.tag = next_decode_tag() * (kPagedTagUnit / 16);
     hipLaunchKernelGGL((sdpa_paged_kernel<T, KIND, HEAD, NR, HALVES>), dim3((unsigned)p.shares),
             dim3(Shape::THREADS), 0, stream, p);
+    if(p.join_behind)
+    {
+        hipLaunchKernelGGL((sdpa_paged_join_kernel<T, HEAD, Shape::QROWS>),
+                dim3((unsigned)(p.c.n_batch * p.units * (Shape::QROWS / kJoinRows))), dim3(256), 0, stream, p);
+    }
     return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;
 }
 
@@ -1284,7 +1432,8 @@ int launch_paged_attend(hipStream_t stream, int dtype, PagedAttendParams &p, int
 {
     const size_t counts = count_bytes(p.c.n_batch, p.c.n_head_kv, p.rows);
     p.counts = static_cast<unsigned long long *>(workspace);
-    p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + counts);
+    p.before = reinterpret_cast<int32_t *>(static_cast<char *>(workspace) + counts);
+    p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + counts + before_bytes(p.c.n_batch));
     p.part_ml = p.part_o + share_rows(p.rows) * (size_t)head;
     if(p.c.k_scales != nullptr)
     {

@@ -123,7 +123,9 @@ def attend_bounds(case, q, q_seq, group, causal, new_rows=None):
     q = q.float().numpy().astype(np.float64).reshape(heads, group, n_batch, q_seq, head)
     bound_a, bound_l = np.zeros(q.shape), np.zeros(q.shape[:4])
     u = {"bf16": 2.0 ** -9, "fp16": 2.0 ** -12, "fp32": 2.0 ** -24}[case.dtype] * 2     # relative to the value
-    up = 2.0 ** -11 if case.packed else u
+    # (a probability is rounded to the tile type whatever the pages hold, in bf16 times the power
+    # of two of its value row, which moves no bit of it: half a step, u, again)
+    up = u
     eps = 2.0 ** -24
     for n in range(n_batch):
         k, ok = case.rows(n, 0)
