@@ -43,7 +43,10 @@ constexpr int kPagedCUs = 256;
 // Workgroups that the keys are shared out to at most: two a CU
 constexpr int kPagedShares = 2 * kPagedCUs;
 // What a unit costs beside its key blocks, in blocks
-constexpr int kPagedUnitCost = 1;
+#ifndef NNTILE_PAGED_UNIT_COST
+#define NNTILE_PAGED_UNIT_COST 1
+#endif
+constexpr int kPagedUnitCost = NNTILE_PAGED_UNIT_COST;
 // fp16 probabilities are kept times 2^14: 2^-28 of the largest still has all of its bits
 constexpr float kPagedLift = 14.0f;
 // A count of shares and the tag above it
@@ -200,16 +203,38 @@ struct PagedSegment
     int u, step, steps;
 };
 
-// Share w of `all` blocks: [begin(w), begin(w + 1)); the share that has a block.
+// Share w of the blocks: [begin(w), begin(w + 1)); the share that has a block.  The blocks come in periods
+// of equal length - a unit where all units are equally long and each gets shares of its own, else
+// all blocks - that as many shares divide.
 struct PagedSplit
 {
-    uint32_t base, rest;    // the first `rest` shares take one block more
-    __device__ __forceinline__ PagedSplit(uint32_t all, uint32_t shares) : base(all / shares), rest(all % shares) {}
-    __device__ __forceinline__ uint32_t begin(uint32_t w) const { return w * base + min(w, rest); }
+    uint32_t period, per_period, shares;
+    uint32_t base, rest;    // of a period the first `rest` shares take one block more
+    __device__ __forceinline__ PagedSplit(uint32_t all, uint32_t places, uint32_t unit_blocks, uint32_t units)
+    {
+        period = all;
+        per_period = min(places, all);
+        shares = per_period;
+        if(unit_blocks != 0 && units <= places)
+        {
+            // as few shares as keep the longest as short as it can be
+            const uint32_t longest = (unit_blocks + places / units - 1) / (places / units);
+            period = unit_blocks;
+            per_period = (unit_blocks + longest - 1) / longest;
+            shares = units * per_period;
+        }
+        base = per_period != 0 ? period / per_period : 0;
+        rest = per_period != 0 ? period % per_period : 0;
+    }
+    __device__ __forceinline__ uint32_t begin(uint32_t w) const
+    {
+        const uint32_t q = w / per_period, r = w - q * per_period;
+        return q * period + r * base + min(r, rest);
+    }
     __device__ __forceinline__ uint32_t of(uint32_t block) const
     {
-        const uint32_t longer = rest * (base + 1);
-        return block < longer ? block / (base + 1) : rest + (block - longer) / base;
+        const uint32_t q = block / period, r = block - q * period, longer = rest * (base + 1);
+        return q * per_period + (r < longer ? r / (base + 1) : rest + (r - longer) / base);
     }
 };
 
@@ -308,84 +333,92 @@ __device__ __forceinline__ int64_t paged_query_row(const PagedAttendParams &p, i
 }
 
 // Joins the shares w0 .. w0 + parts - 1 of a unit, in this order, and finishes rows first_row .. +
-// rows_here - 1 of it.  HEAD/4 threads a
-// row; where the rows leave threads over, they take turns at the shares and the sums
-// are added up through LDS.
-template<typename T, int HEAD, int THREADS, int QROWS>
-__device__ __forceinline__ void paged_join(const PagedAttendParams &p, int n, int h, int rg, int first_row,
+// rows_here - 1 of it.  HEAD/4 threads a row; where the rows leave threads over, they take turns at the
+// shares and the sums are added up through LDS.  A thread has PARTS shares of LINES rows on their way
+// at a time: the round trips are what the join costs.
+template<typename T, int HEAD, int THREADS, int QROWS, int PARTS, int LINES>
+__device__ __forceinline__ void paged_join_by(const PagedAttendParams &p, int n, int h, int rg, int first_row,
         int rows_here, int w0, int parts, float *lds)
 {
     constexpr int TPR = HEAD / 4, ROWS = THREADS / TPR;
-    constexpr int AT_ONCE = 8;
     int turns = 1;
     while(2 * turns * rows_here <= ROWS && 2 * turns <= parts)
     {
         turns *= 2;
     }
     const int d0 = (threadIdx.x % TPR) * 4, slot = threadIdx.x / TPR;
-    const int turn = slot % turns;
-    for(int r0 = 0; r0 < rows_here; r0 += ROWS / turns)
+    const int turn = slot % turns, step = ROWS / turns;
+    // (with more than one turn all rows fit beside each other: one round of one line)
+    for(int r0 = slot / turns; r0 - slot / turns < rows_here; r0 += LINES * step)
     {
-        const int r = r0 + slot / turns;
-        float top = neg_inf(), sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if(r < rows_here)
+        float top[LINES], sum[LINES];
+        f32x4 v[LINES];
+#pragma unroll
+        for(int k = 0; k < LINES; ++k)
         {
-            for(int i0 = turn; i0 < parts; i0 += AT_ONCE * turns)
+            top[k] = neg_inf();
+            sum[k] = 0.0f;
+            v[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        for(int i0 = turn; i0 < parts; i0 += PARTS * turns)
+        {
+            float m[LINES][PARTS], l[LINES][PARTS], x[LINES][PARTS][4];
+#pragma unroll
+            for(int k = 0; k < LINES; ++k)
             {
-                float m[AT_ONCE], l[AT_ONCE], x[AT_ONCE][4];
 #pragma unroll
-                for(int j = 0; j < AT_ONCE; ++j)
+                for(int j = 0; j < PARTS; ++j)
                 {
-                    // (behind the last share: it again, with no weight)
+                    // (behind the last share or row: it again, with no weight)
                     const int i = min(i0 + j * turns, parts - 1);
+                    const int r = min(r0 + k * step, rows_here - 1);
                     const int64_t place = ((int64_t)(w0 + i) * 2 + (i == 0 ? 1 : 0)) * QROWS + first_row + r;
-                    get2(p.part_ml + 2 * place, m[j], l[j]);
-                    get2(p.part_o + place * HEAD + d0, x[j][0], x[j][1]);
-                    get2(p.part_o + place * HEAD + d0 + 2, x[j][2], x[j][3]);
+                    get2(p.part_ml + 2 * place, m[k][j], l[k][j]);
+                    get2(p.part_o + place * HEAD + d0, x[k][j][0], x[k][j][1]);
+                    get2(p.part_o + place * HEAD + d0 + 2, x[k][j][2], x[k][j][3]);
                 }
-                float next = top;
+            }
 #pragma unroll
-                for(int j = 0; j < AT_ONCE; ++j)
+            for(int k = 0; k < LINES; ++k)
+            {
+                float next = top[k];
+#pragma unroll
+                for(int j = 0; j < PARTS; ++j)
                 {
-                    next = i0 + j * turns < parts ? fmaxf(next, m[j]) : next;
+                    next = i0 + j * turns < parts ? fmaxf(next, m[k][j]) : next;
                 }
                 const float safe = next == neg_inf() ? 0.0f : next;
-                const float old = fast_exp2(top - safe);
-                sum *= old;
+                const float old = fast_exp2(top[k] - safe);
+                sum[k] *= old;
+                v[k] *= old;
 #pragma unroll
-                for(int e = 0; e < 4; ++e)
-                {
-                    v[e] *= old;
-                }
-#pragma unroll
-                for(int j = 0; j < AT_ONCE; ++j)
+                for(int j = 0; j < PARTS; ++j)
                 {
                     if(i0 + j * turns < parts)
                     {
-                        const float f = fast_exp2(m[j] - safe);
-                        sum += l[j] * f;
+                        const float f = fast_exp2(m[k][j] - safe);
+                        sum[k] += l[k][j] * f;
 #pragma unroll
                         for(int e = 0; e < 4; ++e)
                         {
-                            v[e] += x[j][e] * f;
+                            v[k][e] += x[k][j][e] * f;
                         }
                     }
                 }
-                top = next;
+                top[k] = next;
             }
         }
         if(turns > 1)
         {
-            // (r0 takes one value only: the rows fit beside each other)
             float *const at = lds + slot * (HEAD + 4);
-            *reinterpret_cast<f32x4 *>(at + d0) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4 *>(at + d0) = v[0];
             if(d0 == 0)
             {
-                at[HEAD] = top;
-                at[HEAD + 1] = sum;
+                at[HEAD] = top[0];
+                at[HEAD + 1] = sum[0];
             }
             __syncthreads();
-            if(turn == 0 && r < rows_here)
+            if(turn == 0 && r0 < rows_here)
             {
                 float next = neg_inf();
                 for(int j = 0; j < turns; ++j)
@@ -393,26 +426,46 @@ __device__ __forceinline__ void paged_join(const PagedAttendParams &p, int n, in
                     next = fmaxf(next, at[j * (HEAD + 4) + HEAD]);
                 }
                 const float safe = next == neg_inf() ? 0.0f : next;
-                sum = 0.0f;
-                f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+                sum[0] = 0.0f;
+                v[0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 for(int j = 0; j < turns; ++j)
                 {
                     const float f = fast_exp2(at[j * (HEAD + 4) + HEAD] - safe);
-                    sum += f * at[j * (HEAD + 4) + HEAD + 1];
-                    o += f * *reinterpret_cast<const f32x4 *>(at + j * (HEAD + 4) + d0);
+                    sum[0] += f * at[j * (HEAD + 4) + HEAD + 1];
+                    v[0] += f * *reinterpret_cast<const f32x4 *>(at + j * (HEAD + 4) + d0);
                 }
-                top = next;
-#pragma unroll
-                for(int e = 0; e < 4; ++e)
-                {
-                    v[e] = o[e];
-                }
+                top[0] = next;
             }
         }
-        if(turn == 0 && r < rows_here)
+#pragma unroll
+        for(int k = 0; k < LINES; ++k)
         {
-            paged_finish_row<T>(p, HEAD, paged_query_row(p, n, h, rg * QROWS + first_row + r), d0, top, sum, v);
+            const int r = r0 + k * step;
+            if(turn == 0 && r < rows_here)
+            {
+                const float out[4] = {v[k][0], v[k][1], v[k][2], v[k][3]};
+                paged_finish_row<T>(p, HEAD, paged_query_row(p, n, h, rg * QROWS + first_row + r), d0, top[k],
+                        sum[k], out);
+            }
         }
+    }
+}
+
+template<typename T, int HEAD, int THREADS, int QROWS>
+__device__ __forceinline__ void paged_join(const PagedAttendParams &p, int n, int h, int rg, int first_row,
+        int rows_here, int w0, int parts, float *lds)
+{
+    if(rows_here > THREADS / (HEAD / 4) && parts <= 4)
+    {
+        paged_join_by<T, HEAD, THREADS, QROWS, 4, 4>(p, n, h, rg, first_row, rows_here, w0, parts, lds);
+    }
+    else if(rows_here > THREADS / (HEAD / 4))
+    {
+        paged_join_by<T, HEAD, THREADS, QROWS, 8, 2>(p, n, h, rg, first_row, rows_here, w0, parts, lds);
+    }
+    else
+    {
+        paged_join_by<T, HEAD, THREADS, QROWS, 8, 1>(p, n, h, rg, first_row, rows_here, w0, parts, lds);
     }
 }
 
@@ -456,21 +509,26 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     const int stream = wave % STREAMS, half = wave / STREAMS;
 
     // ---- the workgroup's run of key blocks ----------------------------------------
-    // Every thread adds up the blocks of a few neighbouring sequences, then a scan.  A unit counts
-    // as a block more than it has: its begin and end cost about as much.  (64 sequences of 17 to 16384
-    // 8-bit rows 82 -> 73 us.)  Where all sequences have as many blocks it does not, so that
-    // shares and units more often end together.
-    const int chunk = (p.c.n_batch + THREADS - 1) / THREADS;
+    // A scan over the sequences' blocks; every lane adds up a few neighbouring sequences.  A unit counts
+    // as a block more than it has: its begin and end cost about as much (64 sequences of 17 to 16384
+    // 8-bit rows 82 -> 73 us).  Where all sequences have as many blocks it does not, so that
+    // shares and units end together.  Up to 64 sequences every wavefront scans for itself,
+    // without LDS and barriers.
+    const bool in_wave = p.c.n_batch <= 64;
+    const int scanner = in_wave ? lane : tid, scanners = in_wave ? 64 : THREADS;
+    const int chunk = (p.c.n_batch + scanners - 1) / scanners;
+    const int n_lo = min(scanner * chunk, p.c.n_batch), n_hi = min(n_lo + chunk, p.c.n_batch);
     auto blocks_of = [&](int n) { return (paged_len(p.c, n) + Shape::BLOCK - 1) / Shape::BLOCK; };
     int unit_cost = kPagedUnitCost;
     auto cost_of = [&](int blocks) { return blocks == 0 ? 0 : blocks + unit_cost; };
-    const int blocks_0 = blocks_of(0);
+    const int blocks_0 = uniform(blocks_of(0));
     int mine = 0;
     bool same = true;
-    for(int n = tid * chunk; n < min((tid + 1) * chunk, p.c.n_batch); ++n)
+    for(int n = n_lo; n < n_hi; ++n)
     {
-        mine += cost_of(blocks_of(n));
-        same = same && blocks_of(n) == blocks_0;
+        const int b = blocks_of(n);
+        mine += cost_of(b);
+        same = same && b == blocks_0;
     }
     same = __all(same);
     int upto = mine;
@@ -480,31 +538,36 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         const int other = __shfl_up(upto, o);
         upto += lane >= o ? other : 0;
     }
-    if(lane == 63)
+    int total = __builtin_amdgcn_readlane(upto, 63);
+    if(!in_wave)
     {
-        wave_sum[wave] = same ? upto : ~upto;
-    }
-    __syncthreads();
-    int total = 0;
+        if(lane == 63)
+        {
+            wave_sum[wave] = same ? upto : ~upto;
+        }
+        __syncthreads();
+        total = 0;
 #pragma unroll
-    for(int w = 0; w < WAVES; ++w)
-    {
-        const int sum = wave_sum[w];
-        same = same && sum >= 0;
-        upto += w < wave ? (sum < 0 ? ~sum : sum) : 0;
-        total += sum < 0 ? ~sum : sum;
+        for(int w = 0; w < WAVES; ++w)
+        {
+            const int sum = uniform(wave_sum[w]);
+            same = same && sum >= 0;
+            upto += w < wave ? (sum < 0 ? ~sum : sum) : 0;
+            total += sum < 0 ? ~sum : sum;
+        }
     }
+    int in_front = upto - mine;         // of the lane's first sequence
     if(same)
     {
         unit_cost = 0;
         total = p.c.n_batch * blocks_0;
+        in_front = n_lo * blocks_0;
     }
-    scan_of[tid] = same ? min(tid * chunk, p.c.n_batch) * blocks_0 : upto - mine;
-    if(p.join_behind && blockIdx.x == 0)
+    if(p.join_behind && blockIdx.x == 0 && (!in_wave || wave == 0))
     {
         // for the launch that joins the shares
-        int sum = scan_of[tid];
-        for(int n = tid * chunk; n < min((tid + 1) * chunk, p.c.n_batch); ++n)
+        int sum = in_front;
+        for(int n = n_lo; n < n_hi; ++n)
         {
             p.before[n] = sum;
             sum += cost_of(blocks_of(n));
@@ -515,49 +578,57 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             p.before[p.c.n_batch + 1] = unit_cost;
         }
     }
+    const uint32_t all = (uint32_t)total * (uint32_t)p.units;
+    const PagedSplit split(all, (uint32_t)p.shares, same ? (uint32_t)blocks_0 : 0u,
+            (uint32_t)p.c.n_batch * (uint32_t)p.units);
     // sequences without rows: shared out, too, for the rows of their queries
-    for(int n = blockIdx.x; n < p.c.n_batch; n += gridDim.x)
+    if(p.overwrite && !(same && blocks_0 != 0))
     {
-        if(uniform(paged_len(p.c, n)) == 0 && p.overwrite)
+        for(int n = blockIdx.x; n < p.c.n_batch; n += gridDim.x)
         {
-            const int rows = p.c.n_head_kv * p.rows;
-            for(int t = tid; t < rows * (HEAD / 4); t += THREADS)
+            if(uniform(paged_len(p.c, n)) == 0)
             {
-                const int r = t / (HEAD / 4);
-                const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                paged_finish_row<T>(p, HEAD, paged_query_row(p, n, r / p.rows, r % p.rows),
-                        4 * (t % (HEAD / 4)), neg_inf(), 0.0f, zero);
+                const int rows = p.c.n_head_kv * p.rows;
+                for(int t = tid; t < rows * (HEAD / 4); t += THREADS)
+                {
+                    const int r = t / (HEAD / 4);
+                    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    paged_finish_row<T>(p, HEAD, paged_query_row(p, n, r / p.rows, r % p.rows),
+                            4 * (t % (HEAD / 4)), neg_inf(), 0.0f, zero);
+                }
             }
         }
     }
-    unit_cost = uniform(unit_cost);
-    const uint32_t all = (uint32_t)uniform(total) * (uint32_t)p.units;
-    const uint32_t shares = min((uint32_t)p.shares, all);
-    if(blockIdx.x >= shares)
+    if(blockIdx.x >= split.shares)
     {
         return;
     }
-    const PagedSplit split(all, shares);
     uint32_t at = split.begin(blockIdx.x);
     const uint32_t end = split.begin(blockIdx.x + 1);
     PagedSegment seg;
     {
-        // the last thread whose sequences begin at or before the block, then sequence by sequence
+        // the last lane whose sequences begin at or before the block, then sequence by sequence
         const int block = (int)(at / (uint32_t)p.units);
-        if(tid == 0)
+        int t, before;
+        if(in_wave)
         {
-            found = 0;
+            t = __popcll(__ballot(scanner * chunk < p.c.n_batch && in_front <= block)) - 1;
+            before = __builtin_amdgcn_readlane(in_front, t);
         }
-        __syncthreads();
-        const bool here = tid * chunk < p.c.n_batch && scan_of[tid] <= block
-            && (tid == THREADS - 1 || (tid + 1) * chunk >= p.c.n_batch || scan_of[tid + 1] > block);
-        if(here)
+        else
         {
-            found = tid;
+            scan_of[tid] = in_front;
+            __syncthreads();
+            const bool here = tid * chunk < p.c.n_batch && in_front <= block
+                && (tid == THREADS - 1 || (tid + 1) * chunk >= p.c.n_batch || scan_of[tid + 1] > block);
+            if(here)
+            {
+                found = tid;
+            }
+            __syncthreads();
+            t = uniform(found);
+            before = uniform(scan_of[t]);
         }
-        __syncthreads();
-        const int t = uniform(found);
-        int before = uniform(scan_of[t]);
         seg.n = t * chunk;
         for(;;)
         {
@@ -774,24 +845,22 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             }
         };
 
+        // The unit's count of shares that are done starts with this call's tag, whatever the workspace
+        // holds.  Mostly it holds the 0 that earlier calls left; what else it held is seen to when the count
+        // is needed.
+        unsigned long long *const count = p.counts + ((int64_t)seg.n * p.units + seg.u);
+        unsigned long long held = 0;
+        if(tid == 0 && !p.join_behind && (seg.step > 0 || seg.steps < seg.blocks))
+        {
+            __hip_atomic_compare_exchange_strong(count, &held, p.tag, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                    __HIP_MEMORY_SCOPE_AGENT);
+        }
         int page[GROUPS], page_next[GROUPS];
         if(n_mine > 0)
         {
             look_up(0, page);
             fetch(0, page, slots);
             look_up(min(1, n_mine - 1), page_next);
-        }
-        if(tid == 0 && !p.join_behind && (seg.step > 0 || seg.steps < seg.blocks))
-        {
-            // The unit's count of shares that are done starts with this call's tag, whatever the
-            // workspace holds: the first share that finds something else puts it there.
-            unsigned long long *const count = p.counts + ((int64_t)seg.n * p.units + seg.u);
-            unsigned long long seen = __hip_atomic_load(count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if((seen & ~(kPagedTagUnit - 1)) != p.tag)
-            {
-                __hip_atomic_compare_exchange_strong(count, &seen, p.tag, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
-                        __HIP_MEMORY_SCOPE_AGENT);
-            }
         }
         const int n_steps = PAIRED ? seg.steps : n_mine;
         auto without_page = [&]()       // groups of the step
@@ -1277,9 +1346,14 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             __syncthreads();
             const uint32_t w0 = split.of(unit_begin);
             const uint32_t parts = split.of(unit_begin + (uint32_t)seg.blocks - 1) - w0 + 1;
-            unsigned long long *const count = p.counts + ((int64_t)seg.n * p.units + seg.u);
             if(tid == 0)
             {
+                if(held != 0 && (held & ~(kPagedTagUnit - 1)) != p.tag)
+                {
+                    // (the first share that gets here puts the tag there)
+                    __hip_atomic_compare_exchange_strong(count, &held, p.tag, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                            __HIP_MEMORY_SCOPE_AGENT);
+                }
                 const unsigned long long old = __hip_atomic_fetch_add(count, 1ull, __ATOMIC_RELAXED,
                         __HIP_MEMORY_SCOPE_AGENT);
                 found = (uint32_t)(old & (kPagedTagUnit - 1)) == parts - 1;
@@ -1338,9 +1412,11 @@ void sdpa_paged_join_kernel(const PagedAttendParams p)
         return;
     }
     const uint32_t all = (uint32_t)p.before[p.c.n_batch] * (uint32_t)p.units;
-    const PagedSplit split(all, min((uint32_t)p.shares, all));
+    const int unit_cost = p.before[p.c.n_batch + 1];
+    // (units that cost no more than their blocks: all are equally long)
+    const PagedSplit split(all, (uint32_t)p.shares, unit_cost == 0 ? cost : 0u, (uint32_t)p.c.n_batch * (uint32_t)p.units);
     const uint32_t begin = before * (uint32_t)p.units + (uint32_t)u * cost;
-    const uint32_t w0 = split.of(begin), w1 = split.of(begin + cost - (uint32_t)p.before[p.c.n_batch + 1] - 1);
+    const uint32_t w0 = split.of(begin), w1 = split.of(begin + cost - (uint32_t)unit_cost - 1);
     if(w0 != w1)
     {
         paged_join<T, HEAD, 256, QROWS>(p, n, h, rg, first_row, rows_here, (int)w0, (int)(w1 - w0 + 1), lds);
@@ -1398,7 +1474,10 @@ static int launch_form(hipStream_t stream, PagedAttendParams &p)
     const int64_t places = kPagedCUs * Shape::WGS_PER_CU;
     p.shares = (int32_t)(most < places ? most : places);
     // (one workgroup would read the shares of 32 or 64 rows for as long as a launch takes, or longer)
-    p.join_behind = Shape::QROWS > 16;
+#ifndef NNTILE_PAGED_JOIN
+#define NNTILE_PAGED_JOIN 0
+#endif
+    p.join_behind = NNTILE_PAGED_JOIN && Shape::QROWS > 16;
     p.tag = next_decode_tag() * (kPagedTagUnit / 16);
     hipLaunchKernelGGL((sdpa_paged_kernel<T, KIND, HEAD, NR, HALVES>), dim3((unsigned)p.shares),
             dim3(Shape::THREADS), 0, stream, p);
