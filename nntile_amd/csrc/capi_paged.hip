@@ -171,8 +171,7 @@ int attend_call(int dtype, void *stream, const nntile_hip_sdpa_paged_args *a, vo
             ? NNTILE_HIP_EUNSUPPORTED : NNTILE_HIP_EINVAL;
     }
     if(workspace == nullptr || !on16(workspace)
-            || workspace_bytes < paged_attend_workspace_bytes(a->cache.n_batch, a->cache.n_head_kv,
-                rows, a->cache.head))
+            || workspace_bytes < paged_attend_workspace_bytes(rows, a->cache.head))
     {
         return NNTILE_HIP_EWORKSPACE;
     }
@@ -251,7 +250,7 @@ size_t nntile_hip_sdpa_fwd_paged_workspace_bytes(const nntile_hip_sdpa_paged_arg
 {
     const int64_t rows = args == nullptr ? -1 : query_rows(args);
     return rows < 0 || args->cache.head <= 0 || args->cache.head > 128 ? 0
-        : paged_attend_workspace_bytes(args->cache.n_batch, args->cache.n_head_kv, rows, args->cache.head);
+        : paged_attend_workspace_bytes(rows, args->cache.head);
 }
 
 #define NNTILE_HIP_PAGED_ENTRY(suffix, dt, ctype) \

@@ -42,11 +42,7 @@ struct PagedAttendParams
     int32_t row_groups;                 // of as many rows as a workgroup takes
     int32_t units;                      // n_head_kv * row_groups, of a sequence
     int32_t shares;                     // workgroups that the key blocks are shared out to
-    unsigned long long *counts;         // workspace: shares that are done, of every unit, above them `tag`
-    unsigned long long tag;             // unique to the call
-    int32_t join_behind;                // the shares are joined by a launch of its own
-    int32_t *before;                    // workspace, for that: cost of the sequences in front of each, n_batch + 1,
-                                        // and what a unit costs beside its blocks
+    unsigned long long *counts;         // workspace: of a shared unit's shares that are done
     float *part_o;                      // workspace: [share][2][rows of a workgroup][head]
     float *part_ml;                     // workspace: [share][2][rows of a workgroup][2]
 };
@@ -71,7 +67,7 @@ int launch_paged_read(hipStream_t stream, int dtype, const PagedView &c, int hea
 int launch_paged_attend(hipStream_t stream, int dtype, PagedAttendParams &p, int head,
         void *workspace);
 // Bytes of workspace for `rows` = kv_group * q_seq query rows of a key/value head.
-size_t paged_attend_workspace_bytes(int64_t n_batch, int64_t n_head_kv, int64_t rows, int64_t head);
+size_t paged_attend_workspace_bytes(int64_t rows, int64_t head);
 int launch_rope_axes(hipStream_t stream, int dtype, bool backward, const RopeAxesParams &p);
 
 } // namespace nntile_hip

@@ -43,17 +43,15 @@ constexpr int kPagedCUs = 256;
 // Workgroups that the keys are shared out to at most: two a CU
 constexpr int kPagedShares = 2 * kPagedCUs;
 // What a unit costs beside its key blocks, in blocks
-#ifndef NNTILE_PAGED_UNIT_COST
-#define NNTILE_PAGED_UNIT_COST 1
-#endif
-constexpr int kPagedUnitCost = NNTILE_PAGED_UNIT_COST;
+constexpr int kPagedUnitCost = 1;
 // fp16 probabilities are kept times 2^14: 2^-28 of the largest still has all of its bits
 constexpr float kPagedLift = 14.0f;
-// A count of shares and the tag above it
-constexpr unsigned long long kPagedTagUnit = 4096;
-static_assert(kPagedShares < (int)kPagedTagUnit, "counts stay below the tag");
-// A value no earlier call of this process has used; its low four bits are clear.
-unsigned long long next_decode_tag();
+// Counts of shares in the workspace: in the low bits, above them a fixed word by which a count is told
+// from what else memory may hold; a cache line each.
+constexpr unsigned long long kPagedCountMask = 4095;
+constexpr unsigned long long kPagedNone = 0x9e3779b97f4a7000ull;
+constexpr int kPagedCountStride = 8;
+static_assert(kPagedShares < (int)kPagedCountMask, "counts stay below the word");
 
 enum PagedKind { kPaged16, kPaged8, kPaged32 };
 
@@ -332,13 +330,13 @@ __device__ __forceinline__ int64_t paged_query_row(const PagedAttendParams &p, i
     return (n + (int64_t)p.c.n_batch * (g + (int64_t)p.kv_group * h)) * p.q_seq + tok;
 }
 
-// Joins the shares w0 .. w0 + parts - 1 of a unit, in this order, and finishes rows first_row .. +
-// rows_here - 1 of it.  HEAD/4 threads a row; where the rows leave threads over, they take turns at the
+// Joins the shares w0 .. w0 + parts - 1 of a unit, in this order, and finishes its rows.
+// HEAD/4 threads a row; where the rows leave threads over, they take turns at the
 // shares and the sums are added up through LDS.  A thread has PARTS shares of LINES rows on their way
 // at a time: the round trips are what the join costs.
 template<typename T, int HEAD, int THREADS, int QROWS, int PARTS, int LINES>
-__device__ __forceinline__ void paged_join_by(const PagedAttendParams &p, int n, int h, int rg, int first_row,
-        int rows_here, int w0, int parts, float *lds)
+__device__ __forceinline__ void paged_join_by(const PagedAttendParams &p, int n, int h, int rg, int rows_here,
+        int w0, int parts, float *lds)
 {
     constexpr int TPR = HEAD / 4, ROWS = THREADS / TPR;
     int turns = 1;
@@ -372,7 +370,7 @@ __device__ __forceinline__ void paged_join_by(const PagedAttendParams &p, int n,
                     // (behind the last share or row: it again, with no weight)
                     const int i = min(i0 + j * turns, parts - 1);
                     const int r = min(r0 + k * step, rows_here - 1);
-                    const int64_t place = ((int64_t)(w0 + i) * 2 + (i == 0 ? 1 : 0)) * QROWS + first_row + r;
+                    const int64_t place = ((int64_t)(w0 + i) * 2 + (i == 0 ? 1 : 0)) * QROWS + r;
                     get2(p.part_ml + 2 * place, m[k][j], l[k][j]);
                     get2(p.part_o + place * HEAD + d0, x[k][j][0], x[k][j][1]);
                     get2(p.part_o + place * HEAD + d0 + 2, x[k][j][2], x[k][j][3]);
@@ -444,7 +442,7 @@ __device__ __forceinline__ void paged_join_by(const PagedAttendParams &p, int n,
             if(turn == 0 && r < rows_here)
             {
                 const float out[4] = {v[k][0], v[k][1], v[k][2], v[k][3]};
-                paged_finish_row<T>(p, HEAD, paged_query_row(p, n, h, rg * QROWS + first_row + r), d0, top[k],
+                paged_finish_row<T>(p, HEAD, paged_query_row(p, n, h, rg * QROWS + r), d0, top[k],
                         sum[k], out);
             }
         }
@@ -452,20 +450,20 @@ __device__ __forceinline__ void paged_join_by(const PagedAttendParams &p, int n,
 }
 
 template<typename T, int HEAD, int THREADS, int QROWS>
-__device__ __forceinline__ void paged_join(const PagedAttendParams &p, int n, int h, int rg, int first_row,
-        int rows_here, int w0, int parts, float *lds)
+__device__ __forceinline__ void paged_join(const PagedAttendParams &p, int n, int h, int rg, int rows_here,
+        int w0, int parts, float *lds)
 {
     if(rows_here > THREADS / (HEAD / 4) && parts <= 4)
     {
-        paged_join_by<T, HEAD, THREADS, QROWS, 4, 4>(p, n, h, rg, first_row, rows_here, w0, parts, lds);
+        paged_join_by<T, HEAD, THREADS, QROWS, 4, 4>(p, n, h, rg, rows_here, w0, parts, lds);
     }
     else if(rows_here > THREADS / (HEAD / 4))
     {
-        paged_join_by<T, HEAD, THREADS, QROWS, 8, 2>(p, n, h, rg, first_row, rows_here, w0, parts, lds);
+        paged_join_by<T, HEAD, THREADS, QROWS, 8, 2>(p, n, h, rg, rows_here, w0, parts, lds);
     }
     else
     {
-        paged_join_by<T, HEAD, THREADS, QROWS, 8, 1>(p, n, h, rg, first_row, rows_here, w0, parts, lds);
+        paged_join_by<T, HEAD, THREADS, QROWS, 8, 1>(p, n, h, rg, rows_here, w0, parts, lds);
     }
 }
 
@@ -495,7 +493,6 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     constexpr int MERGE_LD = HEAD + 4;
     constexpr int MERGE_BYTES = STREAMS * 16 * HALVES * (MERGE_LD + 2) * 4;
     static_assert(MERGE_BYTES <= Shape::RING, "the wavefronts' results of a row block share the ring");
-    static_assert(STREAMS * 64 == 256, "the merge takes 16 threads a row");
     constexpr int JOIN_ROWS = THREADS / (HEAD / 4);     // rows that are joined at a time
     static_assert(JOIN_ROWS * (HEAD + 4) * 4 <= Shape::RING, "... and so do the shares' sums");
     __shared__ __attribute__((aligned(1024))) char ring[Shape::RING];
@@ -562,21 +559,6 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         unit_cost = 0;
         total = p.c.n_batch * blocks_0;
         in_front = n_lo * blocks_0;
-    }
-    if(p.join_behind && blockIdx.x == 0 && (!in_wave || wave == 0))
-    {
-        // for the launch that joins the shares
-        int sum = in_front;
-        for(int n = n_lo; n < n_hi; ++n)
-        {
-            p.before[n] = sum;
-            sum += cost_of(blocks_of(n));
-        }
-        if(tid == 0)
-        {
-            p.before[p.c.n_batch] = total;
-            p.before[p.c.n_batch + 1] = unit_cost;
-        }
     }
     const uint32_t all = (uint32_t)total * (uint32_t)p.units;
     const PagedSplit split(all, (uint32_t)p.shares, same ? (uint32_t)blocks_0 : 0u,
@@ -845,22 +827,23 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             }
         };
 
-        // The unit's count of shares that are done starts with this call's tag, whatever the workspace
-        // holds.  Mostly it holds the 0 that earlier calls left; what else it held is seen to when the count
-        // is needed.
-        unsigned long long *const count = p.counts + ((int64_t)seg.n * p.units + seg.u);
-        unsigned long long held = 0;
-        if(tid == 0 && !p.join_behind && (seg.step > 0 || seg.steps < seg.blocks))
-        {
-            __hip_atomic_compare_exchange_strong(count, &held, p.tag, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
-                    __HIP_MEMORY_SCOPE_AGENT);
-        }
         int page[GROUPS], page_next[GROUPS];
         if(n_mine > 0)
         {
             look_up(0, page);
             fetch(0, page, slots);
             look_up(min(1, n_mine - 1), page_next);
+        }
+        // The count of the unit's shares that are done, at the place of its first share (every share is the
+        // first of one shared unit at most).  It has kPagedNone between calls; if it holds something else,
+        // the workspace is new, which is seen to where the count is needed.
+        const bool whole = seg.step == 0 && seg.steps == seg.blocks;
+        const uint32_t w0 = whole ? blockIdx.x : split.of(unit_begin);
+        unsigned long long *const count = p.counts + w0 * kPagedCountStride;
+        unsigned long long held = kPagedNone;
+        if(tid == 0 && !whole)
+        {
+            held = __hip_atomic_load(count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
         const int n_steps = PAIRED ? seg.steps : n_mine;
         auto without_page = [&]()       // groups of the step
@@ -1255,7 +1238,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         }
 
         // ---- the wavefronts' results, then the unit's or the share's ---------------------
-        const bool begins = seg.step == 0, whole = begins && seg.steps == seg.blocks;
+        const bool begins = seg.step == 0;
         const int rows_here = min(p.rows - rg * QROWS, QROWS);
         float *const merge_o = reinterpret_cast<float *>(ring);
         float *const merge_ml = merge_o + STREAMS * 16 * HALVES * MERGE_LD;
@@ -1338,35 +1321,33 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                 }
             }
         }
-        if(!whole && !p.join_behind)
+        if(!whole)
         {
             // The share's results are with the device once its stores are acknowledged, every
             // wavefront's in front of the barrier.  The workgroup that counts last joins.
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            const uint32_t w0 = split.of(unit_begin);
             const uint32_t parts = split.of(unit_begin + (uint32_t)seg.blocks - 1) - w0 + 1;
             if(tid == 0)
             {
-                if(held != 0 && (held & ~(kPagedTagUnit - 1)) != p.tag)
+                if((held & ~kPagedCountMask) != kPagedNone)
                 {
-                    // (the first share that gets here puts the tag there)
-                    __hip_atomic_compare_exchange_strong(count, &held, p.tag, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
-                            __HIP_MEMORY_SCOPE_AGENT);
+                    // (one of the shares that saw this gets its value in, before any of them counts)
+                    __hip_atomic_compare_exchange_strong(count, &held, kPagedNone, __ATOMIC_RELAXED,
+                            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
                 const unsigned long long old = __hip_atomic_fetch_add(count, 1ull, __ATOMIC_RELAXED,
                         __HIP_MEMORY_SCOPE_AGENT);
-                found = (uint32_t)(old & (kPagedTagUnit - 1)) == parts - 1;
+                found = (uint32_t)(old & kPagedCountMask) == parts - 1;
             }
             __syncthreads();
             if(uniform(found) != 0)
             {
                 if(tid == 0)
                 {
-                    // (a replay of a captured call has this tag again)
-                    __hip_atomic_store(count, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    __hip_atomic_store(count, kPagedNone, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
-                paged_join<T, HEAD, THREADS, QROWS>(p, seg.n, h, rg, 0, rows_here, (int)w0, (int)parts,
+                paged_join<T, HEAD, THREADS, QROWS>(p, seg.n, h, rg, rows_here, (int)w0, (int)parts,
                         reinterpret_cast<float *>(ring));
             }
         }
@@ -1393,70 +1374,22 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     }
 }
 
-// The join as a launch of its own, for units of more rows than one workgroup joins quickly: a
-// workgroup takes kJoinRows rows of a unit.
-constexpr int kJoinRows = 4;
-template<typename T, int HEAD, int QROWS>
-__global__ __launch_bounds__(256)
-void sdpa_paged_join_kernel(const PagedAttendParams p)
-{
-    __shared__ __attribute__((aligned(16))) float lds[256 / (HEAD / 4) * (HEAD + 4)];
-    const int first_row = (int)(blockIdx.x % (QROWS / kJoinRows)) * kJoinRows;
-    const int unit = (int)(blockIdx.x / (QROWS / kJoinRows));
-    const int n = unit / p.units, u = unit - n * p.units;
-    const int h = u / p.row_groups, rg = u - h * p.row_groups;
-    const int rows_here = min(p.rows - rg * QROWS - first_row, kJoinRows);
-    const uint32_t before = (uint32_t)p.before[n], cost = (uint32_t)p.before[n + 1] - before;
-    if(rows_here <= 0 || cost == 0)
-    {
-        return;
-    }
-    const uint32_t all = (uint32_t)p.before[p.c.n_batch] * (uint32_t)p.units;
-    const int unit_cost = p.before[p.c.n_batch + 1];
-    // (units that cost no more than their blocks: all are equally long)
-    const PagedSplit split(all, (uint32_t)p.shares, unit_cost == 0 ? cost : 0u, (uint32_t)p.c.n_batch * (uint32_t)p.units);
-    const uint32_t begin = before * (uint32_t)p.units + (uint32_t)u * cost;
-    const uint32_t w0 = split.of(begin), w1 = split.of(begin + cost - (uint32_t)unit_cost - 1);
-    if(w0 != w1)
-    {
-        paged_join<T, HEAD, 256, QROWS>(p, n, h, rg, first_row, rows_here, (int)w0, (int)(w1 - w0 + 1), lds);
-    }
-}
-
 // Blocks of 16 rows that a workgroup takes: 1, 2, or 4 by two wavefronts a key
 static int row_blocks(bool fp32, int64_t rows)
 {
     return rows <= 16 ? 1 : rows <= 32 || fp32 ? 2 : 4;
 }
 
-static size_t align16(size_t x)
-{
-    return (x + 15) & ~(size_t)15;
-}
-
-// The workspace: a count per unit, the sequences' blocks, the shares' results.  (The larger of the types' sizes,
-// which differ in the rows of a workgroup.)
-static size_t count_bytes(int64_t n_batch, int64_t n_head_kv, int64_t rows)
-{
-    const int64_t of_16bit = 16 * row_blocks(false, rows), of_fp32 = 16 * row_blocks(true, rows);
-    const int64_t groups = (rows + (of_16bit < of_fp32 ? of_16bit : of_fp32) - 1)
-        / (of_16bit < of_fp32 ? of_16bit : of_fp32);
-    return align16(8 * (size_t)(n_batch * n_head_kv) * (size_t)groups);
-}
-
-static size_t before_bytes(int64_t n_batch)
-{
-    return align16(4 * ((size_t)n_batch + 2));
-}
-
+// The workspace: the counts, then the shares' results (the larger size of the types', which differ in
+// the rows of a workgroup).
 static size_t share_rows(int64_t rows)
 {
     return (size_t)kPagedShares * 2 * 16 * (size_t)row_blocks(false, rows);
 }
 
-size_t paged_attend_workspace_bytes(int64_t n_batch, int64_t n_head_kv, int64_t rows, int64_t head)
+size_t paged_attend_workspace_bytes(int64_t rows, int64_t head)
 {
-    return count_bytes(n_batch, n_head_kv, rows) + before_bytes(n_batch) + share_rows(rows) * (size_t)(head + 2) * 4;
+    return sizeof(unsigned long long) * kPagedShares * kPagedCountStride + share_rows(rows) * (size_t)(head + 2) * 4;
 }
 
 template<typename T, int KIND, int HEAD, int NR, int HALVES>
@@ -1467,25 +1400,14 @@ static int launch_form(hipStream_t stream, PagedAttendParams &p)
     p.units = p.c.n_head_kv * p.row_groups;
     // at most as many shares as there can be blocks
     const int64_t most = (int64_t)p.c.n_batch * p.units * (p.c.max_rows / Shape::BLOCK + 1 + kPagedUnitCost);
-    if(most > 0x7fffffffll / (Shape::QROWS / kJoinRows))
+    if(most > 0x7fffffffll)
     {
         return NNTILE_HIP_EINVAL;
     }
     const int64_t places = kPagedCUs * Shape::WGS_PER_CU;
     p.shares = (int32_t)(most < places ? most : places);
-    // (one workgroup would read the shares of 32 or 64 rows for as long as a launch takes, or longer)
-#ifndef NNTILE_PAGED_JOIN
-#define NNTILE_PAGED_JOIN 0
-#endif
-    p.join_behind = NNTILE_PAGED_JOIN && Shape::QROWS > 16;
-    p.tag = next_decode_tag() * (kPagedTagUnit / 16);
     hipLaunchKernelGGL((sdpa_paged_kernel<T, KIND, HEAD, NR, HALVES>), dim3((unsigned)p.shares),
             dim3(Shape::THREADS), 0, stream, p);
-    if(p.join_behind)
-    {
-        hipLaunchKernelGGL((sdpa_paged_join_kernel<T, HEAD, Shape::QROWS>),
-                dim3((unsigned)(p.c.n_batch * p.units * (Shape::QROWS / kJoinRows))), dim3(256), 0, stream, p);
-    }
     return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;
 }
 
@@ -1509,10 +1431,8 @@ static int launch_kind(hipStream_t stream, PagedAttendParams &p, int head)
 
 int launch_paged_attend(hipStream_t stream, int dtype, PagedAttendParams &p, int head, void *workspace)
 {
-    const size_t counts = count_bytes(p.c.n_batch, p.c.n_head_kv, p.rows);
     p.counts = static_cast<unsigned long long *>(workspace);
-    p.before = reinterpret_cast<int32_t *>(static_cast<char *>(workspace) + counts);
-    p.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + counts + before_bytes(p.c.n_batch));
+    p.part_o = reinterpret_cast<float *>(p.counts + kPagedShares * kPagedCountStride);
     p.part_ml = p.part_o + share_rows(p.rows) * (size_t)head;
     if(p.c.k_scales != nullptr)
     {
