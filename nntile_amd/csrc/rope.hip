@@ -21,34 +21,15 @@
 // bf16, one and two columns a thread: 2 x 65536 x 64 (33.6 MB) 7.3 and 6.9 us =
 // 4.9 TB/s, 2 x 65536 x 256 24.0 and 22.3 = 6.0 TB/s; fp32 2 x 65536 x 256 55.1 and
 // 52.6.
+#include "fixed_divide.hpp"
 #include "rope_common.hpp"
 
 namespace nntile_hip
 {
 
-// Quotients of numbers below 2^31 by a fixed divisor: a multiplication by
-// 2^32 (2^shift - by) / by + 1, rounded down, an addition and a shift, exact
-// for every such number (Granlund and Montgomery 1994, theorem 4.2 with N = 32).
-struct RopeDivide
-{
-    uint32_t by, factor, shift;
-    explicit RopeDivide(uint32_t d) : by(d), factor(0), shift(0)
-    {
-        while((1ull << shift) < d)
-        {
-            ++shift;
-        }
-        factor = (uint32_t)((((1ull << shift) - d) << 32) / d + 1);
-    }
-    __device__ __forceinline__ uint32_t quotient(uint32_t t) const
-    {
-        return (__umulhi(t, factor) + t) >> shift;
-    }
-};
-
 template<typename S, bool BACKWARD, int COLS>
 __global__ __launch_bounds__(256)
-void rope_vec_kernel(int64_t m, int n, RopeDivide per_col, const typename S::storage *sin,
+void rope_vec_kernel(int64_t m, int n, FixedDivide per_col, const typename S::storage *sin,
         const typename S::storage *cos, const typename S::storage *src,
         typename S::storage *dst)
 {
@@ -166,7 +147,7 @@ static int launch_rope_typed(hipStream_t stream, int64_t m, int64_t n, const voi
         const bool many = (pairs / 4 + 511) / 512 >= 2048 && 2 * m * (int64_t)sizeof(E) % 128 == 0;
         const int64_t threads = per_col * (many ? (n + 1) / 2 : n);
         const dim3 grid((unsigned)((threads + 255) / 256));
-        const RopeDivide divide((uint32_t)per_col);
+        const FixedDivide divide((uint32_t)per_col);
         if(many)
         {
             hipLaunchKernelGGL((rope_vec_kernel<S, BACKWARD, 2>), grid, dim3(256), 0, stream, m,
