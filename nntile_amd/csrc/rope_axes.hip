@@ -9,9 +9,15 @@
 // The angle is taken in 64 bits and reduced there to less than half a turn: at position
 // 100000 its fp32 product would be off by 0.004 radians.  What is left of it, up to one turn,
 // loses 2^-25 of a turn in fp32 at most; sine and cosine of it are those of the device
-// library.  A thread takes
+// library (the hardware's own, less exact, took as long).  A thread takes
 // four pairs of a token (16 bytes of a 16-bit tensor, 32 of an fp32 one) of HEADS heads and
-// computes their sines and cosines once.
+// computes their sines and cosines once; tokens are numbered through all sequences, whose rows of a
+// head lie behind each other.
+//
+// Bound by HBM where it is large: 4096 tokens of 32 + 8 heads of 128 in bf16, 84 MB, 16.0 us = 5.2 TB/s
+// (17.9 with four heads a thread, 24.1 with two: the sines and cosines are a thread's larger part then);
+// 8192 tokens 28.4 us = 5.9 TB/s.
+#include "fixed_divide.hpp"
 #include "paged.hpp"
 #include "rope_common.hpp"
 
@@ -31,27 +37,26 @@ __device__ __forceinline__ int64_t position_on(const RopeAxesParams &p, int axis
     return axis >= 0 && axis < p.n_axes ? p.positions[axis * p.pos_axis_stride + at] : 0;
 }
 
-// Four pairs a thread.  Threads go along the tokens of a sequence (contiguous for a given
-// head), blockIdx.y over sequences and groups of HEADS heads.
-template<typename S, bool BACKWARD, int HEADS>
+// Four pairs a thread; blockIdx.y over groups of HEADS heads.  STREAM: loads that leave the caches alone.
+template<typename S, bool BACKWARD, int HEADS, bool STREAM>
 __global__ __launch_bounds__(256)
-void rope_axes_vec_kernel(const RopeAxesParams p)
+void rope_axes_vec_kernel(const RopeAxesParams p, const FixedDivide per_row, const FixedDivide per_seq)
 {
     typedef typename S::storage E;
     constexpr int NV = (int)sizeof(E) / 2;      // 16-byte pieces of four pairs
-    const int per_row = (int)(p.head / 8);
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if(t >= p.seq * per_row)
+    const uint32_t tokens = per_seq.by * (uint32_t)p.n_batch;
+    const uint32_t t = blockIdx.x * 256u + threadIdx.x;
+    const uint32_t token = per_row.quotient(t);
+    if(token >= tokens)
     {
         return;
     }
-    const int64_t token = t / per_row;
-    const int i = 4 * (int)(t - token * per_row);
-    const int n = (int)(blockIdx.y % p.n_batch);
-    const int h0 = (int)(blockIdx.y / p.n_batch) * HEADS;
+    const int i = 4 * (int)(t - token * per_row.by);
+    const uint32_t at = p.pos_batch_stride != 0 ? token : token - per_seq.quotient(token) * per_seq.by;
+    const int h0 = (int)blockIdx.y * HEADS;
     const int heads = (int)(p.heads_q + p.heads_k);
-    const int64_t entry = p.seq * p.head;
-    const int64_t in_row = token * p.head + 2 * i;
+    const int64_t of_head = (int64_t)tokens * p.head;
+    const int64_t in_head = (int64_t)token * p.head + 2 * i;
     u32x4 raw[HEADS][NV];
 #pragma unroll
     for(int j = 0; j < HEADS; ++j)
@@ -59,20 +64,19 @@ void rope_axes_vec_kernel(const RopeAxesParams p)
         // (heads past the last re-read it)
         const int h = min(h0 + j, heads - 1);
         const bool key = h >= p.heads_q;
-        const E *from = static_cast<const E *>(key ? p.k : p.q)
-            + ((key ? h - p.heads_q : h) * p.n_batch + n) * entry + in_row;
+        const u32x4 *from = reinterpret_cast<const u32x4 *>(static_cast<const E *>(key ? p.k : p.q)
+                + (key ? h - p.heads_q : h) * of_head + in_head);
 #pragma unroll
         for(int v = 0; v < NV; ++v)
         {
-            raw[j][v] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(from) + v);
+            raw[j][v] = STREAM ? __builtin_nontemporal_load(from + v) : from[v];
         }
     }
     float s[4], c[4];
 #pragma unroll
     for(int k = 0; k < 4; ++k)
     {
-        turn_of(position_on(p, p.axes[i + k], n * p.pos_batch_stride + token), p.freqs[i + k], s[k],
-                c[k]);
+        turn_of(position_on(p, p.axes[i + k], at), p.freqs[i + k], s[k], c[k]);
     }
 #pragma unroll
     for(int j = 0; j < HEADS; ++j)
@@ -96,8 +100,7 @@ void rope_axes_vec_kernel(const RopeAxesParams p)
         if(h < heads)
         {
             const bool key = h >= p.heads_q;
-            E *to = static_cast<E *>(key ? p.k_out : p.q_out)
-                + ((key ? h - p.heads_q : h) * p.n_batch + n) * entry + in_row;
+            E *to = static_cast<E *>(key ? p.k_out : p.q_out) + (key ? h - p.heads_q : h) * of_head + in_head;
 #pragma unroll
             for(int v = 0; v < NV; ++v)
             {
@@ -137,30 +140,51 @@ void rope_axes_pair_kernel(const RopeAxesParams p, int64_t pairs)
     to[1] = S::from_float(y);
 }
 
+template<typename S, bool BACKWARD, int HEADS, bool STREAM>
+static int launch_vec(hipStream_t stream, const RopeAxesParams &p, int64_t blocks_x)
+{
+    const int64_t heads = p.heads_q + p.heads_k;
+    hipLaunchKernelGGL((rope_axes_vec_kernel<S, BACKWARD, HEADS, STREAM>),
+            dim3((unsigned)blocks_x, (unsigned)((heads + HEADS - 1) / HEADS)), dim3(256), 0, stream, p,
+            FixedDivide((uint32_t)(p.head / 8)), FixedDivide((uint32_t)p.seq));
+    return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;
+}
+
 template<typename S, bool BACKWARD>
 static int launch_typed(hipStream_t stream, const RopeAxesParams &p)
 {
     auto aligned = [](const void *x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+    constexpr int64_t E = sizeof(typename S::storage);
     const int64_t heads = p.heads_q + p.heads_k;
-    const int64_t blocks_x = (p.seq * (p.head / 8) + 255) / 256;
-    constexpr int HEADS = 4;
-    const int64_t blocks_y = p.n_batch * ((heads + HEADS - 1) / HEADS);
+    // (a thread's number fits 31 bits)
     if(p.head % 8 == 0 && aligned(p.q) && aligned(p.q_out) && aligned(p.k) && aligned(p.k_out)
-            && blocks_x <= 0x7fffffff && blocks_y <= 65535)
+            && heads <= 2 * 65535 && p.n_batch <= 0x7fffff00 / p.seq / (p.head / 8))
     {
-        hipLaunchKernelGGL((rope_axes_vec_kernel<S, BACKWARD, HEADS>),
-                dim3((unsigned)blocks_x, (unsigned)blocks_y), dim3(256), 0, stream, p);
-    }
-    else
-    {
-        const int64_t pairs = heads * p.n_batch * p.seq * (p.head / 2);
-        if((pairs + 255) / 256 > 0x7fffffff)
+        const int64_t blocks_x = (p.n_batch * p.seq * (p.head / 8) + 255) / 256;
+        // Eight heads a thread where that leaves every CU a workgroup, else two (one token of eight
+        // sequences 4.7 us, so 3.7; 64 of them 5.6 and 3.8).
+        if(blocks_x * ((heads + 7) / 8) < 256)
         {
-            return NNTILE_HIP_EINVAL;
+            return launch_vec<S, BACKWARD, 2, false>(stream, p, blocks_x);
         }
-        hipLaunchKernelGGL((rope_axes_pair_kernel<S, BACKWARD>), dim3((unsigned)((pairs + 255) / 256)),
-                dim3(256), 0, stream, p, pairs);
+        // Large fp32 tensors: four, past the caches.  (49 MB of 24 heads 10.2 us with eight, 12.2 so;
+        // 201 MB 56 and 43: eight streams in and eight out, 4 MB apart.)
+        if constexpr(E == 4)
+        {
+            if(p.n_batch * p.seq * p.head * heads * E * 2 >= 128ll << 20)
+            {
+                return launch_vec<S, BACKWARD, 4, true>(stream, p, blocks_x);
+            }
+        }
+        return launch_vec<S, BACKWARD, 8, false>(stream, p, blocks_x);
     }
+    const int64_t pairs = heads * p.n_batch * p.seq * (p.head / 2);
+    if((pairs + 255) / 256 > 0x7fffffff)
+    {
+        return NNTILE_HIP_EINVAL;
+    }
+    hipLaunchKernelGGL((rope_axes_pair_kernel<S, BACKWARD>), dim3((unsigned)((pairs + 255) / 256)),
+            dim3(256), 0, stream, p, pairs);
     return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;
 }
 
