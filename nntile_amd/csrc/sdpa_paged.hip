@@ -44,8 +44,10 @@ constexpr int kPagedCUs = 256;
 constexpr int kPagedShares = 2 * kPagedCUs;
 // What a unit costs beside its key blocks, in blocks
 constexpr int kPagedUnitCost = 1;
-// fp16 probabilities are kept times 2^14: 2^-28 of the largest still has all of its bits
-constexpr float kPagedLift = 14.0f;
+// How far, in powers of two, probabilities may grow past 1 before they are taken against a new maximum
+constexpr float kPagedSlack = 8.0f;
+// fp16 probabilities are kept times 2^7: they stay below 2^15, and 2^-21 still has all of its bits
+constexpr float kPagedLift = 7.0f;
 // Counts of shares in the workspace: in the low bits, above them a fixed word by which a count is told
 // from what else memory may hold; a cache line each.
 constexpr unsigned long long kPagedCountMask = 4095;
@@ -679,7 +681,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             v_at[db] = (uint32_t)(K_BYTES + r * RB + ((d >> 2) ^ Shape::v_swizzle(r)) * 16 + 4 * (d & 3));
         }
     }
-    const float c_log2 = p.scale * kLog2e;
+    const float c_log2 = p.scale * kLog2e, slack = kPagedSlack / c_log2;
 
     for(;;)
     {
@@ -975,7 +977,6 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             // ---- probabilities -------------------------------------------------------
             // 8-bit pages: what a probability is multiplied by for its value row's power of two
             f32x4 of_scale[GROUPS];
-            float fade_scale = 1.0f;
             if constexpr(KIND == kPaged8)
             {
                 float most = top_scale;
@@ -994,15 +995,27 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                 if constexpr(RANGED)
                 {
                     most = quad_max(most);
-                    fade_scale = fast_exp2(top_scale - most);
-                    top_scale = most;
+                    if(__any(most > top_scale))
+                    {
+                        const float fade = fast_exp2(top_scale - most);
+                        top_scale = most;
+#pragma unroll
+                        for(int nr = 0; nr < NR; ++nr)
+                        {
+#pragma unroll
+                            for(int db = 0; db < DBLOCKS; ++db)
+                            {
+                                o[nr][db] *= fade;
+                            }
+                        }
+                    }
 #pragma unroll
                     for(int g = 0; g < GROUPS; ++g)
                     {
 #pragma unroll
                         for(int e = 0; e < 4; ++e)
                         {
-                            of_scale[g][e] = fast_exp2(of_scale[g][e] - (most - kPagedLift));
+                            of_scale[g][e] = fast_exp2(of_scale[g][e] - (top_scale - kPagedLift));
                         }
                     }
                 }
@@ -1012,7 +1025,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
 #pragma unroll
             for(int nr = 0; nr < NR; ++nr)
             {
-                float top = m_run[nr];
+                float top = neg_inf();
 #pragma unroll
                 for(int g = 0; g < GROUPS; ++g)
                 {
@@ -1033,12 +1046,24 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                         top = fmaxf(top, x);
                     }
                 }
-                // p = 2^(c * score - c * maximum): c is positive, and the product with the
-                // maximum is rounded the same way wherever it is taken
-                const float m_new = quad_max(top);
-                const float mc = m_new == neg_inf() ? 0.0f : m_new * c_log2;
-                const float fade = fast_exp2(m_run[nr] * c_log2 - mc);
-                const float off = kLift - mc;
+                // p = 2^(c * score - c * reference): c is positive, and the product with the
+                // reference is rounded the same way wherever it is taken.  The reference is a
+                // maximum that is replaced once the scores are 2^kPagedSlack past it, so that sums and
+                // products are seldom scaled.
+                top = quad_max(top);
+                if(__any(top > m_run[nr] + slack))
+                {
+                    const float m_new = top > m_run[nr] + slack ? top : m_run[nr];
+                    const float fade = fast_exp2(m_run[nr] * c_log2 - (m_new == neg_inf() ? 0.0f : m_new * c_log2));
+                    l_run[nr] *= fade;
+                    m_run[nr] = m_new;
+#pragma unroll
+                    for(int db = 0; db < DBLOCKS; ++db)
+                    {
+                        o[nr][db] *= fade;
+                    }
+                }
+                const float off = kLift - (m_run[nr] == neg_inf() ? 0.0f : m_run[nr] * c_log2);
                 float sum = 0.0f;
 #pragma unroll
                 for(int g = 0; g < GROUPS; ++g)
@@ -1068,17 +1093,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                         pw[nr][g][1] = PV::pack2(x[2], x[3]);
                     }
                 }
-                l_run[nr] = l_run[nr] * fade + sum;
-                m_run[nr] = m_new;
-                const float fade_o = fade * fade_scale;
-                if(__any(fade_o != 1.0f))
-                {
-#pragma unroll
-                    for(int db = 0; db < DBLOCKS; ++db)
-                    {
-                        o[nr][db] *= fade_o;
-                    }
-                }
+                l_run[nr] += sum;
             }
 
             // ---- output ----------------------------------------------------------------
