@@ -818,23 +818,34 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                 }
             }
         };
-        // the scale bytes of keys 16g + 4 * which .. + 3
-        auto scales = [&](const uint8_t *of, int which, int i, const int (&page)[GROUPS], uint32_t (&out)[GROUPS])
+        // the scale bytes of a step, through the scalar cache, and those of keys 16g + 4 * which .. + 3 of it
+        auto load_scales = [&](int i, const int (&page)[GROUPS], u32x4 (&k)[GROUPS], u32x4 (&v)[GROUPS])
         {
 #pragma unroll
             for(int g = 0; g < GROUPS; ++g)
             {
-                const u32x4 w = scalar_load<u32x4>(of, real_page(page[g]) * p.c.scale_stride + in_page(i, g));
-                out[g] = which == 0 ? w[0] : which == 1 ? w[1] : which == 2 ? w[2] : w[3];
+                const int64_t at_row = real_page(page[g]) * p.c.scale_stride + in_page(i, g);
+                k[g] = scalar_load<u32x4>(p.c.k_scales, at_row);
+                v[g] = scalar_load<u32x4>(p.c.v_scales, at_row);
             }
+        };
+        auto of_lane = [&](const u32x4 &w, int which)
+        {
+            return which == 0 ? w[0] : which == 1 ? w[1] : which == 2 ? w[2] : w[3];
         };
 
         int page[GROUPS], page_next[GROUPS];
+        constexpr int SCALES = KIND == kPaged8 ? GROUPS : 1;
+        u32x4 k_raw[SCALES], v_raw[SCALES];     // of the next step
         if(n_mine > 0)
         {
             look_up(0, page);
             fetch(0, page, slots);
             look_up(min(1, n_mine - 1), page_next);
+            if constexpr(KIND == kPaged8)
+            {
+                load_scales(0, page, k_raw, v_raw);
+            }
         }
         // The count of the unit's shares that are done, at the place of its first share (every share is the
         // first of one shared unit at most).  It has kPagedNone between calls; if it holds something else,
@@ -869,21 +880,20 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             {
                 if constexpr(KIND == kPaged8)
                 {
-                    scales(p.c.k_scales, KSCALE_IN_CODES ? col >> 2 : quad, i, page, ks);
-                    scales(p.c.v_scales, quad, i, page, vs);
+#pragma unroll
+                    for(int g = 0; g < GROUPS; ++g)
+                    {
+                        ks[g] = of_lane(k_raw[g], KSCALE_IN_CODES ? col >> 2 : quad);
+                        vs[g] = of_lane(v_raw[g], quad);
+                    }
                 }
                 hidden = PARTLY ? without_page() : 0;
             }
+            // the reads of the slot that is filled next have returned (to both)
+            paged_wait_lds();
             if constexpr(PAIRED)
             {
-                // both have loaded their half of this step, and are done with the slot filled next
-                paged_wait_loads<0>();
                 __syncthreads();
-            }
-            else
-            {
-                // the reads of the slot that is filled next have returned
-                paged_wait_lds();
             }
             if(i + 1 < n_mine)
             {
@@ -894,14 +904,19 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                     page[g] = page_next[g];
                 }
                 look_up(min(i + 2, n_mine - 1), page_next);
-                if constexpr(!PAIRED)
+                if constexpr(KIND == kPaged8)
                 {
-                    paged_wait_loads<2 * LOADS>();
+                    load_scales(i + 1, page, k_raw, v_raw);
                 }
+                paged_wait_loads<PAIRED ? LOADS : 2 * LOADS>();
             }
-            else if constexpr(!PAIRED)
+            else
             {
                 paged_wait_loads<0>();
+            }
+            if constexpr(PAIRED)
+            {
+                __syncthreads();        // both have loaded their half of this step
             }
             if(PARTLY && PAIRED && i >= n_mine)
             {
