@@ -188,11 +188,23 @@ template<typename T> __device__ __forceinline__ u32x2 widen4(uint32_t codes, flo
     }
 }
 
-// Whether a word of two 16-bit values holds a NaN or an infinity
-template<typename T> __device__ __forceinline__ bool not_finite2(uint32_t w)
+// Whether a word of a page - two 16-bit values, four codes or an fp32 value - holds a NaN or an infinity
+template<typename T, int KIND> __device__ __forceinline__ bool not_numbers(uint32_t w)
 {
-    constexpr uint32_t E = __is_same(T, Bf16) ? 0x7f80u : 0x7c00u;
-    return (w & E) == E || ((w >> 16) & E) == E;
+    if constexpr(KIND == kPaged32)
+    {
+        return (w & 0x7f800000u) == 0x7f800000u;
+    }
+    else if constexpr(KIND == kPaged8)
+    {
+        // a code of all ones behind its sign: adding 1 to it carries into the sign's place
+        return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+    }
+    else
+    {
+        constexpr uint32_t E = __is_same(T, Bf16) ? 0x7f80u : 0x7c00u;
+        return (w & E) == E || ((w >> 16) & E) == E;
+    }
 }
 
 // What a workgroup works on at a time: key blocks [step, step + steps) of unit u (head and row
@@ -203,38 +215,17 @@ struct PagedSegment
     int u, step, steps;
 };
 
-// Share w of the blocks: [begin(w), begin(w + 1)); the share that has a block.  The blocks come in periods
-// of equal length - a unit where all units are equally long and each gets shares of its own, else
-// all blocks - that as many shares divide.
+// Share w of `all` blocks: [begin(w), begin(w + 1)); the share that has a block.
 struct PagedSplit
 {
-    uint32_t period, per_period, shares;
-    uint32_t base, rest;    // of a period the first `rest` shares take one block more
-    __device__ __forceinline__ PagedSplit(uint32_t all, uint32_t places, uint32_t unit_blocks, uint32_t units)
-    {
-        period = all;
-        per_period = min(places, all);
-        shares = per_period;
-        if(unit_blocks != 0 && units <= places)
-        {
-            // as few shares as keep the longest as short as it can be
-            const uint32_t longest = (unit_blocks + places / units - 1) / (places / units);
-            period = unit_blocks;
-            per_period = (unit_blocks + longest - 1) / longest;
-            shares = units * per_period;
-        }
-        base = per_period != 0 ? period / per_period : 0;
-        rest = per_period != 0 ? period % per_period : 0;
-    }
-    __device__ __forceinline__ uint32_t begin(uint32_t w) const
-    {
-        const uint32_t q = w / per_period, r = w - q * per_period;
-        return q * period + r * base + min(r, rest);
-    }
+    uint32_t base, rest;    // the first `rest` shares take one block more
+    __device__ __forceinline__ PagedSplit(uint32_t all, uint32_t shares)
+        : base(shares != 0 ? all / shares : 0), rest(shares != 0 ? all % shares : 0) {}
+    __device__ __forceinline__ uint32_t begin(uint32_t w) const { return w * base + min(w, rest); }
     __device__ __forceinline__ uint32_t of(uint32_t block) const
     {
-        const uint32_t q = block / period, r = block - q * period, longer = rest * (base + 1);
-        return q * per_period + (r < longer ? r / (base + 1) : rest + (r - longer) / base);
+        const uint32_t longer = rest * (base + 1);
+        return block < longer ? block / (base + 1) : rest + (block - longer) / base;
     }
 };
 
@@ -563,8 +554,46 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         in_front = n_lo * blocks_0;
     }
     const uint32_t all = (uint32_t)total * (uint32_t)p.units;
-    const PagedSplit split(all, (uint32_t)p.shares, same ? (uint32_t)blocks_0 : 0u,
-            (uint32_t)p.c.n_batch * (uint32_t)p.units);
+    // Shares of whole units: every unit gets as many as keep each to `longest` blocks, if the workgroups
+    // are enough for that.  A share that ends one unit and begins another costs about two blocks more
+    // than one that does not, so this is done where the longest is no more than that above the
+    // even run, and always where all units are equally long (16 drafted sequences of 300 to 4096 8-bit
+    // rows 21.3 -> 17 us).
+    const uint32_t n_units = (uint32_t)p.c.n_batch * (uint32_t)p.units, places = (uint32_t)p.shares;
+    int of_unit = 0, of_units = 0, shares_in_front = 0;     // shares of the lane's units; of all; in front of its own
+    if(same && n_units <= places && blocks_0 != 0)
+    {
+        const int most = (int)(places / n_units), longest = (blocks_0 + most - 1) / most;
+        of_unit = (blocks_0 + longest - 1) / longest;
+        of_units = p.c.n_batch * of_unit;
+        shares_in_front = n_lo * of_unit;
+    }
+    else if(in_wave && !same && total != 0)
+    {
+        const int even = (int)((all + places - 1) / places);
+        const int b = n_lo < n_hi ? blocks_of(n_lo) : 0;
+        for(int longest = max(even - 1, 1); longest <= even + 2 && of_units == 0; ++longest)
+        {
+            const int k = (b + longest - 1) / longest;
+            int sum = k;
+#pragma unroll
+            for(int o = 1; o < 64; o <<= 1)
+            {
+                const int other = __shfl_up(sum, o);
+                sum += lane >= o ? other : 0;
+            }
+            const int everyone = __builtin_amdgcn_readlane(sum, 63);
+            if((uint32_t)everyone * (uint32_t)p.units <= places)
+            {
+                of_unit = k;
+                of_units = everyone;
+                shares_in_front = sum - k;
+            }
+        }
+    }
+    const bool aligned = of_units != 0;
+    const uint32_t shares = aligned ? (uint32_t)of_units * (uint32_t)p.units : min(places, all);
+    const PagedSplit split(all, shares);
     // sequences without rows: shared out, too, for the rows of their queries
     if(p.overwrite && !(same && blocks_0 != 0))
     {
@@ -583,28 +612,30 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             }
         }
     }
-    if(blockIdx.x >= split.shares)
+    if(blockIdx.x >= shares)
     {
         return;
     }
     uint32_t at = split.begin(blockIdx.x);
     const uint32_t end = split.begin(blockIdx.x + 1);
     PagedSegment seg;
+    uint32_t first_share = blockIdx.x, parts_of_unit = 1;       // where shares are of whole units
     {
-        // the last lane whose sequences begin at or before the block, then sequence by sequence
-        const int block = (int)(at / (uint32_t)p.units);
+        // the last lane whose sequences begin at or before the block or share, then sequence by sequence
+        const int what = aligned ? (int)(blockIdx.x / (uint32_t)p.units) : (int)(at / (uint32_t)p.units);
+        const int front = aligned ? shares_in_front : in_front;
         int t, before;
         if(in_wave)
         {
-            t = __popcll(__ballot(scanner * chunk < p.c.n_batch && in_front <= block)) - 1;
-            before = __builtin_amdgcn_readlane(in_front, t);
+            t = __popcll(__ballot(scanner * chunk < p.c.n_batch && front <= what)) - 1;
+            before = __builtin_amdgcn_readlane(front, t);
         }
         else
         {
-            scan_of[tid] = in_front;
+            scan_of[tid] = front;
             __syncthreads();
-            const bool here = tid * chunk < p.c.n_batch && in_front <= block
-                && (tid == THREADS - 1 || (tid + 1) * chunk >= p.c.n_batch || scan_of[tid + 1] > block);
+            const bool here = tid * chunk < p.c.n_batch && front <= what
+                && (tid == THREADS - 1 || (tid + 1) * chunk >= p.c.n_batch || scan_of[tid + 1] > what);
             if(here)
             {
                 found = tid;
@@ -614,20 +645,36 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             before = uniform(scan_of[t]);
         }
         seg.n = t * chunk;
+        const int parts = __builtin_amdgcn_readlane(of_unit, in_wave ? t : 0);
         for(;;)
         {
             seg.len = uniform(paged_len(p.c, seg.n));
             seg.blocks = (seg.len + Shape::BLOCK - 1) / Shape::BLOCK;
-            if(before + cost_of(seg.blocks) > block || seg.n + 1 >= p.c.n_batch)
+            const int here = aligned ? parts : cost_of(seg.blocks);
+            if(before + here > what || seg.n + 1 >= p.c.n_batch)
             {
                 break;
             }
-            before += cost_of(seg.blocks);
+            before += here;
             ++seg.n;
         }
-        const uint32_t rest = at - (uint32_t)before * (uint32_t)p.units;
-        seg.u = uniform((int)(rest / (uint32_t)cost_of(seg.blocks)));
-        seg.step = uniform((int)(rest % (uint32_t)cost_of(seg.blocks)));
+        if(aligned)
+        {
+            const uint32_t rest = blockIdx.x - (uint32_t)before * (uint32_t)p.units;
+            parts_of_unit = (uint32_t)parts;
+            seg.u = uniform((int)(rest / parts_of_unit));
+            const uint32_t part = rest - (uint32_t)seg.u * parts_of_unit;
+            const PagedSplit of_blocks((uint32_t)seg.blocks, parts_of_unit);
+            first_share = blockIdx.x - part;
+            seg.step = uniform((int)of_blocks.begin(part));
+            seg.steps = uniform((int)of_blocks.begin(part + 1)) - seg.step;
+        }
+        else
+        {
+            const uint32_t rest = at - (uint32_t)before * (uint32_t)p.units;
+            seg.u = uniform((int)(rest / (uint32_t)cost_of(seg.blocks)));
+            seg.step = uniform((int)(rest % (uint32_t)cost_of(seg.blocks)));
+        }
     }
     uint32_t unit_begin = at - (uint32_t)seg.step;      // of the unit's first block among all
 
@@ -685,9 +732,13 @@ void sdpa_paged_kernel(const PagedAttendParams p)
 
     for(;;)
     {
-        // (the last place of a unit has no block: seg.steps may be 0)
-        seg.steps = (int)min((uint32_t)max(seg.blocks - seg.step, 0), end - at);
-        const uint32_t taken = min((uint32_t)(cost_of(seg.blocks) - seg.step), end - at);
+        uint32_t taken = 0;
+        if(!aligned)
+        {
+            // (the last place of a unit has no block: seg.steps may be 0)
+            seg.steps = (int)min((uint32_t)max(seg.blocks - seg.step, 0), end - at);
+            taken = min((uint32_t)(cost_of(seg.blocks) - seg.step), end - at);
+        }
         if(seg.steps > 0)
         {
         const int h = seg.u / p.row_groups, rg = seg.u - h * p.row_groups;
@@ -716,7 +767,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             const int rr = rg * QROWS + (half * NR + nr) * 16 + col;
             token[nr] = rr % p.q_seq;
             row_ok[nr] = rr < p.rows && token[nr] < given;
-            last[nr] = p.causal ? seg.len - given + token[nr] : seg.len - 1;
+            last[nr] = min(p.causal ? seg.len - given + token[nr] : seg.len - 1, seg.len - 1);
         }
         if constexpr(Q_IN_LDS)
         {
@@ -776,16 +827,24 @@ void sdpa_paged_kernel(const PagedAttendParams p)
 
         // ---- pages and loads ------------------------------------------------------------
         const int64_t table_row = (int64_t)seg.n * p.c.max_pages;
+        // Where a page holds a step, its groups lie behind each other in one page: one look-up, one address.
+        const bool one_page = (1 << p.c.page_shift) >= KEYS;
         auto look_up = [&](int i, int (&page)[GROUPS])
         {
-#pragma unroll
-            for(int g = 0; g < GROUPS; ++g)
+            const int row0 = my_first + i * Shape::BLOCK;
+            page[0] = scalar_load<int>(p.c.table, 4 * (table_row + (row0 >> p.c.page_shift)));
+            if(GROUPS > 1 && !one_page)
             {
-                // (groups behind the last row take the page of the last)
-                const int row = min(my_first + i * Shape::BLOCK + 16 * g, seg.len - 1);
-                page[g] = scalar_load<int>(p.c.table, 4 * (table_row + (row >> p.c.page_shift)));
+#pragma unroll
+                for(int g = 1; g < GROUPS; ++g)
+                {
+                    // (groups behind the last row take the page of the last)
+                    const int row = min(row0 + 16 * g, seg.len - 1);
+                    page[g] = scalar_load<int>(p.c.table, 4 * (table_row + (row >> p.c.page_shift)));
+                }
             }
         };
+        // the row of group g among those of the pages' heads
         auto in_page = [&](int i, int g)
         {
             const int row = min(my_first + i * Shape::BLOCK + 16 * g, seg.len - 1) & ~15;
@@ -793,14 +852,31 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         };
         // (a page that is none is read as page 0 and hidden)
         auto real_page = [&](int page) { return (unsigned)page < (unsigned)p.c.n_pages ? page : 0; };
+        // where the groups of a step lie in a pool of rows of `bytes`, `stride` from page to page
+        auto places = [&](int i, const int (&page)[GROUPS], int64_t stride, int bytes, int64_t (&from)[GROUPS])
+        {
+            from[0] = real_page(page[0]) * stride + in_page(i, 0) * bytes;
+            if(GROUPS == 1 || one_page)
+            {
+#pragma unroll
+                for(int g = 1; g < GROUPS; ++g)
+                {
+                    from[g] = from[0] + 16 * g * bytes;
+                }
+            }
+            else
+            {
+#pragma unroll
+                for(int g = 1; g < GROUPS; ++g)
+                {
+                    from[g] = real_page(page[g]) * stride + in_page(i, g) * bytes;
+                }
+            }
+        };
         auto fetch = [&](int i, const int (&page)[GROUPS], char *slot)
         {
             int64_t from[GROUPS];
-#pragma unroll
-            for(int g = 0; g < GROUPS; ++g)
-            {
-                from[g] = real_page(page[g]) * p.c.page_stride + in_page(i, g) * RB;
-            }
+            places(i, page, p.c.page_stride, RB, from);
             const char *const first = PAIRED && half == 1 ? p.c.v_pages : p.c.k_pages;
             char *const to = PAIRED && half == 1 ? slot + K_BYTES : slot;
 #pragma unroll
@@ -821,12 +897,13 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         // the scale bytes of a step, through the scalar cache, and those of keys 16g + 4 * which .. + 3 of it
         auto load_scales = [&](int i, const int (&page)[GROUPS], u32x4 (&k)[GROUPS], u32x4 (&v)[GROUPS])
         {
+            int64_t from[GROUPS];
+            places(i, page, p.c.scale_stride, 1, from);
 #pragma unroll
             for(int g = 0; g < GROUPS; ++g)
             {
-                const int64_t at_row = real_page(page[g]) * p.c.scale_stride + in_page(i, g);
-                k[g] = scalar_load<u32x4>(p.c.k_scales, at_row);
-                v[g] = scalar_load<u32x4>(p.c.v_scales, at_row);
+                k[g] = scalar_load<u32x4>(p.c.k_scales, from[g]);
+                v[g] = scalar_load<u32x4>(p.c.v_scales, from[g]);
             }
         };
         auto of_lane = [&](const u32x4 &w, int which)
@@ -851,7 +928,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         // first of one shared unit at most).  It has kPagedNone between calls; if it holds something else,
         // the workspace is new, which is seen to where the count is needed.
         const bool whole = seg.step == 0 && seg.steps == seg.blocks;
-        const uint32_t w0 = whole ? blockIdx.x : split.of(unit_begin);
+        const uint32_t w0 = aligned || whole ? first_share : split.of(unit_begin);
         unsigned long long *const count = p.counts + w0 * kPagedCountStride;
         unsigned long long held = kPagedNone;
         if(tid == 0 && !whole)
@@ -861,11 +938,14 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         const int n_steps = PAIRED ? seg.steps : n_mine;
         auto without_page = [&]()       // groups of the step
         {
-            uint32_t hidden = 0;
-#pragma unroll
-            for(int g = 0; g < GROUPS; ++g)
+            uint32_t hidden = (unsigned)page[0] < (unsigned)p.c.n_pages ? 0u : GROUPS == 1 || one_page ? ~0u : 1u;
+            if(GROUPS > 1 && !one_page)
             {
-                hidden |= (unsigned)page[g] < (unsigned)p.c.n_pages ? 0u : 1u << g;
+#pragma unroll
+                for(int g = 1; g < GROUPS; ++g)
+                {
+                    hidden |= (unsigned)page[g] < (unsigned)p.c.n_pages ? 0u : 1u << g;
+                }
             }
             return hidden;
         };
@@ -1001,7 +1081,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
 #pragma unroll
                     for(int e = 0; e < 4; ++e)
                     {
-                        const bool there = !PARTLY || (key0 + 16 * g + 4 * quad + e < seg.len && !((hidden >> g) & 1));
+                        const bool there = !PARTLY || 4 * quad + e < ((hidden >> g) & 1 ? 0 : seg.len - key0 - 16 * g);
                         const uint32_t byte = there ? (vs[g] >> (8 * e)) & 255u : 0u;
                         of_scale[g][e] = RANGED ? (float)byte : __uint_as_float(byte << 23);
                         most = RANGED ? fmaxf(most, of_scale[g][e]) : most;
@@ -1054,8 +1134,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                         }
                         if constexpr(PARTLY)
                         {
-                            const int key = key0 + 16 * g + 4 * quad + e;
-                            x = key > last[nr] || key >= seg.len || ((hidden >> g) & 1) ? neg_inf() : x;
+                            x = 4 * quad + e > ((hidden >> g) & 1 ? -1 : last[nr] - key0 - 16 * g) ? neg_inf() : x;
                         }
                         s[nr][g][e] = x;
                         top = fmaxf(top, x);
@@ -1166,7 +1245,25 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                 }
             };
             constexpr int TSTEPS = KIND == kPaged32 ? GROUPS : (GROUPS + 1) / 2;
-            if constexpr(!PARTLY)
+            // Where a value is no number, a probability of 0 does not hide it (0 * NaN).  That matters in the
+            // rows behind all_see, which are hidden from some query: are there any?
+            bool odd = false;
+            if(PARTLY && p.causal && given > 1)
+            {
+                bool any = false;
+                for(int b = max(all_see + 1 - key0, 0) * RB + lane * 16; b < K_BYTES; b += 64 * 16)
+                {
+                    const u32x4 w = *reinterpret_cast<const u32x4 *>(slot + K_BYTES + b);
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
+                    {
+                        any = any || not_numbers<T, KIND>(w[e]);
+                    }
+                }
+                odd = __any(any);
+            }
+            // (in one form with the others where there are many registers to keep, see below)
+            if(!PARTLY || (NR == 1 && !odd))
             {
 #pragma unroll
                 for(int db = 0; db < DBLOCKS; ++db)
@@ -1184,71 +1281,61 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                     }
                 }
             }
-            else
+            else if constexpr(PARTLY)
             {
-                // Where a value is no number, a probability of 0 does not hide it (0 * NaN): then
-                // token by token, with the values behind what the token sees taken out and only
-                // the rows of the token taken over.
-                bool odd = false;
-                if(p.causal && p.q_seq > 1)
+                // If so, token by token, with the values behind what the token sees taken out and only the
+                // rows of the token taken over.
+                const int rounds = odd ? given : 1;
+                for(int tok = 0; tok < rounds; ++tok)
                 {
-                    uint32_t any = 0;
+                    // (nothing is read ahead of the loop: the registers are the other form's)
+                    asm volatile("" ::: "memory");
 #pragma unroll
                     for(int db = 0; db < DBLOCKS; ++db)
                     {
+                        f32x4 fresh[NR];
+#pragma unroll
+                        for(int nr = 0; nr < NR; ++nr)
+                        {
+                            fresh[nr] = o[nr][db];
+                        }
 #pragma unroll
                         for(int t = 0; t < TSTEPS; ++t)
                         {
                             u32x4 w;
                             value_words(db, t, w);
-#pragma unroll
-                            for(int e = 0; e < 4; ++e)
+                            if(odd)
                             {
-                                any |= KIND == kPaged32 ? (w[e] & 0x7f800000u) == 0x7f800000u
-                                    : not_finite2<PV>(w[e]);
-                            }
-                        }
-                    }
-                    odd = __any(any != 0);
-                }
-                const int rounds = odd ? given : 1;
-                for(int tok = 0; tok < rounds; ++tok)
-                {
-                    // (nothing is read ahead of the loop: the registers are the other step's)
-                    asm volatile("" ::: "memory");
-                    const int sees = odd ? all_see + tok : 0x7ffffffe;
-#pragma unroll
-                    for(int db = 0; db < DBLOCKS; ++db)
-                    {
-#pragma unroll
-                        for(int nr = 0; nr < NR; ++nr)
-                        {
-                            f32x4 fresh = o[nr][db];
-#pragma unroll
-                            for(int t = 0; t < TSTEPS; ++t)
-                            {
-                                u32x4 w;
-                                value_words(db, t, w);
+                                // the values of this step's first keys that the token sees
+                                const int seen = all_see + tok + 1 - key0 - (KIND == kPaged32 ? 16 : 32) * t - 4 * quad;
 #pragma unroll
                                 for(int e = 0; e < 4; ++e)
                                 {
                                     if constexpr(KIND == kPaged32)
                                     {
-                                        w[e] = key0 + 16 * t + 4 * quad + e > sees ? 0u : w[e];
+                                        w[e] = e < seen ? w[e] : 0u;
                                     }
                                     else
                                     {
-                                        const int key = key0 + 32 * t + 16 * (e >> 1) + 4 * quad + 2 * (e & 1);
-                                        w[e] &= (key > sees ? 0u : 0xffffu) | (key + 1 > sees ? 0u : 0xffff0000u);
+                                        const int at_key = 16 * (e >> 1) + 2 * (e & 1);
+                                        w[e] &= (at_key < seen ? 0xffffu : 0u) | (at_key + 1 < seen ? 0xffff0000u : 0u);
                                     }
                                 }
-                                fresh = multiply(w, t, nr, fresh);
                             }
+#pragma unroll
+                            for(int nr = 0; nr < NR; ++nr)
+                            {
+                                fresh[nr] = multiply(w, t, nr, fresh[nr]);
+                            }
+                        }
+#pragma unroll
+                        for(int nr = 0; nr < NR; ++nr)
+                        {
                             const bool take = !odd || token[nr] == tok;
 #pragma unroll
                             for(int e = 0; e < 4; ++e)
                             {
-                                o[nr][db][e] = take ? fresh[e] : o[nr][db][e];
+                                o[nr][db][e] = take ? fresh[nr][e] : o[nr][db][e];
                             }
                         }
                     }
@@ -1256,7 +1343,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             }
         };
         // (the steps without hidden keys on their own: two forms behind each other cost fewer
-        // registers than one or the other)
+        // registers than a choice between them)
         int i = 0;
         for(; i < n_mine && my_first + i * Shape::BLOCK + KEYS - 1 <= all_see && without_page() == 0; ++i)
         {
@@ -1357,7 +1444,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             // wavefront's in front of the barrier.  The workgroup that counts last joins.
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            const uint32_t parts = split.of(unit_begin + (uint32_t)seg.blocks - 1) - w0 + 1;
+            const uint32_t parts = aligned ? parts_of_unit : split.of(unit_begin + (uint32_t)seg.blocks - 1) - w0 + 1;
             if(tid == 0)
             {
                 if((held & ~kPagedCountMask) != kPagedNone)
@@ -1383,7 +1470,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         }
         }
         at += taken;
-        if(at >= end)
+        if(aligned || at >= end)
         {
             return;
         }
