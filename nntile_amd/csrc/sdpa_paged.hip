@@ -554,45 +554,19 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         in_front = n_lo * blocks_0;
     }
     const uint32_t all = (uint32_t)total * (uint32_t)p.units;
-    // Shares of whole units: every unit gets as many as keep each to `longest` blocks, if the workgroups
-    // are enough for that.  A share that ends one unit and begins another costs about two blocks more
-    // than one that does not, so this is done where the longest is no more than that above the
-    // even run, and always where all units are equally long (16 drafted sequences of 300 to 4096 8-bit
-    // rows 21.3 -> 17 us).
+    // Where all units are equally long and not more than the workgroups, every unit gets shares of its own, as
+    // few as keep the longest as short as it can be (four sequences of 1024 fp32 rows, 48 units, 15.9 -> 13.5
+    // us); else an even run of blocks is a share.  (Shares of whole units for unequal lengths as well, where
+    // that made the longest no more than two blocks longer: 16 of 500 to 8000 rows 38.0 -> 39.1 us.)
     const uint32_t n_units = (uint32_t)p.c.n_batch * (uint32_t)p.units, places = (uint32_t)p.shares;
-    int of_unit = 0, of_units = 0, shares_in_front = 0;     // shares of the lane's units; of all; in front of its own
-    if(same && n_units <= places && blocks_0 != 0)
+    const bool aligned = same && n_units <= places && blocks_0 != 0;
+    uint32_t of_unit = 1;
+    if(aligned)
     {
-        const int most = (int)(places / n_units), longest = (blocks_0 + most - 1) / most;
-        of_unit = (blocks_0 + longest - 1) / longest;
-        of_units = p.c.n_batch * of_unit;
-        shares_in_front = n_lo * of_unit;
+        const uint32_t most = places / n_units, longest = ((uint32_t)blocks_0 + most - 1) / most;
+        of_unit = ((uint32_t)blocks_0 + longest - 1) / longest;
     }
-    else if(in_wave && !same && total != 0)
-    {
-        const int even = (int)((all + places - 1) / places);
-        const int b = n_lo < n_hi ? blocks_of(n_lo) : 0;
-        for(int longest = max(even - 1, 1); longest <= even + 2 && of_units == 0; ++longest)
-        {
-            const int k = (b + longest - 1) / longest;
-            int sum = k;
-#pragma unroll
-            for(int o = 1; o < 64; o <<= 1)
-            {
-                const int other = __shfl_up(sum, o);
-                sum += lane >= o ? other : 0;
-            }
-            const int everyone = __builtin_amdgcn_readlane(sum, 63);
-            if((uint32_t)everyone * (uint32_t)p.units <= places)
-            {
-                of_unit = k;
-                of_units = everyone;
-                shares_in_front = sum - k;
-            }
-        }
-    }
-    const bool aligned = of_units != 0;
-    const uint32_t shares = aligned ? (uint32_t)of_units * (uint32_t)p.units : min(places, all);
+    const uint32_t shares = aligned ? n_units * of_unit : min(places, all);
     const PagedSplit split(all, shares);
     // sequences without rows: shared out, too, for the rows of their queries
     if(p.overwrite && !(same && blocks_0 != 0))
@@ -619,23 +593,35 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     uint32_t at = split.begin(blockIdx.x);
     const uint32_t end = split.begin(blockIdx.x + 1);
     PagedSegment seg;
-    uint32_t first_share = blockIdx.x, parts_of_unit = 1;       // where shares are of whole units
+    uint32_t first_share = blockIdx.x;
+    if(aligned)
     {
-        // the last lane whose sequences begin at or before the block or share, then sequence by sequence
-        const int what = aligned ? (int)(blockIdx.x / (uint32_t)p.units) : (int)(at / (uint32_t)p.units);
-        const int front = aligned ? shares_in_front : in_front;
+        const uint32_t unit = blockIdx.x / of_unit, part = blockIdx.x - unit * of_unit;
+        const PagedSplit of_blocks((uint32_t)blocks_0, of_unit);
+        first_share = blockIdx.x - part;
+        seg.n = (int)(unit / (uint32_t)p.units);
+        seg.u = (int)(unit - (uint32_t)seg.n * (uint32_t)p.units);
+        seg.len = uniform(paged_len(p.c, seg.n));
+        seg.blocks = blocks_0;
+        seg.step = (int)of_blocks.begin(part);
+        seg.steps = (int)of_blocks.begin(part + 1) - seg.step;
+    }
+    else
+    {
+        // the last lane whose sequences begin at or before the block, then sequence by sequence
+        const int block = (int)(at / (uint32_t)p.units);
         int t, before;
         if(in_wave)
         {
-            t = __popcll(__ballot(scanner * chunk < p.c.n_batch && front <= what)) - 1;
-            before = __builtin_amdgcn_readlane(front, t);
+            t = __popcll(__ballot(scanner * chunk < p.c.n_batch && in_front <= block)) - 1;
+            before = __builtin_amdgcn_readlane(in_front, t);
         }
         else
         {
-            scan_of[tid] = front;
+            scan_of[tid] = in_front;
             __syncthreads();
-            const bool here = tid * chunk < p.c.n_batch && front <= what
-                && (tid == THREADS - 1 || (tid + 1) * chunk >= p.c.n_batch || scan_of[tid + 1] > what);
+            const bool here = tid * chunk < p.c.n_batch && in_front <= block
+                && (tid == THREADS - 1 || (tid + 1) * chunk >= p.c.n_batch || scan_of[tid + 1] > block);
             if(here)
             {
                 found = tid;
@@ -645,36 +631,20 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             before = uniform(scan_of[t]);
         }
         seg.n = t * chunk;
-        const int parts = __builtin_amdgcn_readlane(of_unit, in_wave ? t : 0);
         for(;;)
         {
             seg.len = uniform(paged_len(p.c, seg.n));
             seg.blocks = (seg.len + Shape::BLOCK - 1) / Shape::BLOCK;
-            const int here = aligned ? parts : cost_of(seg.blocks);
-            if(before + here > what || seg.n + 1 >= p.c.n_batch)
+            if(before + cost_of(seg.blocks) > block || seg.n + 1 >= p.c.n_batch)
             {
                 break;
             }
-            before += here;
+            before += cost_of(seg.blocks);
             ++seg.n;
         }
-        if(aligned)
-        {
-            const uint32_t rest = blockIdx.x - (uint32_t)before * (uint32_t)p.units;
-            parts_of_unit = (uint32_t)parts;
-            seg.u = uniform((int)(rest / parts_of_unit));
-            const uint32_t part = rest - (uint32_t)seg.u * parts_of_unit;
-            const PagedSplit of_blocks((uint32_t)seg.blocks, parts_of_unit);
-            first_share = blockIdx.x - part;
-            seg.step = uniform((int)of_blocks.begin(part));
-            seg.steps = uniform((int)of_blocks.begin(part + 1)) - seg.step;
-        }
-        else
-        {
-            const uint32_t rest = at - (uint32_t)before * (uint32_t)p.units;
-            seg.u = uniform((int)(rest / (uint32_t)cost_of(seg.blocks)));
-            seg.step = uniform((int)(rest % (uint32_t)cost_of(seg.blocks)));
-        }
+        const uint32_t rest = at - (uint32_t)before * (uint32_t)p.units;
+        seg.u = uniform((int)(rest / (uint32_t)cost_of(seg.blocks)));
+        seg.step = uniform((int)(rest % (uint32_t)cost_of(seg.blocks)));
     }
     uint32_t unit_begin = at - (uint32_t)seg.step;      // of the unit's first block among all
 
@@ -1444,7 +1414,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             // wavefront's in front of the barrier.  The workgroup that counts last joins.
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            const uint32_t parts = aligned ? parts_of_unit : split.of(unit_begin + (uint32_t)seg.blocks - 1) - w0 + 1;
+            const uint32_t parts = aligned ? of_unit : split.of(unit_begin + (uint32_t)seg.blocks - 1) - w0 + 1;
             if(tid == 0)
             {
                 if((held & ~kPagedCountMask) != kPagedNone)
