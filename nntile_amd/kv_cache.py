@@ -205,3 +205,194 @@ class KVCache:
         hip_sdpa.sdpa_fwd_decode_cache(
             self.k, self.v, k_seq, Q, sliced, lse, A, mode, n_batch, kv_group, workspace,
             causal_offset=k_seq - q_seq, flags=hip_sdpa.OVERWRITE, stream=stream)
+
+
+class PagedKVCache:
+    """Key/value cache whose sequences have lengths of their own: rows lie in
+    pages of a pool that all sequences share, as they are or in 8 bits (e4m3 with
+    one power of two per row).  What `KVCache` does for a batch of equal lengths,
+    for a batch that is served: sequences end (`release`) and their pages go to others.
+
+    Tensors as for `KVCache`: K, V `[n_head_kv * n_batch, rows, head]`, Q, A
+    `[n_head_kv * kv_group * n_batch, q_seq, head]`, entry = sequence + n_batch *
+    head index.  The lengths are known to the host, which hands out the pages;
+    the kernels read lengths and page table on the device.  A caller that
+    captures its steps calls hip_sdpa.paged_kv_append / sdpa_fwd_paged with
+    `table` and a `lens` of its own instead: this class's bookkeeping would run once,
+    at the capture.  Calls of one cache share its workspace: they belong on one stream,
+    or are ordered by the caller.
+    """
+
+    def __init__(self, n_pages, page_rows, n_batch, max_rows, n_head_kv, head, dtype=torch.bfloat16,
+                 packed=False, device="cuda"):
+        if page_rows < 16 or page_rows > 65536 or page_rows & (page_rows - 1):
+            raise ValueError("page_rows is a power of two from 16 to 65536")
+        if min(n_pages, n_batch, max_rows, n_head_kv) < 1 or head not in (64, 128):
+            raise ValueError("a cache needs pages, sequences, rows and heads of size 64 or 128")
+        hip_sdpa.dtype_name(torch.empty(0, dtype=dtype))
+        if packed and dtype == torch.float32:
+            raise TypeError("8-bit pages hold bf16 and fp16 tiles")
+        self.dtype, self.packed = dtype, bool(packed)
+        self.n_batch, self.n_head_kv, self.head = n_batch, n_head_kv, head
+        self.page_rows, self.max_pages = page_rows, -(-max_rows // page_rows)
+        # (a page's keys and values behind each other)
+        shape = (n_pages, 2, n_head_kv, page_rows, head)
+        pool = torch.zeros(shape, dtype=torch.uint8 if packed else dtype, device=device)
+        self.pool = pool.view(torch.float8_e4m3fn) if packed else pool
+        self.k_pages, self.v_pages = self.pool[:, 0], self.pool[:, 1]
+        self.scales = torch.ones(shape[:4], dtype=torch.uint8, device=device) if packed else None
+        self.k_scales, self.v_scales = (self.scales[:, 0], self.scales[:, 1]) if packed else (None, None)
+        self.table = torch.full((n_batch, self.max_pages), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(n_batch, dtype=torch.int32, device=device)
+        self.lengths = [0] * n_batch
+        self._pages = [[] for _ in range(n_batch)]
+        self._free = list(range(n_pages - 1, -1, -1))
+        self._workspace = None
+
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    def _counts(self, rows, new_rows):
+        if new_rows is None:
+            return [rows] * self.n_batch
+        counts = [int(c) for c in new_rows]
+        if len(counts) != self.n_batch or min(counts) < 0 or max(counts) > rows:
+            raise ValueError("new_rows are the new tokens of every sequence, at most the tile's rows")
+        return counts
+
+    def _upload(self, target, values, stream):
+        """Host values into a device tensor, ordered on `stream`."""
+        host = torch.tensor(values, dtype=torch.int32).pin_memory()
+        with torch.cuda.stream(stream):
+            target.copy_(host, non_blocking=True)
+        if stream is not None:
+            target.record_stream(stream)
+
+    def _reserve(self, counts, stream):
+        wanted = []
+        for n, count in enumerate(counts):
+            rows = self.lengths[n] + count
+            if rows > self.max_pages * self.page_rows:
+                raise hip_sdpa.SdpaError(hip_sdpa.EINVAL, "paged_kv_append: sequence %d: %d rows, max: %d"
+                                         % (n, rows, self.max_pages * self.page_rows))
+            wanted.append(max(0, -(-rows // self.page_rows) - len(self._pages[n])))
+        if sum(wanted) > len(self._free):
+            raise hip_sdpa.SdpaError(hip_sdpa.EINVAL, "paged_kv_append: %d pages wanted, %d free"
+                                     % (sum(wanted), len(self._free)))
+        if any(wanted):
+            for n, count in enumerate(wanted):
+                self._pages[n] += [self._free.pop() for _ in range(count)]
+            self._upload(self.table, [p + [-1] * (self.max_pages - len(p)) for p in self._pages], stream)
+
+    def append(self, k, v, new_rows=None, stream=None):
+        """Write k, v ([n_head_kv * n_batch, rows, head]) behind the rows of the
+        sequences; new_rows: how many of `rows` each brings (a list; None: all).
+        More rows than a sequence may have, or than there are pages, raise;
+        nothing is changed then."""
+        if (k.dim() != 3 or k.shape != v.shape or k.dtype != self.dtype or v.dtype != self.dtype
+                or k.shape[0] != self.n_head_kv * self.n_batch or k.shape[2] != self.head):
+            raise ValueError("k and v are tiles [n_head_kv * n_batch, rows, head] of the cache's type")
+        for t in (k, v):
+            if not (t.is_cuda and t.is_contiguous()):
+                raise ValueError("tiles must be contiguous device tensors")
+        rows = k.shape[1]
+        counts = self._counts(rows, new_rows)
+        self._reserve(counts, stream)
+        lengths = [length + count for length, count in zip(self.lengths, counts)]
+        uniform = new_rows is None
+        if uniform:
+            with torch.cuda.stream(stream):
+                self.lens.add_(rows)
+            given = None
+        else:
+            self._upload(self.lens, lengths, stream)
+            given = self._on_device(counts, stream)
+        if stream is not None:
+            for t in (k, v, self.lens, self.pool, self.scales):
+                if t is not None:
+                    t.record_stream(stream)
+        hip_sdpa.paged_kv_append(k, v, self.k_pages, self.v_pages, self.table, self.lens, self.k_scales,
+                                 self.v_scales, new_rows=given, stream=stream)
+        self.lengths = lengths
+
+    def _on_device(self, counts, stream):
+        with torch.cuda.stream(stream):
+            t = torch.empty(self.n_batch, dtype=torch.int32, device=self.lens.device)
+        self._upload(t, counts, stream)
+        return t
+
+    def read(self, first=0, rows=None, stream=None):
+        """Rows [first, first + rows) of every sequence as dense tiles (K, V) of the
+        cache's type; rows behind a sequence's last are zeros.  rows None: up to
+        the longest sequence's end."""
+        rows = max(0, max(self.lengths) - first) if rows is None else rows
+        with torch.cuda.stream(stream):
+            k = torch.empty((self.n_head_kv * self.n_batch, rows, self.head), dtype=self.dtype,
+                            device=self.lens.device)
+            v = torch.empty_like(k)
+        hip_sdpa.paged_kv_read(self.k_pages, self.v_pages, self.table, self.lens, k, v, first=first,
+                               k_scales=self.k_scales, v_scales=self.v_scales, stream=stream)
+        return k, v
+
+    @property
+    def k_partial(self):
+        """The filled rows of the keys (a copy, as the reference's)."""
+        return self.read()[0]
+
+    @property
+    def v_partial(self):
+        return self.read()[1]
+
+    # Queries of a key/value head from which a chunk of a batch of equal lengths is worth the copy
+    # that the tile kernels' denser products need.
+    DENSE_ROWS = 512
+
+    def attend(self, Q, lse, A, kv_group, causal=True, new_rows=None, stream=None):
+        """A = attention of Q over the sequences' rows; the queries of a sequence are
+        its newest tokens (append first), the first new_rows of q_seq (a list; None:
+        all).  lse and A are overwritten; queries without a visible row get
+        lse = -inf, A = 0."""
+        q_seq = Q.shape[1]
+        counts = self._counts(q_seq, new_rows)
+        mode = hip_sdpa.MASK_CAUSAL if causal else hip_sdpa.MASK_NONE
+        length = self.lengths[0]
+        if (kv_group * q_seq >= self.DENSE_ROWS and new_rows is None and length >= q_seq
+                and min(self.lengths) == max(self.lengths)):
+            k, v = self.read(stream=stream)
+            need = hip_sdpa.tile_cache_workspace_bytes(length, Q, mode)
+            workspace = None
+            if need:
+                with torch.cuda.stream(stream):
+                    workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
+            hip_sdpa.sdpa_fwd_tile_cache(k, v, length, Q, None, lse, A, mode, n_batch=self.n_batch,
+                                         kv_group=kv_group, causal_offset=length - q_seq,
+                                         flags=hip_sdpa.OVERWRITE, stream=stream, workspace=workspace)
+            return
+        given = None if new_rows is None else self._on_device(counts, stream)
+        need = hip_sdpa.paged_workspace_bytes(Q, self.n_batch, kv_group)
+        if self._workspace is None or self._workspace.numel() < need:
+            # (a launch of an earlier call may still use the old one: it is kept until the one after
+            # next replaces it)
+            self._retired_workspace = self._workspace
+            self._workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
+        if stream is not None:
+            for t in (Q, lse, A, self._workspace, self.lens, self.table, self.pool, self.scales):
+                if t is not None:
+                    t.record_stream(stream)
+        hip_sdpa.sdpa_fwd_paged(self.k_pages, self.v_pages, self.table, self.lens, Q, lse, A, mode,
+                                kv_group, self._workspace, k_scales=self.k_scales, v_scales=self.v_scales,
+                                new_rows=given, flags=hip_sdpa.OVERWRITE, stream=stream)
+
+    def append_attend(self, k, v, Q, lse, A, kv_group, causal=True, new_rows=None, stream=None):
+        """`append` followed by `attend`: a generation step."""
+        self.append(k, v, new_rows=new_rows, stream=stream)
+        self.attend(Q, lse, A, kv_group, causal=causal, new_rows=new_rows, stream=stream)
+
+    def release(self, n, stream=None):
+        """Sequence n is over: its pages are free for others."""
+        self._free += reversed(self._pages[n])
+        self._pages[n] = []
+        self.lengths[n] = 0
+        self._upload(self.lens, self.lengths, stream)
+        self._upload(self.table, [p + [-1] * (self.max_pages - len(p)) for p in self._pages], stream)
