@@ -558,12 +558,19 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     // few as keep the longest as short as it can be (four sequences of 1024 fp32 rows, 48 units, 15.9 -> 13.5
     // us); else an even run of blocks is a share.  (Shares of whole units for unequal lengths as well, where
     // that made the longest no more than two blocks longer: 16 of 500 to 8000 rows 38.0 -> 39.1 us.)
-    const uint32_t n_units = (uint32_t)p.c.n_batch * (uint32_t)p.units, places = (uint32_t)p.shares;
+    const uint32_t n_units = (uint32_t)p.c.n_batch * (uint32_t)p.units;
+    // The workgroup that joins a unit reads `rows` sums of `head` from every share, alone, while a share
+    // reads its part of the keys: with more shares than about sqrt(keys / rows) a unit the join costs more
+    // than the shorter shares save (one sequence, 8 units, of 4096 16-bit rows, 64 query rows 42.7 us with 32
+    // shares a unit, 26.7 with 8; 4 query rows 16.5 and 11.7).
+    const float keys = (float)all / (float)n_units * (float)Shape::BLOCK;
+    const float most = fmaxf(sqrtf(keys / (float)min(p.rows, QROWS)), 1.0f);
+    const uint32_t places = (uint32_t)uniform((int)fminf((float)p.shares, (float)n_units * most));
     const bool aligned = same && n_units <= places && blocks_0 != 0;
     uint32_t of_unit = 1;
     if(aligned)
     {
-        const uint32_t most = places / n_units, longest = ((uint32_t)blocks_0 + most - 1) / most;
+        const uint32_t each = places / n_units, longest = ((uint32_t)blocks_0 + each - 1) / each;
         of_unit = ((uint32_t)blocks_0 + longest - 1) / longest;
     }
     const uint32_t shares = aligned ? n_units * of_unit : min(places, all);
@@ -1461,17 +1468,19 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     }
 }
 
-// Blocks of 16 rows that a workgroup takes: 1, 2, or 4 by two wavefronts a key
-static int row_blocks(bool fp32, int64_t rows)
+// Blocks of 16 rows that a workgroup takes: 1, 2, or 4 by two wavefronts a key; 1 also where that leaves no
+// more than 64 units, which then have more shares, and joins, between them (8 units of 4096 rows, 64 query
+// rows, 26.7 us with 4 blocks a workgroup, 21.4 with 1; 64 units of 2048 29.2 and 51.9).
+static int row_blocks(bool fp32, int64_t entries, int64_t rows)
 {
-    return rows <= 16 ? 1 : rows <= 32 || fp32 ? 2 : 4;
+    return rows <= 16 || entries * ((rows + 15) / 16) <= 64 ? 1 : rows <= 32 || fp32 ? 2 : 4;
 }
 
 // The workspace: the counts, then the shares' results (the larger size of the types', which differ in
 // the rows of a workgroup).
 static size_t share_rows(int64_t rows)
 {
-    return (size_t)kPagedShares * 2 * 16 * (size_t)row_blocks(false, rows);
+    return (size_t)kPagedShares * 2 * 16 * (size_t)row_blocks(false, 64, rows);
 }
 
 size_t paged_attend_workspace_bytes(int64_t rows, int64_t head)
@@ -1501,7 +1510,7 @@ static int launch_form(hipStream_t stream, PagedAttendParams &p)
 template<typename T, int KIND>
 static int launch_kind(hipStream_t stream, PagedAttendParams &p, int head)
 {
-    switch(row_blocks(KIND == kPaged32, p.rows) * 256 + head)
+    switch(row_blocks(KIND == kPaged32, (int64_t)p.c.n_batch * p.c.n_head_kv, p.rows) * 256 + head)
     {
         case 256 + 64: return launch_form<T, KIND, 64, 1, 1>(stream, p);
         case 256 + 128: return launch_form<T, KIND, 128, 1, 1>(stream, p);
