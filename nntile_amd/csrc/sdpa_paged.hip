@@ -34,6 +34,7 @@
 namespace nntile_hip
 {
 
+typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(2))) int i32x2;
 typedef __attribute__((ext_vector_type(4))) __bf16 bf16x4;
@@ -231,30 +232,28 @@ struct PagedSplit
 
 // Partial results go from one workgroup to another of the same launch, on any XCD: stores and
 // loads that the device serves, not a CU's or an XCD's own cache.
-__device__ __forceinline__ void put2(float *to, float a, float b)
+__device__ __forceinline__ void put2(float *to, f32x2 v)
 {
-    typedef __attribute__((ext_vector_type(2))) float f32x2;
-    __hip_atomic_store(reinterpret_cast<unsigned long long *>(to),
-            __builtin_bit_cast(unsigned long long, f32x2{a, b}), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(reinterpret_cast<unsigned long long *>(to), __builtin_bit_cast(unsigned long long, v),
+            __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-__device__ __forceinline__ void get2(const float *from, float &a, float &b)
+__device__ __forceinline__ f32x2 get2(const float *from)
 {
-    typedef __attribute__((ext_vector_type(2))) float f32x2;
-    const f32x2 v = __builtin_bit_cast(f32x2, __hip_atomic_load(
+    return __builtin_bit_cast(f32x2, __hip_atomic_load(
                 reinterpret_cast<unsigned long long *>(const_cast<float *>(from)), __ATOMIC_RELAXED,
                 __HIP_MEMORY_SCOPE_AGENT));
-    a = v[0];
-    b = v[1];
 }
 
-// The folded row of a unit: (m, l) in log2 units, o unnormalised; into the running pair.
-// Eight (head 128) or four (head 64) values from d0 on.  The threads of a row run in one wavefront,
-// in lock step: every one has read lse before the first writes it.
-template<typename T, int VALUES>
-__device__ __forceinline__ void paged_finish_row(const PagedAttendParams &p, int head, int64_t row,
-        int d0, float m, float l, const float (&o)[VALUES])
+// The folded row of a unit: (m, l) in log2 units, v unnormalised; into the running pair.
+// TPR threads a row, thread t of them with the value pairs 2 * (t + TPR * k), so that neighbours' accesses lie
+// side by side.  The threads of a row run in one wavefront, in lock step: every one has read lse before the
+// first writes it.
+template<typename T, int TPR, int PAIRS>
+__device__ __forceinline__ void paged_finish_row(const PagedAttendParams &p, int64_t row, int t, float m, float l,
+        const f32x2 (&o)[PAIRS])
 {
+    constexpr int HEAD = 2 * TPR * PAIRS;
     const bool none = m == neg_inf() && l == 0.0f;
     float lse_out = neg_inf(), w_old = 0.0f, sc = 0.0f;
     if(none)
@@ -271,46 +270,33 @@ __device__ __forceinline__ void paged_finish_row(const PagedAttendParams &p, int
         merge_weights(p.overwrite ? neg_inf() : p.lse[row], lse_new, w_old, w_new, lse_out);
         sc = w_new / l;
     }
-    float v[VALUES];
 #pragma unroll
-    for(int i = 0; i < VALUES; ++i)
+    for(int k = 0; k < PAIRS; ++k)
     {
-        v[i] = none ? 0.0f : o[i] * sc;
-    }
-    if constexpr(__is_same(T, float))
-    {
-        float *dst = static_cast<float *>(p.A) + row * head + d0;
-#pragma unroll
-        for(int i = 0; i < VALUES; i += 4)
+        f32x2 v = none ? f32x2{0.0f, 0.0f} : o[k] * sc;
+        const int64_t at = row * HEAD + 2 * (t + TPR * k);
+        if constexpr(__is_same(T, float))
         {
-            f32x4 *at = reinterpret_cast<f32x4 *>(dst + i);
-            f32x4 out = {v[i], v[i + 1], v[i + 2], v[i + 3]};
+            f32x2 *dst = reinterpret_cast<f32x2 *>(static_cast<float *>(p.A) + at);
             if(w_old != 0.0f)
             {
-                out += w_old * *at;
+                v += w_old * *dst;
             }
-            *at = out;
+            *dst = v;
         }
-    }
-    else
-    {
-        uint16_t *dst = static_cast<uint16_t *>(p.A) + row * head + d0;
-#pragma unroll
-        for(int i = 0; i < VALUES; i += 4)
+        else
         {
-            u32x2 *at = reinterpret_cast<u32x2 *>(dst + i);
+            uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(p.A) + at);
             if(w_old != 0.0f)
             {
-                const u32x2 old = *at;
-                v[i] += w_old * T::to_float((uint16_t)(old[0] & 0xffffu));
-                v[i + 1] += w_old * T::to_float((uint16_t)(old[0] >> 16));
-                v[i + 2] += w_old * T::to_float((uint16_t)(old[1] & 0xffffu));
-                v[i + 3] += w_old * T::to_float((uint16_t)(old[1] >> 16));
+                const uint32_t old = *dst;
+                v[0] += w_old * T::to_float((uint16_t)(old & 0xffffu));
+                v[1] += w_old * T::to_float((uint16_t)(old >> 16));
             }
-            *at = u32x2{T::pack2(v[i], v[i + 1]), T::pack2(v[i + 2], v[i + 3])};
+            *dst = T::pack2(v[0], v[1]);
         }
     }
-    if(d0 == 0)
+    if(t == 0)
     {
         p.lse[row] = lse_out;
     }
@@ -337,23 +323,23 @@ __device__ __forceinline__ void paged_join_by(const PagedAttendParams &p, int n,
     {
         turns *= 2;
     }
-    const int d0 = (threadIdx.x % TPR) * 4, slot = threadIdx.x / TPR;
+    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;      // pairs 2t and 2t + HEAD/2 of the row
     const int turn = slot % turns, step = ROWS / turns;
     // (with more than one turn all rows fit beside each other: one round of one line)
     for(int r0 = slot / turns; r0 - slot / turns < rows_here; r0 += LINES * step)
     {
         float top[LINES], sum[LINES];
-        f32x4 v[LINES];
+        f32x2 v[LINES][2];
 #pragma unroll
         for(int k = 0; k < LINES; ++k)
         {
             top[k] = neg_inf();
             sum[k] = 0.0f;
-            v[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            v[k][0] = v[k][1] = f32x2{0.0f, 0.0f};
         }
         for(int i0 = turn; i0 < parts; i0 += PARTS * turns)
         {
-            float m[LINES][PARTS], l[LINES][PARTS], x[LINES][PARTS][4];
+            f32x2 ml[LINES][PARTS], x[LINES][PARTS][2];
 #pragma unroll
             for(int k = 0; k < LINES; ++k)
             {
@@ -364,9 +350,9 @@ __device__ __forceinline__ void paged_join_by(const PagedAttendParams &p, int n,
                     const int i = min(i0 + j * turns, parts - 1);
                     const int r = min(r0 + k * step, rows_here - 1);
                     const int64_t place = ((int64_t)(w0 + i) * 2 + (i == 0 ? 1 : 0)) * QROWS + r;
-                    get2(p.part_ml + 2 * place, m[k][j], l[k][j]);
-                    get2(p.part_o + place * HEAD + d0, x[k][j][0], x[k][j][1]);
-                    get2(p.part_o + place * HEAD + d0 + 2, x[k][j][2], x[k][j][3]);
+                    ml[k][j] = get2(p.part_ml + 2 * place);
+                    x[k][j][0] = get2(p.part_o + place * HEAD + 2 * t);
+                    x[k][j][1] = get2(p.part_o + place * HEAD + 2 * t + HEAD / 2);
                 }
             }
 #pragma unroll
@@ -376,24 +362,22 @@ __device__ __forceinline__ void paged_join_by(const PagedAttendParams &p, int n,
 #pragma unroll
                 for(int j = 0; j < PARTS; ++j)
                 {
-                    next = i0 + j * turns < parts ? fmaxf(next, m[k][j]) : next;
+                    next = i0 + j * turns < parts ? fmaxf(next, ml[k][j][0]) : next;
                 }
                 const float safe = next == neg_inf() ? 0.0f : next;
                 const float old = fast_exp2(top[k] - safe);
                 sum[k] *= old;
-                v[k] *= old;
+                v[k][0] *= old;
+                v[k][1] *= old;
 #pragma unroll
                 for(int j = 0; j < PARTS; ++j)
                 {
                     if(i0 + j * turns < parts)
                     {
-                        const float f = fast_exp2(m[k][j] - safe);
-                        sum[k] += l[k][j] * f;
-#pragma unroll
-                        for(int e = 0; e < 4; ++e)
-                        {
-                            v[k][e] += x[k][j][e] * f;
-                        }
+                        const float f = fast_exp2(ml[k][j][0] - safe);
+                        sum[k] += ml[k][j][1] * f;
+                        v[k][0] += x[k][j][0] * f;
+                        v[k][1] += x[k][j][1] * f;
                     }
                 }
                 top[k] = next;
@@ -402,8 +386,9 @@ __device__ __forceinline__ void paged_join_by(const PagedAttendParams &p, int n,
         if(turns > 1)
         {
             float *const at = lds + slot * (HEAD + 4);
-            *reinterpret_cast<f32x4 *>(at + d0) = v[0];
-            if(d0 == 0)
+            *reinterpret_cast<f32x2 *>(at + 2 * t) = v[0][0];
+            *reinterpret_cast<f32x2 *>(at + 2 * t + HEAD / 2) = v[0][1];
+            if(t == 0)
             {
                 at[HEAD] = top[0];
                 at[HEAD + 1] = sum[0];
@@ -418,12 +403,14 @@ __device__ __forceinline__ void paged_join_by(const PagedAttendParams &p, int n,
                 }
                 const float safe = next == neg_inf() ? 0.0f : next;
                 sum[0] = 0.0f;
-                v[0] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                v[0][0] = v[0][1] = f32x2{0.0f, 0.0f};
                 for(int j = 0; j < turns; ++j)
                 {
-                    const float f = fast_exp2(at[j * (HEAD + 4) + HEAD] - safe);
-                    sum[0] += f * at[j * (HEAD + 4) + HEAD + 1];
-                    v[0] += f * *reinterpret_cast<const f32x4 *>(at + j * (HEAD + 4) + d0);
+                    const float *const of = at + j * (HEAD + 4);
+                    const float f = fast_exp2(of[HEAD] - safe);
+                    sum[0] += f * of[HEAD + 1];
+                    v[0][0] += f * *reinterpret_cast<const f32x2 *>(of + 2 * t);
+                    v[0][1] += f * *reinterpret_cast<const f32x2 *>(of + 2 * t + HEAD / 2);
                 }
                 top[0] = next;
             }
@@ -434,9 +421,7 @@ __device__ __forceinline__ void paged_join_by(const PagedAttendParams &p, int n,
             const int r = r0 + k * step;
             if(turn == 0 && r < rows_here)
             {
-                const float out[4] = {v[k][0], v[k][1], v[k][2], v[k][3]};
-                paged_finish_row<T>(p, HEAD, paged_query_row(p, n, h, rg * QROWS + r), d0, top[k],
-                        sum[k], out);
+                paged_finish_row<T, TPR, 2>(p, paged_query_row(p, n, h, rg * QROWS + r), t, top[k], sum[k], v[k]);
             }
         }
     }
@@ -586,9 +571,9 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                 for(int t = tid; t < rows * (HEAD / 4); t += THREADS)
                 {
                     const int r = t / (HEAD / 4);
-                    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    paged_finish_row<T>(p, HEAD, paged_query_row(p, n, r / p.rows, r % p.rows),
-                            4 * (t % (HEAD / 4)), neg_inf(), 0.0f, zero);
+                    const f32x2 zero[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+                    paged_finish_row<T, HEAD / 4, 2>(p, paged_query_row(p, n, r / p.rows, r % p.rows),
+                            t % (HEAD / 4), neg_inf(), 0.0f, zero);
                 }
             }
         }
@@ -1367,13 +1352,14 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             }
             __syncthreads();
             // 16 threads a row; the row of stream w lies at (w + STREAMS * half) * 16 + row
-            constexpr int VALUES = HEAD / 16;
-            const int row = (tid / 16) % 16, its_half = tid / 256, d0 = (tid % 16) * VALUES;
+            constexpr int PAIRS = HEAD / 32;
+            const int row = (tid / 16) % 16, its_half = tid / 256, t = tid % 16;
             const int in_group = (its_half * NR + nr) * 16 + row, rr = rg * QROWS + in_group;
             if(rr < p.rows)
             {
                 const int from = its_half * STREAMS * 16 + row;
-                float top = neg_inf(), sum = 0.0f, v[VALUES];
+                float top = neg_inf(), sum = 0.0f;
+                f32x2 v[PAIRS];
 #pragma unroll
                 for(int w = 0; w < STREAMS; ++w)
                 {
@@ -1381,9 +1367,9 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                 }
                 const float safe = top == neg_inf() ? 0.0f : top;
 #pragma unroll
-                for(int j = 0; j < VALUES; ++j)
+                for(int k = 0; k < PAIRS; ++k)
                 {
-                    v[j] = 0.0f;
+                    v[k] = f32x2{0.0f, 0.0f};
                 }
 #pragma unroll
                 for(int w = 0; w < STREAMS; ++w)
@@ -1391,26 +1377,27 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                     const float f = fast_exp2(merge_ml[2 * (from + w * 16)] - safe);
                     sum += f * merge_ml[2 * (from + w * 16) + 1];
 #pragma unroll
-                    for(int j = 0; j < VALUES; ++j)
+                    for(int k = 0; k < PAIRS; ++k)
                     {
-                        v[j] += f * merge_o[(from + w * 16) * MERGE_LD + d0 + j];
+                        v[k] += f * *reinterpret_cast<const f32x2 *>(merge_o + (from + w * 16) * MERGE_LD
+                                + 2 * (t + 16 * k));
                     }
                 }
                 if(whole)
                 {
-                    paged_finish_row<T>(p, HEAD, paged_query_row(p, seg.n, h, rr), d0, top, sum, v);
+                    paged_finish_row<T, 16, PAIRS>(p, paged_query_row(p, seg.n, h, rr), t, top, sum, v);
                 }
                 else
                 {
                     const int64_t place = ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * QROWS + in_group;
 #pragma unroll
-                    for(int j = 0; j < VALUES; j += 2)
+                    for(int k = 0; k < PAIRS; ++k)
                     {
-                        put2(p.part_o + place * HEAD + d0 + j, v[j], v[j + 1]);
+                        put2(p.part_o + place * HEAD + 2 * (t + 16 * k), v[k]);
                     }
-                    if(d0 == 0)
+                    if(t == 0)
                     {
-                        put2(p.part_ml + 2 * place, top, sum);
+                        put2(p.part_ml + 2 * place, f32x2{top, sum});
                     }
                 }
             }
