@@ -294,8 +294,10 @@ class PagedKVCache:
                 or k.shape[0] != self.n_head_kv * self.n_batch or k.shape[2] != self.head):
             raise ValueError("k and v are tiles [n_head_kv * n_batch, rows, head] of the cache's type")
         for t in (k, v):
-            if not (t.is_cuda and t.is_contiguous()):
-                raise ValueError("tiles must be contiguous device tensors")
+            if not (t.is_cuda and t.is_contiguous() and t.device == self.lens.device
+                    and t.device.index == torch.cuda.current_device()):
+                raise ValueError("tiles must be contiguous device tensors of the cache's device, "
+                                 "which is the current one")
         rows = k.shape[1]
         counts = self._counts(rows, new_rows)
         self._reserve(counts, stream)
@@ -375,7 +377,8 @@ class PagedKVCache:
             # (a launch of an earlier call may still use the old one: it is kept until the one after
             # next replaces it)
             self._retired_workspace = self._workspace
-            self._workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
+            with torch.cuda.stream(stream):
+                self._workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
         if stream is not None:
             for t in (Q, lse, A, self._workspace, self.lens, self.table, self.pool, self.scales):
                 if t is not None:
