@@ -55,21 +55,50 @@ __device__ __forceinline__ int page_of(const PagedView &c, int n, int pos)
     return (unsigned)page < (unsigned)c.n_pages ? page : -1;
 }
 
-// TPR threads a row.
+// The larger of each half, as unsigned 16-bit integers.
+__device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b)
+{
+    typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
+                __builtin_bit_cast(u16x2, b)));
+}
+
+// Over the TPR threads of a row, each half on its own.
 template<int TPR>
 __device__ __forceinline__ uint32_t row_max(uint32_t x)
 {
 #pragma unroll
     for(int o = TPR / 2; o >= 1; o >>= 1)
     {
-        x = max(x, (uint32_t)__shfl_xor((int)x, o, TPR));
+        x = max_halves(x, (uint32_t)__shfl_xor((int)x, o, TPR));
     }
     return x;
 }
 
+// Two values of T divided by a power of two, as codes of one half of a word, to nearest even.
+template<typename T, bool HIGH>
+__device__ __forceinline__ uint32_t narrow2(uint32_t word, uint32_t x, float scale)
+{
+    typedef __attribute__((ext_vector_type(2))) short s16x2;
+    const s16x2 old = __builtin_bit_cast(s16x2, word);
+    if constexpr(__is_same(T, Fp16))
+    {
+        typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+        return __builtin_bit_cast(uint32_t,
+                __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(old, __builtin_bit_cast(f16x2, x), scale, HIGH));
+    }
+    else
+    {
+        typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+        return __builtin_bit_cast(uint32_t,
+                __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(old, __builtin_bit_cast(bf16x2, x), scale, HIGH));
+    }
+}
+
 // T: Bf16 or Fp16 with codes; void: the bytes as they are (row_bytes / 16 threads a row).  A thread
-// takes its 16 bytes of LINES rows, 256 / TPR rows apart.
-template<typename T, int TPR, int LINES>
+// takes its 16 bytes of LINES rows, 256 / TPR rows apart.  AT_ONCE: all of them are on their way beside the
+// lengths, also those that turn out not to be new.
+template<typename T, int TPR, int LINES, bool AT_ONCE>
 __global__ __launch_bounds__(256)
 void paged_append_kernel(const PagedMoveParams p)
 {
@@ -86,7 +115,10 @@ void paged_append_kernel(const PagedMoveParams p)
         // (behind the last row: it again, not written)
         const uint32_t row = min(row0 + k * (256u / TPR), p.all_rows - 1);
         const u32x4 *const from = reinterpret_cast<const u32x4 *>(p.src[which] + (int64_t)row * (TPR * 16)) + piece;
-        raw[k] = *from;         // (on its way beside the lengths)
+        if constexpr(AT_ONCE)
+        {
+            raw[k] = *from;
+        }
         int r;
         dense_row(p, row, n[k], h[k], r);
         const int given = paged_new(p.c, n[k], p.rows);
@@ -95,11 +127,43 @@ void paged_append_kernel(const PagedMoveParams p)
         {
             pos[k] = -1;
         }
+        if constexpr(!AT_ONCE)
+        {
+            raw[k] = pos[k] >= 0 ? *from : u32x4{0, 0, 0, 0};
+        }
     }
 #pragma unroll
     for(int k = 0; k < LINES; ++k)
     {
         page[k] = pos[k] >= 0 ? page_of(p.c, n[k], pos[k]) : -1;
+    }
+    // Largest sizes, as integers: an infinity is larger than every number, a NaN than an infinity.  Two rows
+    // share a word.
+    uint32_t top[LINES];
+    if constexpr(PACK)
+    {
+#pragma unroll
+        for(int k = 0; k < LINES; ++k)
+        {
+            uint32_t x = 0;
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+            {
+                x = max_halves(x, raw[k][i] & 0x7fff7fffu);
+            }
+            top[k] = max(x & 0xffffu, x >> 16);
+        }
+        if constexpr(LINES == 2)
+        {
+            const uint32_t both = row_max<TPR>(top[0] | top[1] << 16);
+            top[0] = both & 0xffffu;
+            top[1] = both >> 16;
+        }
+        else
+        {
+            static_assert(LINES == 1, "one or two rows a thread");
+            top[0] = row_max<TPR>(top[0]);
+        }
     }
 #pragma unroll
     for(int k = 0; k < LINES; ++k)
@@ -116,30 +180,16 @@ void paged_append_kernel(const PagedMoveParams p)
         }
         else
         {
-            float x[8];
-            uint32_t top = 0;
-#pragma unroll
-            for(int i = 0; i < 8; ++i)
-            {
-                x[i] = T::to_float((uint16_t)(raw[k][i / 2] >> (16 * (i % 2))));
-                top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-            }
-            // (as integers: an infinity is larger than every number, a NaN than an infinity)
-            top = row_max<TPR>(top);
             u32x2 codes = {0x7f7f7f7fu, 0x7f7f7f7fu};
             int e = 0;
-            if(top < 0x7f800000u)
+            const uint32_t bits = __float_as_uint(T::to_float((uint16_t)top[k]));
+            if(bits < 0x7f800000u)
             {
                 // 448 = 1.75 * 2^8
-                e = max((int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0), -126);
-                const float scale = __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-                for(int j = 0; j < 2; ++j)
-                {
-                    int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j] * scale, x[4 * j + 1] * scale, 0, false);
-                    c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j + 2] * scale, x[4 * j + 3] * scale, c, true);
-                    codes[j] = (uint32_t)c;
-                }
+                e = max((int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), -126);
+                const float scale = __uint_as_float((uint32_t)(127 + e) << 23);
+                codes[0] = narrow2<T, true>(narrow2<T, false>(0u, raw[k][0], scale), raw[k][1], scale);
+                codes[1] = narrow2<T, true>(narrow2<T, false>(0u, raw[k][2], scale), raw[k][3], scale);
             }
             __builtin_nontemporal_store(codes, reinterpret_cast<u32x2 *>(to + piece * 8));
             if(piece == 0)
@@ -254,11 +304,11 @@ void paged_read_kernel(const PagedMoveParams p)
     }
 }
 
-template<typename T, int TPR, int LINES>
+template<typename T, int TPR, int LINES, bool AT_ONCE>
 static int launch_append(hipStream_t stream, const PagedMoveParams &p)
 {
     constexpr int64_t ROWS = LINES * 256 / TPR;
-    hipLaunchKernelGGL((paged_append_kernel<T, TPR, LINES>), dim3((unsigned)((p.all_rows + ROWS - 1) / ROWS), 2),
+    hipLaunchKernelGGL((paged_append_kernel<T, TPR, LINES, AT_ONCE>), dim3((unsigned)((p.all_rows + ROWS - 1) / ROWS), 2),
             dim3(256), 0, stream, p);
     return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;
 }
@@ -276,14 +326,18 @@ template<typename T, int TPR>
 static int launch_move(hipStream_t stream, const PagedMoveParams &p, bool read)
 {
     // Several rows a thread once that leaves every CU eight workgroups, as many as keep 32 bytes of the
-    // pages on their way: appending 4 x 10240 rows in 8 bits 17.0 us with one, 16.5 with two, 18.9 with four;
+    // pages on their way: appending 4 x 8 x 4096 rows in 8 bits 17.2 us with one, 16.6 with two, 17.6 with four;
     // reading 8 x 8192 rows of 8 bits 78.6 with two, 72.1 with four, 8 x 4096 of 16 bits 44.2 and 47.3.
     constexpr int LINES = __is_same(T, void) ? 2 : 4;
     const int64_t bytes = (int64_t)p.all_rows * TPR * 16 * 2;       // of the dense side
     const bool many = bytes >= 16ll * 256 * 256 * 8 * 2;
     if(!read)
     {
-        return many ? launch_append<T, TPR, 2>(stream, p) : launch_append<T, TPR, 1>(stream, p);
+        // Rows that are not new are not fetched where there are many (4 x 8 x 4096 rows, of which three fifths are
+        // new, 16.5 -> 15.4 us; where all are new, that order costs 18.9 -> 20.0).
+        return !many ? launch_append<T, TPR, 1, true>(stream, p)
+            : p.c.new_rows == nullptr ? launch_append<T, TPR, 2, true>(stream, p)
+            : launch_append<T, TPR, 2, false>(stream, p);
     }
     // What is read stays out of the caches (non-temporal) where it would not stay in the 256 MB of the
     // last level anyway: 34 MB in all 7.2 us, 8.4 non-temporal; 403 MB 78.6 and 72.1.
