@@ -68,16 +68,20 @@ struct PagedShape
     static constexpr int RB = KIND == kPaged32 ? HEAD * 4 : KIND == kPaged8 ? HEAD : HEAD * 2;   // bytes of a row
     static constexpr int CPR = RB / 16;                     // 16-byte chunks of a row
     static constexpr int RPL = RB >= 256 ? 1 : 256 / RB;    // rows per 256-byte line of LDS banks
-    // keys of a wavefront's step: 8 KB of K and V; twice that, up to 64, where two wavefronts share them
+    // keys of a wavefront's step: 8 KB of K and V; twice that where two wavefronts share them and the pages hold
+    // 16 bits (8 sequences of 8192 rows, 8 heads of 128, 64 query rows 54.8 us, 58.7 with 8 KB; 8-bit pages, whose
+    // widened operands are more registers, 51.7 and 47.7)
     static constexpr int ALONE = 4096 / RB > 16 ? 4096 / RB : 16;
-    static constexpr int KEYS = HALVES * ALONE < 64 ? HALVES * ALONE : 64;
+    static constexpr int KEYS = KIND == kPaged8 ? ALONE : HALVES * ALONE < 64 ? HALVES * ALONE : 64;
     static constexpr int BLOCK = STREAMS * KEYS;        // keys of a workgroup's step
     static constexpr int GROUPS = KEYS / 16;
     static constexpr int K_BYTES = KEYS * RB;
     static constexpr int STAGE = 2 * K_BYTES;
     static constexpr int LOADS = K_BYTES / 1024;            // load instructions of a step's K
     static constexpr int ROWS_PER_LOAD = 1024 / RB;
-    static constexpr int RING = STREAMS * 2 * STAGE;
+    // (what a row block of all wavefronts takes at the end, too)
+    static constexpr int MERGE_BYTES = STREAMS * 16 * HALVES * (HEAD + 4 + 2) * 4;
+    static constexpr int RING = STREAMS * 2 * STAGE > MERGE_BYTES ? STREAMS * 2 * STAGE : MERGE_BYTES;
     static constexpr int WGS_PER_CU = RING > 72 * 1024 || WAVES > 4 ? 1 : 2;
     static constexpr int MIN_WAVES = WAVES * WGS_PER_CU / 4;        // of a SIMD
     // the query rows: the operands of one block of 16 stay in registers, those of two in LDS
@@ -469,12 +473,14 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     constexpr float kLift = RANGED && KIND == kPaged16 ? kPagedLift : 0.0f;
 
     constexpr int MERGE_LD = HEAD + 4;
-    constexpr int MERGE_BYTES = STREAMS * 16 * HALVES * (MERGE_LD + 2) * 4;
-    static_assert(MERGE_BYTES <= Shape::RING, "the wavefronts' results of a row block share the ring");
+    static_assert(STREAMS * 16 * HALVES * (MERGE_LD + 2) * 4 <= Shape::RING,
+            "the wavefronts' results of a row block share the ring");
     constexpr int JOIN_ROWS = THREADS / (HEAD / 4);     // rows that are joined at a time
     static_assert(JOIN_ROWS * (HEAD + 4) * 4 <= Shape::RING, "... and so do the shares' sums");
     __shared__ __attribute__((aligned(1024))) char ring[Shape::RING];
     __shared__ __attribute__((aligned(16))) char q_rows[Shape::Q_BYTES];
+    // 8-bit pages: the scale bytes of a wavefront's step and of the next, keys' and values'
+    __shared__ __attribute__((aligned(16))) char scale_bytes[KIND == kPaged8 ? WAVES * 2 * 2 * KEYS : 16];
     __shared__ int scan_of[THREADS], wave_sum[WAVES], found;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
@@ -856,35 +862,43 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                 }
             }
         };
-        // the scale bytes of a step, through the scalar cache, and those of keys 16g + 4 * which .. + 3 of it
-        auto load_scales = [&](int i, const int (&page)[GROUPS], u32x4 (&k)[GROUPS], u32x4 (&v)[GROUPS])
+        // The scale bytes of a step go to LDS like the rows, 16 a lane: lane g < GROUPS has those of the keys of
+        // group g, lane GROUPS + g those of the values.  (Through the scalar cache they take more scalar
+        // registers than there are: 64 sequences of 17 to 16384 rows, 8 heads of 64, 46.9 -> 42.5 us.)
+        char *const scale_slots = scale_bytes + (KIND == kPaged8 ? wave * 4 * KEYS : 0);
+        const char *const scales_of_lane = reinterpret_cast<const char *>(lane < GROUPS ? p.c.k_scales : p.c.v_scales);
+        auto fetch_scales = [&](int i, const int (&page)[GROUPS])
         {
             int64_t from[GROUPS];
             places(i, page, p.c.scale_stride, 1, from);
-#pragma unroll
-            for(int g = 0; g < GROUPS; ++g)
+            const int g = lane % GROUPS;
+            int64_t mine = from[0] + 16 * g;
+            if(GROUPS > 1 && !one_page)
             {
-                k[g] = scalar_load<u32x4>(p.c.k_scales, from[g]);
-                v[g] = scalar_load<u32x4>(p.c.v_scales, from[g]);
+                mine = from[0];
+#pragma unroll
+                for(int j = 1; j < GROUPS; ++j)
+                {
+                    mine = g == j ? from[j] : mine;
+                }
             }
-        };
-        auto of_lane = [&](const u32x4 &w, int which)
-        {
-            return which == 0 ? w[0] : which == 1 ? w[1] : which == 2 ? w[2] : w[3];
+            if(lane < 2 * GROUPS)
+            {
+                load_to_lds16<0, false>(scales_of_lane + mine, scale_slots + (i & 1) * 2 * KEYS);
+            }
         };
 
         int page[GROUPS], page_next[GROUPS];
-        constexpr int SCALES = KIND == kPaged8 ? GROUPS : 1;
-        u32x4 k_raw[SCALES], v_raw[SCALES];     // of the next step
+        constexpr int STEP_LOADS = (PAIRED ? LOADS : 2 * LOADS) + (KIND == kPaged8 ? 1 : 0);
         if(n_mine > 0)
         {
             look_up(0, page);
             fetch(0, page, slots);
-            look_up(min(1, n_mine - 1), page_next);
             if constexpr(KIND == kPaged8)
             {
-                load_scales(0, page, k_raw, v_raw);
+                fetch_scales(0, page);
             }
+            look_up(min(1, n_mine - 1), page_next);
         }
         // The count of the unit's shares that are done, at the place of its first share (every share is the
         // first of one shared unit at most).  It has kPagedNone between calls; if it holds something else,
@@ -916,21 +930,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         {
             constexpr bool PARTLY = decltype(partly)::value;
             char *const slot = slots + (i & 1) * STAGE;
-            uint32_t ks[GROUPS], vs[GROUPS];
-            uint32_t hidden = 0;
-            if(!PARTLY || !PAIRED || i < n_mine)
-            {
-                if constexpr(KIND == kPaged8)
-                {
-#pragma unroll
-                    for(int g = 0; g < GROUPS; ++g)
-                    {
-                        ks[g] = of_lane(k_raw[g], KSCALE_IN_CODES ? col >> 2 : quad);
-                        vs[g] = of_lane(v_raw[g], quad);
-                    }
-                }
-                hidden = PARTLY ? without_page() : 0;
-            }
+            const uint32_t hidden = PARTLY ? without_page() : 0;
             // the reads of the slot that is filled next have returned (to both)
             paged_wait_lds();
             if constexpr(PAIRED)
@@ -940,17 +940,17 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             if(i + 1 < n_mine)
             {
                 fetch(i + 1, page_next, slots + ((i + 1) & 1) * STAGE);
+                if constexpr(KIND == kPaged8)
+                {
+                    fetch_scales(i + 1, page_next);
+                }
 #pragma unroll
                 for(int g = 0; g < GROUPS; ++g)
                 {
                     page[g] = page_next[g];
                 }
                 look_up(min(i + 2, n_mine - 1), page_next);
-                if constexpr(KIND == kPaged8)
-                {
-                    load_scales(i + 1, page, k_raw, v_raw);
-                }
-                paged_wait_loads<PAIRED ? LOADS : 2 * LOADS>();
+                paged_wait_loads<STEP_LOADS>();
             }
             else
             {
@@ -979,6 +979,20 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                     }
                 }
                 paged_wait_lds();
+            }
+
+            // scale bytes of four keys of each group: the keys', of those around the lane's key row where they go
+            // into its codes, else of the lane's scores; the values', of the lane's probabilities
+            uint32_t ks[GROUPS], vs[GROUPS];
+            if constexpr(KIND == kPaged8)
+            {
+                const char *const bytes = scale_slots + (i & 1) * 2 * KEYS;
+#pragma unroll
+                for(int g = 0; g < GROUPS; ++g)
+                {
+                    ks[g] = *reinterpret_cast<const uint32_t *>(bytes + 16 * g + 4 * (KSCALE_IN_CODES ? col >> 2 : quad));
+                    vs[g] = *reinterpret_cast<const uint32_t *>(bytes + KEYS + 16 * g + 4 * quad);
+                }
             }
 
             // ---- scores --------------------------------------------------------------
@@ -1036,7 +1050,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             f32x4 of_scale[GROUPS];
             if constexpr(KIND == kPaged8)
             {
-                float most = top_scale;
+                int most = 0, byte[GROUPS][4];
 #pragma unroll
                 for(int g = 0; g < GROUPS; ++g)
                 {
@@ -1044,18 +1058,18 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                     for(int e = 0; e < 4; ++e)
                     {
                         const bool there = !PARTLY || 4 * quad + e < ((hidden >> g) & 1 ? 0 : seg.len - key0 - 16 * g);
-                        const uint32_t byte = there ? (vs[g] >> (8 * e)) & 255u : 0u;
-                        of_scale[g][e] = RANGED ? (float)byte : __uint_as_float(byte << 23);
-                        most = RANGED ? fmaxf(most, of_scale[g][e]) : most;
+                        byte[g][e] = there ? (int)((vs[g] >> (8 * e)) & 255u) : 0;
+                        most = max(most, byte[g][e]);
                     }
                 }
+                int up = 0;         // what is added to the exponents
                 if constexpr(RANGED)
                 {
-                    most = quad_max(most);
-                    if(__any(most > top_scale))
+                    if(__any((float)most > top_scale))
                     {
-                        const float fade = fast_exp2(top_scale - most);
-                        top_scale = most;
+                        const float next = fmaxf(quad_max((float)most), top_scale);
+                        const float fade = fast_exp2(top_scale - next);
+                        top_scale = next;
 #pragma unroll
                         for(int nr = 0; nr < NR; ++nr)
                         {
@@ -1066,14 +1080,16 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                             }
                         }
                     }
+                    up = 127 + (int)kPagedLift - (int)top_scale;
+                }
 #pragma unroll
-                    for(int g = 0; g < GROUPS; ++g)
+                for(int g = 0; g < GROUPS; ++g)
+                {
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
                     {
-#pragma unroll
-                        for(int e = 0; e < 4; ++e)
-                        {
-                            of_scale[g][e] = fast_exp2(of_scale[g][e] - (top_scale - kPagedLift));
-                        }
+                        // (below 2^-126 of the largest: nothing)
+                        of_scale[g][e] = __uint_as_float((uint32_t)(RANGED ? max(byte[g][e] + up, 0) : byte[g][e]) << 23);
                     }
                 }
             }
