@@ -709,10 +709,25 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         }
         if(seg.steps > 0)
         {
-        const int h = seg.u / p.row_groups, rg = seg.u - h * p.row_groups;
+        // (the row groups of a head from both ends in turn: where the last ones see more keys than the first,
+        // shares of some units have equally much to do)
+        const int h = seg.u / p.row_groups, in_turn = seg.u - h * p.row_groups;
+        const int rg = (in_turn & 1) != 0 ? p.row_groups - 1 - (in_turn >> 1) : in_turn >> 1;
         const int given = uniform(paged_new(p.c, seg.n, p.q_seq));
         const int key_lo = seg.step * Shape::BLOCK;
-        const int key_hi = min(key_lo + seg.steps * Shape::BLOCK, seg.len);
+        // the keys that some row of the group sees, of the tokens of one head: those in front of the newest one's
+        int seen = seg.len;
+        if(p.row_groups > 1)
+        {
+            const int first = rg * QROWS, last_row = min(first + QROWS, p.rows) - 1;
+            const int head_of = uniform(first / p.q_seq);
+            if(last_row < (head_of + 1) * p.q_seq)
+            {
+                const int newest = min(last_row - head_of * p.q_seq, given - 1);
+                seen = first - head_of * p.q_seq >= given ? 0 : p.causal ? max(seg.len - given + newest + 1, 0) : seen;
+            }
+        }
+        const int key_hi = max(min(key_lo + seg.steps * Shape::BLOCK, min(seg.len, seen)), key_lo);
         const int my_first = key_lo + stream * KEYS;
         const int n_mine = my_first < key_hi ? (key_hi - my_first + Shape::BLOCK - 1) / Shape::BLOCK : 0;
 
@@ -911,7 +926,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         {
             held = __hip_atomic_load(count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        const int n_steps = PAIRED ? seg.steps : n_mine;
+        const int n_steps = PAIRED ? (key_hi - key_lo + Shape::BLOCK - 1) / Shape::BLOCK : n_mine;
         auto without_page = [&]()       // groups of the step
         {
             uint32_t hidden = (unsigned)page[0] < (unsigned)p.c.n_pages ? 0u : GROUPS == 1 || one_page ? ~0u : 1u;

@@ -56,3 +56,14 @@ def test_pages_longer_than_the_sequences(dtype, packed):
 def test_nothing_but_empty_sequences():
     for lens in ([0], [0, 0, 0], [-5, 0] * 40):
         _check(P.Case(49, "bf16", False, len(lens), 2, 64, 16, lens), 2, 3)
+
+
+@pytest.mark.parametrize("dtype,packed", KINDS)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("q_seq,group", [(150, 2), (64, 3), (129, 1)])
+def test_chunks_of_padded_sequences(dtype, packed, causal, q_seq, group):
+    """Row blocks whose tokens see a part of the keys, or that hold none of the sequence's tokens; sequences
+    with fewer rows than they bring tokens."""
+    lens, new_rows = [150, 333, 90, 40, 0], [q_seq, 70, 1, 60, q_seq]
+    _check(P.Case(50, dtype, packed, 5, 4, 64, 32, lens), q_seq, group, causal, new_rows)
+    _check(P.Case(51, dtype, packed, 2, 1, 128, 16, [1000, 400]), q_seq, group, causal, [q_seq, 33])
