@@ -652,7 +652,7 @@ int nntile_hip_mask_tile_class_bool(void *stream, int64_t k_rows, int64_t q_cols
  *   k_scales, v_scales [page_rows, n_head_kv, n_pages] bytes, scale_stride apart; both null: the
  *                      pages hold the tile type.  Else they hold e4m3 codes (bf16 and
  *                      fp16 tiles; fp32: NNTILE_HIP_EUNSUPPORTED) and row r of a page
- *                      stands for code * 2^(scale - 127).
+ *                      stands for code * 2^(scale - 127), scales from 1 to 254.
  *   table              [max_pages, n_batch], lens [n_batch]: int32, on the device and
  *                      read when the kernel runs, so a captured call follows them.
  *                      lens counts the rows of a sequence INCLUDING those that the
