@@ -575,20 +575,23 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     }
     const uint32_t shares = aligned ? n_units * of_unit : min(places, all);
     const PagedSplit split(all, shares);
-    // sequences without rows: shared out, too, for the rows of their queries
+    // sequences without rows: shared out, too, for the rows of their queries, some at a time
     if(p.overwrite && !(same && blocks_0 != 0))
     {
-        for(int n = blockIdx.x; n < p.c.n_batch; n += gridDim.x)
+        constexpr int SIDE_BY_SIDE = THREADS / (HEAD / 4), PIECE = 8 * SIDE_BY_SIDE;
+        const int rows = p.c.n_head_kv * p.rows, pieces = (rows - 1) / PIECE + 1;
+        for(uint32_t piece = blockIdx.x; piece < (uint32_t)p.c.n_batch * (uint32_t)pieces; piece += gridDim.x)
         {
+            const int n = (int)(piece / (uint32_t)pieces);
             if(uniform(paged_len(p.c, n)) == 0)
             {
-                const int rows = p.c.n_head_kv * p.rows;
-                for(int t = tid; t < rows * (HEAD / 4); t += THREADS)
+                const int first = (int)(piece - (uint32_t)n * (uint32_t)pieces) * PIECE;
+                const int here = min(rows - first, PIECE);
+                for(int k = tid / (HEAD / 4); k < here; k += SIDE_BY_SIDE)
                 {
-                    const int r = t / (HEAD / 4);
                     const f32x2 zero[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
-                    paged_finish_row<T, HEAD / 4, 2>(p, paged_query_row(p, n, r / p.rows, r % p.rows),
-                            t % (HEAD / 4), neg_inf(), 0.0f, zero);
+                    paged_finish_row<T, HEAD / 4, 2>(p, paged_query_row(p, n, (first + k) / p.rows,
+                                (first + k) % p.rows), tid % (HEAD / 4), neg_inf(), 0.0f, zero);
                 }
             }
         }
