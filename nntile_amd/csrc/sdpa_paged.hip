@@ -566,11 +566,22 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     const float keys = (float)all / (float)n_units * (float)Shape::BLOCK;
     const float most = fmaxf(sqrtf(keys / (float)min(p.rows, QROWS)), 1.0f);
     const uint32_t places = (uint32_t)uniform((int)fminf((float)p.shares, (float)n_units * most));
-    const bool aligned = same && n_units <= places && blocks_0 != 0;
+    // Equal units whose steps wait for memory more than for instructions: a workgroup a CU, where that leaves
+    // none of eight CUs without one (8 heads of 128; 16-bit pages, 32 sequences of 1024, 32 query rows 34.2 ->
+    // 28.0 us, 4 query rows 27.8 -> 25.6, but 20 sequences of 2000, 160 units, 33.4 -> 40.2; 8-bit pages, 32
+    // query rows 26.4 -> 20.9, 4 query rows over 2048 30.4 -> 36.0).  32 query rows over 16-bit pages are better
+    // off in any case (those 160 units 40.7 -> 36.3), unequal units in none (64 of 17 to 8192, 32 query rows
+    // 99 -> 137).
+    constexpr bool ONE_A_CU = KIND == kPaged16 || (KIND == kPaged8 && NR == 2);
+    const uint32_t cus_filled = n_units <= kPagedCUs ? kPagedCUs / n_units * n_units : 0;
+    const uint32_t equal_places = ONE_A_CU && p.row_groups == 1
+        && (8 * cus_filled >= 7 * kPagedCUs || (KIND == kPaged16 && NR == 2 && cus_filled != 0))
+        ? min(places, (uint32_t)kPagedCUs) : places;
+    const bool aligned = same && n_units <= equal_places && blocks_0 != 0;
     uint32_t of_unit = 1;
     if(aligned)
     {
-        const uint32_t each = places / n_units, longest = ((uint32_t)blocks_0 + each - 1) / each;
+        const uint32_t each = equal_places / n_units, longest = ((uint32_t)blocks_0 + each - 1) / each;
         of_unit = ((uint32_t)blocks_0 + longest - 1) / longest;
     }
     const uint32_t shares = aligned ? n_units * of_unit : min(places, all);
