@@ -298,6 +298,8 @@ class PagedKVCache:
                     and t.device.index == torch.cuda.current_device()):
                 raise ValueError("tiles must be contiguous device tensors of the cache's device, "
                                  "which is the current one")
+            if t.data_ptr() % 16:
+                raise ValueError("tiles start at multiples of 16 bytes")
         rows = k.shape[1]
         counts = self._counts(rows, new_rows)
         self._reserve(counts, stream)

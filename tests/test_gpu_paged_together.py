@@ -297,6 +297,11 @@ def test_a_refused_append_changes_nothing(dtype, packed):
         with pytest.raises(ValueError):
             c.append(k, v, new_rows=bad)
     unchanged()
+    off = torch.zeros(k.numel() + 1, dtype=k.dtype, device="cuda")[1:].view(k.shape)
+    for tiles in ((off, v), (k, off), (k.transpose(0, 1), v), (k, v[:, :-1].contiguous()), (k, v.cpu())):
+        with pytest.raises(ValueError):
+            c.append(*tiles, new_rows=[1, 1])
+    unchanged()
     c.attend(Q, lse, A, 1, new_rows=[40, 30])
     mine.check(Q, lse, A, 1, True, [40, 30])
 
