@@ -712,7 +712,9 @@ int nntile_hip_paged_kv_read_fp32(void *stream, const nntile_hip_paged_cache *ca
  * sequences without rows see nothing.  flags: 0 or NNTILE_HIP_SDPA_OVERWRITE, with
  * the meaning they have for the decode entry points (rows that see nothing, rows
  * with a NaN among their scores).  What lies in rows that a query does not see -
- * NaN, infinities - does not reach it.
+ * NaN, infinities, the size of 8-bit rows - does not reach it.  Probabilities are
+ * rounded for the products: over 16-bit pages to the tile type, over 8-bit pages to
+ * 8 bits (bf16 tiles) or 16 (fp16) with the exponents of fp32.
  * The keys of all sequences are shared out evenly over the chip's workgroups,
  * whatever the lengths; shares of one sequence are joined in fp32 in the order of
  * the keys.  The same call gives the same bits every time.

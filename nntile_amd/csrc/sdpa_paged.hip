@@ -27,15 +27,16 @@
 //    What bounds 64 rows is the issue of the softmax's vector instructions.
 //  * 8-bit pages: codes become values of the tile type exactly in front of the matrix instructions.
 //    The power of two of a key row goes into its codes (bf16) or into the score (fp16), that of a value
-//    row into the probability.
+//    row into the probability: as a bf16 number over bf16 tiles, as the sum of two over fp16 tiles, so that it
+//    has fp32's exponents and more bits than fp16, whatever the powers of two of other rows are.
 //
 // What it reaches, 8 heads of 128, bytes of the cache alone: 64 sequences of 1024 bf16 rows, 4 query rows a
 // head 5.9 TB/s, 32 rows 5.7, 64 rows 4.4; 64 of 2048 8-bit rows 5.8, 5.2 and 3.4.  8 of 8192 bf16 rows, 64
 // query rows, 270 MB: 54.7 us = 4.9 TB/s.  A single sequence of 1001 rows, 4 MB: 8.7 us, the chain from
 // the lengths over the table and the keys to the join, a memory latency each.
 //
-// Probabilities are rounded to the tile type for the matrix instruction, as in the other attention
-// kernels; the sum of the softmax takes them unrounded.
+// Probabilities of 16-bit tiles are rounded for the matrix instruction, as in the other attention kernels: to
+// the tile type, over 8-bit pages of fp16 to 16 bits.  The sum of the softmax takes them unrounded.
 #include <type_traits>
 
 #include "paged.hpp"
@@ -56,7 +57,7 @@ constexpr int kPagedShares = 2 * kPagedCUs;
 constexpr int kPagedUnitCost = 1;
 // How far, in powers of two, probabilities may grow past 1 before they are taken against a new maximum
 constexpr float kPagedSlack = 8.0f;
-// fp16 probabilities are kept times 2^7: they stay below 2^15, and 2^-21 still has all of its bits
+// fp16 probabilities of 16-bit pages are kept times 2^7: they stay below 2^15, and 2^-21 still has all of its bits
 constexpr float kPagedLift = 7.0f;
 // Counts of shares in the workspace: in the low bits, above them a fixed word by which a count is told
 // from what else memory may hold; a cache line each.
@@ -471,15 +472,18 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     constexpr int QREGS = KIND == kPaged32 ? HEAD / 16 : HEAD / 32;
     constexpr int QROWS = Shape::QROWS;
     constexpr bool Q_IN_LDS = NR > 1;
-    // the type of the probabilities and values as the matrix instruction takes them
-    typedef typename std::conditional<__is_same(T, float), Fp16, T>::type PV;
-    // 8-bit pages, bf16: the scale of a key row goes into its codes (exact in bf16), that of a value row
-    // into its probabilities.  fp16 has not the range for either: its key scales go into
-    // the scores, and its probabilities take 2^(scale - largest scale so far + kPagedLift).
+    // the type of the probabilities and values as the matrix instruction takes them (fp32 pages: neither)
+    typedef typename std::conditional<KIND == kPaged16, T, Bf16>::type PV;
+    // 8-bit pages: the scale of a key row goes into its codes (exact in bf16; fp16 has not the range: into the
+    // scores), that of a value row into its probabilities, which are bf16 numbers then and the codes exact in
+    // bf16.  For fp16 tiles 8 bits are too few: what the first number leaves of a probability is a second one,
+    // with products of its own (64 of 2048 rows, 8 heads of 128: 47 us with 4 query rows, 55 with 32, 94 with 64;
+    // as one fp16 number against the largest power of two so far 47, 54 and 84, but then a row that is not seen, or
+    // has no weight, takes the bits of smaller ones).
     constexpr bool KSCALE_IN_CODES = KIND == kPaged8 && __is_same(T, Bf16);
-    constexpr bool RANGED = __is_same(PV, Fp16) && KIND != kPaged32;
+    constexpr bool TWO_PARTS = KIND == kPaged8 && __is_same(T, Fp16);
     // the power of two that the probabilities, and so their sum, carry
-    constexpr float kLift = RANGED && KIND == kPaged16 ? kPagedLift : 0.0f;
+    constexpr float kLift = KIND == kPaged16 && __is_same(T, Fp16) ? kPagedLift : 0.0f;
 
     constexpr int MERGE_LD = HEAD + 4;
     static_assert(STREAMS * 16 * HALVES * (MERGE_LD + 2) * 4 <= Shape::RING,
@@ -818,7 +822,6 @@ void sdpa_paged_kernel(const PagedAttendParams p)
 
         f32x4 o[NR][DBLOCKS];
         float m_run[NR], l_run[NR];
-        float top_scale = 0.0f;         // the largest scale byte of the value rows so far
 #pragma unroll
         for(int nr = 0; nr < NR; ++nr)
         {
@@ -1088,50 +1091,20 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             f32x4 of_scale[GROUPS];
             if constexpr(KIND == kPaged8)
             {
-                int most = 0, byte[GROUPS][4];
 #pragma unroll
                 for(int g = 0; g < GROUPS; ++g)
                 {
 #pragma unroll
                     for(int e = 0; e < 4; ++e)
                     {
+                        // (a row that does not exist: whatever its byte, times a probability of 0)
                         const bool there = !PARTLY || 4 * quad + e < ((hidden >> g) & 1 ? 0 : seg.len - key0 - 16 * g);
-                        byte[g][e] = there ? (int)((vs[g] >> (8 * e)) & 255u) : 0;
-                        most = max(most, byte[g][e]);
-                    }
-                }
-                int up = 0;         // what is added to the exponents
-                if constexpr(RANGED)
-                {
-                    if(__any((float)most > top_scale))
-                    {
-                        const float next = fmaxf(quad_max((float)most), top_scale);
-                        const float fade = fast_exp2(top_scale - next);
-                        top_scale = next;
-#pragma unroll
-                        for(int nr = 0; nr < NR; ++nr)
-                        {
-#pragma unroll
-                            for(int db = 0; db < DBLOCKS; ++db)
-                            {
-                                o[nr][db] *= fade;
-                            }
-                        }
-                    }
-                    up = 127 + (int)kPagedLift - (int)top_scale;
-                }
-#pragma unroll
-                for(int g = 0; g < GROUPS; ++g)
-                {
-#pragma unroll
-                    for(int e = 0; e < 4; ++e)
-                    {
-                        // (below 2^-126 of the largest: nothing)
-                        of_scale[g][e] = __uint_as_float((uint32_t)(RANGED ? max(byte[g][e] + up, 0) : byte[g][e]) << 23);
+                        of_scale[g][e] = there ? scale_of(vs[g], e) : 0.0f;
                     }
                 }
             }
             uint32_t pw[NR][GROUPS][2];                 // 16-bit pairs
+            uint32_t pw_rest[TWO_PARTS ? NR : 1][TWO_PARTS ? GROUPS : 1][2];        // what they leave
             f32x4 pf[NR][GROUPS];                       // fp32
 #pragma unroll
             for(int nr = 0; nr < NR; ++nr)
@@ -1197,6 +1170,16 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                     {
                         pf[nr][g] = x;
                     }
+                    else if constexpr(TWO_PARTS)
+                    {
+                        // the first 8 bits as they are, the next 8 rounded: 2^-16 of a probability is lost at most
+                        const u32x4 bits = __builtin_bit_cast(u32x4, x);
+                        const f32x4 rest = x - __builtin_bit_cast(f32x4, bits & 0xffff0000u);
+                        pw[nr][g][0] = __builtin_amdgcn_perm(bits[1], bits[0], 0x07060302u);
+                        pw[nr][g][1] = __builtin_amdgcn_perm(bits[3], bits[2], 0x07060302u);
+                        pw_rest[nr][g][0] = PV::pack2(rest[0], rest[1]);
+                        pw_rest[nr][g][1] = PV::pack2(rest[2], rest[3]);
+                    }
                     else
                     {
                         pw[nr][g][0] = PV::pack2(x[0], x[1]);
@@ -1256,8 +1239,14 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                 }
                 else
                 {
-                    return mfma32<PV>(w, u32x4{pw[nr][2 * t][0], pw[nr][2 * t][1], pw[nr][2 * t + 1][0],
+                    c = mfma32<PV>(w, u32x4{pw[nr][2 * t][0], pw[nr][2 * t][1], pw[nr][2 * t + 1][0],
                             pw[nr][2 * t + 1][1]}, c);
+                    if constexpr(TWO_PARTS)
+                    {
+                        c = mfma32<PV>(w, u32x4{pw_rest[nr][2 * t][0], pw_rest[nr][2 * t][1],
+                                pw_rest[nr][2 * t + 1][0], pw_rest[nr][2 * t + 1][1]}, c);
+                    }
+                    return c;
                 }
             };
             constexpr int TSTEPS = KIND == kPaged32 ? GROUPS : (GROUPS + 1) / 2;
@@ -1381,8 +1370,6 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             __syncthreads();        // every wavefront is done with the ring, or with the last row block
             const int mine = wave * 16 + col;
             float m = m_run[nr] * c_log2 - kLift, l = quad_sum(l_run[nr]);
-            // what the products of this wavefront are times
-            const float to_m = KIND == kPaged8 && RANGED ? fast_exp2(top_scale - (127.0f + kPagedLift)) : 1.0f;
             if(!row_ok[nr])
             {
                 m = neg_inf();
@@ -1391,13 +1378,8 @@ void sdpa_paged_kernel(const PagedAttendParams p)
 #pragma unroll
             for(int db = 0; db < DBLOCKS; ++db)
             {
-                f32x4 x = o[nr][db];
-                if constexpr(KIND == kPaged8 && RANGED)
-                {
-                    x *= to_m;
-                }
                 *reinterpret_cast<f32x4 *>(merge_o + mine * MERGE_LD + 16 * db + 4 * quad)
-                    = row_ok[nr] ? x : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    = row_ok[nr] ? o[nr][db] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
             if(quad == 0)
             {
