@@ -714,7 +714,10 @@ int nntile_hip_paged_kv_read_fp32(void *stream, const nntile_hip_paged_cache *ca
  * with a NaN among their scores).  What lies in rows that a query does not see -
  * NaN, infinities, the size of 8-bit rows - does not reach it.  Probabilities are
  * rounded for the products: over 16-bit pages to the tile type, over 8-bit pages to
- * 8 bits (bf16 tiles) or 16 (fp16) with the exponents of fp32.
+ * 8 bits (bf16 tiles) or 16 (fp16) with the exponents of fp32.  Values are summed up
+ * in fp32 with weights of at most 1, the largest from 2^-8 on, and divided by the
+ * sum of the weights at the end: where the sum is past fp32, A is infinite or NaN
+ * though its own values might not be.
  * The keys of all sequences are shared out evenly over the chip's workgroups,
  * whatever the lengths; shares of one sequence are joined in fp32 in the order of
  * the keys.  The same call gives the same bits every time.

@@ -55,7 +55,7 @@ constexpr int kPagedCUs = 256;
 constexpr int kPagedShares = 2 * kPagedCUs;
 // What a unit costs beside its key blocks, in blocks
 constexpr int kPagedUnitCost = 1;
-// How far, in powers of two, probabilities may grow past 1 before they are taken against a new maximum
+// How far, in powers of two, probabilities may grow past the first before they are taken against a new maximum
 constexpr float kPagedSlack = 8.0f;
 // fp16 probabilities of 16-bit pages are kept times 2^7: they stay below 2^15, and 2^-21 still has all of its bits
 constexpr float kPagedLift = 7.0f;
@@ -482,8 +482,9 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     // has no weight, takes the bits of smaller ones).
     constexpr bool KSCALE_IN_CODES = KIND == kPaged8 && __is_same(T, Bf16);
     constexpr bool TWO_PARTS = KIND == kPaged8 && __is_same(T, Fp16);
-    // the power of two that the probabilities, and so their sum, carry
-    constexpr float kLift = KIND == kPaged16 && __is_same(T, Fp16) ? kPagedLift : 0.0f;
+    // the power of two that the probabilities, and so their sum, carry: where they have fp32's exponents, they
+    // stay below 1, so that products with the largest values do not overflow
+    constexpr float kLift = KIND == kPaged16 && __is_same(T, Fp16) ? kPagedLift : -kPagedSlack;
 
     constexpr int MERGE_LD = HEAD + 4;
     static_assert(STREAMS * 16 * HALVES * (MERGE_LD + 2) * 4 <= Shape::RING,

@@ -94,3 +94,28 @@ def test_rows_of_all_sizes(dtype, lens, q_seq, group):
     x[~c.there[:, None, None].expand(x.shape[:4])] = float("nan")
     c.pool = x.to(c.pool.dtype)
     _check(c, _queries(66, c, q_seq, group), q_seq, group)
+
+
+@pytest.mark.parametrize("dtype,packed", [("bf16", False), ("fp32", False), ("bf16", True)])
+@pytest.mark.parametrize("head", [64, 128])
+@pytest.mark.parametrize("q_seq,group", [(1, 1), (2, 12), (5, 12)])
+def test_large_values_behind_small_scores(dtype, packed, head, q_seq, group):
+    """A few keys late in the sequence score a little more than those before them, less than makes the running
+    maximum worth replacing, and have values of 2^124: their sum is a number of the type."""
+    n_batch, heads, length = 8, 24, 1024
+    c = P.Case(67, dtype, packed, n_batch, heads, head, 128, [length] * n_batch, spread=0)
+    c.scales[:] = 127
+    x = c.pool.float()
+    x[:, 0] = 0.0
+    for n in range(n_batch):
+        for pos in (length - 301, length - 200, length - 99):
+            page, at = _row(c, n, pos)
+            # a score of 4.85, so a probability of 2^7 times the others'
+            x[page, 0, :, at] = 4.85 / head ** 0.5
+            big = 1.0 + 0.25 * (torch.arange(head) % 4)
+            x[page, 1, :, at] = 64.0 * big if packed else 2.0 ** 124 * big
+            c.scales[page, 1, :, at] = 127 + 118
+    c.pool = x.to(c.pool.dtype)
+    q = torch.ones(heads * group * n_batch, q_seq, head).to(P.TORCH_DT[dtype])
+    A, _ = _check(c, q, q_seq, group)
+    assert float(A.float().min()) > 2.0 ** 121
