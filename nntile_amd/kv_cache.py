@@ -269,6 +269,14 @@ class PagedKVCache:
         if stream is not None:
             target.record_stream(stream)
 
+    def _in_use(self, stream, *tensors):
+        """The cache's tensors and these are in use on a stream that is given: memory of
+        theirs that is freed waits for it."""
+        if stream is not None:
+            for t in (self.pool, self.scales, self.table, self.lens) + tensors:
+                if t is not None:
+                    t.record_stream(stream)
+
     def _reserve(self, counts, stream):
         wanted = []
         for n, count in enumerate(counts):
@@ -312,10 +320,7 @@ class PagedKVCache:
         else:
             self._upload(self.lens, lengths, stream)
             given = self._on_device(counts, stream)
-        if stream is not None:
-            for t in (k, v, self.lens, self.pool, self.scales):
-                if t is not None:
-                    t.record_stream(stream)
+        self._in_use(stream, k, v)
         hip_sdpa.paged_kv_append(k, v, self.k_pages, self.v_pages, self.table, self.lens, self.k_scales,
                                  self.v_scales, new_rows=given, stream=stream)
         self.lengths = lengths
@@ -335,6 +340,7 @@ class PagedKVCache:
             k = torch.empty((self.n_head_kv * self.n_batch, rows, self.head), dtype=self.dtype,
                             device=self.lens.device)
             v = torch.empty_like(k)
+        self._in_use(stream)
         hip_sdpa.paged_kv_read(self.k_pages, self.v_pages, self.table, self.lens, k, v, first=first,
                                k_scales=self.k_scales, v_scales=self.v_scales, stream=stream)
         return k, v
@@ -361,6 +367,7 @@ class PagedKVCache:
         counts = self._counts(q_seq, new_rows)
         mode = hip_sdpa.MASK_CAUSAL if causal else hip_sdpa.MASK_NONE
         length = self.lengths[0]
+        self._in_use(stream, Q, lse, A)
         if (kv_group * q_seq >= self.DENSE_ROWS and new_rows is None and length >= q_seq
                 and min(self.lengths) == max(self.lengths)):
             k, v = self.read(stream=stream)
@@ -382,9 +389,7 @@ class PagedKVCache:
             with torch.cuda.stream(stream):
                 self._workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
         if stream is not None:
-            for t in (Q, lse, A, self._workspace, self.lens, self.table, self.pool, self.scales):
-                if t is not None:
-                    t.record_stream(stream)
+            self._workspace.record_stream(stream)
         hip_sdpa.sdpa_fwd_paged(self.k_pages, self.v_pages, self.table, self.lens, Q, lse, A, mode,
                                 kv_group, self._workspace, k_scales=self.k_scales, v_scales=self.v_scales,
                                 new_rows=given, flags=hip_sdpa.OVERWRITE, stream=stream)

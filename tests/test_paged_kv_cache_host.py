@@ -1,0 +1,84 @@
+"""What PagedKVCache does on the host around its calls: which tensors it tells the allocator of, which memory it keeps
+(no GPU: the calls are taken by doubles that note what they get)."""
+import contextlib
+
+import pytest
+import torch
+
+from nntile_amd import hip_sdpa as h
+from nntile_amd.kv_cache import PagedKVCache
+
+
+def _place(t):
+    return t.untyped_storage().data_ptr()
+
+
+class Doubles:
+    """Stand in for the calls of hip_sdpa and for the streams."""
+
+    def __init__(self, monkeypatch):
+        self.calls, self.recorded = [], []
+        for name in ("paged_kv_read", "sdpa_fwd_tile_cache", "sdpa_fwd_paged"):
+            monkeypatch.setattr(h, name, lambda *a, _name=name, **kw: self.calls.append((_name, a, kw)))
+        monkeypatch.setattr(h, "tile_cache_workspace_bytes", lambda *a, **kw: 4096)
+        monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext())
+        monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: self.recorded.append((_place(t), s)))
+
+    def told(self, stream):
+        return {place for place, s in self.recorded if s == stream}
+
+    def names(self):
+        return [name for name, _, _ in self.calls]
+
+    def tensors(self):
+        return {_place(t) for _, a, kw in self.calls for t in list(a) + list(kw.values()) if isinstance(t, torch.Tensor)}
+
+
+def _cache(lengths, packed=True, **kw):
+    c = PagedKVCache(**dict(dict(n_pages=64, page_rows=64, n_batch=len(lengths), max_rows=1024, n_head_kv=2, head=64,
+                                 packed=packed, device="cpu"), **kw))
+    c.lengths = list(lengths)
+    return c
+
+
+def _queries(c, q_seq, group):
+    Q = torch.zeros(c.n_head_kv * group * c.n_batch, q_seq, c.head, dtype=c.dtype)
+    return Q, torch.zeros(Q.shape[:2]), torch.zeros_like(Q)
+
+
+def test_a_chunk_that_is_read_back_tells_of_its_tensors(monkeypatch):
+    """As many queries as go through the tile kernels, on a stream that is given: queries, results and the
+    cache's tensors are in use there."""
+    d = Doubles(monkeypatch)
+    c = _cache([600, 600])
+    tiles = _queries(c, 512, 1)
+    c.attend(*tiles, 1, stream="side")
+    assert d.names() == ["paged_kv_read", "sdpa_fwd_tile_cache"]
+    for t in tiles + (c.pool, c.scales, c.lens, c.table):
+        assert _place(t) in d.tensors() and _place(t) in d.told("side")
+
+
+def test_reading_back_tells_of_the_cache(monkeypatch):
+    d = Doubles(monkeypatch)
+    c = _cache([600, 30])
+    c.read(stream="side")
+    for t in (c.pool, c.scales, c.lens, c.table):
+        assert _place(t) in d.tensors() and _place(t) in d.told("side")
+
+
+def test_attention_over_the_pages_tells_of_its_tensors(monkeypatch):
+    d = Doubles(monkeypatch)
+    c = _cache([600, 30])
+    tiles = _queries(c, 5, 4)
+    c.attend(*tiles, 4, stream="side")
+    assert d.names() == ["sdpa_fwd_paged"]
+    assert d.tensors() <= d.told("side")
+
+
+def test_nothing_is_told_of_the_current_stream(monkeypatch):
+    d = Doubles(monkeypatch)
+    c = _cache([600, 600])
+    c.attend(*_queries(c, 512, 1), 1)
+    c.attend(*_queries(c, 3, 1), 1)
+    c.read()
+    assert d.recorded == []
