@@ -247,7 +247,7 @@ class PagedKVCache:
         self.lengths = [0] * n_batch
         self._pages = [[] for _ in range(n_batch)]
         self._free = list(range(n_pages - 1, -1, -1))
-        self._workspace = None
+        self._workspace, self._old_workspaces = None, []
 
     @property
     def free_pages(self):
@@ -383,9 +383,8 @@ class PagedKVCache:
         given = None if new_rows is None else self._on_device(counts, stream)
         need = hip_sdpa.paged_workspace_bytes(Q, self.n_batch, kv_group)
         if self._workspace is None or self._workspace.numel() < need:
-            # (a launch of an earlier call may still use the old one: it is kept until the one after
-            # next replaces it)
-            self._retired_workspace = self._workspace
+            # (a launch of an earlier call, on whatever stream, may still use the old one; there are three sizes)
+            self._old_workspaces.append(self._workspace)
             with torch.cuda.stream(stream):
                 self._workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
         if stream is not None:

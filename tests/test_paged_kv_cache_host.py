@@ -1,6 +1,7 @@
 """What PagedKVCache does on the host around its calls: which tensors it tells the allocator of, which memory it keeps
 (no GPU: the calls are taken by doubles that note what they get)."""
 import contextlib
+import weakref
 
 import pytest
 import torch
@@ -82,3 +83,19 @@ def test_nothing_is_told_of_the_current_stream(monkeypatch):
     c.attend(*_queries(c, 3, 1), 1)
     c.read()
     assert d.recorded == []
+
+
+def test_a_workspace_is_not_let_go(monkeypatch):
+    """Calls of more and more query rows, down to a generation step again: what an earlier call on whatever stream may
+    still use stays with the cache."""
+    d = Doubles(monkeypatch)
+    c = _cache([600, 30])
+    given = []
+    for q_seq, group in ((1, 1), (1, 4), (5, 4), (9, 4), (40, 4), (300, 1), (1, 1)):
+        c.attend(*_queries(c, q_seq, group), group)
+        name, a, kw = d.calls.pop()
+        assert name == "sdpa_fwd_paged" and a[9].numel() >= h.paged_workspace_bytes(a[4], 2, group)
+        given.append(weakref.ref(a[9]))
+        del a, kw
+    # (some sizes only: those of 16, 32 and 64 rows)
+    assert all(ref() is not None for ref in given) and len({_place(ref()) for ref in given}) == 3
