@@ -358,6 +358,19 @@ class PagedKVCache:
     # that the tile kernels' denser products need.
     DENSE_ROWS = 512
 
+    def _read_back(self, length, Q, mode, stream):
+        """Dense keys and values for the tile kernels, and their workspace; None where the pool
+        leaves no memory for them."""
+        try:
+            k, v = self.read(rows=length, stream=stream)
+            need = hip_sdpa.tile_cache_workspace_bytes(length, Q, mode)
+            if not need:
+                return k, v, None
+            with torch.cuda.stream(stream):
+                return k, v, torch.empty(need, dtype=torch.uint8, device=Q.device)
+        except torch.OutOfMemoryError:
+            return None
+
     def attend(self, Q, lse, A, kv_group, causal=True, new_rows=None, stream=None):
         """A = attention of Q over the sequences' rows; the queries of a sequence are
         its newest tokens (append first), the first new_rows of q_seq (a list; None:
@@ -370,16 +383,13 @@ class PagedKVCache:
         self._in_use(stream, Q, lse, A)
         if (kv_group * q_seq >= self.DENSE_ROWS and new_rows is None and length >= q_seq
                 and min(self.lengths) == max(self.lengths)):
-            k, v = self.read(stream=stream)
-            need = hip_sdpa.tile_cache_workspace_bytes(length, Q, mode)
-            workspace = None
-            if need:
-                with torch.cuda.stream(stream):
-                    workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)
-            hip_sdpa.sdpa_fwd_tile_cache(k, v, length, Q, None, lse, A, mode, n_batch=self.n_batch,
-                                         kv_group=kv_group, causal_offset=length - q_seq,
-                                         flags=hip_sdpa.OVERWRITE, stream=stream, workspace=workspace)
-            return
+            dense = self._read_back(length, Q, mode, stream)
+            if dense is not None:
+                k, v, workspace = dense
+                hip_sdpa.sdpa_fwd_tile_cache(k, v, length, Q, None, lse, A, mode, n_batch=self.n_batch,
+                                             kv_group=kv_group, causal_offset=length - q_seq,
+                                             flags=hip_sdpa.OVERWRITE, stream=stream, workspace=workspace)
+                return
         given = None if new_rows is None else self._on_device(counts, stream)
         need = hip_sdpa.paged_workspace_bytes(Q, self.n_batch, kv_group)
         if self._workspace is None or self._workspace.numel() < need:

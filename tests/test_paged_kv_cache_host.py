@@ -99,3 +99,27 @@ def test_a_workspace_is_not_let_go(monkeypatch):
         del a, kw
     # (some sizes only: those of 16, 32 and 64 rows)
     assert all(ref() is not None for ref in given) and len({_place(ref()) for ref in given}) == 3
+
+
+@pytest.mark.parametrize("which", ["tiles", "workspace"])
+def test_a_chunk_without_memory_for_the_copy_takes_the_pages(monkeypatch, which):
+    """The pool may fill the device: a chunk whose copy has no place is answered all the same."""
+    d = Doubles(monkeypatch)
+    c = _cache([600, 600])
+    tiles = _queries(c, 512, 1)
+    empty = torch.empty
+
+    def full(*a, **kw):
+        if (which == "tiles") == (kw.get("dtype") == c.dtype):
+            raise torch.OutOfMemoryError("no memory")
+        return empty(*a, **kw)
+
+    def paged_only(*a, **kw):
+        monkeypatch.setattr(torch, "empty", empty)
+        return bytes_of(*a, **kw)
+
+    bytes_of = h.paged_workspace_bytes
+    monkeypatch.setattr(h, "paged_workspace_bytes", paged_only)
+    monkeypatch.setattr(torch, "empty", full)
+    c.attend(*tiles, 1)
+    assert d.names()[-1] == "sdpa_fwd_paged" and "sdpa_fwd_tile_cache" not in d.names()
