@@ -229,6 +229,8 @@ class PagedKVCache:
             raise ValueError("page_rows is a power of two from 16 to 65536")
         if min(n_pages, n_batch, max_rows, n_head_kv) < 1 or head not in (64, 128):
             raise ValueError("a cache needs pages, sequences, rows and heads of size 64 or 128")
+        if -(-max_rows // page_rows) * page_rows > 0x7fffffff or n_batch * n_head_kv > 0x7fffffff:
+            raise ValueError("the rows of a sequence's pages, and sequences times heads, are below 2^31")
         hip_sdpa.dtype_name(torch.empty(0, dtype=dtype))
         if packed and dtype == torch.float32:
             raise TypeError("8-bit pages hold bf16 and fp16 tiles")

@@ -123,3 +123,12 @@ def test_a_chunk_without_memory_for_the_copy_takes_the_pages(monkeypatch, which)
     monkeypatch.setattr(torch, "empty", full)
     c.attend(*tiles, 1)
     assert d.names()[-1] == "sdpa_fwd_paged" and "sdpa_fwd_tile_cache" not in d.names()
+
+
+@pytest.mark.parametrize("sizes", [dict(max_rows=1 << 31, page_rows=65536), dict(max_rows=(1 << 31) - 15, page_rows=16),
+                                   dict(max_rows=1 << 40, page_rows=4096)])
+def test_more_rows_than_the_calls_take(sizes):
+    """max_pages * page_rows is below 2^31 for every call: refused where the cache is made, not by an append that has
+    counted its rows already."""
+    with pytest.raises(ValueError, match="below 2\\^31"):
+        _cache([0], n_pages=1, n_head_kv=1, packed=False, **sizes)
