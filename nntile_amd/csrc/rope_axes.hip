@@ -20,6 +20,7 @@
 #include "fixed_divide.hpp"
 #include "paged.hpp"
 #include "rope_common.hpp"
+#include "wide_grid.hpp"
 
 namespace nntile_hip
 {
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(256)
 void rope_axes_pair_kernel(const RopeAxesParams p, int64_t pairs)
 {
     typedef typename S::storage E;
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t t = wide_block() * 256 + threadIdx.x;
     if(t >= pairs)
     {
         return;
@@ -178,13 +179,12 @@ static int launch_typed(hipStream_t stream, const RopeAxesParams &p)
         }
         return launch_vec<S, BACKWARD, 8, false>(stream, p, blocks_x);
     }
-    const int64_t pairs = heads * p.n_batch * p.seq * (p.head / 2);
-    if((pairs + 255) / 256 > 0x7fffffff)
+    const int64_t pairs = heads * p.n_batch * p.seq * (p.head / 2), blocks = (pairs + 255) / 256;
+    if(blocks > kGridMost)
     {
         return NNTILE_HIP_EINVAL;
     }
-    hipLaunchKernelGGL((rope_axes_pair_kernel<S, BACKWARD>), dim3((unsigned)((pairs + 255) / 256)),
-            dim3(256), 0, stream, p, pairs);
+    hipLaunchKernelGGL((rope_axes_pair_kernel<S, BACKWARD>), wide_grid(blocks), dim3(256), 0, stream, p, pairs);
     return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;
 }
 
