@@ -23,6 +23,7 @@
 // 52.6.
 #include "fixed_divide.hpp"
 #include "rope_common.hpp"
+#include "wide_grid.hpp"
 
 namespace nntile_hip
 {
@@ -107,7 +108,7 @@ void rope_pair_kernel(int64_t m, int64_t pairs, const typename S::storage *sin,
         const typename S::storage *cos, const typename S::storage *src,
         typename S::storage *dst)
 {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t t = wide_block() * 256 + threadIdx.x;
     if(t >= pairs)
     {
         return;
@@ -162,11 +163,11 @@ static int launch_rope_typed(hipStream_t stream, int64_t m, int64_t n, const voi
     else
     {
         const int64_t blocks = (pairs + 255) / 256;
-        if(blocks > 0x7fffffff)
+        if(blocks > kGridMost)
         {
             return NNTILE_HIP_EINVAL;
         }
-        hipLaunchKernelGGL((rope_pair_kernel<S, BACKWARD>), dim3((unsigned)blocks), dim3(256), 0,
+        hipLaunchKernelGGL((rope_pair_kernel<S, BACKWARD>), wide_grid(blocks), dim3(256), 0,
                 stream, m, pairs, sin, cos, src, dst);
     }
     return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;

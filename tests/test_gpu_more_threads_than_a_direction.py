@@ -1,0 +1,33 @@
+"""Calls of 2^32 threads and more: a launch has less in one direction, and runs the rest of a larger one without an
+error only if its workgroups are numbered through two."""
+import math
+
+import pytest
+import torch
+
+from nntile_amd import hip_sdpa as h
+
+pytestmark = pytest.mark.gpu
+
+
+def _spots(total):
+    """Four elements at the front, around 2^31 and 2^32, and at the end."""
+    return [0, 2 ** 31 - 2, 2 ** 32 - 2, total - 4]
+
+
+def test_rope_by_single_pairs():
+    m, n = 3, 2 ** 32 // 3 + 1000           # (rows of no whole 16 bytes)
+    print("rope", m, n, flush=True)
+    src = torch.zeros(n, m, 2, dtype=torch.bfloat16, device="cuda")
+    dst = torch.full_like(src, 7.0)
+    sin, cos = (torch.tensor(x).to(torch.bfloat16).cuda() for x in ([0.5, 0.25, 0.0], [0.5, 1.0, -1.0]))
+    pairs, out = src.view(-1, 2), dst.view(-1, 2)
+    for at in _spots(m * n):
+        pairs[at:at + 4] = torch.tensor([1.0, 2.0])
+    h.rope(sin, cos, src, dst)
+    torch.cuda.synchronize()
+    for at in _spots(m * n):
+        i = torch.arange(at, at + 4) % m
+        s, c = sin.cpu().float()[i], cos.cpu().float()[i]
+        assert torch.equal(out[at:at + 4].cpu().float(), torch.stack((c - 2 * s, s + 2 * c), dim=1))
+    assert not out[2 ** 31 + 4:2 ** 32 - 4:1000003].any() and not out[2 ** 32 + 4:-4:101].any()
