@@ -11,6 +11,7 @@
 // bytes and addresses allow it, elements otherwise.  The decode entry point
 // that takes the capacity then reads the cache where it lies.
 #include "sdpa_common.hpp"
+#include "wide_grid.hpp"
 
 namespace nntile_hip
 {
@@ -30,7 +31,7 @@ template<int PIECE>
 __global__ __launch_bounds__(256)
 void kv_cache_append_kernel(KvAppendParams p)
 {
-    const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t t = wide_block() * 256 + threadIdx.x;
     if(t >= p.pieces)
     {
         return;
@@ -84,11 +85,11 @@ int launch_kv_cache_append(hipStream_t stream, int elem, int64_t head, int64_t r
     }
     p.pieces = entries * rows * (p.row_bytes / piece);
     const int64_t blocks = (p.pieces + 255) / 256;
-    if(blocks > 0x7fffffff)
+    if(blocks > kGridMost)
     {
         return NNTILE_HIP_EINVAL;
     }
-    const dim3 grid((unsigned)blocks, 2);
+    const dim3 grid = wide_grid(blocks, 2);
     if(piece == 16)
     {
         hipLaunchKernelGGL(kv_cache_append_kernel<16>, grid, dim3(256), 0, stream, p);

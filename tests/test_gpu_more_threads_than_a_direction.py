@@ -31,3 +31,20 @@ def test_rope_by_single_pairs():
         s, c = sin.cpu().float()[i], cos.cpu().float()[i]
         assert torch.equal(out[at:at + 4].cpu().float(), torch.stack((c - 2 * s, s + 2 * c), dim=1))
     assert not out[2 ** 31 + 4:2 ** 32 - 4:1000003].any() and not out[2 ** 32 + 4:-4:101].any()
+
+
+def test_kv_cache_append_by_single_values():
+    entries, rows, head = 2, 2 ** 31 // 5 + 1000, 5
+    print("append", entries, rows, head, flush=True)
+    new = torch.zeros(entries, rows, head, dtype=torch.bfloat16, device="cuda")
+    flat = new.view(-1)
+    for at in _spots(flat.numel()):
+        flat[at:at + 4] = torch.tensor([1.0, 2.0, 3.0, 4.0])
+    caches = [torch.full((entries, rows + 3, head), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    h.kv_cache_append(new, new, *caches, 2)
+    torch.cuda.synchronize()
+    for c in caches:
+        assert torch.all(c[:, :2] == 7) and torch.all(c[:, -1] == 7)
+        for e in range(entries):
+            for at in range(0, rows, 1 << 27):
+                assert torch.equal(c[e, 2 + at:2 + min(at + (1 << 27), rows)], new[e, at:at + (1 << 27)])
