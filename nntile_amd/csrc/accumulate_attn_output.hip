@@ -6,6 +6,7 @@
 // at -inf are left untouched.  Pure streaming: 16-byte accesses, one row's
 // chunks on neighbouring lanes.
 #include "sdpa_common.hpp"
+#include "wide_grid.hpp"
 
 namespace nntile_hip
 {
@@ -57,7 +58,7 @@ void accumulate_attn_output_vec_kernel(int64_t head, int64_t nrows,
     typedef typename S::storage E;
     const int r_in_block = threadIdx.x / chunks_per_row;
     const int chunk = threadIdx.x % chunks_per_row;
-    const int64_t row = (int64_t)blockIdx.x * rows_per_block + r_in_block;
+    const int64_t row = wide_block() * rows_per_block + r_in_block;
     const bool active = r_in_block < rows_per_block && row < nrows;
     float w_have = 1.0f, w_inc = 0.0f, merged = 0.0f;
     bool touch = false;
@@ -106,7 +107,7 @@ void accumulate_attn_output_row_kernel(int64_t head, int64_t nrows,
         const float *src_lse, const typename S::storage *src_attn,
         float *dst_lse, typename S::storage *dst_attn)
 {
-    const int64_t row = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t row = wide_block() * blockDim.x + threadIdx.x;
     if(row >= nrows)
     {
         return;
@@ -141,23 +142,23 @@ int launch_accumulate(hipStream_t stream, int64_t head, int64_t seq,
         const int cpr = (int)(head / S::VEC);
         const int rpb = 256 / cpr;
         const int64_t blocks = (nrows + rpb - 1) / rpb;
-        if(blocks > 0x7fffffff)
+        if(blocks > kGridMost)
         {
             return NNTILE_HIP_EINVAL;
         }
         hipLaunchKernelGGL((accumulate_attn_output_vec_kernel<S>),
-                dim3((unsigned)blocks), dim3(256), 0, stream, head, nrows, cpr,
+                wide_grid(blocks), dim3(256), 0, stream, head, nrows, cpr,
                 rpb, src_lse, src, dst_lse, dst);
     }
     else
     {
         const int64_t blocks = (nrows + 255) / 256;
-        if(blocks > 0x7fffffff)
+        if(blocks > kGridMost)
         {
             return NNTILE_HIP_EINVAL;
         }
         hipLaunchKernelGGL((accumulate_attn_output_row_kernel<S>),
-                dim3((unsigned)blocks), dim3(256), 0, stream, head, nrows,
+                wide_grid(blocks), dim3(256), 0, stream, head, nrows,
                 src_lse, src, dst_lse, dst);
     }
     return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;

@@ -48,3 +48,18 @@ def test_kv_cache_append_by_single_values():
         for e in range(entries):
             for at in range(0, rows, 1 << 27):
                 assert torch.equal(c[e, 2 + at:2 + min(at + (1 << 27), rows)], new[e, at:at + (1 << 27)])
+
+
+def test_accumulate_by_single_rows():
+    batch, seq, head = 2, 2 ** 31 + 1000, 1
+    print("accumulate", batch, seq, head, flush=True)
+    src, dst = (torch.zeros(batch, seq, head, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    src_lse, dst_lse = (torch.zeros(batch, seq, device="cuda") for _ in range(2))
+    for at in _spots(src.numel()):
+        src.view(-1)[at:at + 4] = torch.tensor([1.0, 2.0, 3.0, 4.0])
+    h.accumulate_attn_output(src_lse, src, dst_lse, dst)
+    torch.cuda.synchronize()
+    for at in _spots(src.numel()):
+        assert torch.equal(dst.view(-1)[at:at + 4].cpu().float(), torch.tensor([0.5, 1.0, 1.5, 2.0]))
+    for part in dst_lse.view(-1).split(1 << 30):
+        assert float((part - math.log(2.0)).abs().max()) <= 2.0 ** -22
