@@ -5,6 +5,7 @@
 // one rounding to the tile type).  A workgroup moves a 64 x 64 block through
 // LDS: reads run along i, writes along j, both over whole 64-element rows.
 #include "sdpa_common.hpp"
+#include "wide_grid.hpp"
 
 namespace nntile_hip
 {
@@ -38,8 +39,8 @@ void transpose_kernel(int64_t m, int64_t n, int64_t tiles_m, float alpha,
     typedef typename S::storage E;
     // one column of padding: the transposed reads of a wave fall on 64 banks
     __shared__ E tile[kTrTile][kTrTile + (sizeof(E) == 2 ? 2 : 1)];
-    const int64_t i0 = (int64_t)(blockIdx.x % tiles_m) * kTrTile;
-    const int64_t j0 = (int64_t)(blockIdx.x / tiles_m) * kTrTile;
+    const int64_t i0 = (wide_block() % tiles_m) * kTrTile;
+    const int64_t j0 = (wide_block() / tiles_m) * kTrTile;
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
     // tile[j][i] = src(i0 + i, j0 + j): 64 consecutive i per wave load
 #pragma unroll
@@ -82,8 +83,8 @@ void transpose16_kernel(int64_t m, int64_t n, int64_t tiles_m, float alpha,
         const uint16_t *src, uint16_t *dst)
 {
     __shared__ uint32_t tile[kTr16I * kTr16Pitch];
-    const int64_t i0 = (int64_t)(blockIdx.x % tiles_m) * kTr16I;
-    const int64_t j0 = (int64_t)(blockIdx.x / tiles_m) * kTr16J;
+    const int64_t i0 = (wide_block() % tiles_m) * kTr16I;
+    const int64_t j0 = (wide_block() / tiles_m) * kTr16J;
     const int tid = threadIdx.x;
     {
         const int c = tid % 16, jp = tid / 16;          // 8 rows i, column pair
@@ -335,22 +336,22 @@ static int launch_transpose_typed(hipStream_t stream, int64_t m, int64_t n, floa
         if(m % 8 == 0 && n % 8 == 0 && aligned)
         {
             const int64_t tm = (m + kTr16I - 1) / kTr16I, tn = (n + kTr16J - 1) / kTr16J;
-            if(tm > 0x7fffffff / tn)
+            if(tm > kGridMost / tn)
             {
                 return NNTILE_HIP_EINVAL;
             }
-            hipLaunchKernelGGL((transpose16_kernel<S>), dim3((unsigned)(tm * tn)), dim3(256), 0,
+            hipLaunchKernelGGL((transpose16_kernel<S>), wide_grid(tm * tn), dim3(256), 0,
                     stream, m, n, tm, alpha, static_cast<const uint16_t *>(src),
                     static_cast<uint16_t *>(dst));
             return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;
         }
     }
     const int64_t tiles_m = (m + kTrTile - 1) / kTrTile, tiles_n = (n + kTrTile - 1) / kTrTile;
-    if(tiles_m > 0x7fffffff / tiles_n)
+    if(tiles_m > kGridMost / tiles_n)
     {
         return NNTILE_HIP_EINVAL;
     }
-    hipLaunchKernelGGL((transpose_kernel<S>), dim3((unsigned)(tiles_m * tiles_n)), dim3(256), 0,
+    hipLaunchKernelGGL((transpose_kernel<S>), wide_grid(tiles_m * tiles_n), dim3(256), 0,
             stream, m, n, tiles_m, alpha, static_cast<const E *>(src), static_cast<E *>(dst));
     return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;
 }

@@ -63,3 +63,17 @@ def test_accumulate_by_single_rows():
         assert torch.equal(dst.view(-1)[at:at + 4].cpu().float(), torch.tensor([0.5, 1.0, 1.5, 2.0]))
     for part in dst_lse.view(-1).split(1 << 30):
         assert float((part - math.log(2.0)).abs().max()) <= 2.0 ** -22
+
+
+def test_transpose_of_one_row():
+    """A row of 2^30 elements and some is as many tiles of 64 x 64 as 2^32 threads take."""
+    n = 2 ** 30 + 1001
+    print("transpose", n, flush=True)
+    src = torch.zeros(n, 1, dtype=torch.bfloat16, device="cuda")
+    spots = [0, 2 ** 29 - 2, 2 ** 30 - 2, n - 4]
+    for at in spots:
+        src[at:at + 4, 0] = torch.tensor([1.0, 2.0, 3.0, 4.0])
+    dst = torch.full((1, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    h.transpose(2.0, src, dst, 1, n)
+    torch.cuda.synchronize()
+    assert torch.equal(dst.view(-1), 2 * src.view(-1))
