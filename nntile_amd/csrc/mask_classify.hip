@@ -14,6 +14,7 @@
 //   OFF_RULE some element differs from the rule  visible <=> k <= q + offset
 // HBM-bound: reads the tile once, writes nothing but the word.
 #include "sdpa_common.hpp"
+#include "wide_grid.hpp"
 
 namespace nntile_hip
 {
@@ -62,7 +63,7 @@ __global__ __launch_bounds__(256)
 void mask_classify_kernel(int64_t k_rows, int64_t total, int64_t offset,
         const typename M::storage *mask, uint32_t *flags)
 {
-    const int64_t base = (int64_t)blockIdx.x * kClassifyChunk;
+    const int64_t base = wide_block() * kClassifyChunk;
     const int64_t end = min(base + kClassifyChunk, total);
     uint32_t seen = 0;
     // position of the first element of this thread, then advanced by 256
@@ -116,12 +117,12 @@ int launch_mask_classify(hipStream_t stream, int dtype, int64_t k_rows, int64_t 
 {
     const int64_t total = k_rows * q_cols;
     const int64_t blocks = (total + kClassifyChunk - 1) / kClassifyChunk;
-    if(blocks > 0x7fffffff)
+    if(blocks > kGridMost)
     {
         return NNTILE_HIP_EINVAL;
     }
     hipLaunchKernelGGL(mask_classify_clear_kernel, dim3(1), dim3(1), 0, stream, flags);
-    const dim3 grid((unsigned)blocks), block(256);
+    const dim3 grid = wide_grid(blocks), block(256);
     switch(dtype)
     {
         case 0:
