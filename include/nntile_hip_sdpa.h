@@ -667,7 +667,8 @@ int nntile_hip_mask_tile_class_bool(void *stream, int64_t k_rows, int64_t q_cols
  * page_rows is a power of two from 16 to 65536, head 64 or 128 (other head sizes and
  * page sizes: NNTILE_HIP_EUNSUPPORTED).  Pages, scales, and tiles start at
  * multiples of 16 bytes; page_stride bytes and scale_stride are multiples of 16.
- * max_pages * page_rows and n_batch * n_head_kv * kv_group * rows are below 2^31, for
+ * max_pages * page_rows and n_batch * n_head_kv * kv_group * rows are below 2^31, the
+ * tiles of an append or read below 128 GiB, for
  * the attention also n_batch * n_head_kv * ceil(kv_group * q_seq / 16) * (max_pages *
  * page_rows / 64 + 2) (else NNTILE_HIP_EINVAL). */
 typedef struct nntile_hip_paged_cache

@@ -304,12 +304,19 @@ void paged_read_kernel(const PagedMoveParams p)
     }
 }
 
+// Workgroups of 256 threads that a direction of a launch takes: it has less than 2^32 threads
+constexpr int64_t kMoveBlocks = (1 << 24) - 1;
+
 template<typename T, int TPR, int LINES, bool AT_ONCE>
 static int launch_append(hipStream_t stream, const PagedMoveParams &p)
 {
     constexpr int64_t ROWS = LINES * 256 / TPR;
-    hipLaunchKernelGGL((paged_append_kernel<T, TPR, LINES, AT_ONCE>), dim3((unsigned)((p.all_rows + ROWS - 1) / ROWS), 2),
-            dim3(256), 0, stream, p);
+    const int64_t blocks = (p.all_rows + ROWS - 1) / ROWS;
+    if(blocks > kMoveBlocks)
+    {
+        return NNTILE_HIP_EINVAL;
+    }
+    hipLaunchKernelGGL((paged_append_kernel<T, TPR, LINES, AT_ONCE>), dim3((unsigned)blocks, 2), dim3(256), 0, stream, p);
     return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;
 }
 
@@ -317,8 +324,12 @@ template<typename T, int TPR, int LINES, bool STREAM>
 static int launch_read(hipStream_t stream, const PagedMoveParams &p)
 {
     constexpr int64_t ROWS = LINES * 256 / TPR;
-    hipLaunchKernelGGL((paged_read_kernel<T, TPR, LINES, STREAM>),
-            dim3((unsigned)((p.all_rows + ROWS - 1) / ROWS), 2), dim3(256), 0, stream, p);
+    const int64_t blocks = (p.all_rows + ROWS - 1) / ROWS;
+    if(blocks > kMoveBlocks)
+    {
+        return NNTILE_HIP_EINVAL;
+    }
+    hipLaunchKernelGGL((paged_read_kernel<T, TPR, LINES, STREAM>), dim3((unsigned)blocks, 2), dim3(256), 0, stream, p);
     return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;
 }
 
