@@ -31,3 +31,25 @@ def test_more_pairs_than_a_launch_has_threads(head, heads):
         off = np.abs(x[at:at + 4].double().cpu().numpy() - want)
         assert np.all(off <= HALF_STEP["bf16"] * np.abs(want) + 2.0 ** -21 * size)
     assert not x[spots[1] + 4:spots[2]:1000003].any()
+
+
+@pytest.mark.parametrize("dtype", sorted(DT))
+@pytest.mark.parametrize("backward,inplace", [(False, False), (True, True), (False, True)])
+@pytest.mark.parametrize("n_batch,seq,heads_q,heads_k,head,sections,shared", [
+    (1, 4099, 9, 4, 128, [22, 21, 21], False),          # queries end and keys begin within eight heads
+    (3, 1367, 5, 8, 128, [64], True),
+    (2, 8200, 3, 2, 64, [16, 16], False),               # fewer than eight heads
+    (5, 1639, 16, 0, 64, [20, 12], False),
+    (1, 30000, 1, 1, 40, [12, 8], False)])
+def test_eight_heads_a_thread(dtype, backward, inplace, n_batch, seq, heads_q, heads_k, head, sections, shared):
+    """Calls large enough that every CU has a workgroup with eight heads a thread."""
+    assert -(-n_batch * seq * (head // 8) // 256) * -(-(heads_q + heads_k) // 8) >= 256
+    _check(dtype, n_batch, seq, heads_q, heads_k, head, sections, 5000, backward, shared=shared, inplace=inplace)
+
+
+@pytest.mark.parametrize("backward,inplace", [(False, False), (True, True)])
+@pytest.mark.parametrize("heads_q,heads_k", [(9, 4), (10, 0), (3, 11)])
+def test_four_heads_a_thread_past_the_caches(backward, inplace, heads_q, heads_k):
+    """fp32 tensors of 128 MB and more, read and written."""
+    seq, head = 128 * 2 ** 20 // (8 * 128 * (heads_q + heads_k)) + 3, 128
+    _check("fp32", 1, seq, heads_q, heads_k, head, [32, 32], 5000, backward, inplace=inplace)
