@@ -36,3 +36,19 @@ def test_a_chunk_that_is_read_back_on_another_stream(packed, causal):
         torch.cuda.synchronize()
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_a_chunk_that_is_kept_to_the_pages(packed):
+    """NaN among the newest values: with DENSE_ROWS out of reach the tokens before do not notice."""
+    g = torch.Generator().manual_seed(71)
+    c = PagedKVCache(20, 64, 1, 600, 1, 64, packed=packed)
+    c.DENSE_ROWS = 1 << 62
+    q_seq, group = 200, 4
+    k, v = (torch.randn(1, q_seq, 64, generator=g).to(torch.bfloat16) for _ in range(2))
+    v[0, q_seq - 3, 5] = float("nan")
+    Q = torch.randn(group, q_seq, 64, generator=g).to(torch.bfloat16).cuda()
+    lse, A = torch.empty(group, q_seq, device="cuda"), torch.empty_like(Q)
+    c.append_attend(k.cuda(), v.cuda(), Q, lse, A, group)
+    odd = A.isnan().any(-1)
+    assert not odd[:, :-3].any() and odd[:, -3:].all() and not lse.isnan().any()
