@@ -31,7 +31,7 @@
 //    has fp32's exponents and more bits than fp16, whatever the powers of two of other rows are.
 //
 // What it reaches, 8 heads of 128, bytes of the cache alone: 64 sequences of 1024 bf16 rows, 4 query rows a
-// head 5.9 TB/s, 32 rows 5.7, 64 rows 4.4; 64 of 2048 8-bit rows 5.8, 5.2 and 3.4.  8 of 8192 bf16 rows, 64
+// head 5.9 TB/s, 32 rows 5.7, 64 rows 4.4; 64 of 2048 8-bit rows (bf16) 5.8, 5.2 and 3.5.  8 of 8192 bf16 rows, 64
 // query rows, 270 MB: 54.7 us = 4.9 TB/s.  A single sequence of 1001 rows, 4 MB: 8.7 us, the chain from
 // the lengths over the table and the keys to the join, a memory latency each.
 //
