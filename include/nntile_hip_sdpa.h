@@ -743,6 +743,89 @@ int nntile_hip_sdpa_fwd_paged_fp16(void *stream, const nntile_hip_sdpa_paged_arg
 int nntile_hip_sdpa_fwd_paged_fp32(void *stream, const nntile_hip_sdpa_paged_args *args,
         void *workspace, size_t workspace_bytes);
 
+/* ---- 11b. pages of 4-bit codes ------------------------------------------------------
+ * The calls of section 11 on pages of e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign):
+ *   k_pages, v_pages   [head, page_rows, n_head_kv, n_pages] codes, two a byte, the lower half
+ *                      first; page_stride counts codes and is a multiple of 32
+ *   k_scales, v_scales [head/32, page_rows, n_head_kv, n_pages] bytes, scale_stride apart (a
+ *                      multiple of 16): values 32b .. 32b + 31 of a row stand for
+ *                      code * 2^(scale - 127), scales from 1 to 252; or scale 255 over codes of 0:
+ *                      the 32 values are NaN
+ * Everything else is as there.  bf16 and fp16 tiles.  The append takes the smallest power of two, from
+ * 2^-125 to 2^125, that leaves none of the 32 values above 7 (the largest code, 6, is no further from
+ * what it stands for than half a step then; what 2^125 leaves above becomes 6 * 2^125), and rounds to
+ * nearest even; 32 values with a NaN or an infinity among them are stored as NaN.  What is read back is exact in bf16.  The attention's
+ * workspace is nntile_hip_sdpa_fwd_paged_workspace_bytes; its probabilities are rounded to 8 bits
+ * (bf16 tiles) or 16 (fp16), with the exponents of fp32. */
+int nntile_hip_paged4_kv_append_bf16(void *stream, const nntile_hip_paged_cache *cache,
+        int64_t rows, const uint16_t *k_new, const uint16_t *v_new);
+int nntile_hip_paged4_kv_append_fp16(void *stream, const nntile_hip_paged_cache *cache,
+        int64_t rows, const uint16_t *k_new, const uint16_t *v_new);
+int nntile_hip_paged4_kv_read_bf16(void *stream, const nntile_hip_paged_cache *cache,
+        int64_t first, int64_t rows, uint16_t *k_out, uint16_t *v_out);
+int nntile_hip_paged4_kv_read_fp16(void *stream, const nntile_hip_paged_cache *cache,
+        int64_t first, int64_t rows, uint16_t *k_out, uint16_t *v_out);
+int nntile_hip_sdpa_fwd_paged4_bf16(void *stream, const nntile_hip_sdpa_paged_args *args,
+        void *workspace, size_t workspace_bytes);
+int nntile_hip_sdpa_fwd_paged4_fp16(void *stream, const nntile_hip_sdpa_paged_args *args,
+        void *workspace, size_t workspace_bytes);
+
+/* ---- 11c. the attention that cached rows receive, and eviction by it ------------------
+ * No counterpart in the reference.  For pages of any kind (..._paged4_...: 4-bit codes).
+ *
+ * weights [columns, n_batch, n_head_kv] fp32, columns >= max_pages * page_rows: for every row p
+ * below lens of sequence n and head h
+ *   weights = decay * weights + sum over the queries that see the row of exp(s - lse),
+ * s their scores with the row's key, over the kv_group query heads of h and the q_seq newest
+ * tokens; Q and lse as nntile_hip_sdpa_fwd_paged_* takes and (with NNTILE_HIP_SDPA_OVERWRITE) leaves
+ * them, mask_mode and new_rows as there.  Queries with lse = -inf count nothing.  decay lies
+ * in [0, 1]; with 0 what weights held does not matter.  Columns at or behind lens are left as
+ * they are.  cache.v_pages and cache.v_scales are not looked at.  The same call gives the same
+ * bits every time.
+ * n_batch * n_head_kv * ceil(max_pages * page_rows / 64) is below 2^31 (else NNTILE_HIP_EINVAL). */
+typedef struct nntile_hip_paged_weights_args
+{
+    nntile_hip_paged_cache cache;
+    int64_t q_seq, kv_group, columns;
+    int32_t mask_mode;
+    float decay;
+    const void *Q;
+    const float *lse;
+    float *weights;
+} nntile_hip_paged_weights_args;
+
+int nntile_hip_paged_attn_weights_bf16(void *stream, const nntile_hip_paged_weights_args *args);
+int nntile_hip_paged_attn_weights_fp16(void *stream, const nntile_hip_paged_weights_args *args);
+int nntile_hip_paged_attn_weights_fp32(void *stream, const nntile_hip_paged_weights_args *args);
+int nntile_hip_paged4_attn_weights_bf16(void *stream, const nntile_hip_paged_weights_args *args);
+int nntile_hip_paged4_attn_weights_fp16(void *stream, const nntile_hip_paged_weights_args *args);
+
+/* Of every sequence with more than `keep` rows, and every head, `keep` rows stay: its last
+ * `recent` (at most keep) and, of those in front, the ones with the largest weights - of equal
+ * ones the lower row; a NaN counts as larger than every number.  They move to rows 0 .. keep - 1, in
+ * their order, in place; rows from `keep` on hold what they held.  Shorter sequences are
+ * left as they are.  The caller lowers lens to min(lens, keep) behind the call.
+ *   kept         [keep, n_batch, n_head_kv] int32, written: the row that row d was; -1 from min(lens,
+ *                keep) on
+ *   weights      as above; weights_out: the same array, or another of the same size, whose
+ *                columns below lens are written: the weights of the rows that stayed, then zeros
+ * A row without a page moves as zeros, and none is written where the new place has no page.  No page
+ * belongs to two sequences.  cache.new_rows is not looked at. */
+typedef struct nntile_hip_paged_evict_args
+{
+    nntile_hip_paged_cache cache;
+    int64_t keep, recent, columns;
+    const float *weights;
+    float *weights_out;
+    int32_t *kept;
+} nntile_hip_paged_evict_args;
+
+int nntile_hip_paged_kv_evict_bf16(void *stream, const nntile_hip_paged_evict_args *args);
+int nntile_hip_paged_kv_evict_fp16(void *stream, const nntile_hip_paged_evict_args *args);
+int nntile_hip_paged_kv_evict_fp32(void *stream, const nntile_hip_paged_evict_args *args);
+int nntile_hip_paged4_kv_evict_bf16(void *stream, const nntile_hip_paged_evict_args *args);
+int nntile_hip_paged4_kv_evict_fp16(void *stream, const nntile_hip_paged_evict_args *args);
+
 /* ---- 12. rotary embedding with positions of several axes --------------------------
  * nntile_hip_rope_* takes tables of sines and cosines; here they follow from the
  * positions, of one axis (text) or several (time, rows and columns of video

@@ -1,5 +1,5 @@
-// C ABI of the paged key/value cache and of the rotary embedding with positions of several axes:
-// argument checks and dispatch to the kernels.
+// C ABI of the paged key/value cache, of the weights its rows receive and their eviction, and of the rotary
+// embedding with positions of several axes: argument checks and dispatch to the kernels.
 #include "paged.hpp"
 
 using namespace nntile_hip;
@@ -25,10 +25,12 @@ int64_t small_product(int64_t a, int64_t b)
     return a < 0 || b < 0 || (b != 0 && a > kMost / b) ? -1 : a * b;
 }
 
-int paged_view(const nntile_hip_paged_cache *c, int dtype, PagedView &v)
+// four: pages of 4-bit codes.  values: the call looks at the values, too.
+int paged_view(const nntile_hip_paged_cache *c, int dtype, PagedView &v, bool four = false, bool values = true)
 {
-    if(c == nullptr || c->k_pages == nullptr || c->v_pages == nullptr || c->table == nullptr
-            || c->lens == nullptr || (c->k_scales == nullptr) != (c->v_scales == nullptr)
+    if(c == nullptr || c->k_pages == nullptr || (values && c->v_pages == nullptr) || c->table == nullptr
+            || c->lens == nullptr || (values && (c->k_scales == nullptr) != (c->v_scales == nullptr))
+            || (four && c->k_scales == nullptr)
             || c->head <= 0 || c->page_rows <= 0 || c->n_head_kv <= 0 || c->n_pages <= 0
             || c->max_pages <= 0 || c->n_batch <= 0 || c->n_pages > kMost)
     {
@@ -50,18 +52,20 @@ int paged_view(const nntile_hip_paged_cache *c, int dtype, PagedView &v)
     {
         return NNTILE_HIP_EINVAL;
     }
-    const int64_t e = packed ? 1 : elem_bytes(dtype);
+    // half bytes of a value; scale bytes of a page, of 32 values or of a row
+    const int64_t e2 = four ? 1 : packed ? 2 : 2 * elem_bytes(dtype);
+    const int64_t scales = page_of_heads * (four ? c->head / 32 : 1);
     constexpr int64_t kStride = (int64_t)1 << 55;       // (times the number of pages it stays an address)
     if(c->page_stride < page_of_heads * c->head || c->page_stride > kStride / c->n_pages
-            || c->page_stride * e % 16 != 0 || !on16(c->k_pages)
-            || !on16(c->v_pages) || (reinterpret_cast<uintptr_t>(c->table) & 3u) != 0
+            || c->page_stride * e2 % 32 != 0 || !on16(c->k_pages)
+            || (values && !on16(c->v_pages)) || (reinterpret_cast<uintptr_t>(c->table) & 3u) != 0
             || (reinterpret_cast<uintptr_t>(c->lens) & 3u) != 0
             || (reinterpret_cast<uintptr_t>(c->new_rows) & 3u) != 0)
     {
         return NNTILE_HIP_EINVAL;
     }
-    if(packed && (c->scale_stride < page_of_heads || c->scale_stride > kStride / c->n_pages
-                || c->scale_stride % 16 != 0 || !on16(c->k_scales) || !on16(c->v_scales)))
+    if(packed && (c->scale_stride < scales || c->scale_stride > kStride / c->n_pages
+                || c->scale_stride % 16 != 0 || !on16(c->k_scales) || (values && !on16(c->v_scales))))
     {
         return NNTILE_HIP_EINVAL;
     }
@@ -72,7 +76,7 @@ int paged_view(const nntile_hip_paged_cache *c, int dtype, PagedView &v)
     v.table = c->table;
     v.lens = c->lens;
     v.new_rows = c->new_rows;
-    v.page_stride = c->page_stride * e;
+    v.page_stride = c->page_stride * e2 / 2;
     v.scale_stride = packed ? c->scale_stride : 0;
     v.n_batch = (int32_t)c->n_batch;
     v.n_head_kv = (int32_t)c->n_head_kv;
@@ -83,11 +87,11 @@ int paged_view(const nntile_hip_paged_cache *c, int dtype, PagedView &v)
     return NNTILE_HIP_OK;
 }
 
-int append_call(int dtype, void *stream, const nntile_hip_paged_cache *c, int64_t rows,
+int append_call(int dtype, bool four, void *stream, const nntile_hip_paged_cache *c, int64_t rows,
         const void *k_new, const void *v_new)
 {
     PagedView v;
-    const int rc = paged_view(c, dtype, v);
+    const int rc = paged_view(c, dtype, v, four);
     if(rc != NNTILE_HIP_OK)
     {
         return rc;
@@ -104,14 +108,15 @@ int append_call(int dtype, void *stream, const nntile_hip_paged_cache *c, int64_
     {
         return NNTILE_HIP_EINVAL;
     }
-    return launch_paged_append(static_cast<hipStream_t>(stream), dtype, v, (int)c->head, rows, k_new, v_new);
+    return (four ? launch_paged4_append : launch_paged_append)(static_cast<hipStream_t>(stream), dtype, v,
+            (int)c->head, rows, k_new, v_new);
 }
 
-int read_call(int dtype, void *stream, const nntile_hip_paged_cache *c, int64_t first, int64_t rows,
+int read_call(int dtype, bool four, void *stream, const nntile_hip_paged_cache *c, int64_t first, int64_t rows,
         void *k_out, void *v_out)
 {
     PagedView v;
-    const int rc = paged_view(c, dtype, v);
+    const int rc = paged_view(c, dtype, v, four);
     if(rc != NNTILE_HIP_OK)
     {
         return rc;
@@ -129,23 +134,31 @@ int read_call(int dtype, void *stream, const nntile_hip_paged_cache *c, int64_t 
     {
         return NNTILE_HIP_EINVAL;
     }
-    return launch_paged_read(static_cast<hipStream_t>(stream), dtype, v, (int)c->head, first, rows,
-            k_out, v_out);
+    return (four ? launch_paged4_read : launch_paged_read)(static_cast<hipStream_t>(stream), dtype, v, (int)c->head,
+            first, rows, k_out, v_out);
 }
 
 // kv_group * q_seq, or -1
-int64_t query_rows(const nntile_hip_sdpa_paged_args *a)
+int64_t query_rows(const nntile_hip_paged_cache &c, int64_t q_seq, int64_t kv_group)
 {
-    if(a->q_seq <= 0 || a->kv_group <= 0 || a->cache.n_batch <= 0 || a->cache.n_head_kv <= 0)
+    if(q_seq <= 0 || kv_group <= 0 || c.n_batch <= 0 || c.n_head_kv <= 0)
     {
         return -1;
     }
-    const int64_t rows = small_product(a->q_seq, a->kv_group);
-    const int64_t entries = small_product(a->cache.n_batch, a->cache.n_head_kv);
+    const int64_t rows = small_product(q_seq, kv_group);
+    const int64_t entries = small_product(c.n_batch, c.n_head_kv);
     return rows < 0 || entries < 0 || small_product(rows, entries) < 0 ? -1 : rows;
 }
 
-int attend_call(int dtype, void *stream, const nntile_hip_sdpa_paged_args *a, void *workspace,
+// What the attention over pages refuses of masks
+int mask_check(int32_t mode)
+{
+    return mode == NNTILE_HIP_MASK_CAUSAL || mode == NNTILE_HIP_MASK_NONE ? NNTILE_HIP_OK
+        : mode == NNTILE_HIP_MASK_ADDITIVE || mode == NNTILE_HIP_MASK_BOOL ? NNTILE_HIP_EUNSUPPORTED
+        : NNTILE_HIP_EINVAL;
+}
+
+int attend_call(int dtype, bool four, void *stream, const nntile_hip_sdpa_paged_args *a, void *workspace,
         size_t workspace_bytes)
 {
     if(a == nullptr)
@@ -153,22 +166,21 @@ int attend_call(int dtype, void *stream, const nntile_hip_sdpa_paged_args *a, vo
         return NNTILE_HIP_EINVAL;
     }
     PagedAttendParams p = {};
-    const int rc = paged_view(&a->cache, dtype, p.c);
+    const int rc = paged_view(&a->cache, dtype, p.c, four);
     if(rc != NNTILE_HIP_OK)
     {
         return rc;
     }
-    const int64_t rows = query_rows(a);
+    const int64_t rows = query_rows(a->cache, a->q_seq, a->kv_group);
     if(rows < 0 || a->Q == nullptr || a->lse == nullptr || a->A == nullptr || !on16(a->Q) || !on16(a->A)
             || (reinterpret_cast<uintptr_t>(a->lse) & 3u) != 0
             || (a->flags & ~NNTILE_HIP_SDPA_OVERWRITE) != 0)
     {
         return NNTILE_HIP_EINVAL;
     }
-    if(a->mask_mode != NNTILE_HIP_MASK_CAUSAL && a->mask_mode != NNTILE_HIP_MASK_NONE)
+    if(mask_check(a->mask_mode) != NNTILE_HIP_OK)
     {
-        return a->mask_mode == NNTILE_HIP_MASK_ADDITIVE || a->mask_mode == NNTILE_HIP_MASK_BOOL
-            ? NNTILE_HIP_EUNSUPPORTED : NNTILE_HIP_EINVAL;
+        return mask_check(a->mask_mode);
     }
     if(workspace == nullptr || !on16(workspace)
             || workspace_bytes < paged_attend_workspace_bytes(rows, a->cache.head))
@@ -184,7 +196,78 @@ int attend_call(int dtype, void *stream, const nntile_hip_sdpa_paged_args *a, vo
     p.causal = a->mask_mode == NNTILE_HIP_MASK_CAUSAL;
     p.overwrite = (a->flags & NNTILE_HIP_SDPA_OVERWRITE) != 0;
     p.scale = 1.0f / sqrtf((float)a->cache.head);
-    return launch_paged_attend(static_cast<hipStream_t>(stream), dtype, p, (int)a->cache.head, workspace);
+    return (four ? launch_paged4_attend : launch_paged_attend)(static_cast<hipStream_t>(stream), dtype, p,
+            (int)a->cache.head, workspace);
+}
+
+int page_bits(const nntile_hip_paged_cache &c, int dtype, bool four)
+{
+    return four ? 4 : c.k_scales != nullptr ? 8 : 8 * elem_bytes(dtype);
+}
+
+int weights_call(int dtype, bool four, void *stream, const nntile_hip_paged_weights_args *a)
+{
+    if(a == nullptr)
+    {
+        return NNTILE_HIP_EINVAL;
+    }
+    PagedWeightsParams p = {};
+    const int rc = paged_view(&a->cache, dtype, p.c, four, false);
+    if(rc != NNTILE_HIP_OK)
+    {
+        return rc;
+    }
+    const int64_t rows = query_rows(a->cache, a->q_seq, a->kv_group);
+    if(rows < 0 || a->Q == nullptr || a->lse == nullptr || a->weights == nullptr || !on16(a->Q)
+            || (reinterpret_cast<uintptr_t>(a->lse) & 3u) != 0 || (reinterpret_cast<uintptr_t>(a->weights) & 3u) != 0
+            || a->columns < p.c.max_rows || a->columns > kMost || !(a->decay >= 0.0f && a->decay <= 1.0f))
+    {
+        return NNTILE_HIP_EINVAL;
+    }
+    if(mask_check(a->mask_mode) != NNTILE_HIP_OK)
+    {
+        return mask_check(a->mask_mode);
+    }
+    p.Q = a->Q;
+    p.lse = a->lse;
+    p.weights = a->weights;
+    p.columns = a->columns;
+    p.q_seq = (int32_t)a->q_seq;
+    p.kv_group = (int32_t)a->kv_group;
+    p.rows = (int32_t)rows;
+    p.causal = a->mask_mode == NNTILE_HIP_MASK_CAUSAL;
+    p.decay = a->decay;
+    p.scale = 1.0f / sqrtf((float)a->cache.head);
+    return launch_paged_weights(static_cast<hipStream_t>(stream), dtype, page_bits(a->cache, dtype, four), p,
+            (int)a->cache.head);
+}
+
+int evict_call(int dtype, bool four, void *stream, const nntile_hip_paged_evict_args *a)
+{
+    if(a == nullptr)
+    {
+        return NNTILE_HIP_EINVAL;
+    }
+    PagedEvictParams p = {};
+    const int rc = paged_view(&a->cache, dtype, p.c, four);
+    if(rc != NNTILE_HIP_OK)
+    {
+        return rc;
+    }
+    if(a->keep <= 0 || a->keep > kMost || a->recent < 0 || a->recent > a->keep || a->weights == nullptr
+            || a->weights_out == nullptr || a->kept == nullptr || (reinterpret_cast<uintptr_t>(a->weights) & 3u) != 0
+            || (reinterpret_cast<uintptr_t>(a->weights_out) & 3u) != 0
+            || (reinterpret_cast<uintptr_t>(a->kept) & 3u) != 0 || a->columns < p.c.max_rows || a->columns > kMost)
+    {
+        return NNTILE_HIP_EINVAL;
+    }
+    p.weights = a->weights;
+    p.weights_out = a->weights_out;
+    p.kept = a->kept;
+    p.columns = a->columns;
+    p.keep = (int32_t)a->keep;
+    p.recent = (int32_t)a->recent;
+    return launch_paged_evict(static_cast<hipStream_t>(stream), page_bits(a->cache, dtype, four), p, (int)a->cache.head);
 }
 
 int rope_axes_call(int dtype, void *stream, const nntile_hip_rope_axes_args *a)
@@ -248,7 +331,7 @@ extern "C"
 
 size_t nntile_hip_sdpa_fwd_paged_workspace_bytes(const nntile_hip_sdpa_paged_args *args)
 {
-    const int64_t rows = args == nullptr ? -1 : query_rows(args);
+    const int64_t rows = args == nullptr ? -1 : query_rows(args->cache, args->q_seq, args->kv_group);
     return rows < 0 || args->cache.head <= 0 || args->cache.head > 128 ? 0
         : paged_attend_workspace_bytes(rows, args->cache.head);
 }
@@ -257,17 +340,25 @@ size_t nntile_hip_sdpa_fwd_paged_workspace_bytes(const nntile_hip_sdpa_paged_arg
     int nntile_hip_paged_kv_append_##suffix(void *stream, const nntile_hip_paged_cache *cache, \
             int64_t rows, const ctype *k_new, const ctype *v_new) \
     { \
-        return append_call(dt, stream, cache, rows, k_new, v_new); \
+        return append_call(dt, false, stream, cache, rows, k_new, v_new); \
     } \
     int nntile_hip_paged_kv_read_##suffix(void *stream, const nntile_hip_paged_cache *cache, \
             int64_t first, int64_t rows, ctype *k_out, ctype *v_out) \
     { \
-        return read_call(dt, stream, cache, first, rows, k_out, v_out); \
+        return read_call(dt, false, stream, cache, first, rows, k_out, v_out); \
     } \
     int nntile_hip_sdpa_fwd_paged_##suffix(void *stream, const nntile_hip_sdpa_paged_args *args, \
             void *workspace, size_t workspace_bytes) \
     { \
-        return attend_call(dt, stream, args, workspace, workspace_bytes); \
+        return attend_call(dt, false, stream, args, workspace, workspace_bytes); \
+    } \
+    int nntile_hip_paged_attn_weights_##suffix(void *stream, const nntile_hip_paged_weights_args *args) \
+    { \
+        return weights_call(dt, false, stream, args); \
+    } \
+    int nntile_hip_paged_kv_evict_##suffix(void *stream, const nntile_hip_paged_evict_args *args) \
+    { \
+        return evict_call(dt, false, stream, args); \
     } \
     int nntile_hip_rope_axes_##suffix(void *stream, const nntile_hip_rope_axes_args *args) \
     { \
@@ -277,5 +368,33 @@ NNTILE_HIP_PAGED_ENTRY(bf16, 0, uint16_t)
 NNTILE_HIP_PAGED_ENTRY(fp16, 1, uint16_t)
 NNTILE_HIP_PAGED_ENTRY(fp32, 2, float)
 #undef NNTILE_HIP_PAGED_ENTRY
+
+#define NNTILE_HIP_PAGED4_ENTRY(suffix, dt) \
+    int nntile_hip_paged4_kv_append_##suffix(void *stream, const nntile_hip_paged_cache *cache, \
+            int64_t rows, const uint16_t *k_new, const uint16_t *v_new) \
+    { \
+        return append_call(dt, true, stream, cache, rows, k_new, v_new); \
+    } \
+    int nntile_hip_paged4_kv_read_##suffix(void *stream, const nntile_hip_paged_cache *cache, \
+            int64_t first, int64_t rows, uint16_t *k_out, uint16_t *v_out) \
+    { \
+        return read_call(dt, true, stream, cache, first, rows, k_out, v_out); \
+    } \
+    int nntile_hip_sdpa_fwd_paged4_##suffix(void *stream, const nntile_hip_sdpa_paged_args *args, \
+            void *workspace, size_t workspace_bytes) \
+    { \
+        return attend_call(dt, true, stream, args, workspace, workspace_bytes); \
+    } \
+    int nntile_hip_paged4_attn_weights_##suffix(void *stream, const nntile_hip_paged_weights_args *args) \
+    { \
+        return weights_call(dt, true, stream, args); \
+    } \
+    int nntile_hip_paged4_kv_evict_##suffix(void *stream, const nntile_hip_paged_evict_args *args) \
+    { \
+        return evict_call(dt, true, stream, args); \
+    }
+NNTILE_HIP_PAGED4_ENTRY(bf16, 0)
+NNTILE_HIP_PAGED4_ENTRY(fp16, 1)
+#undef NNTILE_HIP_PAGED4_ENTRY
 
 } // extern "C"

@@ -677,13 +677,21 @@ int64_t pool_stride(const at::Tensor &t)
     return t.size(0) > 1 ? t.stride(0) : inner;
 }
 
+// Whether the pages of a call hold 4-bit codes.
+bool four_bits(PyObject *k_pages)
+{
+    return tensor(k_pages).scalar_type() == at::ScalarType::Float4_e2m1fn_x2;
+}
+
 // Pools, table, lengths, scales and new rows into the argument block; false: they
-// do not fit each other.  `ty`: the type of the tiles.
+// do not fit each other.  `ty`: the type of the tiles.  (The keys in the place of the values: a call that
+// does not look at values.)
 bool fill_paged(nntile_hip_paged_cache &c, const SameDevice &dev, Type ty, PyObject *k_pages_,
         PyObject *v_pages_, PyObject *table_, PyObject *lens_, PyObject *k_scales_,
         PyObject *v_scales_, PyObject *new_rows_)
 {
     const at::Tensor &k_pages = tensor(k_pages_), &v_pages = tensor(v_pages_);
+    const bool four = four_bits(k_pages_);
     const at::Tensor &table = dev.dense(table_), &lens = dev.dense(lens_);
     dev.check(k_pages);
     dev.check(v_pages);
@@ -695,10 +703,14 @@ bool fill_paged(nntile_hip_paged_cache &c, const SameDevice &dev, Type ty, PyObj
     {
         return false;
     }
-    const at::ScalarType held = packed ? at::kFloat8_e4m3fn
+    if(four && !packed)
+    {
+        return false;
+    }
+    const at::ScalarType held = four ? at::ScalarType::Float4_e2m1fn_x2 : packed ? at::kFloat8_e4m3fn
         : ty == BF16 ? at::kBFloat16 : ty == FP16 ? at::kHalf : at::kFloat;
     const char *text = "pages are tensors [n_pages, n_head_kv, page_rows, head] of the tiles' type, "
-        "or torch.float8_e4m3fn with scales";
+        "or torch.float8_e4m3fn or torch.float4_e2m1fn_x2 (head/2) with scales";
     wants(k_pages, held, 4, text);
     wants(v_pages, held, 4, text);
     c.page_stride = pool_stride(k_pages);
@@ -712,8 +724,27 @@ bool fill_paged(nntile_hip_paged_cache &c, const SameDevice &dev, Type ty, PyObj
     c.n_pages = k_pages.size(0);
     c.n_head_kv = k_pages.size(1);
     c.page_rows = k_pages.size(2);
-    c.head = k_pages.size(3);
-    if(packed)
+    c.head = four ? 2 * k_pages.size(3) : k_pages.size(3);
+    if(four)
+    {
+        const at::Tensor &ks = tensor(k_scales_), &vs = tensor(v_scales_);
+        dev.check(ks);
+        dev.check(vs);
+        const char *scales = "scales of 4-bit pages are uint8 tensors [n_pages, n_head_kv, page_rows, head/32]";
+        wants(ks, at::kByte, 4, scales);
+        wants(vs, at::kByte, 4, scales);
+        // (codes, not bytes)
+        c.page_stride *= 2;
+        c.scale_stride = pool_stride(ks);
+        if(ks.sizes() != vs.sizes() || pool_stride(vs) != c.scale_stride || c.head % 32 != 0
+                || ks.sizes().slice(0, 3) != k_pages.sizes().slice(0, 3) || ks.size(3) != c.head / 32)
+        {
+            return false;
+        }
+        c.k_scales = static_cast<uint8_t *>(ks.data_ptr());
+        c.v_scales = static_cast<uint8_t *>(vs.data_ptr());
+    }
+    else if(packed)
     {
         const at::Tensor &ks = tensor(k_scales_), &vs = tensor(v_scales_);
         dev.check(ks);
@@ -773,6 +804,13 @@ PyObject *paged_append(PyObject *, PyObject *const *v, Py_ssize_t n)
         }
         void *s = stream_of(v[9]);
         const int64_t rows = k.size(1);
+        if(four_bits(v[2]))
+        {
+            return ty == FP32 ? NNTILE_HIP_EUNSUPPORTED
+                : unlocked(ty == BF16 ? nntile_hip_paged4_kv_append_bf16 : nntile_hip_paged4_kv_append_fp16,
+                        s, &c, rows, static_cast<const uint16_t *>(k.data_ptr()),
+                        static_cast<const uint16_t *>(w.data_ptr()));
+        }
         if(ty == FP32)
         {
             return unlocked(nntile_hip_paged_kv_append_fp32, s, &c, rows,
@@ -803,6 +841,13 @@ PyObject *paged_read(PyObject *, PyObject *const *v, Py_ssize_t n)
         }
         const int64_t first = integer(v[6]), rows = k.size(1);
         void *s = stream_of(v[9]);
+        if(four_bits(v[0]))
+        {
+            return ty == FP32 ? NNTILE_HIP_EUNSUPPORTED
+                : unlocked(ty == BF16 ? nntile_hip_paged4_kv_read_bf16 : nntile_hip_paged4_kv_read_fp16,
+                        s, &c, first, rows, static_cast<uint16_t *>(k.data_ptr()),
+                        static_cast<uint16_t *>(w.data_ptr()));
+        }
         if(ty == FP32)
         {
             return unlocked(nntile_hip_paged_kv_read_fp32, s, &c, first, rows,
@@ -848,9 +893,107 @@ PyObject *fwd_paged(PyObject *, PyObject *const *v, Py_ssize_t n)
         a.Q = Q.data_ptr();
         a.lse = static_cast<float *>(lse.data_ptr());
         a.A = A.data_ptr();
+        if(four_bits(v[0]))
+        {
+            return ty == FP32 ? NNTILE_HIP_EUNSUPPORTED
+                : unlocked(ty == BF16 ? nntile_hip_sdpa_fwd_paged4_bf16 : nntile_hip_sdpa_fwd_paged4_fp16,
+                        stream_of(v[14]), &a, ws.data_ptr(), nbytes(&ws));
+        }
         return unlocked(ty == BF16 ? nntile_hip_sdpa_fwd_paged_bf16
                 : ty == FP16 ? nntile_hip_sdpa_fwd_paged_fp16 : nntile_hip_sdpa_fwd_paged_fp32,
                 stream_of(v[14]), &a, ws.data_ptr(), nbytes(&ws));
+    });
+}
+
+// (k_pages, table, lens, Q, lse, weights, mask_mode, kv_group, k_scales, new_rows, decay, stream)
+PyObject *paged_attn_weights(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+    return guarded(n, 12, [&]() -> int
+    {
+        const at::Tensor &Q = tile(v[3]), &lse = tile(v[4]), &weights = tile(v[5]);
+        const SameDevice dev;
+        for(const at::Tensor *t : {&Q, &lse, &weights})
+        {
+            dev.check(*t);
+        }
+        rank3(Q);
+        const Type ty = type_of(v[3], Q);
+        wants(lse, at::kFloat, 2, "lse is an fp32 tensor [batch, q_seq]");
+        wants(weights, at::kFloat, 2, "weights are an fp32 tensor [n_head_kv * n_batch, columns]");
+        nntile_hip_paged_weights_args a = {};
+        if(!fill_paged(a.cache, dev, ty, v[0], v[0], v[1], v[2], v[8], v[8], v[9]))
+        {
+            return NNTILE_HIP_EINVAL;
+        }
+        a.q_seq = Q.size(1);
+        a.kv_group = integer(v[7]);
+        a.mask_mode = (int32_t)integer(v[6]);
+        const double decay = PyFloat_AsDouble(v[10]);
+        if(decay == -1.0 && PyErr_Occurred())
+        {
+            throw Bad();
+        }
+        a.decay = (float)decay;
+        const int64_t entries = a.cache.n_head_kv * a.cache.n_batch;
+        if(a.kv_group < 1 || a.kv_group > Q.size(0) || Q.size(0) != entries * a.kv_group
+                || Q.size(2) != a.cache.head || lse.size(0) != Q.size(0) || lse.size(1) != Q.size(1)
+                || weights.size(0) != entries)
+        {
+            return NNTILE_HIP_EINVAL;
+        }
+        a.columns = weights.size(1);
+        a.Q = Q.data_ptr();
+        a.lse = static_cast<const float *>(lse.data_ptr());
+        a.weights = static_cast<float *>(weights.data_ptr());
+        if(four_bits(v[0]))
+        {
+            return ty == FP32 ? NNTILE_HIP_EUNSUPPORTED
+                : unlocked(ty == BF16 ? nntile_hip_paged4_attn_weights_bf16 : nntile_hip_paged4_attn_weights_fp16,
+                        stream_of(v[11]), &a);
+        }
+        return unlocked(ty == BF16 ? nntile_hip_paged_attn_weights_bf16
+                : ty == FP16 ? nntile_hip_paged_attn_weights_fp16 : nntile_hip_paged_attn_weights_fp32,
+                stream_of(v[11]), &a);
+    });
+}
+
+// (k_pages, v_pages, table, lens, weights, weights_out, kept, recent, k_scales, v_scales, stream)
+PyObject *paged_evict(PyObject *, PyObject *const *v, Py_ssize_t n)
+{
+    return guarded(n, 11, [&]() -> int
+    {
+        const at::Tensor &weights = tile(v[4]), &out = tile(v[5]), &kept = tile(v[6]);
+        const SameDevice dev;
+        for(const at::Tensor *t : {&weights, &out, &kept})
+        {
+            dev.check(*t);
+        }
+        wants(weights, at::kFloat, 2, "weights are an fp32 tensor [n_head_kv * n_batch, columns]");
+        wants(out, at::kFloat, 2, "weights_out is an fp32 tensor like weights");
+        wants(kept, at::kInt, 2, "kept is an int32 tensor [n_head_kv * n_batch, keep]");
+        // (what pages of codes stand for does not matter here)
+        const at::ScalarType held = tensor(v[0]).scalar_type();
+        const Type ty = held == at::kFloat ? FP32 : held == at::kHalf ? FP16 : BF16;
+        nntile_hip_paged_evict_args a = {};
+        if(!fill_paged(a.cache, dev, ty, v[0], v[1], v[2], v[3], v[8], v[9], Py_None))
+        {
+            return NNTILE_HIP_EINVAL;
+        }
+        const int64_t entries = a.cache.n_head_kv * a.cache.n_batch;
+        if(weights.size(0) != entries || out.sizes() != weights.sizes() || kept.size(0) != entries)
+        {
+            return NNTILE_HIP_EINVAL;
+        }
+        a.keep = kept.size(1);
+        a.recent = integer(v[7]);
+        a.columns = weights.size(1);
+        a.weights = static_cast<const float *>(weights.data_ptr());
+        a.weights_out = static_cast<float *>(out.data_ptr());
+        a.kept = static_cast<int32_t *>(kept.data_ptr());
+        return unlocked(four_bits(v[0]) ? nntile_hip_paged4_kv_evict_bf16
+                : ty == BF16 ? nntile_hip_paged_kv_evict_bf16
+                : ty == FP16 ? nntile_hip_paged_kv_evict_fp16 : nntile_hip_paged_kv_evict_fp32,
+                stream_of(v[10]), &a);
     });
 }
 
@@ -1025,7 +1168,8 @@ PyMethodDef methods[] = {
     FAST(fwd_tile), FAST(fwd_tile_cache), FAST(fwd_tile_cache_ws), FAST(tile_cache_workspace), FAST(fwd_decode), FAST(fwd_decode_cache),
     FAST(fwd_decode_append_cache), FAST(cache_step), FAST(kv_append), FAST(flash_fwd),
     FAST(flash_bwd), FAST(bwd_tile), FAST(accumulate), FAST(rope), FAST(transpose),
-    FAST(paged_append), FAST(paged_read), FAST(fwd_paged), FAST(rope_axes),
+    FAST(paged_append), FAST(paged_read), FAST(fwd_paged), FAST(paged_attn_weights), FAST(paged_evict),
+    FAST(rope_axes),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_front", nullptr, -1, methods, nullptr, nullptr,

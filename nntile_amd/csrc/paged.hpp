@@ -47,6 +47,30 @@ struct PagedAttendParams
     float *part_ml;                     // workspace: [share][2][rows of a workgroup][2]
 };
 
+struct PagedWeightsParams
+{
+    PagedView c;                        // (the values are not read)
+    const void *Q;
+    const float *lse;
+    float *weights;                     // [entry][columns]
+    int64_t columns;
+    int32_t q_seq, kv_group, rows;      // rows = kv_group * q_seq, of a key/value head
+    int32_t causal;
+    float decay;
+    float scale;                        // 1/sqrt(head)
+    int32_t shares;                     // workgroups
+};
+
+struct PagedEvictParams
+{
+    PagedView c;
+    const float *weights;               // [entry][columns]
+    float *weights_out;                 // may be the same
+    int32_t *kept;                      // [entry][keep]
+    int64_t columns;
+    int32_t keep, recent;
+};
+
 struct RopeAxesParams
 {
     int64_t head, seq, n_batch, heads_q, heads_k;
@@ -66,6 +90,15 @@ int launch_paged_read(hipStream_t stream, int dtype, const PagedView &c, int hea
         int64_t rows, void *k_out, void *v_out);
 int launch_paged_attend(hipStream_t stream, int dtype, PagedAttendParams &p, int head,
         void *workspace);
+// Pages of 4-bit codes
+int launch_paged4_append(hipStream_t stream, int dtype, const PagedView &c, int head, int64_t rows,
+        const void *k_new, const void *v_new);
+int launch_paged4_read(hipStream_t stream, int dtype, const PagedView &c, int head, int64_t first,
+        int64_t rows, void *k_out, void *v_out);
+int launch_paged4_attend(hipStream_t stream, int dtype, PagedAttendParams &p, int head, void *workspace);
+// bits: of a page's values, 4, 8 or those of the tile type
+int launch_paged_weights(hipStream_t stream, int dtype, int bits, PagedWeightsParams &p, int head);
+int launch_paged_evict(hipStream_t stream, int bits, const PagedEvictParams &p, int head);
 // Bytes of workspace for `rows` = kv_group * q_seq query rows of a key/value head.
 size_t paged_attend_workspace_bytes(int64_t rows, int64_t head);
 int launch_rope_axes(hipStream_t stream, int dtype, bool backward, const RopeAxesParams &p);

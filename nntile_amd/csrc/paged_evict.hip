@@ -1,0 +1,316 @@
+// Eviction from a cache in pages: of every sequence and head the rows that received most of the attention stay,
+// and move together.
+//
+// Of a sequence with more rows than `keep` stay its last `recent` ones and, of those in front, the heaviest; of equal
+// ones the lower row.  They keep their order: row d of what is left is row kept[d] of what was there, kept[d] >= d,
+// and moves down in place.  Two launches:
+//
+//  * selection, a workgroup for every (sequence, head): the threshold by counting the weights' bits from the top, 11,
+//    11 and 10 of them, in LDS; then one walk over the rows that numbers those that stay.
+//  * the moves, a workgroup for every (sequence, head), K or V, and 64 bytes of the rows: several hundred rows at a
+//    time are read into registers, and when all of them are there, written.  A row's new place lies at or in front of
+//    its old one, so rows that are read later are never in the way.
+#include "paged_operands.hpp"
+#include "paged_rows.hpp"
+
+namespace nntile_hip
+{
+
+constexpr int kSelectThreads = 1024;
+constexpr int kSelectWaves = kSelectThreads / 64;
+constexpr int kSelectChunk = 4 * kSelectThreads;    // weights of a step, four a thread
+
+// A weight as an integer of the same order: -0 as 0, a NaN above all
+__device__ __forceinline__ uint32_t weight_key(float w)
+{
+    const uint32_t u = __float_as_uint(w + 0.0f);
+    return w != w ? ~0u : (u >> 31) != 0 ? ~u : u | 0x80000000u;
+}
+
+// The sums of `x` over the threads in front of this one, and over all.
+__device__ __forceinline__ uint32_t workgroup_scan(uint32_t x, uint32_t *wave_sum, uint32_t &all)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t upto = x;
+#pragma unroll
+    for(int o = 1; o < 64; o <<= 1)
+    {
+        const uint32_t other = __shfl_up(upto, o);
+        upto += lane >= o ? other : 0;
+    }
+    if(lane == 63)
+    {
+        wave_sum[wave] = upto;
+    }
+    __syncthreads();
+    uint32_t before = 0;
+    all = 0;
+#pragma unroll
+    for(int w = 0; w < kSelectWaves; ++w)
+    {
+        before += w < wave ? wave_sum[w] : 0;
+        all += wave_sum[w];
+    }
+    return before + upto - x;
+}
+
+__global__ __launch_bounds__(kSelectThreads)
+void paged_select_kernel(const PagedEvictParams p)
+{
+    constexpr int BINS = 2048;
+    __shared__ uint32_t bins[BINS];
+    __shared__ uint32_t wave_sum[2][kSelectWaves];
+    __shared__ uint32_t found[2];
+    const int tid = threadIdx.x;
+    const uint32_t entries = (uint32_t)p.c.n_batch * (uint32_t)p.c.n_head_kv;
+    for(uint32_t entry = blockIdx.x; entry < entries; entry += gridDim.x)
+    {
+        const int n = (int)(entry % (uint32_t)p.c.n_batch);
+        const int len = uniform(paged_len(p.c, n));
+        const float *const w_in = p.weights + (int64_t)entry * p.columns;
+        float *const w_out = p.weights_out + (int64_t)entry * p.columns;
+        int32_t *const kept = p.kept + (int64_t)entry * p.keep;
+        const int stay = min(len, p.keep);
+        for(int d = stay + tid; d < p.keep; d += kSelectThreads)
+        {
+            kept[d] = -1;
+        }
+        if(len <= p.keep)
+        {
+            for(int d = tid; d < len; d += kSelectThreads)
+            {
+                kept[d] = d;
+                if(w_out != w_in)
+                {
+                    w_out[d] = w_in[d];
+                }
+            }
+            continue;
+        }
+        const int old = len - p.recent;             // rows that are chosen from (recent <= keep < len)
+        uint32_t wanted = (uint32_t)(p.keep - p.recent);
+        // ---- the key of the wanted-th heaviest row ------------------------------------
+        uint32_t prefix = wanted == 0 ? ~0u : 0u;   // (nothing lies above it)
+        if(wanted != 0)
+        {
+            for(int pass = 0; pass < 3; ++pass)
+            {
+                const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 1024 : 2048;
+                for(int b = tid; b < BINS; b += kSelectThreads)
+                {
+                    bins[b] = 0;
+                }
+                __syncthreads();
+                for(int at = tid; at < old; at += kSelectThreads)
+                {
+                    const uint32_t key = weight_key(w_in[at]);
+                    if(pass == 0 || (key >> (pass == 1 ? 21 : 10)) == prefix)
+                    {
+                        atomicAdd(&bins[(key >> shift) & (width - 1)], 1u);
+                    }
+                }
+                __syncthreads();
+                // the largest bits first, two a thread
+                const uint32_t high = bins[BINS - 1 - 2 * tid], low = bins[BINS - 2 - 2 * tid];
+                uint32_t all;
+                const uint32_t before = workgroup_scan(high + low, wave_sum[pass & 1], all);
+                if(before < wanted && wanted <= before + high + low)
+                {
+                    const bool in_high = wanted <= before + high;
+                    found[0] = (uint32_t)(in_high ? BINS - 1 - 2 * tid : BINS - 2 - 2 * tid);
+                    found[1] = wanted - before - (in_high ? 0 : high);
+                }
+                __syncthreads();
+                prefix = prefix << (pass == 2 ? 10 : 11) | found[0];
+                wanted = found[1];
+            }
+        }
+        // ---- the rows that stay, in order ------------------------------------------------
+        // all above the key, and the first `wanted` that have it
+        uint32_t above_before = 0, equal_before = 0;
+        for(int at0 = 0, turn = 0; at0 < len; at0 += kSelectChunk, ++turn)
+        {
+            const int at = at0 + 4 * tid;
+            float w[4];
+            uint32_t above = 0, equal = 0;          // a bit for each of the four
+#pragma unroll
+            for(int k = 0; k < 4; ++k)
+            {
+                w[k] = at + k < len ? w_in[at + k] : 0.0f;
+                const uint32_t key = weight_key(w[k]);
+                above |= (at + k < old ? key > prefix : at + k < len) ? 1u << k : 0u;
+                equal |= at + k < old && key == prefix ? 1u << k : 0u;
+            }
+            // (at most 4096 of each in a step)
+            uint32_t all;
+            const uint32_t before = workgroup_scan((uint32_t)__popc(above) | (uint32_t)__popc(equal) << 16,
+                    wave_sum[turn & 1], all);
+            uint32_t a = above_before + (before & 0xffffu), e = equal_before + (before >> 16);
+#pragma unroll
+            for(int k = 0; k < 4; ++k)
+            {
+                if((above >> k & 1) != 0 || ((equal >> k & 1) != 0 && e < wanted))
+                {
+                    const uint32_t d = a + min(e, wanted);
+                    kept[d] = at + k;
+                    w_out[d] = w[k];
+                }
+                a += above >> k & 1;
+                e += equal >> k & 1;
+            }
+            above_before += all & 0xffffu;
+            equal_before += all >> 16;
+        }
+        // (the last step's weights have been read by all: the barrier in its scan)
+        for(int d = p.keep + tid; d < len; d += kSelectThreads)
+        {
+            w_out[d] = 0.0f;
+        }
+        __syncthreads();        // the next entry's bins and sums
+    }
+}
+
+constexpr int kEvictThreads = 1024;
+
+// The scale bytes of a row, 1, 2 or 4
+template<int SB> __device__ __forceinline__ uint32_t load_scales(const uint8_t *from)
+{
+    if constexpr(SB == 4)
+    {
+        return *reinterpret_cast<const uint32_t *>(from);
+    }
+    return SB == 2 ? *reinterpret_cast<const uint16_t *>(from) : *from;
+}
+
+template<int SB> __device__ __forceinline__ void store_scales(uint8_t *to, uint32_t x)
+{
+    if constexpr(SB == 4)
+    {
+        *reinterpret_cast<uint32_t *>(to) = x;
+    }
+    else if constexpr(SB == 2)
+    {
+        *reinterpret_cast<uint16_t *>(to) = (uint16_t)x;
+    }
+    else
+    {
+        *to = (uint8_t)x;
+    }
+}
+
+// SB: scale bytes of a row.  LANES threads have 16 bytes each of a row's slice.
+template<int ROW_BYTES, int SB>
+__global__ __launch_bounds__(kEvictThreads)
+void paged_evict_kernel(const PagedEvictParams p)
+{
+    constexpr int SLICE = ROW_BYTES < 64 ? ROW_BYTES : 64, SLICES = ROW_BYTES / SLICE, LANES = SLICE / 16;
+    constexpr int ROWS = kEvictThreads / LANES, AT_ONCE = 4;
+    const int piece = threadIdx.x % LANES, slot = threadIdx.x / LANES;
+    const uint32_t entries = (uint32_t)p.c.n_batch * (uint32_t)p.c.n_head_kv;
+    for(uint32_t work = blockIdx.x; work < entries * (2 * SLICES); work += gridDim.x)
+    {
+        const uint32_t entry = work / (2 * SLICES), slice = work % SLICES, which = work / SLICES % 2;
+        const int n = (int)(entry % (uint32_t)p.c.n_batch), h = (int)(entry / (uint32_t)p.c.n_batch);
+        const int len = uniform(paged_len(p.c, n));
+        if(len <= p.keep)
+        {
+            continue;
+        }
+        const int32_t *const kept = p.kept + (int64_t)entry * p.keep;
+        char *const pages = (which ? p.c.v_pages : p.c.k_pages) + slice * SLICE + piece * 16;
+        uint8_t *const scales = which ? p.c.v_scales : p.c.k_scales;
+        for(int d0 = 0; d0 < p.keep; d0 += ROWS * AT_ONCE)
+        {
+            u32x4 x[AT_ONCE];
+            uint32_t size[AT_ONCE];
+            int src[AT_ONCE];
+#pragma unroll
+            for(int k = 0; k < AT_ONCE; ++k)
+            {
+                const int d = d0 + k * ROWS + slot;
+                src[k] = d < p.keep ? kept[d] : -1;
+                src[k] = src[k] > d && src[k] < len ? src[k] : -1;      // (a row that stays where it is)
+            }
+#pragma unroll
+            for(int k = 0; k < AT_ONCE; ++k)
+            {
+                // (a row without a page: zeros)
+                x[k] = u32x4{0, 0, 0, 0};
+                size[k] = 0x7f7f7f7fu;
+                const int page = src[k] >= 0 ? page_of(p.c, n, src[k]) : -1;
+                if(page >= 0)
+                {
+                    const int64_t at = row_in_page(p.c, h, src[k]);
+                    x[k] = *reinterpret_cast<const u32x4 *>(pages + page * p.c.page_stride + at * ROW_BYTES);
+                    if constexpr(SB != 0)
+                    {
+                        if(slice == 0 && piece == 0)
+                        {
+                            size[k] = load_scales<SB>(scales + page * p.c.scale_stride + at * SB);
+                        }
+                    }
+                }
+            }
+            // all rows of the step are read before the first is written
+            paged_wait_loads<0>();
+            __syncthreads();
+#pragma unroll
+            for(int k = 0; k < AT_ONCE; ++k)
+            {
+                const int d = d0 + k * ROWS + slot;
+                const int page = src[k] >= 0 ? page_of(p.c, n, d) : -1;
+                if(page >= 0)
+                {
+                    const int64_t at = row_in_page(p.c, h, d);
+                    *reinterpret_cast<u32x4 *>(pages + page * p.c.page_stride + at * ROW_BYTES) = x[k];
+                    if constexpr(SB != 0)
+                    {
+                        if(slice == 0 && piece == 0)
+                        {
+                            store_scales<SB>(scales + page * p.c.scale_stride + at * SB, size[k]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+}
+
+template<int ROW_BYTES, int SB>
+static int launch_evict(hipStream_t stream, const PagedEvictParams &p)
+{
+    constexpr int SLICES = ROW_BYTES < 64 ? 1 : ROW_BYTES / 64;
+    const int64_t entries = (int64_t)p.c.n_batch * p.c.n_head_kv, work = entries * 2 * SLICES;
+    if(work > 0x7fffffff)
+    {
+        return NNTILE_HIP_EINVAL;
+    }
+    // (a direction of a launch has less than 2^32 threads)
+    constexpr int64_t MOST = 1 << 20;
+    hipLaunchKernelGGL(paged_select_kernel, dim3((unsigned)(entries < MOST ? entries : MOST)), dim3(kSelectThreads), 0, stream, p);
+    if(hipGetLastError() != hipSuccess)
+    {
+        return NNTILE_HIP_ELAUNCH;
+    }
+    hipLaunchKernelGGL((paged_evict_kernel<ROW_BYTES, SB>), dim3((unsigned)(work < MOST ? work : MOST)), dim3(kEvictThreads), 0,
+            stream, p);
+    return hipGetLastError() == hipSuccess ? NNTILE_HIP_OK : NNTILE_HIP_ELAUNCH;
+}
+
+int launch_paged_evict(hipStream_t stream, int bits, const PagedEvictParams &p, int head)
+{
+    switch(bits * 256 + head)
+    {
+        case 4 * 256 + 64: return launch_evict<32, 2>(stream, p);
+        case 4 * 256 + 128: return launch_evict<64, 4>(stream, p);
+        case 8 * 256 + 64: return launch_evict<64, 1>(stream, p);
+        case 8 * 256 + 128: return launch_evict<128, 1>(stream, p);
+        case 16 * 256 + 64: return launch_evict<128, 0>(stream, p);
+        case 16 * 256 + 128: return launch_evict<256, 0>(stream, p);
+        case 32 * 256 + 64: return launch_evict<256, 0>(stream, p);
+        case 32 * 256 + 128: return launch_evict<512, 0>(stream, p);
+        default: return NNTILE_HIP_EUNSUPPORTED;
+    }
+}
+
+} // namespace nntile_hip

@@ -104,6 +104,19 @@ class PagedArgs(ctypes.Structure):
                 ("Q", _vp), ("lse", _vp), ("A", _vp)]
 
 
+class PagedWeightsArgs(ctypes.Structure):
+    """nntile_hip_paged_weights_args."""
+    _fields_ = [("cache", PagedCacheArgs), ("q_seq", _i64), ("kv_group", _i64), ("columns", _i64),
+                ("mask_mode", ctypes.c_int32), ("decay", ctypes.c_float),
+                ("Q", _vp), ("lse", _vp), ("weights", _vp)]
+
+
+class PagedEvictArgs(ctypes.Structure):
+    """nntile_hip_paged_evict_args."""
+    _fields_ = [("cache", PagedCacheArgs), ("keep", _i64), ("recent", _i64), ("columns", _i64),
+                ("weights", _vp), ("weights_out", _vp), ("kept", _vp)]
+
+
 class RopeAxesArgs(ctypes.Structure):
     """nntile_hip_rope_axes_args."""
     _fields_ = [("head", _i64), ("seq", _i64), ("n_batch", _i64), ("heads_q", _i64),
@@ -165,6 +178,11 @@ EXPORTS = (
     + ["nntile_hip_paged_kv_read_" + t for t in ("bf16", "fp16", "fp32")]
     + ["nntile_hip_sdpa_fwd_paged_" + t for t in ("bf16", "fp16", "fp32")]
     + ["nntile_hip_sdpa_fwd_paged_workspace_bytes"]
+    + ["nntile_hip_paged_attn_weights_" + t for t in ("bf16", "fp16", "fp32")]
+    + ["nntile_hip_paged_kv_evict_" + t for t in ("bf16", "fp16", "fp32")]
+    + [f + t for t in ("bf16", "fp16")
+       for f in ("nntile_hip_paged4_kv_append_", "nntile_hip_paged4_kv_read_", "nntile_hip_sdpa_fwd_paged4_",
+                 "nntile_hip_paged4_attn_weights_", "nntile_hip_paged4_kv_evict_")]
     + ["nntile_hip_rope_axes_" + t for t in ("bf16", "fp16", "fp32")]
     + ["nntile_hip_mask_tile_class_" + t for t in ("bf16", "fp16", "fp32", "bool")]
     + ["nntile_hip_sdpa_fwd_grid_codelet_" + t for t in ("bf16", "fp16", "fp32")]
@@ -242,15 +260,22 @@ def lib():
             f = getattr(L, "nntile_hip_kv_cache_append_" + t)
             f.argtypes = [_vp] + [_i64] * 5 + [_vp] * 4
             f.restype = ctypes.c_int
-            f = getattr(L, "nntile_hip_paged_kv_append_" + t)
-            f.argtypes = [_vp, ctypes.POINTER(PagedCacheArgs), _i64, _vp, _vp]
-            f.restype = ctypes.c_int
-            f = getattr(L, "nntile_hip_paged_kv_read_" + t)
-            f.argtypes = [_vp, ctypes.POINTER(PagedCacheArgs), _i64, _i64, _vp, _vp]
-            f.restype = ctypes.c_int
-            f = getattr(L, "nntile_hip_sdpa_fwd_paged_" + t)
-            f.argtypes = [_vp, ctypes.POINTER(PagedArgs), _vp, ctypes.c_size_t]
-            f.restype = ctypes.c_int
+            for kind in ("paged", "paged4") if t != "fp32" else ("paged",):
+                f = getattr(L, "nntile_hip_%s_kv_append_%s" % (kind, t))
+                f.argtypes = [_vp, ctypes.POINTER(PagedCacheArgs), _i64, _vp, _vp]
+                f.restype = ctypes.c_int
+                f = getattr(L, "nntile_hip_%s_kv_read_%s" % (kind, t))
+                f.argtypes = [_vp, ctypes.POINTER(PagedCacheArgs), _i64, _i64, _vp, _vp]
+                f.restype = ctypes.c_int
+                f = getattr(L, "nntile_hip_sdpa_fwd_%s_%s" % (kind, t))
+                f.argtypes = [_vp, ctypes.POINTER(PagedArgs), _vp, ctypes.c_size_t]
+                f.restype = ctypes.c_int
+                f = getattr(L, "nntile_hip_%s_attn_weights_%s" % (kind, t))
+                f.argtypes = [_vp, ctypes.POINTER(PagedWeightsArgs)]
+                f.restype = ctypes.c_int
+                f = getattr(L, "nntile_hip_%s_kv_evict_%s" % (kind, t))
+                f.argtypes = [_vp, ctypes.POINTER(PagedEvictArgs)]
+                f.restype = ctypes.c_int
             f = getattr(L, "nntile_hip_rope_axes_" + t)
             f.argtypes = [_vp, ctypes.POINTER(RopeAxesArgs)]
             f.restype = ctypes.c_int
@@ -790,7 +815,9 @@ def paged_kv_append(k_new, v_new, k_pages, v_pages, table, lens, k_scales=None, 
     """Write k_new, v_new ([n_head_kv*n_batch, rows, head]) into the pages of a
     cache: k_pages, v_pages [n_pages, n_head_kv, page_rows, head] in the type of
     the tiles, or torch.float8_e4m3fn with k_scales, v_scales [n_pages,
-    n_head_kv, page_rows] (uint8, the exponent of a row's power of two + 127);
+    n_head_kv, page_rows] (uint8, the exponent of a row's power of two + 127), or
+    torch.float4_e2m1fn_x2 (head/2 elements a row, two codes each) with scales
+    [n_pages, n_head_kv, page_rows, head/32], one for every 32 values of a row;
     only their first axis may be strided.  table: [n_batch, max_pages] int32 page
     numbers; lens: [n_batch] int32 rows of each sequence, the new ones included;
     new_rows: [n_batch] int32, how many of `rows` each sequence brings (None: all).
@@ -830,6 +857,32 @@ def sdpa_fwd_paged(k_pages, v_pages, table, lens, Q, lse, A, mask_mode, kv_group
     _check(_native().fwd_paged(k_pages, v_pages, table, lens, Q, lse, A, mask_mode, kv_group,
                                workspace, k_scales, v_scales, new_rows, flags, stream),
            "sdpa_fwd_paged")
+
+
+def paged_attn_weights(k_pages, table, lens, Q, lse, weights, mask_mode, kv_group, k_scales=None,
+                       new_rows=None, decay=1.0, stream=None):
+    """weights = decay * weights + the probabilities with which the newest tokens'
+    queries attend to each row of a paged cache (see paged_kv_append), summed over
+    the tokens and the kv_group heads: Q and lse as sdpa_fwd_paged took and, with
+    OVERWRITE, left them; weights [n_head_kv*n_batch, columns] fp32, columns at
+    least the rows that the table has pages for.  Columns at or behind lens stay
+    as they are; decay (0 to 1) 0: what weights held does not matter."""
+    _check(_native().paged_attn_weights(k_pages, table, lens, Q, lse, weights, mask_mode, kv_group,
+                                        k_scales, new_rows, decay, stream), "paged_attn_weights")
+
+
+def paged_kv_evict(k_pages, v_pages, table, lens, weights, weights_out, kept, recent, k_scales=None,
+                   v_scales=None, stream=None):
+    """Of every sequence of a paged cache (see paged_kv_append) with more than keep =
+    kept.shape[1] rows, keep stay, for each head: the last `recent` and the ones
+    with the largest weights ([n_head_kv*n_batch, columns], see
+    paged_attn_weights) of those in front; of equal ones the lower.  They move to
+    the first rows, in their order.  kept [n_head_kv*n_batch, keep] int32: the row
+    that each was, -1 behind the last.  weights_out (may be weights): columns
+    below lens are written, the weights of the rows that stayed, then zeros.  The
+    caller lowers lens to at most keep behind the call."""
+    _check(_native().paged_evict(k_pages, v_pages, table, lens, weights, weights_out, kept, recent,
+                                 k_scales, v_scales, stream), "paged_kv_evict")
 
 
 def rope_axes_freqs(head, sections, base=10000.0, own=False, device="cuda"):

@@ -209,8 +209,9 @@ class KVCache:
 
 class PagedKVCache:
     """Key/value cache whose sequences have lengths of their own: rows lie in
-    pages of a pool that all sequences share, as they are or in 8 bits (e4m3 with
-    one power of two per row).  What `KVCache` does for a batch of equal lengths,
+    pages of a pool that all sequences share, as they are, in 8 bits (packed, or bits=8:
+    e4m3 with one power of two per row) or in 4 (bits=4: e2m1 with one power of two
+    per 32 values).  What `KVCache` does for a batch of equal lengths,
     for a batch that is served: sequences end (`release`) and their pages go to others.
 
     Tensors as for `KVCache`: K, V `[n_head_kv * n_batch, rows, head]`, Q, A
@@ -221,10 +222,15 @@ class PagedKVCache:
     `table` and a `lens` of its own instead: this class's bookkeeping would run once,
     at the capture.  Calls of one cache share its workspace: they belong on one stream,
     or are ordered by the caller.
+
+    weighted: the cache keeps, for every row and head, the attention that the row
+    received (`weights`, added to by `observe`), by which `evict` chooses the rows that stay
+    when sequences are cut down.  A row is then no longer a token's position: whoever
+    turns keys and queries by their positions counts the tokens.
     """
 
     def __init__(self, n_pages, page_rows, n_batch, max_rows, n_head_kv, head, dtype=torch.bfloat16,
-                 packed=False, device="cuda"):
+                 packed=False, device="cuda", bits=None, weighted=False):
         if page_rows < 16 or page_rows > 65536 or page_rows & (page_rows - 1):
             raise ValueError("page_rows is a power of two from 16 to 65536")
         if min(n_pages, n_batch, max_rows, n_head_kv) < 1 or head not in (64, 128):
@@ -232,20 +238,32 @@ class PagedKVCache:
         if -(-max_rows // page_rows) * page_rows > 0x7fffffff or n_batch * n_head_kv > 0x7fffffff:
             raise ValueError("the rows of a sequence's pages, and sequences times heads, are below 2^31")
         hip_sdpa.dtype_name(torch.empty(0, dtype=dtype))
+        if bits not in (None, 4, 8) or (packed and bits == 4):
+            raise ValueError("pages hold the tile type, or 8 (packed) or 4 bits")
+        packed = bool(packed) or bits is not None
         if packed and dtype == torch.float32:
-            raise TypeError("8-bit pages hold bf16 and fp16 tiles")
-        self.dtype, self.packed = dtype, bool(packed)
+            raise TypeError("8-bit pages hold bf16 and fp16 tiles" if bits != 4 else "4-bit pages hold bf16 and fp16 tiles")
+        self.dtype, self.packed = dtype, packed
+        self.bits = 4 if bits == 4 else 8 if packed else 8 * dtype.itemsize
         self.n_batch, self.n_head_kv, self.head = n_batch, n_head_kv, head
         self.page_rows, self.max_pages = page_rows, -(-max_rows // page_rows)
         # (a page's keys and values behind each other)
         shape = (n_pages, 2, n_head_kv, page_rows, head)
-        pool = torch.zeros(shape, dtype=torch.uint8 if packed else dtype, device=device)
-        self.pool = pool.view(torch.float8_e4m3fn) if packed else pool
+        if self.bits == 4:
+            pool = torch.zeros(shape[:4] + (head // 2,), dtype=torch.uint8, device=device)
+            self.pool = pool.view(torch.float4_e2m1fn_x2)
+        else:
+            pool = torch.zeros(shape, dtype=torch.uint8 if packed else dtype, device=device)
+            self.pool = pool.view(torch.float8_e4m3fn) if packed else pool
         self.k_pages, self.v_pages = self.pool[:, 0], self.pool[:, 1]
-        self.scales = torch.ones(shape[:4], dtype=torch.uint8, device=device) if packed else None
+        of_row = (head // 32,) if self.bits == 4 else ()
+        self.scales = torch.ones(shape[:4] + of_row, dtype=torch.uint8, device=device) if packed else None
         self.k_scales, self.v_scales = (self.scales[:, 0], self.scales[:, 1]) if packed else (None, None)
         self.table = torch.full((n_batch, self.max_pages), -1, dtype=torch.int32, device=device)
         self.lens = torch.zeros(n_batch, dtype=torch.int32, device=device)
+        # (columns behind a sequence's rows are zeros)
+        self.weights = torch.zeros(n_head_kv * n_batch, self.max_pages * page_rows, dtype=torch.float32,
+                                   device=device) if weighted else None
         self.lengths = [0] * n_batch
         self._pages = [[] for _ in range(n_batch)]
         self._free = list(range(n_pages - 1, -1, -1))
@@ -275,7 +293,7 @@ class PagedKVCache:
         """The cache's tensors and these are in use on a stream that is given: memory of
         theirs that is freed waits for it."""
         if stream is not None:
-            for t in (self.pool, self.scales, self.table, self.lens) + tensors:
+            for t in (self.pool, self.scales, self.table, self.lens, self.weights) + tensors:
                 if t is not None:
                     t.record_stream(stream)
 
@@ -416,10 +434,57 @@ class PagedKVCache:
         self.append(k, v, new_rows=new_rows, stream=stream)
         self.attend(Q, lse, A, kv_group, causal=causal, new_rows=new_rows, stream=stream)
 
+    def _has_weights(self):
+        if self.weights is None:
+            raise ValueError("the cache was made without weights (weighted=True)")
+
+    def observe(self, Q, lse, kv_group, causal=True, new_rows=None, decay=1.0, stream=None):
+        """Behind an `attend` with the same Q, kv_group, causal and new_rows, and with the lse that
+        it left: weights = decay * weights + the attention that every row received, over the
+        queries and the kv_group heads."""
+        self._has_weights()
+        counts = self._counts(Q.shape[1], new_rows)
+        mode = hip_sdpa.MASK_CAUSAL if causal else hip_sdpa.MASK_NONE
+        self._in_use(stream, Q, lse)
+        given = None if new_rows is None else self._on_device(counts, stream)
+        hip_sdpa.paged_attn_weights(self.k_pages, self.table, self.lens, Q, lse, self.weights, mode, kv_group,
+                                    k_scales=self.k_scales, new_rows=given, decay=decay, stream=stream)
+
+    def evict(self, keep, recent=0, stream=None):
+        """Cut every sequence with more than `keep` rows down to that many: for each head the
+        last `recent` and the ones with the largest weights of those in front (of equal ones the
+        lower row), in their order.  Pages that are no longer needed are free for others.  Returns kept
+        [n_head_kv * n_batch, keep] int32: the row that each was, -1 behind a sequence's last."""
+        self._has_weights()
+        if keep < 1 or recent < 0 or recent > keep:
+            raise ValueError("keep is at least 1, recent between 0 and keep")
+        with torch.cuda.stream(stream):
+            kept = torch.empty((self.n_head_kv * self.n_batch, keep), dtype=torch.int32, device=self.lens.device)
+        self._in_use(stream)
+        hip_sdpa.paged_kv_evict(self.k_pages, self.v_pages, self.table, self.lens, self.weights, self.weights,
+                                kept, recent, k_scales=self.k_scales, v_scales=self.v_scales, stream=stream)
+        # (only now: a refused call leaves the cache as it was)
+        if max(self.lengths) > keep:
+            self.lengths = [min(length, keep) for length in self.lengths]
+            for n, length in enumerate(self.lengths):
+                stay = -(-length // self.page_rows)
+                self._free += reversed(self._pages[n][stay:])
+                del self._pages[n][stay:]
+            self._upload_places(stream)
+        return kept
+
+    def _upload_places(self, stream):
+        self._upload(self.lens, self.lengths, stream)
+        self._upload(self.table, [p + [-1] * (self.max_pages - len(p)) for p in self._pages], stream)
+
     def release(self, n, stream=None):
         """Sequence n is over: its pages are free for others."""
         self._free += reversed(self._pages[n])
         self._pages[n] = []
         self.lengths[n] = 0
-        self._upload(self.lens, self.lengths, stream)
-        self._upload(self.table, [p + [-1] * (self.max_pages - len(p)) for p in self._pages], stream)
+        if self.weights is not None:
+            with torch.cuda.stream(stream):
+                self.weights.view(self.n_head_kv, self.n_batch, -1)[:, n].zero_()
+            if stream is not None:
+                self.weights.record_stream(stream)
+        self._upload_places(stream)
