@@ -37,6 +37,14 @@ __device__ __forceinline__ W scalar_load(const void *base, int64_t byte)
     return *reinterpret_cast<ptr>(reinterpret_cast<uintptr_t>(base) + byte);
 }
 
+// x, of which the compiler knows nothing: what follows from it is not worked out in front of a loop, to be kept
+// there in registers that the loop has other use for
+__device__ __forceinline__ int fresh(int x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 __device__ __forceinline__ int uniform(int x)
 {
     return __builtin_amdgcn_readfirstlane(x);
@@ -142,6 +150,23 @@ template<typename T> __device__ __forceinline__ u32x4 widen8_of_4(uint32_t codes
         w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3));
     }
     return w;
+}
+
+// Two bf16 numbers, not below 0, at most 1 and taken down by 127 << 7, times 2^byte each (what falls below the
+// smallest number becomes 0): the exponents are integers above the seven bits of the mantissa.
+__device__ __forceinline__ uint32_t add_exponents(uint32_t lowered, uint32_t two_bytes)
+{
+    typedef __attribute__((ext_vector_type(2))) int16_t i16x2;
+    uint32_t sum;
+    asm("v_pk_mad_u16 %0, %1, %2, %3" : "=v"(sum) : "v"(two_bytes), "s"(0x00800080u), "v"(lowered));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(i16x2, sum), i16x2{0, 0}));
+}
+
+// ... and down by 127 << 7
+__device__ __forceinline__ uint32_t lower_exponents(uint32_t x)
+{
+    typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2, x) - (uint16_t)(127 << 7));
 }
 
 // Eight fp16 values as sums of two bf16 numbers: the first 8 bits, and what they leave, exactly.

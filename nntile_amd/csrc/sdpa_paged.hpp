@@ -41,70 +41,10 @@
 
 #include <type_traits>
 
-#include "paged_operands.hpp"
+#include "sdpa_paged4_walk.hpp"
 
 namespace nntile_hip
 {
-
-constexpr int kPagedCUs = 256;
-// Workgroups that the keys are shared out to at most: two a CU
-constexpr int kPagedShares = 2 * kPagedCUs;
-// What a unit costs beside its key blocks, in blocks
-constexpr int kPagedUnitCost = 1;
-// How far, in powers of two, probabilities may grow past the first before they are taken against a new maximum
-constexpr float kPagedSlack = 8.0f;
-// fp16 probabilities of 16-bit pages are kept times 2^7: they stay below 2^15, and 2^-21 still has all of its bits
-constexpr float kPagedLift = 7.0f;
-// Counts of shares in the workspace: in the low bits, above them a fixed word by which a count is told
-// from what else memory may hold; a cache line each.
-constexpr unsigned long long kPagedCountMask = 4095;
-constexpr unsigned long long kPagedNone = 0x9e3779b97f4a7000ull;
-constexpr int kPagedCountStride = 8;
-static_assert(kPagedShares < (int)kPagedCountMask, "counts stay below the word");
-
-template<int KIND, int HEAD, int NR, int HALVES>
-struct PagedShape
-{
-    static constexpr int STREAMS = 4;                       // wavefronts that take different keys
-    static constexpr int WAVES = STREAMS * HALVES;
-    static constexpr int THREADS = 64 * WAVES;
-    static constexpr int QROWS = 16 * NR * HALVES;          // query rows of a workgroup
-    static constexpr int RB = KIND == kPaged32 ? HEAD * 4 : KIND == kPaged8 ? HEAD : KIND == kPaged4 ? HEAD / 2
-        : HEAD * 2;                                         // bytes of a row
-    static constexpr int SB = KIND == kPaged8 ? 1 : KIND == kPaged4 ? HEAD / 32 : 0;     // scale bytes of a row
-    static constexpr int CPR = RB / 16;                     // 16-byte chunks of a row
-    static constexpr int RPL = RB >= 256 ? 1 : 256 / RB;    // rows per 256-byte line of LDS banks
-    // keys of a wavefront's step: 8 KB of K and V; twice that where two wavefronts share them and the pages hold
-    // 16 bits (8 sequences of 8192 rows, 8 heads of 128, 64 query rows 54.8 us, 58.7 with 8 KB; 8-bit pages, whose
-    // widened operands are more registers, 51.7 and 47.7)
-    static constexpr int ALONE = 4096 / RB > 16 ? 4096 / RB : 16;
-    static constexpr int KEYS = KIND == kPaged8 ? ALONE : HALVES * ALONE < 64 ? HALVES * ALONE : 64;
-    static_assert(KIND != kPaged4 || KEYS == 64, "a transposing read of 4-bit values takes 64 keys");
-    static constexpr int BLOCK = STREAMS * KEYS;        // keys of a workgroup's step
-    static constexpr int GROUPS = KEYS / 16;
-    static constexpr int K_BYTES = KEYS * RB;
-    static constexpr int STAGE = 2 * K_BYTES;
-    static constexpr int LOADS = K_BYTES / 1024;            // load instructions of a step's K
-    static constexpr int ROWS_PER_LOAD = 1024 / RB;
-    // (what a row block of all wavefronts takes at the end, too)
-    static constexpr int MERGE_BYTES = STREAMS * 16 * HALVES * (HEAD + 4 + 2) * 4;
-    static constexpr int RING = STREAMS * 2 * STAGE > MERGE_BYTES ? STREAMS * 2 * STAGE : MERGE_BYTES;
-    static constexpr int WGS_PER_CU = RING > 72 * 1024 || WAVES > 4 ? 1 : 2;
-    static constexpr int MIN_WAVES = WAVES * WGS_PER_CU / 4;        // of a SIMD
-    // the query rows: the operands of one block of 16 stay in registers, those of two in LDS
-    static constexpr int QB = HEAD * (KIND == kPaged32 ? 4 : 2);
-    static constexpr int Q_BYTES = NR > 1 ? QROWS * QB : 16;
-    static __host__ __device__ constexpr int q_swizzle(int r) { return r % (QB / 16 < 16 ? QB / 16 : 16); }
-
-    // Where chunk c of row r lies: chunk position c ^ swizzle(r) of the row, so that the
-    // rows one LDS instruction reads fall on different banks.
-    static __host__ __device__ constexpr int k_swizzle(int r) { return (r / RPL) % CPR; }
-    static __host__ __device__ constexpr int v_swizzle(int r)
-    {
-        return KIND == kPaged16 ? 2 * ((r / RPL) % (CPR / 2))
-            : KIND == kPaged8 ? k_swizzle(r) : KIND == kPaged4 ? (r >> 4) % CPR : 4 * ((r >> 2) & 3);
-    }
-};
 
 // Whether a word of a page - two 16-bit values, four codes or an fp32 value - holds a NaN or an infinity
 template<typename T, int KIND> __device__ __forceinline__ bool not_numbers(uint32_t w)
@@ -124,14 +64,6 @@ template<typename T, int KIND> __device__ __forceinline__ bool not_numbers(uint3
         return (w & E) == E || ((w >> 16) & E) == E;
     }
 }
-
-// What a workgroup works on at a time: key blocks [step, step + steps) of unit u (head and row
-// group) of sequence n.
-struct PagedSegment
-{
-    int n, len, blocks;     // sequence, its rows, their key blocks
-    int u, step, steps;
-};
 
 // Partial results go from one workgroup to another of the same launch, on any XCD: stores and
 // loads that the device serves, not a CU's or an XCD's own cache.
@@ -205,20 +137,13 @@ __device__ __forceinline__ void paged_finish_row(const PagedAttendParams &p, int
     }
 }
 
-// Row of lse (times head: of Q and A) of query row rr of key/value head h of sequence n
-__device__ __forceinline__ int64_t paged_query_row(const PagedAttendParams &p, int n, int h, int rr)
-{
-    const int g = rr / p.q_seq, tok = rr % p.q_seq;
-    return (n + (int64_t)p.c.n_batch * (g + (int64_t)p.kv_group * h)) * p.q_seq + tok;
-}
-
 // Joins the shares w0 .. w0 + parts - 1 of a unit, in this order, and finishes its rows.
 // HEAD/4 threads a row; where the rows leave threads over, they take turns at the
 // shares and the sums are added up through LDS.  A thread has PARTS shares of LINES rows on their way
 // at a time: the round trips are what the join costs.
 template<typename T, int HEAD, int THREADS, int QROWS, int PARTS, int LINES>
 __device__ __forceinline__ void paged_join_by(const PagedAttendParams &p, int n, int h, int rg, int rows_here,
-        int w0, int parts, float *lds)
+        int w0, int parts, float *lds, int tid)
 {
     constexpr int TPR = HEAD / 4, ROWS = THREADS / TPR;
     int turns = 1;
@@ -226,7 +151,7 @@ __device__ __forceinline__ void paged_join_by(const PagedAttendParams &p, int n,
     {
         turns *= 2;
     }
-    const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;      // pairs 2t and 2t + HEAD/2 of the row
+    const int t = tid % TPR, slot = tid / TPR;      // pairs 2t and 2t + HEAD/2 of the row
     const int turn = slot % turns, step = ROWS / turns;
     // (with more than one turn all rows fit beside each other: one round of one line)
     for(int r0 = slot / turns; r0 - slot / turns < rows_here; r0 += LINES * step)
@@ -332,53 +257,45 @@ __device__ __forceinline__ void paged_join_by(const PagedAttendParams &p, int n,
 
 template<typename T, int HEAD, int THREADS, int QROWS>
 __device__ __forceinline__ void paged_join(const PagedAttendParams &p, int n, int h, int rg, int rows_here,
-        int w0, int parts, float *lds)
+        int w0, int parts, float *lds, int tid)
 {
     if(rows_here > THREADS / (HEAD / 4) && parts <= 4)
     {
-        paged_join_by<T, HEAD, THREADS, QROWS, 4, 4>(p, n, h, rg, rows_here, w0, parts, lds);
+        paged_join_by<T, HEAD, THREADS, QROWS, 4, 4>(p, n, h, rg, rows_here, w0, parts, lds, tid);
     }
     else if(rows_here > THREADS / (HEAD / 4))
     {
-        paged_join_by<T, HEAD, THREADS, QROWS, 8, 2>(p, n, h, rg, rows_here, w0, parts, lds);
+        paged_join_by<T, HEAD, THREADS, QROWS, 8, 2>(p, n, h, rg, rows_here, w0, parts, lds, tid);
     }
     else
     {
-        paged_join_by<T, HEAD, THREADS, QROWS, 8, 1>(p, n, h, rg, rows_here, w0, parts, lds);
+        paged_join_by<T, HEAD, THREADS, QROWS, 8, 1>(p, n, h, rg, rows_here, w0, parts, lds, tid);
     }
 }
 
 template<typename T, int KIND, int HEAD, int NR, int HALVES>
-__global__ __launch_bounds__((PagedShape<KIND, HEAD, NR, HALVES>::THREADS), (PagedShape<KIND, HEAD, NR, HALVES>::MIN_WAVES))
+__global__ __launch_bounds__((PagedShape<T, KIND, HEAD, NR, HALVES>::THREADS), (PagedShape<T, KIND, HEAD, NR, HALVES>::MIN_WAVES))
 void sdpa_paged_kernel(const PagedAttendParams p)
 {
-    typedef PagedShape<KIND, HEAD, NR, HALVES> Shape;
+    typedef PagedShape<T, KIND, HEAD, NR, HALVES> Shape;
     constexpr int RB = Shape::RB, CPR = Shape::CPR, KEYS = Shape::KEYS, GROUPS = Shape::GROUPS;
     constexpr int LOADS = Shape::LOADS, K_BYTES = Shape::K_BYTES, STAGE = Shape::STAGE;
     constexpr int WAVES = Shape::WAVES, STREAMS = Shape::STREAMS, THREADS = Shape::THREADS;
     constexpr int DBLOCKS = HEAD / 16;
     // registers of a row block's query operand: 16 bytes each
     constexpr int QREGS = KIND == kPaged32 ? HEAD / 16 : HEAD / 32;
-    // 4-bit pages: keys become bf16 numbers, whose exponents take any power of two of a block; an fp16 query is the
-    // sum of two of them then (11 bits in 8 and 3, exactly), with products of its own each
-    constexpr bool TWO_Q = KIND == kPaged4 && __is_same(T, Fp16);
-    constexpr int QPARTS = TWO_Q ? 2 : 1;
-    typedef typename std::conditional<KIND == kPaged4, Bf16, T>::type QK;
     constexpr int QROWS = Shape::QROWS;
-    constexpr bool Q_IN_LDS = NR > 1;
+    constexpr bool Q_IN_LDS = NR > 1 && KIND != kPaged4;
     // the type of the probabilities and values as the matrix instruction takes them (fp32 pages: neither)
     typedef typename std::conditional<KIND == kPaged16, T, Bf16>::type PV;
-    constexpr bool CODES = KIND == kPaged8 || KIND == kPaged4;
-    constexpr int SB = Shape::SB;
     // 8-bit pages: the scale of a key row goes into its codes (exact in bf16; fp16 has not the range: into the
     // scores), that of a value row into its probabilities, which are bf16 numbers then and the codes exact in
     // bf16.  For fp16 tiles 8 bits are too few: what the first number leaves of a probability is a second one,
     // with products of its own (64 of 2048 rows, 8 heads of 128: 47 us with 4 query rows, 55 with 32, 94 with 64;
     // as one fp16 number against the largest power of two so far 47, 54 and 84, but then a row that is not seen, or
     // has no weight, takes the bits of smaller ones).
-    // 4-bit pages: the same, with a power of two of its own for every 32 values of a row.
-    constexpr bool KSCALE_IN_CODES = KIND == kPaged4 || (KIND == kPaged8 && __is_same(T, Bf16));
-    constexpr bool TWO_PARTS = CODES && __is_same(T, Fp16);
+    constexpr bool KSCALE_IN_CODES = KIND == kPaged8 && __is_same(T, Bf16);
+    constexpr bool TWO_PARTS = KIND == kPaged8 && __is_same(T, Fp16);
     // the power of two that the probabilities, and so their sum, carry: where they have fp32's exponents, they
     // stay below 1, so that products with the largest values do not overflow
     constexpr float kLift = KIND == kPaged16 && __is_same(T, Fp16) ? kPagedLift : -kPagedSlack;
@@ -389,9 +306,9 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     constexpr int JOIN_ROWS = THREADS / (HEAD / 4);     // rows that are joined at a time
     static_assert(JOIN_ROWS * (HEAD + 4) * 4 <= Shape::RING, "... and so do the shares' sums");
     __shared__ __attribute__((aligned(1024))) char ring[Shape::RING];
-    __shared__ __attribute__((aligned(16))) char q_rows[Shape::Q_BYTES * QPARTS];
-    // pages of codes: the scale bytes of a wavefront's step and of the next, keys' and values'
-    __shared__ __attribute__((aligned(16))) char scale_bytes[CODES ? WAVES * 2 * 2 * KEYS * SB : 16];
+    __shared__ __attribute__((aligned(16))) char q_rows[KIND == kPaged4 ? 16 : Shape::Q_BYTES];
+    // 8-bit pages: the scale bytes of a wavefront's step and of the next, keys' and values'
+    __shared__ __attribute__((aligned(16))) char scale_bytes[KIND == kPaged8 ? WAVES * 2 * 2 * KEYS : 16];
     __shared__ int scan_of[THREADS], wave_sum[WAVES], found;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
@@ -589,13 +506,12 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     }
     // lane's addresses of the operands in a slot; the 16-key groups lie 16 * RB apart
     // (the swizzles have a period of 16 rows)
-    constexpr int KREADS = RB < 64 ? 1 : RB / 64;       // 16-byte reads of a key row by its four lanes (or one of 8)
+    constexpr int KREADS = RB < 64 ? 1 : RB / 64;       // 16-byte reads of a key row by its four lanes
     uint32_t k_at[KREADS];
 #pragma unroll
     for(int i = 0; i < KREADS; ++i)
     {
-        k_at[i] = RB < 64 ? (uint32_t)(col * RB + ((quad >> 1) ^ Shape::k_swizzle(col)) * 16 + 8 * (quad & 1))
-            : (uint32_t)(col * RB + ((4 * i + quad) ^ Shape::k_swizzle(col)) * 16);
+        k_at[i] = (uint32_t)(col * RB + ((4 * i + quad) ^ Shape::k_swizzle(col)) * 16);
     }
     uint32_t v_at[DBLOCKS];
 #pragma unroll
@@ -614,12 +530,6 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             // next 16-key group's
             const int j = col >> 1, r = 4 * quad + (j & 3) + 16 * (j >> 2);
             v_at[db] = (uint32_t)(K_BYTES + r * RB + (db ^ Shape::v_swizzle(r)) * 16 + 8 * (col & 1));
-        }
-        else if constexpr(KIND == kPaged4)
-        {
-            // ... of row i, sixteen values; rows 4g .. 4g + 3 are the 16-key group g's
-            const int r = 16 * (col >> 2) + 4 * quad + (col & 3);
-            v_at[db] = (uint32_t)(K_BYTES + r * RB + ((db >> 1) ^ Shape::v_swizzle(r)) * 16 + 8 * (db & 1));
         }
         else
         {
@@ -665,15 +575,14 @@ void sdpa_paged_kernel(const PagedAttendParams p)
 
         // ---- the lane's query rows ---------------------------------------------------
         // 16-byte pieces of an operand begin at head values: 16-bit 32i + 8*quad; 8-bit pages, whose
-        // 16-byte reads hold 16 values, 64(i/2) + 16*quad + 8(i%2); 4-bit pages, where a lane has a fourth of
-        // the row, (head/4)*quad + 8i; fp32 16i + 4*quad
+        // 16-byte reads hold 16 values, 64(i/2) + 16*quad + 8(i%2); fp32 16i + 4*quad
         constexpr int E = KIND == kPaged32 ? 4 : 2;
         auto q_piece = [&](int i)
         {
             return (KIND == kPaged16 ? 32 * i + 8 * quad : KIND == kPaged8 ? 64 * (i / 2) + 16 * quad + 8 * (i % 2)
-                    : KIND == kPaged4 ? HEAD / 4 * quad + 8 * i : 16 * i + 4 * quad) * E / 16;
+                    : 16 * i + 4 * quad) * E / 16;
         };
-        u32x4 qf[Q_IN_LDS ? 1 : QREGS * QPARTS];
+        u32x4 qf[Q_IN_LDS ? 1 : QREGS];
         int last[NR];           // the last key the row sees
         int token[NR];
         bool row_ok[NR];
@@ -697,18 +606,11 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                     x = *reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.Q)
                             + paged_query_row(p, seg.n, h, rr) * Shape::QB + piece * 16);
                 }
-                char *const to = q_rows + r * Shape::QB + (piece ^ Shape::q_swizzle(r)) * 16;
-                if constexpr(TWO_Q)
-                {
-                    u32x4 rest;
-                    two_bf16(x, x, rest);
-                    *reinterpret_cast<u32x4 *>(to + Shape::Q_BYTES) = rest;
-                }
-                *reinterpret_cast<u32x4 *>(to) = x;
+                *reinterpret_cast<u32x4 *>(q_rows + r * Shape::QB + (piece ^ Shape::q_swizzle(r)) * 16) = x;
             }
             __syncthreads();
         }
-        else
+        else if constexpr(KIND != kPaged4)
         {
             const char *src = static_cast<const char *>(p.Q)
                 + paged_query_row(p, seg.n, h, row_ok[0] ? rg * 16 + col : 0) * Shape::QB;
@@ -716,22 +618,18 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             for(int i = 0; i < QREGS; ++i)
             {
                 qf[i] = row_ok[0] ? *reinterpret_cast<const u32x4 *>(src + q_piece(i) * 16) : u32x4{0, 0, 0, 0};
-                if constexpr(TWO_Q)
-                {
-                    two_bf16(qf[i], qf[i], qf[QREGS + i]);
-                }
             }
         }
-        auto q_operand = [&](int nr, int i, int part) -> u32x4
+        auto q_operand = [&](int nr, int i) -> u32x4
         {
             if constexpr(Q_IN_LDS)
             {
-                return *reinterpret_cast<const u32x4 *>(q_rows + part * Shape::Q_BYTES
-                        + ((half * NR + nr) * 16 + col) * Shape::QB + (q_piece(i) ^ Shape::q_swizzle(col)) * 16);
+                return *reinterpret_cast<const u32x4 *>(q_rows + ((half * NR + nr) * 16 + col) * Shape::QB
+                        + (q_piece(i) ^ Shape::q_swizzle(col)) * 16);
             }
             else
             {
-                return qf[part * QREGS + i];
+                return qf[i];
             }
         };
         // below it every row sees every key
@@ -751,6 +649,24 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             }
         }
 
+        // The count of the unit's shares that are done, at the place of its first share (every share is the
+        // first of one shared unit at most).  It has kPagedNone between calls; if it holds something else,
+        // the workspace is new, which is seen to where the count is needed.
+        const bool whole = seg.step == 0 && seg.steps == seg.blocks;
+        const uint32_t w0 = aligned || whole ? first_share : split.of(unit_begin);
+        unsigned long long *const count = p.counts + w0 * kPagedCountStride;
+        unsigned long long held = kPagedNone;
+        auto count_so_far = [&]() -> unsigned long long
+        {
+            return tid == 0 && !whole ? __hip_atomic_load(count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : kPagedNone;
+        };
+        if constexpr(KIND == kPaged4)
+        {
+            held = count_so_far();
+            paged4_walk<T, HEAD, NR>(p, seg, h, rg, given, my_first, n_mine, all_see, last, ring, o, m_run, l_run);
+        }
+        else
+        {
         // ---- pages and loads ------------------------------------------------------------
         const int64_t table_row = (int64_t)seg.n * p.c.max_pages;
         // Where a page holds a step, its groups lie behind each other in one page: one look-up, one address.
@@ -805,21 +721,6 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             places(i, page, p.c.page_stride, RB, from);
             const char *const first = PAIRED && half == 1 ? p.c.v_pages : p.c.k_pages;
             char *const to = PAIRED && half == 1 ? slot + K_BYTES : slot;
-            if constexpr(Shape::ROWS_PER_LOAD > 16)
-            {
-                // (a load takes two groups, which may lie in two pages)
-#pragma unroll
-                for(int ld = 0; ld < LOADS; ++ld)
-                {
-                    const int64_t mine = lane < 32 ? from[2 * ld] : from[2 * ld + 1];
-                    load_to_lds16<0, true>(first + mine + k_off[ld], to + ld * 1024);
-                    if constexpr(!PAIRED)
-                    {
-                        load_to_lds16<0, true>(p.c.v_pages + mine + v_off[ld], slot + K_BYTES + ld * 1024);
-                    }
-                }
-                return;
-            }
 #pragma unroll
             for(int ld = 0; ld < LOADS; ++ld)
             {
@@ -838,16 +739,14 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         // The scale bytes of a step go to LDS like the rows, 16 a lane: lane g < GROUPS has those of the keys of
         // group g, lane GROUPS + g those of the values.  (Through the scalar cache they take more scalar
         // registers than there are: 64 sequences of 17 to 16384 rows, 8 heads of 64, 46.9 -> 42.5 us.)
-        // 4-bit pages have SB times as many: SB lanes a group.
-        constexpr int SLANES = CODES ? GROUPS * SB : 1;     // lanes that have the keys'
-        char *const scale_slots = scale_bytes + (CODES ? wave * 4 * KEYS * SB : 0);
-        const char *const scales_of_lane = reinterpret_cast<const char *>(lane < SLANES ? p.c.k_scales : p.c.v_scales);
+        char *const scale_slots = scale_bytes + (KIND == kPaged8 ? wave * 4 * KEYS : 0);
+        const char *const scales_of_lane = reinterpret_cast<const char *>(lane < GROUPS ? p.c.k_scales : p.c.v_scales);
         auto fetch_scales = [&](int i, const int (&page)[GROUPS])
         {
             int64_t from[GROUPS];
-            places(i, page, p.c.scale_stride, SB, from);
-            const int g = lane % SLANES / (SB > 1 ? SB : 1);
-            int64_t mine = from[0] + 16 * SB * g;
+            places(i, page, p.c.scale_stride, 1, from);
+            const int g = lane % GROUPS;
+            int64_t mine = from[0] + 16 * g;
             if(GROUPS > 1 && !one_page)
             {
                 mine = from[0];
@@ -857,39 +756,25 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                     mine = g == j ? from[j] : mine;
                 }
             }
-            if constexpr(SB > 1)
+            if(lane < 2 * GROUPS)
             {
-                mine += 16 * (lane % SB);
-            }
-            if(lane < 2 * SLANES)
-            {
-                load_to_lds16<0, false>(scales_of_lane + mine, scale_slots + (i & 1) * 2 * KEYS * SB);
+                load_to_lds16<0, false>(scales_of_lane + mine, scale_slots + (i & 1) * 2 * KEYS);
             }
         };
 
         int page[GROUPS], page_next[GROUPS];
-        constexpr int STEP_LOADS = (PAIRED ? LOADS : 2 * LOADS) + (CODES ? 1 : 0);
+        constexpr int STEP_LOADS = (PAIRED ? LOADS : 2 * LOADS) + (KIND == kPaged8 ? 1 : 0);
         if(n_mine > 0)
         {
             look_up(0, page);
             fetch(0, page, slots);
-            if constexpr(CODES)
+            if constexpr(KIND == kPaged8)
             {
                 fetch_scales(0, page);
             }
             look_up(min(1, n_mine - 1), page_next);
         }
-        // The count of the unit's shares that are done, at the place of its first share (every share is the
-        // first of one shared unit at most).  It has kPagedNone between calls; if it holds something else,
-        // the workspace is new, which is seen to where the count is needed.
-        const bool whole = seg.step == 0 && seg.steps == seg.blocks;
-        const uint32_t w0 = aligned || whole ? first_share : split.of(unit_begin);
-        unsigned long long *const count = p.counts + w0 * kPagedCountStride;
-        unsigned long long held = kPagedNone;
-        if(tid == 0 && !whole)
-        {
-            held = __hip_atomic_load(count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
+        held = count_so_far();
         const int n_steps = PAIRED ? (key_hi - key_lo + Shape::BLOCK - 1) / Shape::BLOCK : n_mine;
         auto without_page = [&]()       // groups of the step
         {
@@ -919,7 +804,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             if(i + 1 < n_mine)
             {
                 fetch(i + 1, page_next, slots + ((i + 1) & 1) * STAGE);
-                if constexpr(CODES)
+                if constexpr(KIND == kPaged8)
                 {
                     fetch_scales(i + 1, page_next);
                 }
@@ -944,10 +829,10 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                 return;
             }
             const int key0 = my_first + i * Shape::BLOCK;
-            if(PARTLY && KIND != kPaged4 && (key0 + KEYS > seg.len || hidden != 0))
+            if(PARTLY && (key0 + KEYS > seg.len || hidden != 0))
             {
                 // values of rows that are none: zeros, so that what lies there does not
-                // get into the products (their probabilities are exactly 0; 4-bit codes are all numbers)
+                // get into the products (their probabilities are exactly 0)
 #pragma unroll
                 for(int g = 0; g < GROUPS; ++g)
                 {
@@ -963,7 +848,6 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             // scale bytes of four keys of each group: the keys', of those around the lane's key row where they go
             // into its codes, else of the lane's scores; the values', of the lane's probabilities
             uint32_t ks[GROUPS], vs[GROUPS];
-            uint32_t vs4[KIND == kPaged4 ? GROUPS : 1][SB > 0 ? SB : 1];    // (4-bit pages: SB bytes a value row)
             if constexpr(KIND == kPaged8)
             {
                 const char *const bytes = scale_slots + (i & 1) * 2 * KEYS;
@@ -972,22 +856,6 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                 {
                     ks[g] = *reinterpret_cast<const uint32_t *>(bytes + 16 * g + 4 * (KSCALE_IN_CODES ? col >> 2 : quad));
                     vs[g] = *reinterpret_cast<const uint32_t *>(bytes + KEYS + 16 * g + 4 * quad);
-                }
-            }
-
-            else if constexpr(KIND == kPaged4)
-            {
-                const char *const bytes = scale_slots + (i & 1) * 2 * KEYS * SB;
-#pragma unroll
-                for(int g = 0; g < GROUPS; ++g)
-                {
-                    // the byte of the lane's fourth of the lane's key row
-                    ks[g] = *reinterpret_cast<const uint8_t *>(bytes + (16 * g + col) * SB + quad * SB / 4);
-#pragma unroll
-                    for(int w = 0; w < SB; ++w)
-                    {
-                        vs4[g][w] = *reinterpret_cast<const uint32_t *>(bytes + (KEYS + 16 * g + 4 * quad) * SB + 4 * w);
-                    }
                 }
             }
 
@@ -1000,28 +868,11 @@ void sdpa_paged_kernel(const PagedAttendParams p)
 #pragma unroll
                 for(int r = 0; r < KREADS; ++r)
                 {
-                    if constexpr(RB < 64)
-                    {
-                        const u32x2 half = *reinterpret_cast<const u32x2 *>(slot + k_at[r] + g * 16 * RB);
-                        kf[r] = u32x4{half[0], half[1], 0, 0};
-                    }
-                    else
-                    {
-                        kf[r] = *reinterpret_cast<const u32x4 *>(slot + k_at[r] + g * 16 * RB);
-                    }
+                    kf[r] = *reinterpret_cast<const u32x4 *>(slot + k_at[r] + g * 16 * RB);
                 }
-                u32x4 wide[KIND == kPaged8 ? 2 * KREADS : KIND == kPaged4 ? QREGS : 1];
+                u32x4 wide[KIND == kPaged8 ? 2 * KREADS : 1];
                 // (of the lane's key row)
-                const float k_scale = KIND == kPaged4 ? __uint_as_float(ks[g] << 23)
-                    : KSCALE_IN_CODES ? scale_of(ks[g], col & 3) : 1.0f;
-                if constexpr(KIND == kPaged4)
-                {
-#pragma unroll
-                    for(int r = 0; r < QREGS; ++r)
-                    {
-                        wide[r] = widen8_of_4<Bf16>(kf[0][r], k_scale);
-                    }
-                }
+                const float k_scale = KSCALE_IN_CODES ? scale_of(ks[g], col & 3) : 1.0f;
                 if constexpr(KIND == kPaged8)
                 {
 #pragma unroll
@@ -1039,16 +890,8 @@ void sdpa_paged_kernel(const PagedAttendParams p)
 #pragma unroll
                     for(int i = 0; i < QREGS; ++i)
                     {
-                        const u32x4 q = q_operand(nr, i, 0);
-                        if constexpr(KIND == kPaged4)
-                        {
-                            x = mfma32<QK>(wide[i], q, x);
-                            if constexpr(TWO_Q)
-                            {
-                                x = mfma32<QK>(wide[i], q_operand(nr, i, 1), x);
-                            }
-                        }
-                        else if constexpr(KIND == kPaged32)
+                        const u32x4 q = q_operand(nr, i);
+                        if constexpr(KIND == kPaged32)
                         {
 #pragma unroll
                             for(int e = 0; e < 4; ++e)
@@ -1086,25 +929,6 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             uint32_t pw[NR][GROUPS][2];                 // 16-bit pairs
             uint32_t pw_rest[TWO_PARTS ? NR : 1][TWO_PARTS ? GROUPS : 1][2];        // what they leave
             f32x4 pf[NR][GROUPS];                       // fp32
-            // four probabilities as the matrix instruction takes them
-            auto in_two = [&](const f32x4 &x, uint32_t (&first)[2], uint32_t (&more)[2])
-            {
-                if constexpr(TWO_PARTS)
-                {
-                    // the first 8 bits as they are, the next 8 rounded: 2^-16 of a probability is lost at most
-                    const u32x4 bits = __builtin_bit_cast(u32x4, x);
-                    const f32x4 rest = x - __builtin_bit_cast(f32x4, bits & 0xffff0000u);
-                    first[0] = __builtin_amdgcn_perm(bits[1], bits[0], 0x07060302u);
-                    first[1] = __builtin_amdgcn_perm(bits[3], bits[2], 0x07060302u);
-                    more[0] = PV::pack2(rest[0], rest[1]);
-                    more[1] = PV::pack2(rest[2], rest[3]);
-                }
-                else if constexpr(!__is_same(T, float))
-                {
-                    first[0] = PV::pack2(x[0], x[1]);
-                    first[1] = PV::pack2(x[2], x[3]);
-                }
-            };
 #pragma unroll
             for(int nr = 0; nr < NR; ++nr)
             {
@@ -1165,71 +989,30 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                             x[e] *= of_scale[g][e];
                         }
                     }
-                    if constexpr(KIND == kPaged32 || KIND == kPaged4)
+                    if constexpr(KIND == kPaged32)
                     {
                         pf[nr][g] = x;
                     }
+                    else if constexpr(TWO_PARTS)
+                    {
+                        // the first 8 bits as they are, the next 8 rounded: 2^-16 of a probability is lost at most
+                        const u32x4 bits = __builtin_bit_cast(u32x4, x);
+                        const f32x4 rest = x - __builtin_bit_cast(f32x4, bits & 0xffff0000u);
+                        pw[nr][g][0] = __builtin_amdgcn_perm(bits[1], bits[0], 0x07060302u);
+                        pw[nr][g][1] = __builtin_amdgcn_perm(bits[3], bits[2], 0x07060302u);
+                        pw_rest[nr][g][0] = PV::pack2(rest[0], rest[1]);
+                        pw_rest[nr][g][1] = PV::pack2(rest[2], rest[3]);
+                    }
                     else
                     {
-                        in_two(x, pw[nr][g], pw_rest[TWO_PARTS ? nr : 0][TWO_PARTS ? g : 0]);
+                        pw[nr][g][0] = PV::pack2(x[0], x[1]);
+                        pw[nr][g][1] = PV::pack2(x[2], x[3]);
                     }
                 }
                 l_run[nr] += sum;
             }
 
             // ---- output ----------------------------------------------------------------
-            if constexpr(KIND == kPaged4)
-            {
-                // 32 columns at a time, which have their powers of two in common
-#pragma unroll
-                for(int b = 0; b < SB; ++b)
-                {
-#pragma unroll
-                    for(int nr = 0; nr < NR; ++nr)
-                    {
-#pragma unroll
-                        for(int g = 0; g < GROUPS; ++g)
-                        {
-                            f32x4 x;
-#pragma unroll
-                            for(int e = 0; e < 4; ++e)
-                            {
-                                x[e] = pf[nr][g][e] * scale_of(vs4[g][e * SB / 4], (e * SB + b) % 4);
-                                if constexpr(PARTLY)
-                                {
-                                    // (whatever the power of two of a row that is not seen, also none)
-                                    x[e] = 4 * quad + e > ((hidden >> g) & 1 ? -1 : last[nr] - key0 - 16 * g) ? 0.0f : x[e];
-                                }
-                            }
-                            in_two(x, pw[nr][g], pw_rest[TWO_PARTS ? nr : 0][TWO_PARTS ? g : 0]);
-                        }
-                    }
-#pragma unroll
-                    for(int db = 2 * b; db < 2 * b + 2; ++db)
-                    {
-                        typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-                        const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-                                    (lds_i32x2 *)(slot + v_at[db])));
-#pragma unroll
-                        for(int t = 0; t < GROUPS / 2; ++t)
-                        {
-                            const u32x4 w = widen8_of_4<PV>(v[t], 1.0f);
-#pragma unroll
-                            for(int nr = 0; nr < NR; ++nr)
-                            {
-                                o[nr][db] = mfma32<PV>(w, u32x4{pw[nr][2 * t][0], pw[nr][2 * t][1],
-                                        pw[nr][2 * t + 1][0], pw[nr][2 * t + 1][1]}, o[nr][db]);
-                                if constexpr(TWO_PARTS)
-                                {
-                                    o[nr][db] = mfma32<PV>(w, u32x4{pw_rest[nr][2 * t][0], pw_rest[nr][2 * t][1],
-                                            pw_rest[nr][2 * t + 1][0], pw_rest[nr][2 * t + 1][1]}, o[nr][db]);
-                                }
-                            }
-                        }
-                    }
-                }
-                return;
-            }
             auto value_words = [&](int db, int t, u32x4 &w)
             {
                 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -1398,8 +1181,11 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         {
             take_step(i, std::true_type());
         }
+        }
 
         // ---- the wavefronts' results, then the unit's or the share's ---------------------
+        const int my_tid = KIND == kPaged4 ? fresh(tid) : tid, my_wave = KIND == kPaged4 ? uniform(my_tid >> 6) : wave;
+        const int my_col = KIND == kPaged4 ? my_tid & 15 : col, my_quad = KIND == kPaged4 ? (my_tid & 63) >> 4 : quad;
         const bool begins = seg.step == 0;
         const int rows_here = min(p.rows - rg * QROWS, QROWS);
         float *const merge_o = reinterpret_cast<float *>(ring);
@@ -1408,7 +1194,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         for(int nr = 0; nr < NR; ++nr)
         {
             __syncthreads();        // every wavefront is done with the ring, or with the last row block
-            const int mine = wave * 16 + col;
+            const int mine = my_wave * 16 + my_col;
             float m = m_run[nr] * c_log2 - kLift, l = quad_sum(l_run[nr]);
             if(!row_ok[nr])
             {
@@ -1418,10 +1204,10 @@ void sdpa_paged_kernel(const PagedAttendParams p)
 #pragma unroll
             for(int db = 0; db < DBLOCKS; ++db)
             {
-                *reinterpret_cast<f32x4 *>(merge_o + mine * MERGE_LD + 16 * db + 4 * quad)
+                *reinterpret_cast<f32x4 *>(merge_o + mine * MERGE_LD + 16 * db + 4 * my_quad)
                     = row_ok[nr] ? o[nr][db] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
-            if(quad == 0)
+            if(my_quad == 0)
             {
                 merge_ml[2 * mine] = m;
                 merge_ml[2 * mine + 1] = l;
@@ -1429,7 +1215,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             __syncthreads();
             // 16 threads a row; the row of stream w lies at (w + STREAMS * half) * 16 + row
             constexpr int PAIRS = HEAD / 32;
-            const int row = (tid / 16) % 16, its_half = tid / 256, t = tid % 16;
+            const int row = (my_tid / 16) % 16, its_half = my_tid / 256, t = my_tid % 16;
             const int in_group = (its_half * NR + nr) * 16 + row, rr = rg * QROWS + in_group;
             if(rr < p.rows)
             {
@@ -1505,7 +1291,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                     __hip_atomic_store(count, kPagedNone, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
                 paged_join<T, HEAD, THREADS, QROWS>(p, seg.n, h, rg, rows_here, (int)w0, (int)parts,
-                        reinterpret_cast<float *>(ring));
+                        reinterpret_cast<float *>(ring), my_tid);
             }
         }
         }
@@ -1534,29 +1320,29 @@ void sdpa_paged_kernel(const PagedAttendParams p)
 // Blocks of 16 rows that a workgroup takes: 1, 2, or 4 by two wavefronts a key; 1 also where that leaves no
 // more than 64 units, which then have more shares, and joins, between them (8 units of 4096 rows, 64 query
 // rows, 26.7 us with 4 blocks a workgroup, 21.4 with 1; 64 units of 2048 29.2 and 51.9).
-static int row_blocks(bool fp32, int64_t entries, int64_t rows)
+static int row_blocks(bool two_at_most, int64_t entries, int64_t rows)
 {
-    return rows <= 16 || entries * ((rows + 15) / 16) <= 64 ? 1 : rows <= 32 || fp32 ? 2 : 4;
+    return rows <= 16 || entries * ((rows + 15) / 16) <= 64 ? 1 : rows <= 32 || two_at_most ? 2 : 4;
 }
 
 // The workspace: the counts, then the shares' results (the larger size of the types', which differ in
 // the rows of a workgroup).
 static size_t share_rows(int64_t rows)
 {
-    return (size_t)kPagedShares * 2 * 16 * (size_t)row_blocks(false, 64, rows);
+    return (size_t)(rows <= 16 ? kPagedMoreShares : kPagedShares) * 2 * 16 * (size_t)row_blocks(false, 64, rows);
 }
 
 static void place_workspace(PagedAttendParams &p, int head, void *workspace)
 {
     p.counts = static_cast<unsigned long long *>(workspace);
-    p.part_o = reinterpret_cast<float *>(p.counts + kPagedShares * kPagedCountStride);
+    p.part_o = reinterpret_cast<float *>(p.counts + kPagedMoreShares * kPagedCountStride);
     p.part_ml = p.part_o + share_rows(p.rows) * (size_t)head;
 }
 
 template<typename T, int KIND, int HEAD, int NR, int HALVES>
 static int launch_form(hipStream_t stream, PagedAttendParams &p)
 {
-    typedef PagedShape<KIND, HEAD, NR, HALVES> Shape;
+    typedef PagedShape<T, KIND, HEAD, NR, HALVES> Shape;
     p.row_groups = (p.rows + Shape::QROWS - 1) / Shape::QROWS;
     p.units = p.c.n_head_kv * p.row_groups;
     // at most as many shares as there can be blocks
@@ -1575,7 +1361,7 @@ static int launch_form(hipStream_t stream, PagedAttendParams &p)
 template<typename T, int KIND>
 static int launch_kind(hipStream_t stream, PagedAttendParams &p, int head)
 {
-    switch(row_blocks(KIND == kPaged32, (int64_t)p.c.n_batch * p.c.n_head_kv, p.rows) * 256 + head)
+    switch(row_blocks(KIND == kPaged32 || KIND == kPaged4, (int64_t)p.c.n_batch * p.c.n_head_kv, p.rows) * 256 + head)
     {
         case 256 + 64: return launch_form<T, KIND, 64, 1, 1>(stream, p);
         case 256 + 128: return launch_form<T, KIND, 128, 1, 1>(stream, p);
@@ -1583,7 +1369,7 @@ static int launch_kind(hipStream_t stream, PagedAttendParams &p, int head)
         case 512 + 128: return launch_form<T, KIND, 128, 2, 1>(stream, p);
         default: break;
     }
-    if constexpr(KIND != kPaged32)
+    if constexpr(KIND != kPaged32 && KIND != kPaged4)
     {
         return head == 64 ? launch_form<T, KIND, 64, 2, 2>(stream, p) : launch_form<T, KIND, 128, 2, 2>(stream, p);
     }
