@@ -211,8 +211,8 @@ int weights_call(int dtype, bool four, void *stream, const nntile_hip_paged_weig
     {
         return NNTILE_HIP_EINVAL;
     }
-    PagedWeightsParams p = {};
-    const int rc = paged_view(&a->cache, dtype, p.c, four, false);
+    PagedView view;
+    const int rc = paged_view(&a->cache, dtype, view, four, false);
     if(rc != NNTILE_HIP_OK)
     {
         return rc;
@@ -220,7 +220,7 @@ int weights_call(int dtype, bool four, void *stream, const nntile_hip_paged_weig
     const int64_t rows = query_rows(a->cache, a->q_seq, a->kv_group);
     if(rows < 0 || a->Q == nullptr || a->lse == nullptr || a->weights == nullptr || !on16(a->Q)
             || (reinterpret_cast<uintptr_t>(a->lse) & 3u) != 0 || (reinterpret_cast<uintptr_t>(a->weights) & 3u) != 0
-            || a->columns < p.c.max_rows || a->columns > kMost || !(a->decay >= 0.0f && a->decay <= 1.0f))
+            || a->columns < view.max_rows || a->columns > kMost || !(a->decay >= 0.0f && a->decay <= 1.0f))
     {
         return NNTILE_HIP_EINVAL;
     }
@@ -228,16 +228,9 @@ int weights_call(int dtype, bool four, void *stream, const nntile_hip_paged_weig
     {
         return mask_check(a->mask_mode);
     }
-    p.Q = a->Q;
-    p.lse = a->lse;
-    p.weights = a->weights;
-    p.columns = a->columns;
-    p.q_seq = (int32_t)a->q_seq;
-    p.kv_group = (int32_t)a->kv_group;
-    p.rows = (int32_t)rows;
-    p.causal = a->mask_mode == NNTILE_HIP_MASK_CAUSAL;
-    p.decay = a->decay;
-    p.scale = 1.0f / sqrtf((float)a->cache.head);
+    PagedWeightsParams p = {view, a->Q, a->lse, a->weights, a->columns, (int32_t)a->q_seq, (int32_t)a->kv_group,
+        (int32_t)rows, a->mask_mode == NNTILE_HIP_MASK_CAUSAL, a->decay, 1.0f / sqrtf((float)a->cache.head), 0,
+        FixedDivide((uint32_t)a->q_seq)};
     return launch_paged_weights(static_cast<hipStream_t>(stream), dtype, page_bits(a->cache, dtype, four), p,
             (int)a->cache.head);
 }

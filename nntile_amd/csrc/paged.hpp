@@ -1,6 +1,7 @@
 // What the kernels on a paged key/value cache share.
 #pragma once
 
+#include "fixed_divide.hpp"
 #include "sdpa_common.hpp"
 
 namespace nntile_hip
@@ -59,6 +60,7 @@ struct PagedWeightsParams
     float decay;
     float scale;                        // 1/sqrt(head)
     int32_t shares;                     // workgroups
+    FixedDivide by_seq;                 // by q_seq
 };
 
 struct PagedEvictParams

@@ -10,9 +10,11 @@
 //    every workgroup takes an equal run of them, whatever the lengths (which live on the device).
 //  * S = Q K^T with matrix instructions of 16 x 16: a lane has one key and four queries, so that a key's sum stays in
 //    the lane but for the last two steps, across the four lanes that share it.
-//  * A wavefront's keys stay in registers while the queries, 64 rows at a time, come from LDS.
+//  * A wavefront's keys stay in registers while the queries, up to 128 rows at a time, come from LDS; the next
+//    block's keys, and the pages of the one behind it, are on their way meanwhile.
 #include <type_traits>
 
+#include "fixed_divide.hpp"
 #include "paged_operands.hpp"
 
 namespace nntile_hip
@@ -20,27 +22,29 @@ namespace nntile_hip
 
 constexpr int kWeightsCUs = 256;
 
-// Where a workgroup stands: block `block` of `blocks` of head h of sequence n
+// Where a workgroup stands: block `block` of `blocks` of head h of sequence n, which has `given` new tokens
 struct WeightsPlace
 {
-    int n, h, len, block, blocks;
+    int n, h, len, given, block, blocks;
 };
 
 // GK: groups of 16 keys of a wavefront.
 template<typename T, int KIND, int HEAD, int GK>
-__global__ __launch_bounds__(256)
+__global__ __launch_bounds__(256, (GK == 1 ? 4 : 2))
 void paged_weights_kernel(const PagedWeightsParams p)
 {
     constexpr int RB = KIND == kPaged32 ? HEAD * 4 : KIND == kPaged8 ? HEAD : KIND == kPaged4 ? HEAD / 2 : HEAD * 2;
     constexpr int KEYS = 16 * GK, BLOCK = 4 * KEYS;     // keys of a wavefront's step, of a workgroup's
-    constexpr int ROWS = 64;                            // query rows that lie in LDS
-    // registers of 16 bytes of a row's operand, for keys and queries
-    constexpr int QREGS = KIND == kPaged32 ? HEAD / 16 : HEAD / 32;
+    constexpr int ROWS = GK == 1 ? 32 : 128;            // query rows that lie in LDS
+    constexpr int BLOCKS = GK == 1 ? 1 : 2;             // blocks of 16 of them side by side: one's sums wait for each other
+    // registers of 16 bytes: of a row's operand, for keys and queries, and of a key row as it lies in its page
+    constexpr int QREGS = KIND == kPaged32 ? HEAD / 16 : HEAD / 32, RAW = RB < 64 ? 1 : RB / 64;
     // keys of 4 bits become bf16 numbers, and an fp16 query the sum of two
     constexpr bool TWO_Q = KIND == kPaged4 && __is_same(T, Fp16);
     constexpr int QPARTS = TWO_Q ? 2 : 1;
     typedef typename std::conditional<KIND == kPaged4, Bf16, T>::type QK;
     constexpr int QB = HEAD * (KIND == kPaged32 ? 4 : 2), PIECES = QB / 16;
+    constexpr bool CODES = KIND == kPaged4 || KIND == kPaged8;
     __shared__ __attribute__((aligned(16))) char q_rows[QPARTS * ROWS * QB];
     __shared__ __attribute__((aligned(16))) float off_of[ROWS];     // -lse in log2 units; -inf: the row counts nothing
     __shared__ __attribute__((aligned(16))) int last_of[ROWS];      // the last key the row sees
@@ -51,111 +55,267 @@ void paged_weights_kernel(const PagedWeightsParams p)
     // the 16-byte piece of a query row that goes with a lane's operand i
     auto q_piece = [&](int i)
     {
-        return KIND == kPaged16 ? 4 * i + quad : KIND == kPaged8 ? 8 * (i / 2) + 2 * quad + i % 2
-            : KIND == kPaged4 ? HEAD / 32 * quad + i : 4 * i + quad;
+        return KIND == kPaged8 ? 8 * (i / 2) + 2 * quad + i % 2 : KIND == kPaged4 ? HEAD / 32 * quad + i : 4 * i + quad;
     };
 
     // ---- the workgroup's run of blocks ----------------------------------------------
     auto blocks_of = [&](int len) { return (len + BLOCK - 1) / BLOCK; };
-    int mine = 0;
-    for(int n = lane; n < p.c.n_batch; n += 64)
+    auto len_of = [&](int n) { return n < p.c.n_batch ? paged_len(p.c, n) : 0; };
+    auto scan = [&](int len)        // blocks of the lanes up to this one
     {
-        mine += blocks_of(paged_len(p.c, n));
-    }
+        uint32_t upto = (uint32_t)blocks_of(len);
 #pragma unroll
-    for(int o = 32; o >= 1; o >>= 1)
+        for(int o = 1; o < 64; o <<= 1)
+        {
+            const uint32_t other = __shfl_up(upto, o);
+            upto += lane >= o ? other : 0;
+        }
+        return upto;
+    };
+    auto last_lane = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); };
+    int len_of_lane = len_of(lane);
+    uint32_t upto = scan(len_of_lane), all = last_lane(upto);
+    if(p.c.n_batch > 64)
     {
-        mine += __shfl_xor(mine, o);
+        int more = 0;
+        for(int n = lane + 64; n < p.c.n_batch; n += 64)
+        {
+            more += blocks_of(paged_len(p.c, n));
+        }
+#pragma unroll
+        for(int o = 32; o >= 1; o >>= 1)
+        {
+            more += __shfl_xor(more, o);
+        }
+        all += (uint32_t)uniform(more);
     }
-    const uint32_t all = (uint32_t)uniform(mine) * (uint32_t)p.c.n_head_kv;
+    all *= (uint32_t)p.c.n_head_kv;
     const uint32_t shares = min((uint32_t)p.shares, all);
     if(blockIdx.x >= shares)
     {
         return;
     }
     const PagedSplit split(all, shares);
-    const uint32_t at = split.begin(blockIdx.x);
+    uint32_t at = split.begin(blockIdx.x);
     int left = (int)(split.begin(blockIdx.x + 1) - at);
     WeightsPlace place = {};
+    // 64 sequences at a time
+    for(int n0 = 0;;)
     {
-        uint32_t before = 0;
-        for(;; ++place.n)
+        const uint32_t here = last_lane(upto) * (uint32_t)p.c.n_head_kv;
+        if(at < here)           // (there is one)
         {
-            place.len = uniform(paged_len(p.c, place.n));
+            // the first sequence that ends behind the block
+            const int t = __popcll(__ballot(upto * (uint32_t)p.c.n_head_kv <= at));
+            place.n = n0 + t;
+            place.len = __builtin_amdgcn_readlane(len_of_lane, t);
             place.blocks = blocks_of(place.len);
-            const uint32_t here = (uint32_t)place.blocks * (uint32_t)p.c.n_head_kv;
-            if(at < before + here)
-            {
-                break;      // (at < all: there is one)
-            }
-            before += here;
+            at -= ((uint32_t)__builtin_amdgcn_readlane((int)upto, t) - (uint32_t)place.blocks) * (uint32_t)p.c.n_head_kv;
+            break;
         }
-        place.h = uniform((int)((at - before) / (uint32_t)place.blocks));
-        place.block = uniform((int)((at - before) % (uint32_t)place.blocks));
+        at -= here;
+        n0 += 64;
+        len_of_lane = len_of(n0 + lane);
+        upto = scan(len_of_lane);
     }
+    place.given = uniform(paged_new(p.c, place.n, p.q_seq));
+    place.h = uniform((int)(at / (uint32_t)place.blocks));
+    place.block = uniform((int)(at % (uint32_t)place.blocks));
     const float c_log2 = p.scale * kLog2e;
 
-    bool staged = false;        // the pair's queries lie in LDS, all of them
-    bool dead = false;          // a query of those in LDS counts nothing, whatever its scores are
-    for(;;)
+    auto next_of = [&](WeightsPlace x)
     {
-        const int given = uniform(paged_new(p.c, place.n, p.q_seq));
-        const int key0 = place.block * BLOCK + wave * KEYS;
-        const bool here = key0 < place.len;
+        if(++x.block == x.blocks)
+        {
+            x.block = 0;
+            if(++x.h == p.c.n_head_kv)
+            {
+                x.h = 0;
+                do
+                {
+                    ++x.n;
+                    x.len = uniform(paged_len(p.c, x.n));
+                    x.blocks = blocks_of(x.len);
+                } while(x.blocks == 0);     // (there is a block left)
+                x.given = uniform(paged_new(p.c, x.n, p.q_seq));
+            }
+        }
+        return x;
+    };
 
-        // ---- keys ----------------------------------------------------------------------
-        u32x4 kf[GK][QREGS];
-        float s_scale[GK];
-        uint32_t hidden = 0;        // groups without a page
+    // ---- keys: the pages of the block after the next, the next one's rows, and this one's operands ------------
+    // (groups behind the last row: the last one's rows, not written)
+    auto group_row = [&](const WeightsPlace &x, int g)
+    {
+        return max(min(x.block * BLOCK + wave * KEYS + 16 * g, x.len - 1), 0) & ~15;
+    };
+    auto look_up = [&](const WeightsPlace &x, int (&page)[GK])
+    {
 #pragma unroll
         for(int g = 0; g < GK; ++g)
         {
-            s_scale[g] = 1.0f;
-            // (groups behind the last row: the last one's rows, not written)
-            const int row = max(min(key0 + 16 * g, place.len - 1), 0) & ~15;
-            const int page_in = scalar_load<int>(p.c.table, 4 * ((int64_t)place.n * p.c.max_pages + (row >> p.c.page_shift)));
-            const bool real = (unsigned)page_in < (unsigned)p.c.n_pages;
+            page[g] = scalar_load<int>(p.c.table, 4 * ((int64_t)x.n * p.c.max_pages + (group_row(x, g) >> p.c.page_shift)));
+        }
+    };
+    auto weights_at = [&](const WeightsPlace &x)
+    {
+        return p.weights + (x.n + (int64_t)p.c.n_batch * x.h) * p.columns + x.block * BLOCK + wave * KEYS + col;
+    };
+    auto load = [&](const WeightsPlace &x, const int (&page)[GK], u32x4 (&raw)[GK][RAW], uint32_t (&byte)[GK], float (&old)[GK],
+            uint32_t &hidden)
+    {
+        hidden = 0;
+#pragma unroll
+        for(int g = 0; g < GK; ++g)
+        {
+            const bool real = (unsigned)page[g] < (unsigned)p.c.n_pages;
             hidden |= real ? 0u : 1u << g;
-            const int64_t page = real ? page_in : 0;
-            const int64_t in_page = ((int64_t)place.h << p.c.page_shift) + (row & ((1 << p.c.page_shift) - 1)) + col;
-            const char *const from = p.c.k_pages + page * p.c.page_stride + in_page * RB;
-            if constexpr(KIND == kPaged4)
+            const int64_t pg = real ? page[g] : 0;
+            const int64_t in_page = ((int64_t)x.h << p.c.page_shift) + (group_row(x, g) & ((1 << p.c.page_shift) - 1)) + col;
+            const char *const from = p.c.k_pages + pg * p.c.page_stride + in_page * RB;
+            if constexpr(RB < 64)
             {
-                constexpr int W = HEAD / 32;        // words of a lane
-                const float scale = __uint_as_float((uint32_t)p.c.k_scales[page * p.c.scale_stride + in_page * W
-                        + quad * W / 4] << 23);
-#pragma unroll
-                for(int i = 0; i < W; ++i)
-                {
-                    kf[g][i] = widen8_of_4<Bf16>(*reinterpret_cast<const uint32_t *>(from + 4 * (W * quad + i)), scale);
-                }
-            }
-            else if constexpr(KIND == kPaged8)
-            {
-                const float scale = __uint_as_float((uint32_t)p.c.k_scales[page * p.c.scale_stride + in_page] << 23);
-                s_scale[g] = __is_same(T, Bf16) ? 1.0f : scale;
-#pragma unroll
-                for(int i = 0; i < QREGS / 2; ++i)
-                {
-                    const u32x4 x = *reinterpret_cast<const u32x4 *>(from + 16 * (4 * i + quad));
-#pragma unroll
-                    for(int j = 0; j < 2; ++j)
-                    {
-                        const u32x2 a = widen4<T>(x[2 * j], __is_same(T, Bf16) ? scale : 1.0f),
-                            b = widen4<T>(x[2 * j + 1], __is_same(T, Bf16) ? scale : 1.0f);
-                        kf[g][2 * i + j] = u32x4{a[0], a[1], b[0], b[1]};
-                    }
-                }
+                const u32x2 two = *reinterpret_cast<const u32x2 *>(from + 8 * quad);
+                raw[g][0] = u32x4{two[0], two[1], 0, 0};
             }
             else
             {
 #pragma unroll
-                for(int i = 0; i < QREGS; ++i)
+                for(int i = 0; i < RAW; ++i)
                 {
-                    kf[g][i] = *reinterpret_cast<const u32x4 *>(from + 16 * (4 * i + quad));
+                    raw[g][i] = *reinterpret_cast<const u32x4 *>(from + 16 * (4 * i + quad));
+                }
+            }
+            if constexpr(CODES)
+            {
+                constexpr int SB = KIND == kPaged4 ? HEAD / 32 : 1;
+                byte[g] = p.c.k_scales[pg * p.c.scale_stride + in_page * SB + quad * SB / 4];
+            }
+            if(p.decay != 0.0f && quad == 0 && x.block * BLOCK + wave * KEYS + 16 * g + col < x.len)
+            {
+                old[g] = weights_at(x)[16 * g];
+            }
+        }
+    };
+    int page[GK];
+    u32x4 raw[GK][RAW];
+    uint32_t byte[GK] = {}, hidden = 0;
+    float old[GK] = {};
+    look_up(place, page);
+    load(place, page, raw, byte, old, hidden);
+    WeightsPlace next = left > 1 ? next_of(place) : place;
+    look_up(next, page);
+
+    // Query rows from row0 on into LDS.  True: one of them counts nothing, whatever its scores are.
+    auto stage = [&](const WeightsPlace &x, int row0) -> bool
+    {
+        const int rows = min(p.rows - row0, ROWS), pieces = (rows + 16 * BLOCKS - 1) / (16 * BLOCKS) * (16 * BLOCKS) * PIECES;
+        // row r's place in lse (times head: in Q); of a row that is none: the pair's first
+        auto place_of = [&](int r, int &tok, bool &ok)
+        {
+            const int rr = min(row0 + r, p.rows - 1), g = (int)p.by_seq.quotient((uint32_t)rr);
+            tok = rr - g * p.q_seq;
+            ok = r < rows && tok < x.given;
+            return (x.n + (int64_t)p.c.n_batch * ((ok ? g : 0) + (int64_t)p.kv_group * x.h)) * p.q_seq + (ok ? tok : 0);
+        };
+        int my_tok;
+        bool my_ok;
+        const int64_t my_row = place_of(min(tid, ROWS - 1), my_tok, my_ok);
+        const float lse = my_ok ? p.lse[my_row] : neg_inf();
+        __syncthreads();        // the rows before these are done with
+        // (several loads on their way at a time)
+        constexpr int AT_ONCE = 4;
+        for(int t0 = 0; t0 < pieces; t0 += 256 * AT_ONCE)
+        {
+            u32x4 v[AT_ONCE];
+            bool ok[AT_ONCE];
+#pragma unroll
+            for(int k = 0; k < AT_ONCE; ++k)
+            {
+                const int t = min(t0 + 256 * k + tid, pieces - 1);
+                int tok;
+                const int64_t row = place_of(t / PIECES, tok, ok[k]);
+                v[k] = *reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.Q) + row * QB + t % PIECES * 16);
+            }
+#pragma unroll
+            for(int k = 0; k < AT_ONCE; ++k)
+            {
+                const int t = t0 + 256 * k + tid, r = t / PIECES;
+                u32x4 first = ok[k] ? v[k] : u32x4{0, 0, 0, 0};
+                if(t < pieces)
+                {
+                    char *const to = q_rows + r * QB + swizzled(r, t % PIECES) * 16;
+                    if constexpr(TWO_Q)
+                    {
+                        u32x4 rest;
+                        two_bf16(first, first, rest);
+                        *reinterpret_cast<u32x4 *>(to + ROWS * QB) = rest;
+                    }
+                    *reinterpret_cast<u32x4 *>(to) = first;
                 }
             }
         }
+        if(tid < ROWS)
+        {
+            off_of[tid] = lse == neg_inf() ? neg_inf() : -lse * kLog2e;
+            last_of[tid] = lse == neg_inf() ? -1 : p.causal ? x.len - x.given + my_tok : x.len - 1;
+        }
+        return __syncthreads_or(my_ok && lse == neg_inf());
+    };
+    bool staged = false;        // the pair's queries lie in LDS, all of them
+    bool dead = false;
+    for(;;)
+    {
+        // (the queries in front of the wait for the keys)
+        if(!staged && p.rows <= ROWS && place.given > 0)
+        {
+            dead = stage(place, 0);
+            staged = true;
+        }
+        // this block's operands
+        u32x4 kf[GK][QREGS];
+        float s_scale[GK], kept[GK];
+        const uint32_t without = hidden;
+#pragma unroll
+        for(int g = 0; g < GK; ++g)
+        {
+            const float scale = CODES ? __uint_as_float(byte[g] << 23) : 1.0f;
+            s_scale[g] = KIND == kPaged8 && !__is_same(T, Bf16) ? scale : 1.0f;
+            kept[g] = old[g];
+#pragma unroll
+            for(int i = 0; i < QREGS; ++i)
+            {
+                if constexpr(KIND == kPaged4)
+                {
+                    kf[g][i] = widen8_of_4<Bf16>(raw[g][0][i], scale);
+                }
+                else if constexpr(KIND == kPaged8)
+                {
+                    const float of_codes = __is_same(T, Bf16) ? scale : 1.0f;
+                    const u32x2 a = widen4<T>(raw[g][i / 2][2 * (i % 2)], of_codes),
+                        b = widen4<T>(raw[g][i / 2][2 * (i % 2) + 1], of_codes);
+                    kf[g][i] = u32x4{a[0], a[1], b[0], b[1]};
+                }
+                else
+                {
+                    kf[g][i] = raw[g][i];
+                }
+            }
+        }
+        // the next block's rows are on their way meanwhile
+        const WeightsPlace now = place;
+        if(left > 1)
+        {
+            load(next, page, raw, byte, old, hidden);
+            place = next;
+            if(left > 2)
+            {
+                next = next_of(next);
+                look_up(next, page);
+            }
+        }
+        const int key0 = now.block * BLOCK + wave * KEYS;
+        const bool here = key0 < now.len;
 
         // ---- sums over the queries -------------------------------------------------------
         float sum[GK];
@@ -165,115 +325,98 @@ void paged_weights_kernel(const PagedWeightsParams p)
             sum[g] = 0.0f;
         }
         // below it every row sees every key
-        const int all_see = p.causal ? place.len - given : place.len - 1;
-        const bool partly = key0 + KEYS - 1 > all_see || hidden != 0;
-        for(int row0 = 0; row0 < (given > 0 ? p.rows : 0); row0 += ROWS)
+        const int all_see = p.causal ? now.len - now.given : now.len - 1;
+        const bool partly = key0 + KEYS - 1 > all_see || without != 0;
+        for(int row0 = 0; row0 < (now.given > 0 ? p.rows : 0); row0 += ROWS)
         {
             const int rows = min(p.rows - row0, ROWS);
             if(!staged)
             {
-                __syncthreads();        // the rows before these are done with
-                bool counts_not = false;
-                for(int t = tid; t < ROWS * PIECES; t += 256)
-                {
-                    const int r = t / PIECES, piece = t % PIECES, rr = row0 + r;
-                    const int g = rr / p.q_seq, tok = rr % p.q_seq;
-                    const bool ok = r < rows && tok < given;
-                    const int64_t row = (place.n + (int64_t)p.c.n_batch * (g + (int64_t)p.kv_group * place.h)) * p.q_seq + tok;
-                    u32x4 x = {0, 0, 0, 0};
-                    if(ok)
-                    {
-                        x = *reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.Q) + row * QB + piece * 16);
-                    }
-                    char *const to = q_rows + r * QB + swizzled(r, piece) * 16;
-                    if constexpr(TWO_Q)
-                    {
-                        u32x4 rest;
-                        two_bf16(x, x, rest);
-                        *reinterpret_cast<u32x4 *>(to + ROWS * QB) = rest;
-                    }
-                    *reinterpret_cast<u32x4 *>(to) = x;
-                    if(piece == 0)
-                    {
-                        const float lse = ok ? p.lse[row] : neg_inf();
-                        counts_not = counts_not || (ok && lse == neg_inf());
-                        off_of[r] = lse == neg_inf() ? neg_inf() : -lse * kLog2e;
-                        last_of[r] = lse == neg_inf() ? -1 : p.causal ? place.len - given + tok : place.len - 1;
-                    }
-                }
-                dead = __syncthreads_or(counts_not);
+                dead = stage(now, row0);
                 staged = p.rows <= ROWS;
             }
             if(!here)
             {
                 continue;
             }
-            for(int rb = 0; rb < rows; rb += 16)
+            for(int rb = 0; rb < rows; rb += 16 * BLOCKS)
             {
-                const f32x4 off = *reinterpret_cast<const f32x4 *>(off_of + rb + 4 * quad);
-                f32x4 s[GK];
+                f32x4 s[BLOCKS][GK];
 #pragma unroll
-                for(int g = 0; g < GK; ++g)
+                for(int k = 0; k < BLOCKS; ++k)
                 {
-                    s[g] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for(int g = 0; g < GK; ++g)
+                    {
+                        s[k][g] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    }
                 }
 #pragma unroll
                 for(int i = 0; i < QREGS; ++i)
                 {
-                    const char *const q_at = q_rows + (rb + col) * QB + swizzled(col, q_piece(i)) * 16;
-                    const u32x4 q = *reinterpret_cast<const u32x4 *>(q_at);
 #pragma unroll
-                    for(int g = 0; g < GK; ++g)
+                    for(int part = 0; part < QPARTS; ++part)
                     {
-                        if constexpr(KIND == kPaged32)
-                        {
 #pragma unroll
-                            for(int e = 0; e < 4; ++e)
+                        for(int k = 0; k < BLOCKS; ++k)
+                        {
+                            const u32x4 q = *reinterpret_cast<const u32x4 *>(q_rows + (part * ROWS + rb + 16 * k + col) * QB
+                                    + swizzled(col, q_piece(i)) * 16);
+#pragma unroll
+                            for(int g = 0; g < GK; ++g)
                             {
-                                s[g] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(q[e]),
-                                        __uint_as_float(kf[g][i][e]), s[g], 0, 0, 0);
-                            }
-                        }
-                        else
-                        {
-                            s[g] = mfma32<QK>(q, kf[g][i], s[g]);
-                        }
-                    }
-                    if constexpr(TWO_Q)
-                    {
-                        const u32x4 rest = *reinterpret_cast<const u32x4 *>(q_at + ROWS * QB);
+                                if constexpr(KIND == kPaged32)
+                                {
 #pragma unroll
-                        for(int g = 0; g < GK; ++g)
-                        {
-                            s[g] = mfma32<QK>(rest, kf[g][i], s[g]);
+                                    for(int e = 0; e < 4; ++e)
+                                    {
+                                        s[k][g] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(q[e]),
+                                                __uint_as_float(kf[g][i][e]), s[k][g], 0, 0, 0);
+                                    }
+                                }
+                                else
+                                {
+                                    s[k][g] = mfma32<QK>(q, kf[g][i], s[k][g]);
+                                }
+                            }
                         }
                     }
                 }
                 if(partly || dead)
                 {
-                    typedef __attribute__((ext_vector_type(4))) int i32x4;
-                    const i32x4 last = *reinterpret_cast<const i32x4 *>(last_of + rb + 4 * quad);
 #pragma unroll
-                    for(int g = 0; g < GK; ++g)
+                    for(int k = 0; k < BLOCKS; ++k)
                     {
+                        typedef __attribute__((ext_vector_type(4))) int i32x4;
+                        const f32x4 off = *reinterpret_cast<const f32x4 *>(off_of + rb + 16 * k + 4 * quad);
+                        const i32x4 last = *reinterpret_cast<const i32x4 *>(last_of + rb + 16 * k + 4 * quad);
 #pragma unroll
-                        for(int e = 0; e < 4; ++e)
+                        for(int g = 0; g < GK; ++g)
                         {
-                            const float x = fast_exp2(fmaf(s[g][e] * s_scale[g], c_log2, off[e]));
-                            sum[g] += key0 + 16 * g + col <= ((hidden >> g) & 1 ? -1 : last[e]) ? x : 0.0f;
+#pragma unroll
+                            for(int e = 0; e < 4; ++e)
+                            {
+                                const float x = fast_exp2(fmaf(s[k][g][e] * s_scale[g], c_log2, off[e]));
+                                sum[g] += key0 + 16 * g + col <= ((without >> g) & 1 ? -1 : last[e]) ? x : 0.0f;
+                            }
                         }
                     }
                 }
                 else
                 {
 #pragma unroll
-                    for(int g = 0; g < GK; ++g)
+                    for(int k = 0; k < BLOCKS; ++k)
                     {
-                        const float c = KIND == kPaged8 ? c_log2 * s_scale[g] : c_log2;
+                        const f32x4 off = *reinterpret_cast<const f32x4 *>(off_of + rb + 16 * k + 4 * quad);
 #pragma unroll
-                        for(int e = 0; e < 4; ++e)
+                        for(int g = 0; g < GK; ++g)
                         {
-                            sum[g] += fast_exp2(fmaf(s[g][e], c, off[e]));
+                            const float c = KIND == kPaged8 ? c_log2 * s_scale[g] : c_log2;
+#pragma unroll
+                            for(int e = 0; e < 4; ++e)
+                            {
+                                sum[g] += fast_exp2(fmaf(s[k][g][e], c, off[e]));
+                            }
                         }
                     }
                 }
@@ -281,15 +424,14 @@ void paged_weights_kernel(const PagedWeightsParams p)
         }
         if(here)
         {
-            float *const to = p.weights + (place.n + (int64_t)p.c.n_batch * place.h) * p.columns + key0;
+            float *const to = weights_at(now);
 #pragma unroll
             for(int g = 0; g < GK; ++g)
             {
                 const float x = quad_sum(sum[g]);
-                if(quad == 0 && key0 + 16 * g + col < place.len)
+                if(quad == 0 && key0 + 16 * g + col < now.len)
                 {
-                    float *const w = to + 16 * g + col;
-                    *w = p.decay == 0.0f ? x : fmaf(p.decay, *w, x);
+                    to[16 * g] = p.decay == 0.0f ? x : fmaf(p.decay, kept[g], x);
                 }
             }
         }
@@ -297,21 +439,7 @@ void paged_weights_kernel(const PagedWeightsParams p)
         {
             return;
         }
-        if(++place.block == place.blocks)
-        {
-            place.block = 0;
-            staged = false;
-            if(++place.h == p.c.n_head_kv)
-            {
-                place.h = 0;
-                do
-                {
-                    ++place.n;
-                    place.len = uniform(paged_len(p.c, place.n));
-                    place.blocks = blocks_of(place.len);
-                } while(place.blocks == 0);     // (there is a block left)
-            }
-        }
+        staged = staged && place.n == now.n && place.h == now.h;
     }
 }
 
