@@ -16,10 +16,6 @@
 namespace nntile_hip
 {
 
-constexpr int kSelectThreads = 1024;
-constexpr int kSelectWaves = kSelectThreads / 64;
-constexpr int kSelectChunk = 4 * kSelectThreads;    // weights of a step, four a thread
-
 // A weight as an integer of the same order: -0 as 0, a NaN above all
 __device__ __forceinline__ uint32_t weight_key(float w)
 {
@@ -27,7 +23,9 @@ __device__ __forceinline__ uint32_t weight_key(float w)
     return w != w ? ~0u : (u >> 31) != 0 ? ~u : u | 0x80000000u;
 }
 
-// The sums of `x` over the threads in front of this one, and over all.
+// The sums of `x` over the threads in front of this one, and over all.  wave_sum is the call's until the second barrier
+// from here.
+template<int WAVES>
 __device__ __forceinline__ uint32_t workgroup_scan(uint32_t x, uint32_t *wave_sum, uint32_t &all)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -46,7 +44,7 @@ __device__ __forceinline__ uint32_t workgroup_scan(uint32_t x, uint32_t *wave_su
     uint32_t before = 0;
     all = 0;
 #pragma unroll
-    for(int w = 0; w < kSelectWaves; ++w)
+    for(int w = 0; w < WAVES; ++w)
     {
         before += w < wave ? wave_sum[w] : 0;
         all += wave_sum[w];
@@ -54,13 +52,17 @@ __device__ __forceinline__ uint32_t workgroup_scan(uint32_t x, uint32_t *wave_su
     return before + upto - x;
 }
 
-__global__ __launch_bounds__(kSelectThreads)
+// A step of the walk over the weights is four of them a thread.  HELD: steps whose weights stay in registers from the
+// first look at them to the last; 0: as many as there are rows for, from memory each time.
+template<int THREADS, int HELD>
+__global__ __launch_bounds__(THREADS)
 void paged_select_kernel(const PagedEvictParams p)
 {
-    constexpr int BINS = 2048;
+    constexpr int STEP = 4 * THREADS, WAVES = THREADS / 64, BINS = 2048, MINE = BINS / THREADS;
+    constexpr int KEPT = HELD > 0 ? HELD : 1;
     __shared__ uint32_t bins[BINS];
-    __shared__ uint32_t wave_sum[2][kSelectWaves];
-    __shared__ uint32_t found[2];
+    __shared__ uint32_t wave_sum[2][WAVES];
+    __shared__ uint32_t found[3];
     const int tid = threadIdx.x;
     const uint32_t entries = (uint32_t)p.c.n_batch * (uint32_t)p.c.n_head_kv;
     for(uint32_t entry = blockIdx.x; entry < entries; entry += gridDim.x)
@@ -71,13 +73,13 @@ void paged_select_kernel(const PagedEvictParams p)
         float *const w_out = p.weights_out + (int64_t)entry * p.columns;
         int32_t *const kept = p.kept + (int64_t)entry * p.keep;
         const int stay = min(len, p.keep);
-        for(int d = stay + tid; d < p.keep; d += kSelectThreads)
+        for(int d = stay + tid; d < p.keep; d += THREADS)
         {
             kept[d] = -1;
         }
         if(len <= p.keep)
         {
-            for(int d = tid; d < len; d += kSelectThreads)
+            for(int d = tid; d < len; d += THREADS)
             {
                 kept[d] = d;
                 if(w_out != w_in)
@@ -88,63 +90,138 @@ void paged_select_kernel(const PagedEvictParams p)
             continue;
         }
         const int old = len - p.recent;             // rows that are chosen from (recent <= keep < len)
-        uint32_t wanted = (uint32_t)(p.keep - p.recent);
+        const int steps = (len + STEP - 1) / STEP;
+        // the thread's weights of step s: rows s * STEP + 4 * tid and on; behind the last: 0
+        float held[KEPT][4];
+        auto look = [&](int s, float (&w)[4])
+        {
+            const int at = s * STEP + 4 * tid;
+            if(at + 3 < len)
+            {
+                __builtin_memcpy(w, w_in + at, 16);
+            }
+            else
+            {
+#pragma unroll
+                for(int k = 0; k < 4; ++k)
+                {
+                    w[k] = at + k < len ? w_in[at + k] : 0.0f;
+                }
+            }
+        };
+        // f(s, weights of step s) for all steps, in order
+        auto walk = [&](auto f)
+        {
+            if constexpr(HELD > 0)
+            {
+#pragma unroll
+                for(int s = 0; s < HELD; ++s)
+                {
+                    if(s < steps)
+                    {
+                        f(s, held[s]);
+                    }
+                }
+            }
+            else
+            {
+                for(int s = 0; s < steps; ++s)
+                {
+                    look(s, held[0]);
+                    f(s, held[0]);
+                }
+            }
+        };
+        if constexpr(HELD > 0)
+        {
+#pragma unroll
+            for(int s = 0; s < HELD; ++s)
+            {
+                if(s < steps)
+                {
+                    look(s, held[s]);
+                }
+            }
+        }
         // ---- the key of the wanted-th heaviest row ------------------------------------
-        uint32_t prefix = wanted == 0 ? ~0u : 0u;   // (nothing lies above it)
+        // All rows with a key above `key` stay, and the first `wanted` that have it.
+        uint32_t wanted = (uint32_t)(p.keep - p.recent), key = ~0u;
         if(wanted != 0)
         {
+            uint32_t prefix = 0;
             for(int pass = 0; pass < 3; ++pass)
             {
                 const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, width = pass == 2 ? 1024 : 2048;
-                for(int b = tid; b < BINS; b += kSelectThreads)
+#pragma unroll
+                for(int b = 0; b < MINE; ++b)
                 {
-                    bins[b] = 0;
+                    bins[tid + b * THREADS] = 0;
                 }
                 __syncthreads();
-                for(int at = tid; at < old; at += kSelectThreads)
+                walk([&](int s, const float (&w)[4])
                 {
-                    const uint32_t key = weight_key(w_in[at]);
-                    if(pass == 0 || (key >> (pass == 1 ? 21 : 10)) == prefix)
+#pragma unroll
+                    for(int k = 0; k < 4; ++k)
                     {
-                        atomicAdd(&bins[(key >> shift) & (width - 1)], 1u);
+                        const uint32_t of = weight_key(w[k]);
+                        if(s * STEP + 4 * tid + k < old && (pass == 0 || (of >> (pass == 1 ? 21 : 10)) == prefix))
+                        {
+                            atomicAdd(&bins[(of >> shift) & (width - 1)], 1u);
+                        }
                     }
-                }
+                });
                 __syncthreads();
-                // the largest bits first, two a thread
-                const uint32_t high = bins[BINS - 1 - 2 * tid], low = bins[BINS - 2 - 2 * tid];
-                uint32_t all;
-                const uint32_t before = workgroup_scan(high + low, wave_sum[pass & 1], all);
-                if(before < wanted && wanted <= before + high + low)
+                // the largest bits first, some a thread
+                uint32_t count[MINE], sum = 0;
+#pragma unroll
+                for(int b = 0; b < MINE; ++b)
                 {
-                    const bool in_high = wanted <= before + high;
-                    found[0] = (uint32_t)(in_high ? BINS - 1 - 2 * tid : BINS - 2 - 2 * tid);
-                    found[1] = wanted - before - (in_high ? 0 : high);
+                    count[b] = bins[BINS - 1 - MINE * tid - b];
+                    sum += count[b];
+                }
+                uint32_t all, before = workgroup_scan<WAVES>(sum, wave_sum[pass & 1], all);
+#pragma unroll
+                for(int b = 0; b < MINE; ++b)
+                {
+                    if(before < wanted && wanted <= before + count[b])
+                    {
+                        found[0] = (uint32_t)(BINS - 1 - MINE * tid - b);
+                        found[1] = wanted - before;
+                        found[2] = count[b];
+                    }
+                    before += count[b];
                 }
                 __syncthreads();
                 prefix = prefix << (pass == 2 ? 10 : 11) | found[0];
                 wanted = found[1];
+                key = prefix << shift;
+                if(wanted == found[2] && key != 0)
+                {
+                    // all rows with these bits stay, whatever the bits below
+                    key -= 1;
+                    wanted = 0;
+                    break;
+                }
             }
         }
         // ---- the rows that stay, in order ------------------------------------------------
-        // all above the key, and the first `wanted` that have it
         uint32_t above_before = 0, equal_before = 0;
-        for(int at0 = 0, turn = 0; at0 < len; at0 += kSelectChunk, ++turn)
+        __syncthreads();        // (found and wave_sum have been read)
+        walk([&](int s, const float (&w)[4])
         {
-            const int at = at0 + 4 * tid;
-            float w[4];
+            const int at = s * STEP + 4 * tid;
             uint32_t above = 0, equal = 0;          // a bit for each of the four
 #pragma unroll
             for(int k = 0; k < 4; ++k)
             {
-                w[k] = at + k < len ? w_in[at + k] : 0.0f;
-                const uint32_t key = weight_key(w[k]);
-                above |= (at + k < old ? key > prefix : at + k < len) ? 1u << k : 0u;
-                equal |= at + k < old && key == prefix ? 1u << k : 0u;
+                const uint32_t of = weight_key(w[k]);
+                above |= (at + k < old ? of > key : at + k < len) ? 1u << k : 0u;
+                equal |= at + k < old && of == key ? 1u << k : 0u;
             }
             // (at most 4096 of each in a step)
             uint32_t all;
-            const uint32_t before = workgroup_scan((uint32_t)__popc(above) | (uint32_t)__popc(equal) << 16,
-                    wave_sum[turn & 1], all);
+            const uint32_t before = workgroup_scan<WAVES>((uint32_t)__popc(above) | (uint32_t)__popc(equal) << 16,
+                    wave_sum[s & 1], all);
             uint32_t a = above_before + (before & 0xffffu), e = equal_before + (before >> 16);
 #pragma unroll
             for(int k = 0; k < 4; ++k)
@@ -160,9 +237,9 @@ void paged_select_kernel(const PagedEvictParams p)
             }
             above_before += all & 0xffffu;
             equal_before += all >> 16;
-        }
+        });
         // (the last step's weights have been read by all: the barrier in its scan)
-        for(int d = p.keep + tid; d < len; d += kSelectThreads)
+        for(int d = p.keep + tid; d < len; d += THREADS)
         {
             w_out[d] = 0.0f;
         }
@@ -223,7 +300,7 @@ void paged_evict_kernel(const PagedEvictParams p)
         {
             u32x4 x[AT_ONCE];
             uint32_t size[AT_ONCE];
-            int src[AT_ONCE];
+            int src[AT_ONCE], to[AT_ONCE];
 #pragma unroll
             for(int k = 0; k < AT_ONCE; ++k)
             {
@@ -238,6 +315,7 @@ void paged_evict_kernel(const PagedEvictParams p)
                 x[k] = u32x4{0, 0, 0, 0};
                 size[k] = 0x7f7f7f7fu;
                 const int page = src[k] >= 0 ? page_of(p.c, n, src[k]) : -1;
+                to[k] = src[k] >= 0 ? page_of(p.c, n, d0 + k * ROWS + slot) : -1;
                 if(page >= 0)
                 {
                     const int64_t at = row_in_page(p.c, h, src[k]);
@@ -258,16 +336,15 @@ void paged_evict_kernel(const PagedEvictParams p)
             for(int k = 0; k < AT_ONCE; ++k)
             {
                 const int d = d0 + k * ROWS + slot;
-                const int page = src[k] >= 0 ? page_of(p.c, n, d) : -1;
-                if(page >= 0)
+                if(to[k] >= 0)
                 {
                     const int64_t at = row_in_page(p.c, h, d);
-                    *reinterpret_cast<u32x4 *>(pages + page * p.c.page_stride + at * ROW_BYTES) = x[k];
+                    *reinterpret_cast<u32x4 *>(pages + to[k] * p.c.page_stride + at * ROW_BYTES) = x[k];
                     if constexpr(SB != 0)
                     {
                         if(slice == 0 && piece == 0)
                         {
-                            store_scales<SB>(scales + page * p.c.scale_stride + at * SB, size[k]);
+                            store_scales<SB>(scales + to[k] * p.c.scale_stride + at * SB, size[k]);
                         }
                     }
                 }
@@ -287,7 +364,23 @@ static int launch_evict(hipStream_t stream, const PagedEvictParams &p)
     }
     // (a direction of a launch has less than 2^32 threads)
     constexpr int64_t MOST = 1 << 20;
-    hipLaunchKernelGGL(paged_select_kernel, dim3((unsigned)(entries < MOST ? entries : MOST)), dim3(kSelectThreads), 0, stream, p);
+    const dim3 grid((unsigned)(entries < MOST ? entries : MOST));
+    if(p.c.max_rows <= 4096)
+    {
+        hipLaunchKernelGGL((paged_select_kernel<256, 4>), grid, dim3(256), 0, stream, p);
+    }
+    else if(p.c.max_rows <= 8192)
+    {
+        hipLaunchKernelGGL((paged_select_kernel<1024, 2>), grid, dim3(1024), 0, stream, p);
+    }
+    else if(p.c.max_rows <= 32768)
+    {
+        hipLaunchKernelGGL((paged_select_kernel<1024, 8>), grid, dim3(1024), 0, stream, p);
+    }
+    else
+    {
+        hipLaunchKernelGGL((paged_select_kernel<1024, 0>), grid, dim3(1024), 0, stream, p);
+    }
     if(hipGetLastError() != hipSuccess)
     {
         return NNTILE_HIP_ELAUNCH;
