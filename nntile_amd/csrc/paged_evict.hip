@@ -29,13 +29,7 @@ template<int WAVES>
 __device__ __forceinline__ uint32_t workgroup_scan(uint32_t x, uint32_t *wave_sum, uint32_t &all)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t upto = x;
-#pragma unroll
-    for(int o = 1; o < 64; o <<= 1)
-    {
-        const uint32_t other = __shfl_up(upto, o);
-        upto += lane >= o ? other : 0;
-    }
+    const uint32_t upto = wave_scan(x);
     if(lane == 63)
     {
         wave_sum[wave] = upto;

@@ -50,6 +50,20 @@ __device__ __forceinline__ int uniform(int x)
     return __builtin_amdgcn_readfirstlane(x);
 }
 
+// Sums over the wavefront's lanes up to this one, by moves between the vector unit's lanes (through LDS each of the six
+// steps waits for a round trip).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x)
+{
+    // one, two, four and eight lanes up in each row of 16, then the last lane of a row to the rows behind it
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+
 template<int N> __device__ __forceinline__ void paged_wait_loads()
 {
     static_assert(N >= 0 && N < 64, "vmcnt is a 6-bit counter");

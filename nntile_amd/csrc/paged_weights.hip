@@ -61,33 +61,18 @@ void paged_weights_kernel(const PagedWeightsParams p)
     // ---- the workgroup's run of blocks ----------------------------------------------
     auto blocks_of = [&](int len) { return (len + BLOCK - 1) / BLOCK; };
     auto len_of = [&](int n) { return n < p.c.n_batch ? paged_len(p.c, n) : 0; };
-    auto scan = [&](int len)        // blocks of the lanes up to this one
-    {
-        uint32_t upto = (uint32_t)blocks_of(len);
-#pragma unroll
-        for(int o = 1; o < 64; o <<= 1)
-        {
-            const uint32_t other = __shfl_up(upto, o);
-            upto += lane >= o ? other : 0;
-        }
-        return upto;
-    };
+    auto scan = [&](int len) { return wave_scan((uint32_t)blocks_of(len)); };      // blocks of the lanes up to this one
     auto last_lane = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); };
     int len_of_lane = len_of(lane);
     uint32_t upto = scan(len_of_lane), all = last_lane(upto);
     if(p.c.n_batch > 64)
     {
-        int more = 0;
+        uint32_t more = 0;
         for(int n = lane + 64; n < p.c.n_batch; n += 64)
         {
-            more += blocks_of(paged_len(p.c, n));
+            more += (uint32_t)blocks_of(paged_len(p.c, n));
         }
-#pragma unroll
-        for(int o = 32; o >= 1; o >>= 1)
-        {
-            more += __shfl_xor(more, o);
-        }
-        all += (uint32_t)uniform(more);
+        all += last_lane(wave_scan(more));
     }
     all *= (uint32_t)p.c.n_head_kv;
     const uint32_t shares = min((uint32_t)p.shares, all);
