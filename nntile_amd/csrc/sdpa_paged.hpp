@@ -327,26 +327,40 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     const int scanner = in_wave ? lane : tid, scanners = in_wave ? 64 : THREADS;
     const int chunk = (p.c.n_batch + scanners - 1) / scanners;
     const int n_lo = min(scanner * chunk, p.c.n_batch), n_hi = min(n_lo + chunk, p.c.n_batch);
-    auto blocks_of = [&](int n) { return (paged_len(p.c, n) + Shape::BLOCK - 1) / Shape::BLOCK; };
+    auto blocks_of_rows = [&](int rows) { return (rows + Shape::BLOCK - 1) / Shape::BLOCK; };
+    // Up to 64 sequences: a lane has one's length and new tokens, for whoever asks later.
+    int len_of_lane = 0, given_of_lane = 0;
+    if(in_wave && lane < p.c.n_batch)
+    {
+        len_of_lane = paged_len(p.c, lane);
+        given_of_lane = paged_new(p.c, lane, p.q_seq);
+    }
+    auto len_of = [&](int n)
+    {
+        return in_wave ? __builtin_amdgcn_readlane(len_of_lane, n) : uniform(paged_len(p.c, n));
+    };
     int unit_cost = kPagedUnitCost;
     auto cost_of = [&](int blocks) { return blocks == 0 ? 0 : blocks + unit_cost; };
-    const int blocks_0 = uniform(blocks_of(0));
+    const int blocks_0 = blocks_of_rows(len_of(0));
     int mine = 0;
     bool same = true;
-    for(int n = n_lo; n < n_hi; ++n)
+    if(in_wave)
     {
-        const int b = blocks_of(n);
-        mine += cost_of(b);
-        same = same && b == blocks_0;
+        const int b = blocks_of_rows(len_of_lane);
+        mine = cost_of(b);
+        same = lane >= p.c.n_batch || b == blocks_0;
+    }
+    else
+    {
+        for(int n = n_lo; n < n_hi; ++n)
+        {
+            const int b = blocks_of_rows(paged_len(p.c, n));
+            mine += cost_of(b);
+            same = same && b == blocks_0;
+        }
     }
     same = __all(same);
-    int upto = mine;
-#pragma unroll
-    for(int o = 1; o < 64; o <<= 1)
-    {
-        const int other = __shfl_up(upto, o);
-        upto += lane >= o ? other : 0;
-    }
+    int upto = (int)wave_scan((uint32_t)mine);
     int total = __builtin_amdgcn_readlane(upto, 63);
     if(!in_wave)
     {
@@ -413,7 +427,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         for(uint32_t piece = blockIdx.x; piece < (uint32_t)p.c.n_batch * (uint32_t)pieces; piece += gridDim.x)
         {
             const int n = (int)(piece / (uint32_t)pieces);
-            if(uniform(paged_len(p.c, n)) == 0)
+            if(len_of(n) == 0)
             {
                 const int first = (int)(piece - (uint32_t)n * (uint32_t)pieces) * PIECE;
                 const int here = min(rows - first, PIECE);
@@ -441,7 +455,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         first_share = blockIdx.x - part;
         seg.n = (int)(unit / (uint32_t)p.units);
         seg.u = (int)(unit - (uint32_t)seg.n * (uint32_t)p.units);
-        seg.len = uniform(paged_len(p.c, seg.n));
+        seg.len = len_of(seg.n);
         seg.blocks = blocks_0;
         seg.step = (int)of_blocks.begin(part);
         seg.steps = (int)of_blocks.begin(part + 1) - seg.step;
@@ -473,7 +487,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         seg.n = t * chunk;
         for(;;)
         {
-            seg.len = uniform(paged_len(p.c, seg.n));
+            seg.len = len_of(seg.n);
             seg.blocks = (seg.len + Shape::BLOCK - 1) / Shape::BLOCK;
             if(before + cost_of(seg.blocks) > block || seg.n + 1 >= p.c.n_batch)
             {
@@ -555,7 +569,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
         // shares of some units have equally much to do)
         const int h = seg.u / p.row_groups, in_turn = seg.u - h * p.row_groups;
         const int rg = (in_turn & 1) != 0 ? p.row_groups - 1 - (in_turn >> 1) : in_turn >> 1;
-        const int given = uniform(paged_new(p.c, seg.n, p.q_seq));
+        const int given = in_wave ? __builtin_amdgcn_readlane(given_of_lane, seg.n) : uniform(paged_new(p.c, seg.n, p.q_seq));
         const int key_lo = seg.step * Shape::BLOCK;
         // the keys that some row of the group sees, of the tokens of one head: those in front of the newest one's
         int seen = seg.len;
@@ -1310,7 +1324,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
             do
             {
                 ++seg.n;
-                seg.len = uniform(paged_len(p.c, seg.n));
+                seg.len = len_of(seg.n);
                 seg.blocks = (seg.len + Shape::BLOCK - 1) / Shape::BLOCK;
             } while(seg.blocks == 0);       // (`end` lies behind a block that exists)
         }
