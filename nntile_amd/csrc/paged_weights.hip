@@ -195,7 +195,8 @@ void paged_weights_kernel(const PagedWeightsParams p)
     auto stage = [&](const WeightsPlace &x, int row0) -> bool
     {
         const int rows = min(p.rows - row0, ROWS), pieces = (rows + 16 * BLOCKS - 1) / (16 * BLOCKS) * (16 * BLOCKS) * PIECES;
-        // row r's place in lse (times head: in Q); of a row that is none: the pair's first
+        // Row r's place in lse (times head: in Q); of a row that is none: the pair's first, whose scores are numbers wherever
+        // a row that counts has one (those of a row of zeros are NaN for a key with an infinity).
         auto place_of = [&](int r, int &tok, bool &ok)
         {
             const int rr = min(row0 + r, p.rows - 1), g = (int)p.by_seq.quotient((uint32_t)rr);
@@ -213,20 +214,20 @@ void paged_weights_kernel(const PagedWeightsParams p)
         for(int t0 = 0; t0 < pieces; t0 += 256 * AT_ONCE)
         {
             u32x4 v[AT_ONCE];
-            bool ok[AT_ONCE];
 #pragma unroll
             for(int k = 0; k < AT_ONCE; ++k)
             {
                 const int t = min(t0 + 256 * k + tid, pieces - 1);
                 int tok;
-                const int64_t row = place_of(t / PIECES, tok, ok[k]);
+                bool ok;
+                const int64_t row = place_of(t / PIECES, tok, ok);
                 v[k] = *reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.Q) + row * QB + t % PIECES * 16);
             }
 #pragma unroll
             for(int k = 0; k < AT_ONCE; ++k)
             {
                 const int t = t0 + 256 * k + tid, r = t / PIECES;
-                u32x4 first = ok[k] ? v[k] : u32x4{0, 0, 0, 0};
+                u32x4 first = v[k];
                 if(t < pieces)
                 {
                     char *const to = q_rows + r * QB + swizzled(r, t % PIECES) * 16;

@@ -112,6 +112,25 @@ def test_a_seen_key_that_is_no_number(dtype, bits):
     assert torch.isnan(after[0]).nonzero().flatten().tolist() == [37]
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("group", [3, 16, 37])
+def test_a_seen_key_that_is_infinite(dtype, group):
+    """Scores of -inf: a weight of 0, and none that the rows which fill up a block of 16 make NaN."""
+    c = F.make(11, dtype, 32 if dtype == "fp32" else 16, 1, 1, 64, 16, [90])
+    page = int(c.table[0, 2])
+    q = torch.randn(group, 1, 64)
+    q[:, 0, 9] = -0.5 - torch.rand(group)
+    q = q.to(P.TORCH_DT[dtype])
+    rest = torch.arange(c.max_pages * 16) != 37
+    runs = []
+    for key in (1.0, float("inf")):
+        c.pool[page, 0, 0, 5, 9] = key
+        c.device()
+        runs.append(_run(c, q, torch.full((group, 1), 2.0), torch.zeros(1, c.max_pages * 16), group, True)[0])
+    assert torch.equal(runs[0][rest], runs[1][rest])
+    assert float(runs[0][37]) > 0 and float(runs[1][37]) == 0
+
+
 @pytest.mark.parametrize("dtype,bits", F.KINDS)
 @pytest.mark.parametrize("q_seq,n_batch", [(1, 150), (40, 70)])
 def test_weights_of_many_sequences(dtype, bits, q_seq, n_batch):
