@@ -366,17 +366,18 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
                 }
             }
         };
-        // A power of two that is that of NaN?
+        // A power of two that is that of NaN, or 2^65 and more?
         bool odd = false;
         if constexpr(!PARTLY)
         {
             const uint32_t w = *reinterpret_cast<const uint32_t *>(v_scales + 4 * (lane % (16 * SB)));
-            odd = __any((((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u) != 0);
+            odd = __any((w & w << 1 & 0x80808080u) != 0);
         }
         if(!PARTLY && !odd)
         {
             // As bf16 numbers probabilities take a power of two by an addition to their exponents (what falls below the
-            // smallest number becomes 0, and a probability of 0 at most 2^-127).
+            // smallest number becomes 0; a probability of 0 counts as 2^-127, 2^-119 of the sum: of values up to
+            // 6 * 2^64 that is 2^-52).
             uint32_t pw[NR][GROUPS][2], pw_rest[NT][GT][2];
 #pragma unroll
             for(int nr = 0; nr < NR; ++nr)
@@ -427,8 +428,8 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
         }
         else
         {
-            // Probabilities that have to be exactly 0, of rows that are hidden or none, and powers of two that are those
-            // of NaN: the product in fp32.
+            // Probabilities that have to be exactly 0, of rows that are hidden or none or whose values are that large, and
+            // powers of two that are those of NaN: the product in fp32.
 #pragma unroll
             for(int b = 0; b < SB; ++b)
             {

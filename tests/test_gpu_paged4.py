@@ -229,6 +229,23 @@ def test_blocks_of_sizes_far_apart(dtype, q_seq, group):
     _check(c, q, q_seq, group, True, None, A, lse)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("head", [64, 128])
+@pytest.mark.parametrize("byte", [191, 192, 252])
+def test_the_largest_values_of_a_row_without_weight(dtype, head, byte):
+    """A row that every query sees, with a score of some -1000 and values of 6 * 2^(byte - 127), among rows of usual ones:
+    it leaves them as they are."""
+    c = F.Case4(53, dtype, 1, 1, head, 64, [900])
+    page = int(c.table[0, 2])
+    c.pool[page, :, 0, 11] = 0x77          # 6 everywhere
+    c.scales[page, 0, 0, 11] = 127 + 6
+    c.scales[page, 1, 0, 11] = byte
+    c.device()
+    q = -torch.rand(16, 1, head, generator=torch.Generator().manual_seed(54)).to(P.TORCH_DT[dtype])
+    A, lse = _attend(c, q, 16, True)
+    _check(c, q, 1, 16, True, None, A, lse)
+
+
 def test_a_table_with_entries_that_are_no_pages():
     c = F.Case4(61, "bf16", 2, 2, 64, 16, [100, 90])
     c.table[0, 2], c.table[1, 5], c.table[1, 0] = -1, c.n_pages, 1 << 30
