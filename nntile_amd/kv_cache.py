@@ -419,7 +419,7 @@ class PagedKVCache:
         given = None if new_rows is None else self._on_device(counts, stream)
         need = hip_sdpa.paged_workspace_bytes(Q, self.n_batch, kv_group)
         if self._workspace is None or self._workspace.numel() < need:
-            # (a launch of an earlier call, on whatever stream, may still use the old one; there are three sizes)
+            # (a launch of an earlier call, on whatever stream, may still use the old one; there are two sizes)
             self._old_workspaces.append(self._workspace)
             with torch.cuda.stream(stream):
                 self._workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)

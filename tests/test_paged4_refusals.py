@@ -144,6 +144,17 @@ def test_more_work_than_a_launch_has():
     assert h.lib().nntile_hip_paged_kv_evict_fp32(None, ctypes.byref(e)) == h.EINVAL
 
 
+@pytest.mark.parametrize("t,head", [("bf16", 128), ("bf16", 64), ("fp16", 128), ("fp16", 64)])
+def test_tiles_of_128_gib(t, head):
+    """2^30 rows of 128 bytes and more take 2^32 threads and more in one direction of a launch."""
+    c = _cache("paged4", head=head, page_rows=1024, n_head_kv=2, n_pages=5, max_pages=1 << 20, n_batch=2,
+               page_stride=head * 2048, scale_stride=head // 32 * 2048)
+    rows = 1 << 28
+    assert getattr(h.lib(), "nntile_hip_paged4_kv_append_" + t)(None, ctypes.byref(c), rows, 4096, 4096) == h.EINVAL
+    if head == 128:         # (four rows a thread: 2^30 rows of 64 values are 2^31 threads)
+        assert getattr(h.lib(), "nntile_hip_paged4_kv_read_" + t)(None, ctypes.byref(c), 0, rows, 4096, 4096) == h.EINVAL
+
+
 def test_caches_that_are_not_made():
     make = lambda **kw: PagedKVCache(4, 16, 1, 64, 1, 64, device="cpu", **kw)
     for bits in (0, 1, 2, 3, 16, 32, "4"):
