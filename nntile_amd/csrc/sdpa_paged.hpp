@@ -444,15 +444,22 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     {
         return;
     }
-    uint32_t at = split.begin(blockIdx.x);
-    const uint32_t end = split.begin(blockIdx.x + 1);
+    // The workgroup's share.  Where a head's row groups read the same keys, neighbouring shares go to workgroups of equal
+    // index modulo 8, to one XCD and its L2.
+    uint32_t me = blockIdx.x;
+    if(p.row_groups > 1 && me < (shares & ~7u))
+    {
+        me = me % 8 * (shares / 8) + me / 8;
+    }
+    uint32_t at = split.begin(me);
+    const uint32_t end = split.begin(me + 1);
     PagedSegment seg;
-    uint32_t first_share = blockIdx.x;
+    uint32_t first_share = me;
     if(aligned)
     {
-        const uint32_t unit = blockIdx.x / of_unit, part = blockIdx.x - unit * of_unit;
+        const uint32_t unit = me / of_unit, part = me - unit * of_unit;
         const PagedSplit of_blocks((uint32_t)blocks_0, of_unit);
-        first_share = blockIdx.x - part;
+        first_share = me - part;
         seg.n = (int)(unit / (uint32_t)p.units);
         seg.u = (int)(unit - (uint32_t)seg.n * (uint32_t)p.units);
         seg.len = len_of(seg.n);
@@ -1265,7 +1272,7 @@ void sdpa_paged_kernel(const PagedAttendParams p)
                 }
                 else
                 {
-                    const int64_t place = ((int64_t)blockIdx.x * 2 + (begins ? 1 : 0)) * QROWS + in_group;
+                    const int64_t place = ((int64_t)me * 2 + (begins ? 1 : 0)) * QROWS + in_group;
 #pragma unroll
                     for(int k = 0; k < PAIRS; ++k)
                     {

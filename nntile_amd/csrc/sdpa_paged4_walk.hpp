@@ -35,6 +35,9 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
     // Keys become bf16 numbers, whose exponents take any power of two of a block; an fp16 query is the sum of two of them
     // then (11 bits in 8 and 3, exactly), and so is a probability (16 bits), with products of their own each.
     constexpr bool TWO = __is_same(T, Fp16);
+    // Rows that another workgroup reads, too, may stay in the caches: 8 sequences of 8192 rows, 8 heads of 128, bf16, 32 and
+    // 64 query rows 33.1 -> 31.6 and 42.4 -> 40.8 us (fp16 38.8 -> 40.3 and 62.2 -> 63.3: not there).
+    constexpr bool PAST_CACHES = NR == 1 || TWO;
     constexpr int SLANES = GROUPS * SB;         // lanes that have the scale bytes of a step's keys, 16 each
     constexpr int STEP_LOADS = 2 * LOADS + 1;   // load instructions of a step
     const int tid = fresh(threadIdx.x), lane = tid & 63, wave = uniform(tid >> 6);
@@ -102,12 +105,12 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
 #pragma unroll
         for(int ld = 0; ld < LOADS; ++ld)
         {
-            load_to_lds16<0, true>(k_from + off[ld], slot + ld * 1024);
+            load_to_lds16<0, PAST_CACHES>(k_from + off[ld], slot + ld * 1024);
         }
 #pragma unroll
         for(int ld = 0; ld < LOADS; ++ld)
         {
-            load_to_lds16<0, true>(v_from + off[ld], slot + K_BYTES + ld * 1024);
+            load_to_lds16<0, PAST_CACHES>(v_from + off[ld], slot + K_BYTES + ld * 1024);
         }
         const int g = lane % SLANES / SB;
         const uint8_t *const scale_from = scales_of_lane + group_page(page, g) * p.c.scale_stride + group_row(i, g) * SB;
