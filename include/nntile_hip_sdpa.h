@@ -754,9 +754,10 @@ int nntile_hip_sdpa_fwd_paged_fp32(void *stream, const nntile_hip_sdpa_paged_arg
  * Everything else is as there.  bf16 and fp16 tiles.  The append takes the smallest power of two, from
  * 2^-125 to 2^125, that leaves none of the 32 values above 7 (the largest code, 6, is no further from
  * what it stands for than half a step then; what 2^125 leaves above becomes 6 * 2^125), and rounds to
- * nearest even; 32 values with a NaN or an infinity among them are stored as NaN.  What is read back is exact in bf16.  The attention's
+ * nearest even; 32 values with a NaN or an infinity among them are stored as NaN.  What is read
+ * back is exact in bf16, in fp16 rounded once and at most its largest number.  The attention's
  * workspace is nntile_hip_sdpa_fwd_paged_workspace_bytes; its probabilities are rounded to 8 bits
- * (bf16 tiles) or 16 (fp16), with the exponents of fp32. */
+ * (bf16 tiles) or 16 (fp16), with the exponents of fp32; max_pages * page_rows is at most 2^30. */
 int nntile_hip_paged4_kv_append_bf16(void *stream, const nntile_hip_paged_cache *cache,
         int64_t rows, const uint16_t *k_new, const uint16_t *v_new);
 int nntile_hip_paged4_kv_append_fp16(void *stream, const nntile_hip_paged_cache *cache,
@@ -782,7 +783,8 @@ int nntile_hip_sdpa_fwd_paged4_fp16(void *stream, const nntile_hip_sdpa_paged_ar
  * in [0, 1]; with 0 what weights held does not matter.  Columns at or behind lens are left as
  * they are.  cache.v_pages and cache.v_scales are not looked at.  The same call gives the same
  * bits every time.
- * n_batch * n_head_kv * ceil(max_pages * page_rows / 64) is below 2^31 (else NNTILE_HIP_EINVAL). */
+ * max_pages * page_rows is at most 2^30, n_batch * n_head_kv * ceil(max_pages * page_rows / 64) below
+ * 2^31 (else NNTILE_HIP_EINVAL). */
 typedef struct nntile_hip_paged_weights_args
 {
     nntile_hip_paged_cache cache;
@@ -809,7 +811,7 @@ int nntile_hip_paged4_attn_weights_fp16(void *stream, const nntile_hip_paged_wei
  *                keep) on
  *   weights      as above; weights_out: the same array, or another of the same size, whose
  *                columns below lens are written: the weights of the rows that stayed, then zeros
- * A row without a page moves as zeros, and none is written where the new place has no page.  No page
+ * max_pages * page_rows and keep are at most 2^30.  A row without a page moves as zeros, and none is written where the new place has no page.  No page
  * belongs to two sequences.  cache.new_rows is not looked at. */
 typedef struct nntile_hip_paged_evict_args
 {

@@ -7,9 +7,18 @@
 //
 //  * selection, a workgroup for every (sequence, head): the threshold by counting the weights' bits from the top, 11,
 //    11 and 10 of them, in LDS; then one walk over the rows that numbers those that stay.
-//  * the moves, a workgroup for every (sequence, head), K or V, and 64 bytes of the rows: several hundred rows at a
+//  * the moves, a workgroup for every (sequence, head), K or V, and 64 bytes of the rows: some thousand rows at a
 //    time are read into registers, and when all of them are there, written.  A row's new place lies at or in front of
-//    its old one, so rows that are read later are never in the way.
+//    its old one, so rows that are read later are never in the way.  What is kept and where it lies is looked up a step
+//    ahead, and the first rows, which stay where they are, are skipped (64 of 8192 bf16 rows of 128 values, 8128 kept at
+//    random 143 -> 123 us, 1088 of 8128 behind the first that goes 27.9 -> 17).
+//
+// Bound by latency where little moves: 12 heads of 1024 fp32 rows down to 512 take 9.3 us, half of it the launches,
+// the rest the chain of loads, counts and barriers of the selection, and length, kept, table and row of a move.  64 of
+// 700 to 8192 4-bit rows down to 1024, 57 MB, 25 us with what reads the pages back; the selection is 8.6 us of them (12.5
+// with the weights read again in every pass), the moves 6.6.  With much to move by HBM and the last-level cache: those 8128
+// of 8192 rows are 525 MB read and written, 4.7 TB/s in the moves alone.  Slices of 64 bytes of a row: with whole rows a
+// workgroup there were a quarter as many to have loads on their way.
 #include "paged_operands.hpp"
 #include "paged_rows.hpp"
 
@@ -280,7 +289,9 @@ void paged_evict_kernel(const PagedEvictParams p)
     const uint32_t entries = (uint32_t)p.c.n_batch * (uint32_t)p.c.n_head_kv;
     for(uint32_t work = blockIdx.x; work < entries * (2 * SLICES); work += gridDim.x)
     {
-        const uint32_t entry = work / (2 * SLICES), slice = work % SLICES, which = work / SLICES % 2;
+        // (the slices of a row, halves of the same cache lines, have equal index modulo 8 where the pairs are a multiple of 4:
+        // one XCD)
+        const uint32_t slice = work / (2 * entries), pair = work - slice * (2 * entries), entry = pair / 2, which = pair % 2;
         const int n = (int)(entry % (uint32_t)p.c.n_batch), h = (int)(entry / (uint32_t)p.c.n_batch);
         const int len = uniform(paged_len(p.c, n));
         if(len <= p.keep)
@@ -290,35 +301,59 @@ void paged_evict_kernel(const PagedEvictParams p)
         const int32_t *const kept = p.kept + (int64_t)entry * p.keep;
         char *const pages = (which ? p.c.v_pages : p.c.k_pages) + slice * SLICE + piece * 16;
         uint8_t *const scales = which ? p.c.v_scales : p.c.k_scales;
-        for(int d0 = 0; d0 < p.keep; d0 += ROWS * AT_ONCE)
+        constexpr int MOVES = ROWS * AT_ONCE;       // of a step
+        int d0 = 0;
+        if(p.keep > MOVES)
         {
-            u32x4 x[AT_ONCE];
-            uint32_t size[AT_ONCE];
-            int src[AT_ONCE], to[AT_ONCE];
+            // rows in front of the first that goes stay where they are: looked for at every `apart`-th
+            const int apart = (p.keep + kEvictThreads - 1) / kEvictThreads, d = (int)threadIdx.x * apart;
+            d0 = max(__syncthreads_count(d < p.keep && kept[d] == d) - 1, 0) * apart;
+        }
+        // What is kept in places d0 + slot .. and, for rows that move, the pages they come from and go to.
+        auto places = [&](int d0, int (&src)[AT_ONCE])
+        {
 #pragma unroll
             for(int k = 0; k < AT_ONCE; ++k)
             {
                 const int d = d0 + k * ROWS + slot;
                 src[k] = d < p.keep ? kept[d] : -1;
-                src[k] = src[k] > d && src[k] < len ? src[k] : -1;      // (a row that stays where it is)
             }
+        };
+        auto look_up = [&](int d0, int (&src)[AT_ONCE], int (&from)[AT_ONCE], int (&to)[AT_ONCE])
+        {
+#pragma unroll
+            for(int k = 0; k < AT_ONCE; ++k)
+            {
+                const int d = d0 + k * ROWS + slot;
+                src[k] = src[k] > d && src[k] < len ? src[k] : -1;      // (a row that stays where it is)
+                from[k] = src[k] >= 0 ? page_of(p.c, n, src[k]) : -1;
+                to[k] = src[k] >= 0 ? page_of(p.c, n, d) : -1;
+            }
+        };
+        int src[AT_ONCE], from[AT_ONCE], to[AT_ONCE];
+        places(d0, src);
+        look_up(d0, src, from, to);
+        for(; d0 < p.keep; d0 += MOVES)
+        {
+            u32x4 x[AT_ONCE];
+            uint32_t size[AT_ONCE];
+            int next[AT_ONCE], next_from[AT_ONCE], next_to[AT_ONCE];
+            places(d0 + MOVES, next);
 #pragma unroll
             for(int k = 0; k < AT_ONCE; ++k)
             {
                 // (a row without a page: zeros)
                 x[k] = u32x4{0, 0, 0, 0};
                 size[k] = 0x7f7f7f7fu;
-                const int page = src[k] >= 0 ? page_of(p.c, n, src[k]) : -1;
-                to[k] = src[k] >= 0 ? page_of(p.c, n, d0 + k * ROWS + slot) : -1;
-                if(page >= 0)
+                if(from[k] >= 0)
                 {
                     const int64_t at = row_in_page(p.c, h, src[k]);
-                    x[k] = *reinterpret_cast<const u32x4 *>(pages + page * p.c.page_stride + at * ROW_BYTES);
+                    x[k] = *reinterpret_cast<const u32x4 *>(pages + from[k] * p.c.page_stride + at * ROW_BYTES);
                     if constexpr(SB != 0)
                     {
                         if(slice == 0 && piece == 0)
                         {
-                            size[k] = load_scales<SB>(scales + page * p.c.scale_stride + at * SB);
+                            size[k] = load_scales<SB>(scales + from[k] * p.c.scale_stride + at * SB);
                         }
                     }
                 }
@@ -326,13 +361,13 @@ void paged_evict_kernel(const PagedEvictParams p)
             // all rows of the step are read before the first is written
             paged_wait_loads<0>();
             __syncthreads();
+            look_up(d0 + MOVES, next, next_from, next_to);
 #pragma unroll
             for(int k = 0; k < AT_ONCE; ++k)
             {
-                const int d = d0 + k * ROWS + slot;
                 if(to[k] >= 0)
                 {
-                    const int64_t at = row_in_page(p.c, h, d);
+                    const int64_t at = row_in_page(p.c, h, d0 + k * ROWS + slot);
                     *reinterpret_cast<u32x4 *>(pages + to[k] * p.c.page_stride + at * ROW_BYTES) = x[k];
                     if constexpr(SB != 0)
                     {
@@ -342,6 +377,9 @@ void paged_evict_kernel(const PagedEvictParams p)
                         }
                     }
                 }
+                src[k] = next[k];
+                from[k] = next_from[k];
+                to[k] = next_to[k];
             }
         }
     }

@@ -8,7 +8,7 @@
 //
 //  * The kv_group query heads of a key/value head are taken together, rows = kv_group * q_seq in blocks
 //    of 16: one or two of them a wavefront, up to four a workgroup (more rows: several workgroups read the
-//    keys, each up to the last one that its rows see).
+//    keys, each up to the last one that its rows see, on one XCD, so that all but the first read them from its L2).
 //  * The keys of a sequence are cut into blocks of 4 * KEYS, the blocks of all (sequence, head, row
 //    group) units are numbered through, and every workgroup takes an equal run of them, whatever the
 //    lengths: it finds its first unit by a scan of the lengths (they live on the device, so a captured

@@ -8,10 +8,12 @@
 //  * Values come through the transposing reads as codes, sixteen keys of a column, and their powers of two go into the
 //    probabilities, for every 32 columns anew: as bf16 numbers those take them by an addition to their exponents.
 //  * What bounds it is the issue of vector instructions, some 400 a step with one row block, 560 with two, beside what
-//    a unit's begin and end take: 64 sequences of 17 to 16384 rows, 8 heads of 128, 4 query rows a head, 173 MB, 44.1 us
-//    (46.8 with widened probabilities of fp32 and scalar addresses; loads alone 37).  Half the LDS, each half of a
-//    step fetched as soon as it was read, and three workgroups a CU for it: 47.0.  Values widened row by row and written
-//    back to LDS to be read transposed as bf16 numbers: 47.9.
+//    a unit's begin and end take: 64 sequences of 17 to 16384 rows, 8 heads of 128, 4 query rows a head, bf16, 173 MB,
+//    43.2 us = 4.0 TB/s (loads alone 37); 8 of 8192 rows, 64 query rows, 73 MB and 17 GFLOP, 40.7 us, of which 26 are the
+//    issue of these instructions, 6 the beginning, 2 the wavefronts' results and 4 the join.  Probabilities widened in
+//    fp32 and scalar addresses took 2.7 us more of the first and 0.6 less of the second.  Half the LDS, each half of a
+//    step fetched as soon as it was read, and three workgroups a CU for it: 2.9 more.  Values widened row by row and
+//    written back to LDS to be read transposed as bf16 numbers: 3.8 more.
 #pragma once
 
 #include <type_traits>

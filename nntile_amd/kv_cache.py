@@ -378,7 +378,8 @@ class PagedKVCache:
     # that the tile kernels' denser products need: one number for all types and sizes, on either side of
     # where they meet (us over the pages, read back).  bf16, 8 heads of 128, 4 x 2048 rows: 256 queries
     # 36.3, 47.9, 512 50.1, 46.9, 1024 95.1, 54.0; one sequence of 4096: 512 34.0, 37.8, 1024 50.9, 41.1.
-    # fp32, 12 heads of 64, 2 x 2048: 128 31.1, 33.8, 256 56.2, 45.2, 512 93.4, 53.5.
+    # fp32, 12 heads of 64, 2 x 2048: 128 31.1, 33.8, 256 56.2, 45.2, 512 93.4, 53.5.  4 bits, 4 x 2048 and 8 x 8192 rows
+    # of bf16: 256 27.7, 50.0 and 111, 216, 512 36.2, 46.8 and 217, 203, 1024 68.9, 54.2 and 495, 304.
     DENSE_ROWS = 512
 
     def _read_back(self, length, Q, mode, stream):

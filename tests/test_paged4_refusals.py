@@ -144,6 +144,21 @@ def test_more_work_than_a_launch_has():
     assert h.lib().nntile_hip_paged_kv_evict_fp32(None, ctypes.byref(e)) == h.EINVAL
 
 
+def test_sequences_longer_than_the_walks_count():
+    """2^31 - 2^16 rows: their number and a step more are no 32-bit integers."""
+    big = dict(page_rows=65536, n_head_kv=1, n_batch=1, max_pages=32767, page_stride=64 * 65536)
+    for kind in ("paged", "paged4"):
+        c = _cache(kind, **dict(big, **({} if kind == "paged" else dict(scale_stride=2 * 65536))))
+        w, e = _weights(kind, cache=c, columns=(1 << 31) - 1), _evict(kind, cache=c, columns=(1 << 31) - 1)
+        assert getattr(h.lib(), "nntile_hip_%s_attn_weights_bf16" % kind)(None, ctypes.byref(w)) == h.EINVAL
+        assert getattr(h.lib(), "nntile_hip_%s_kv_evict_bf16" % kind)(None, ctypes.byref(e)) == h.EINVAL
+    a = _attend(c)
+    a.q_seq = a.kv_group = 1
+    assert h.lib().nntile_hip_sdpa_fwd_paged4_bf16(None, ctypes.byref(a), 4096, 1 << 40) == h.EINVAL
+    e = _evict("paged", keep=(1 << 30) + 1)
+    assert h.lib().nntile_hip_paged_kv_evict_bf16(None, ctypes.byref(e)) == h.EINVAL
+
+
 @pytest.mark.parametrize("t,head", [("bf16", 128), ("bf16", 64), ("fp16", 128), ("fp16", 64)])
 def test_tiles_of_128_gib(t, head):
     """2^30 rows of 128 bytes and more take 2^32 threads and more in one direction of a launch."""
