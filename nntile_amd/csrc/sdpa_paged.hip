@@ -6,7 +6,7 @@ namespace nntile_hip
 
 size_t paged_attend_workspace_bytes(int64_t rows, int64_t head)
 {
-    return sizeof(unsigned long long) * kPagedMoreShares * kPagedCountStride + share_rows(rows) * (size_t)(head + 2) * 4;
+    return sizeof(unsigned long long) * kPagedShares * kPagedCountStride + share_rows(rows) * (size_t)(head + 2) * 4;
 }
 
 int launch_paged_attend(hipStream_t stream, int dtype, PagedAttendParams &p, int head, void *workspace)

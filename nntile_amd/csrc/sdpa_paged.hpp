@@ -1350,13 +1350,13 @@ static int row_blocks(bool two_at_most, int64_t entries, int64_t rows)
 // the rows of a workgroup).
 static size_t share_rows(int64_t rows)
 {
-    return (size_t)(rows <= 16 ? kPagedMoreShares : kPagedShares) * 2 * 16 * (size_t)row_blocks(false, 64, rows);
+    return (size_t)kPagedShares * 2 * 16 * (size_t)row_blocks(false, 64, rows);
 }
 
 static void place_workspace(PagedAttendParams &p, int head, void *workspace)
 {
     p.counts = static_cast<unsigned long long *>(workspace);
-    p.part_o = reinterpret_cast<float *>(p.counts + kPagedMoreShares * kPagedCountStride);
+    p.part_o = reinterpret_cast<float *>(p.counts + kPagedShares * kPagedCountStride);
     p.part_ml = p.part_o + share_rows(p.rows) * (size_t)head;
 }
 

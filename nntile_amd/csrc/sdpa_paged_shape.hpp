@@ -9,8 +9,6 @@ namespace nntile_hip
 constexpr int kPagedCUs = 256;
 // Workgroups that the keys are shared out to at most: two a CU
 constexpr int kPagedShares = 2 * kPagedCUs;
-// ... and where LDS has room for four
-constexpr int kPagedMoreShares = 4 * kPagedCUs;
 // What a unit costs beside its key blocks, in blocks
 constexpr int kPagedUnitCost = 1;
 // How far, in powers of two, probabilities may grow past the first before they are taken against a new maximum
@@ -22,7 +20,7 @@ constexpr float kPagedLift = 7.0f;
 constexpr unsigned long long kPagedCountMask = 4095;
 constexpr unsigned long long kPagedNone = 0x9e3779b97f4a7000ull;
 constexpr int kPagedCountStride = 8;
-static_assert(kPagedMoreShares < (int)kPagedCountMask, "counts stay below the word");
+static_assert(kPagedShares < (int)kPagedCountMask, "counts stay below the word");
 
 template<typename T, int KIND, int HEAD, int NR, int HALVES>
 struct PagedShape
@@ -59,7 +57,9 @@ struct PagedShape
     static constexpr int WALK = STREAMS * 2 * (STAGE + 2 * KEYS * SB) + QPARTS * QROWS * QB;
     static constexpr int FILL = KIND == kPaged4 ? WALK : STREAMS * 2 * STAGE;
     static constexpr int RING = FILL > MERGE_BYTES ? FILL : MERGE_BYTES;
-    static constexpr int WGS_PER_CU = KIND == kPaged4 ? (HEAD == 64 && NR == 1 ? 4 : RING > 79 * 1024 ? 1 : 2)
+    // (4-bit pages, head 64, one row block, as many as LDS has room for, four: 64 sequences of 1024 rows, 4 query rows,
+    // 12.2 -> 16.6 us, of 4096 32 -> 37; two row blocks, three: 16 of 300 to 4096 fp16 rows 19 -> 26, by spills)
+    static constexpr int WGS_PER_CU = KIND == kPaged4 ? (RING > 79 * 1024 ? 1 : 2)
         : RING > 72 * 1024 || WAVES > 4 ? 1 : 2;
     static constexpr int MIN_WAVES = WAVES * WGS_PER_CU / 4;        // of a SIMD
     static __host__ __device__ constexpr int q_swizzle(int r) { return r % (QB / 16 < 16 ? QB / 16 : 16); }

@@ -377,9 +377,10 @@ class PagedKVCache:
     # Queries of a key/value head from which a chunk of a batch of equal lengths is worth the copy
     # that the tile kernels' denser products need: one number for all types and sizes, on either side of
     # where they meet (us over the pages, read back).  bf16, 8 heads of 128, 4 x 2048 rows: 256 queries
-    # 36.3, 47.9, 512 50.1, 46.9, 1024 95.1, 54.0; one sequence of 4096: 512 34.0, 37.8, 1024 50.9, 41.1.
-    # fp32, 12 heads of 64, 2 x 2048: 128 31.1, 33.8, 256 56.2, 45.2, 512 93.4, 53.5.  4 bits, 4 x 2048 and 8 x 8192 rows
-    # of bf16: 256 27.7, 50.0 and 111, 216, 512 36.2, 46.8 and 217, 203, 1024 68.9, 54.2 and 495, 304.
+    # 31.4, 52.3, 512 40.6, 48.8, 1024 75.5, 56.1; one sequence of 4096: 512 30.3, 36.0, 1024 46.4, 40.0;
+    # 8 x 8192: 256 133, 226, 512 261, 219.  fp32, 12 heads of 64, 2 x 2048: 256 54.2, 44.1, 512 91.8,
+    # 49.8.  4 bits, 4 x 2048 and 8 x 8192 rows of bf16: 256 26.8, 49.7 and 110, 216, 512 36.1, 46.5 and
+    # 218, 203, 1024 65.3, 54.2 and 432, 305; of fp16 512 65.0, 46.6 and 424, 217.
     DENSE_ROWS = 512
 
     def _read_back(self, length, Q, mode, stream):
@@ -420,7 +421,7 @@ class PagedKVCache:
         given = None if new_rows is None else self._on_device(counts, stream)
         need = hip_sdpa.paged_workspace_bytes(Q, self.n_batch, kv_group)
         if self._workspace is None or self._workspace.numel() < need:
-            # (a launch of an earlier call, on whatever stream, may still use the old one; there are two sizes)
+            # (a launch of an earlier call, on whatever stream, may still use the old one; there are three sizes)
             self._old_workspaces.append(self._workspace)
             with torch.cuda.stream(stream):
                 self._workspace = torch.empty(need, dtype=torch.uint8, device=Q.device)

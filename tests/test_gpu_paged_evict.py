@@ -114,6 +114,16 @@ def test_long_sequences(bits, length, keep, recent, kind):
     _check(c, _weights(2, c, kind), keep, recent)
 
 
+@pytest.mark.parametrize("dtype,bits,head", [("bf16", 4, 64), ("fp16", 4, 128), ("bf16", 8, 64), ("fp16", 16, 128), ("fp32", 32, 128)])
+@pytest.mark.parametrize("first", [0, 1, 1023, 1024, 2047, 2049, 4100, 5890])
+def test_rows_that_stay_where_they_are(dtype, bits, head, first):
+    """One row goes, and the others behind it move by one; another head loses its last that may go."""
+    c = F.make(21, dtype, bits, 1, 2, head, 64, [6000]).device()
+    w = torch.ones(2, c.max_pages * c.page_rows)
+    w[0, first] = 0.5
+    _check(c, w, 5999, 100)
+
+
 def test_many_entries():
     c = F.make(3, "bf16", 16, 300, 9, 64, 16, [i % 40 for i in range(300)]).device()
     _check(c, _weights(3, c, "any"), 16, 4)
