@@ -16,7 +16,8 @@
 //    query rows, 50 MB, 11.3 us = 4.5 TB/s.  More rows: 64 keys (fp32 of 128 values 32), two blocks of 16 rows side by
 //    side, since the products of one wait for each other, and two workgroups a CU; bound by vector instructions, of each
 //    score an fma, an exponential and an addition: 4-bit fp16 pages of 16384 rows in all, 8 heads of 128, 128 query rows,
-//    4.3 GFLOP, 14.4 us, of which 8 are that issue (one block of rows at a time and keys fetched where they are used 16.8).
+//    4.3 GFLOP, 11.6 us, of which 5 are that issue and 3 the launch (every query as the sum of two bf16 numbers 14.4, one
+//    block of rows at a time and keys fetched where they are used as well 16.8).
 #include <type_traits>
 
 #include "fixed_divide.hpp"
@@ -44,13 +45,12 @@ void paged_weights_kernel(const PagedWeightsParams p)
     constexpr int BLOCKS = GK == 1 ? 1 : 2;             // blocks of 16 of them side by side: one's sums wait for each other
     // registers of 16 bytes: of a row's operand, for keys and queries, and of a key row as it lies in its page
     constexpr int QREGS = KIND == kPaged32 ? HEAD / 16 : HEAD / 32, RAW = RB < 64 ? 1 : RB / 64;
-    // keys of 4 bits become bf16 numbers, and an fp16 query the sum of two
-    constexpr bool TWO_Q = KIND == kPaged4 && __is_same(T, Fp16);
-    constexpr int QPARTS = TWO_Q ? 2 : 1;
-    typedef typename std::conditional<KIND == kPaged4, Bf16, T>::type QK;
+    // Keys of 4 bits become numbers of the tile type exactly, those of fp16 tiles while their powers of two lie from 2^-13
+    // to 2^13: a wavefront that has others makes bf16 numbers of its keys, and of a query the sum of two.
+    constexpr bool NARROW = KIND == kPaged4 && __is_same(T, Fp16);
     constexpr int QB = HEAD * (KIND == kPaged32 ? 4 : 2), PIECES = QB / 16;
     constexpr bool CODES = KIND == kPaged4 || KIND == kPaged8;
-    __shared__ __attribute__((aligned(16))) char q_rows[QPARTS * ROWS * QB];
+    __shared__ __attribute__((aligned(16))) char q_rows[ROWS * QB];
     __shared__ __attribute__((aligned(16))) float off_of[ROWS];     // -lse in log2 units; -inf: the row counts nothing
     __shared__ __attribute__((aligned(16))) int last_of[ROWS];      // the last key the row sees
 
@@ -232,17 +232,9 @@ void paged_weights_kernel(const PagedWeightsParams p)
             for(int k = 0; k < AT_ONCE; ++k)
             {
                 const int t = t0 + 256 * k + tid, r = t / PIECES;
-                u32x4 first = v[k];
                 if(t < pieces)
                 {
-                    char *const to = q_rows + r * QB + swizzled(r, t % PIECES) * 16;
-                    if constexpr(TWO_Q)
-                    {
-                        u32x4 rest;
-                        two_bf16(first, first, rest);
-                        *reinterpret_cast<u32x4 *>(to + ROWS * QB) = rest;
-                    }
-                    *reinterpret_cast<u32x4 *>(to) = first;
+                    *reinterpret_cast<u32x4 *>(q_rows + r * QB + swizzled(r, t % PIECES) * 16) = v[k];
                 }
             }
         }
@@ -267,6 +259,16 @@ void paged_weights_kernel(const PagedWeightsParams p)
         u32x4 kf[GK][QREGS];
         float s_scale[GK], kept[GK];
         const uint32_t without = hidden;
+        bool far = false;
+        if constexpr(NARROW)
+        {
+#pragma unroll
+            for(int g = 0; g < GK; ++g)
+            {
+                far = far || byte[g] - (127u - 13u) > 26u;
+            }
+            far = __any(far);
+        }
 #pragma unroll
         for(int g = 0; g < GK; ++g)
         {
@@ -278,7 +280,14 @@ void paged_weights_kernel(const PagedWeightsParams p)
             {
                 if constexpr(KIND == kPaged4)
                 {
-                    kf[g][i] = widen8_of_4<Bf16>(raw[g][0][i], scale);
+                    if(!NARROW || far)
+                    {
+                        kf[g][i] = widen8_of_4<Bf16>(raw[g][0][i], scale);
+                    }
+                    else
+                    {
+                        kf[g][i] = widen8_of_4<T>(raw[g][0][i], scale);
+                    }
                 }
                 else if constexpr(KIND == kPaged8)
                 {
@@ -308,6 +317,57 @@ void paged_weights_kernel(const PagedWeightsParams p)
         const int key0 = now.block * BLOCK + wave * KEYS;
         const bool here = key0 < now.len;
 
+        // scores of the rows from rb on
+        auto scores = [&](int rb, f32x4 (&s)[BLOCKS][GK], auto two)
+        {
+            constexpr bool TWO = decltype(two)::value;
+#pragma unroll
+            for(int k = 0; k < BLOCKS; ++k)
+            {
+#pragma unroll
+                for(int g = 0; g < GK; ++g)
+                {
+                    s[k][g] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+            }
+#pragma unroll
+            for(int i = 0; i < QREGS; ++i)
+            {
+#pragma unroll
+                for(int k = 0; k < BLOCKS; ++k)
+                {
+                    u32x4 q = *reinterpret_cast<const u32x4 *>(q_rows + (rb + 16 * k + col) * QB + swizzled(col, q_piece(i)) * 16);
+                    u32x4 rest = q;
+                    if constexpr(TWO)
+                    {
+                        two_bf16(q, q, rest);
+                    }
+#pragma unroll
+                    for(int g = 0; g < GK; ++g)
+                    {
+                        if constexpr(KIND == kPaged32)
+                        {
+#pragma unroll
+                            for(int e = 0; e < 4; ++e)
+                            {
+                                s[k][g] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(q[e]),
+                                        __uint_as_float(kf[g][i][e]), s[k][g], 0, 0, 0);
+                            }
+                        }
+                        else if constexpr(TWO)
+                        {
+                            s[k][g] = mfma32<Bf16>(q, kf[g][i], s[k][g]);
+                            s[k][g] = mfma32<Bf16>(rest, kf[g][i], s[k][g]);
+                        }
+                        else
+                        {
+                            s[k][g] = mfma32<T>(q, kf[g][i], s[k][g]);
+                        }
+                    }
+                }
+            }
+        };
+
         // ---- sums over the queries -------------------------------------------------------
         float sum[GK];
 #pragma unroll
@@ -333,45 +393,13 @@ void paged_weights_kernel(const PagedWeightsParams p)
             for(int rb = 0; rb < rows; rb += 16 * BLOCKS)
             {
                 f32x4 s[BLOCKS][GK];
-#pragma unroll
-                for(int k = 0; k < BLOCKS; ++k)
+                if(NARROW && far)
                 {
-#pragma unroll
-                    for(int g = 0; g < GK; ++g)
-                    {
-                        s[k][g] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                    }
+                    scores(rb, s, std::bool_constant<NARROW>());
                 }
-#pragma unroll
-                for(int i = 0; i < QREGS; ++i)
+                else
                 {
-#pragma unroll
-                    for(int part = 0; part < QPARTS; ++part)
-                    {
-#pragma unroll
-                        for(int k = 0; k < BLOCKS; ++k)
-                        {
-                            const u32x4 q = *reinterpret_cast<const u32x4 *>(q_rows + (part * ROWS + rb + 16 * k + col) * QB
-                                    + swizzled(col, q_piece(i)) * 16);
-#pragma unroll
-                            for(int g = 0; g < GK; ++g)
-                            {
-                                if constexpr(KIND == kPaged32)
-                                {
-#pragma unroll
-                                    for(int e = 0; e < 4; ++e)
-                                    {
-                                        s[k][g] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(q[e]),
-                                                __uint_as_float(kf[g][i][e]), s[k][g], 0, 0, 0);
-                                    }
-                                }
-                                else
-                                {
-                                    s[k][g] = mfma32<QK>(q, kf[g][i], s[k][g]);
-                                }
-                            }
-                        }
-                    }
+                    scores(rb, s, std::false_type());
                 }
                 if(partly || dead)
                 {

@@ -112,6 +112,27 @@ def test_a_seen_key_that_is_no_number(dtype, bits):
     assert torch.isnan(after[0]).nonzero().flatten().tolist() == [37]
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("head", [64, 128])
+@pytest.mark.parametrize("q_seq,group", [(1, 4), (5, 4), (10, 16)])
+def test_four_bit_keys_of_sizes_far_apart(dtype, head, q_seq, group):
+    """Powers of two that fp16 has no exponents for, beside usual ones: in one block of 32 values of a sequence, in all."""
+    c = F.make(12, dtype, 4, 2, 2, head, 64, [300, 200])
+    g = torch.Generator().manual_seed(13)
+    size = torch.randint(127 - 30, 127 + 15, c.scales[:, 0].shape, generator=g).to(torch.uint8)
+    there = c.there[:, None, :, None].expand(size.shape).clone()
+    for page in set(c.table[0].tolist()) - {-1}:
+        there[page] = False
+    c.scales[:, 0] = torch.where(there, size, c.scales[:, 0])
+    c.scales[int(c.table[0, 1]), 0, 1, 6, 1] = 127 - 17
+    c.device()
+    q = (2.0 ** -7 * torch.randn(4 * group, q_seq, head, generator=g)).to(P.TORCH_DT[dtype])
+    lse = torch.from_numpy(P.attend(c, q, q_seq, group, True, None)[1]).float()
+    weights = torch.rand(4, c.max_pages * 64, generator=g)
+    after = _run(c, q, lse, weights, group, True, None, 0.5)
+    _check(c, q, lse, weights, after, q_seq, group, True, None, 0.5)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("group", [3, 16, 37])
 def test_a_seen_key_that_is_infinite(dtype, group):
