@@ -3,11 +3,12 @@
 //
 // A row is e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), two a byte, the lower half first, and one power of
 // two 2^k for every 32 values, kept as the byte k + 127: with a the largest absolute value of the 32, k is the
-// smallest integer from -125 to 125 with a <= 7 * 2^k (or 125: what lies above becomes 6 * 2^125).  What lies between 6
-// and 7 rounds to 6, by no more than what lies between 4 and 6 is rounded by; on normal values the codes then err by 11.2 % (root mean square), by 11.5 %
-// with the power that leaves nothing above 6 or with that of the largest value's exponent.  Every
-// value that a code stands for is a normal, finite number of bf16.  The division is exact, so a code is one rounding of its
-// value, to nearest even, and what is read back is exact in bf16.  A block with a NaN or an infinity has the byte 255.
+// smallest integer from -125 to 125 with a <= 7 * 2^k (or 125: what lies above becomes 6 * 2^125).  What lies
+// between 6 and 7 rounds to 6, by no more than what lies between 4 and 6 is rounded by; on normal values the codes
+// then err by 11.2 % (root mean square), by 11.5 % with the power that leaves nothing above 6 or with that of the
+// largest value's exponent.  Every value that a code stands for is a normal, finite number of bf16.  The division
+// is exact, so a code is one rounding of its value, to nearest even, and what is read back is exact in bf16.  A
+// block with a NaN or an infinity has the byte 255.
 //
 // Like the moves of 8-bit rows: a thread has 16 bytes of the dense side, eight values, of a row or of a few at
 // once; the four threads of a block are neighbours.  Bound by HBM, the dense side's bytes: 4 x 4096 rows, 8 heads of 128,
