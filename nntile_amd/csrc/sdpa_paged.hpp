@@ -405,9 +405,14 @@ void sdpa_paged_kernel(const PagedAttendParams p)
     // query rows 26.4 -> 20.9, 4 query rows over 2048 30.4 -> 36.0).  32 query rows over 16-bit pages are better
     // off in any case (those 160 units 40.7 -> 36.3), unequal units in none (64 of 17 to 8192, 32 query rows
     // 99 -> 137).
+    // 4-bit pages, whose joins weigh more beside their keys: where a share of two workgroups a CU has two blocks at most,
+    // any rows (8 heads; of 128, 32 of 1024 rows, 4, 16 and 32 query rows 14.5, 15.6, 23.5 -> 12.7, 12.8, 17.9, 4 of 2048, 64
+    // query rows 20.7 -> 16.3, of 8192, 4 and 16 query rows 14.5, 19.9 -> 15.0, 16.3; of 64, 32 of 1024, 4 query rows 12.3 ->
+    // 9.8), not with more (8 of 8192, 64 query rows 40.7 -> 45.8).
     constexpr bool ONE_A_CU = KIND == kPaged16 || (KIND == kPaged8 && NR == 2);
+    const bool one_a_cu = KIND == kPaged4 ? all <= 2 * (uint32_t)p.shares : ONE_A_CU && p.row_groups == 1;
     const uint32_t cus_filled = n_units <= kPagedCUs ? kPagedCUs / n_units * n_units : 0;
-    const uint32_t equal_places = ONE_A_CU && p.row_groups == 1
+    const uint32_t equal_places = one_a_cu
         && (8 * cus_filled >= 7 * kPagedCUs || (KIND == kPaged16 && NR == 2 && cus_filled != 0))
         ? min(places, (uint32_t)kPagedCUs) : places;
     const bool aligned = same && n_units <= equal_places && blocks_0 != 0;

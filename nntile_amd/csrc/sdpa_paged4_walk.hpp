@@ -34,8 +34,11 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
     constexpr int RB = Shape::RB, SB = Shape::SB, CPR = Shape::CPR, KEYS = Shape::KEYS, GROUPS = Shape::GROUPS;
     constexpr int LOADS = Shape::LOADS, K_BYTES = Shape::K_BYTES, STREAMS = Shape::STREAMS, QROWS = Shape::QROWS, QB = Shape::QB;
     constexpr int DBLOCKS = HEAD / 16, QREGS = HEAD / 32;
-    // Keys become bf16 numbers, whose exponents take any power of two of a block; an fp16 query is the sum of two of them
-    // then (11 bits in 8 and 3, exactly), and so is a probability (16 bits), with products of their own each.
+    // Keys become numbers of the tile type exactly; where a step has powers of two below 2^-13 or above 2^13, for which
+    // fp16 has no exponents, bf16 numbers, and an fp16 query is the sum of two of them then (11 bits in 8 and 3, exactly).
+    // (64 sequences of 2048 rows, 8 heads of 128, 32, 64 and 256 query rows 69, 132 and 512 us with sums of two always, 59,
+    // 110 and 414 now; 8 of 8192, 32 query rows, 39.7 and 43.9, the registers now being those of two workgroups a CU.)
+    // Probabilities of fp16 tiles are always the sum of two bf16 numbers (16 bits), with products of their own each.
     constexpr bool TWO = __is_same(T, Fp16);
     // Rows that another workgroup reads, too, may stay in the caches: 8 sequences of 8192 rows, 8 heads of 128, bf16, 32 and
     // 64 query rows 33.1 -> 31.6 and 42.4 -> 40.8 us (fp16 38.8 -> 40.3 and 62.2 -> 63.3: not there).
@@ -141,21 +144,14 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
                 x = *reinterpret_cast<const u32x4 *>(static_cast<const char *>(p.Q)
                         + paged_query_row(p, seg.n, h, rr) * QB + piece * 16);
             }
-            char *const to = q_rows + r * QB + (piece ^ Shape::q_swizzle(r)) * 16;
-            if constexpr(TWO)
-            {
-                u32x4 rest;
-                two_bf16(x, x, rest);
-                *reinterpret_cast<u32x4 *>(to + QROWS * QB) = rest;
-            }
-            *reinterpret_cast<u32x4 *>(to) = x;
+            *reinterpret_cast<u32x4 *>(q_rows + r * QB + (piece ^ Shape::q_swizzle(r)) * 16) = x;
         }
         __syncthreads();
     }
     // a lane's operands begin at (head/4)*quad + 8i of its row
-    auto q_operand = [&](int nr, int i, int part)
+    auto q_operand = [&](int nr, int i)
     {
-        return *reinterpret_cast<const u32x4 *>(q_rows + (part * QROWS + nr * 16 + col) * QB
+        return *reinterpret_cast<const u32x4 *>(q_rows + (nr * 16 + col) * QB
                 + ((HEAD / 32 * quad + i) ^ Shape::q_swizzle(col)) * 16);
     };
 
@@ -216,12 +212,14 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
         f32x4 s[NR][GROUPS];
         uint32_t codes[GROUPS][QREGS];
         float scale[GROUPS];
+        bool far = false;
 #pragma unroll
         for(int g = 0; g < GROUPS; ++g)
         {
             // the power of two of the lane's fourth of its key row
-            scale[g] = __uint_as_float((uint32_t)*reinterpret_cast<const uint8_t *>(k_scales + (16 * g + col) * SB
-                        + quad * SB / 4) << 23);
+            const uint32_t byte = *reinterpret_cast<const uint8_t *>(k_scales + (16 * g + col) * SB + quad * SB / 4);
+            scale[g] = __uint_as_float(byte << 23);
+            far = far || (TWO && byte - (127u - 13u) > 26u);
 #pragma unroll
             for(int i = 0; i < QREGS; ++i)
             {
@@ -234,27 +232,50 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
             }
         }
         // (the groups' sums side by side: a sum's products wait for each other)
-#pragma unroll
-        for(int i = 0; i < QREGS; ++i)
+        if(!TWO || !__any(far))
         {
-            u32x4 q[NR], q_rest[NR];
 #pragma unroll
-            for(int nr = 0; nr < NR; ++nr)
+            for(int i = 0; i < QREGS; ++i)
             {
-                q[nr] = q_operand(nr, i, 0);
-                q_rest[nr] = TWO ? q_operand(nr, i, 1) : q[nr];
-            }
-#pragma unroll
-            for(int g = 0; g < GROUPS; ++g)
-            {
-                const u32x4 wide = widen8_of_4<Bf16>(codes[g][i], scale[g]);
+                u32x4 q[NR];
 #pragma unroll
                 for(int nr = 0; nr < NR; ++nr)
                 {
-                    s[nr][g] = mfma32<Bf16>(wide, q[nr], s[nr][g]);
-                    if constexpr(TWO)
+                    q[nr] = q_operand(nr, i);
+                }
+#pragma unroll
+                for(int g = 0; g < GROUPS; ++g)
+                {
+                    const u32x4 wide = widen8_of_4<T>(codes[g][i], scale[g]);
+#pragma unroll
+                    for(int nr = 0; nr < NR; ++nr)
                     {
-                        s[nr][g] = mfma32<Bf16>(wide, q_rest[nr], s[nr][g]);
+                        s[nr][g] = mfma32<T>(wide, q[nr], s[nr][g]);
+                    }
+                }
+            }
+        }
+        else if constexpr(TWO)
+        {
+#pragma unroll
+            for(int i = 0; i < QREGS; ++i)
+            {
+                u32x4 wide[GROUPS];
+#pragma unroll
+                for(int g = 0; g < GROUPS; ++g)
+                {
+                    wide[g] = widen8_of_4<Bf16>(codes[g][i], scale[g]);
+                }
+#pragma unroll
+                for(int nr = 0; nr < NR; ++nr)
+                {
+                    u32x4 q = q_operand(nr, i), rest;
+                    two_bf16(q, q, rest);
+#pragma unroll
+                    for(int g = 0; g < GROUPS; ++g)
+                    {
+                        s[nr][g] = mfma32<Bf16>(wide[g], q, s[nr][g]);
+                        s[nr][g] = mfma32<Bf16>(wide[g], rest, s[nr][g]);
                     }
                 }
             }

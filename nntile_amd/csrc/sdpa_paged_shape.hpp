@@ -51,16 +51,15 @@ struct PagedShape
     // the query rows: the operands of one block of 16 stay in registers, those of two in LDS
     static constexpr int QB = HEAD * (KIND == kPaged32 ? 4 : 2);
     static constexpr int Q_BYTES = NR > 1 ? QROWS * QB : 16;
-    // 4-bit pages: two steps' keys, values and scales of every wavefront, and the query rows behind them (fp16 ones
-    // as two numbers)
-    static constexpr int QPARTS = __is_same(T, Fp16) ? 2 : 1;
-    static constexpr int WALK = STREAMS * 2 * (STAGE + 2 * KEYS * SB) + QPARTS * QROWS * QB;
+    // 4-bit pages: two steps' keys, values and scales of every wavefront, and the query rows behind them
+    static constexpr int WALK = STREAMS * 2 * (STAGE + 2 * KEYS * SB) + QROWS * QB;
     static constexpr int FILL = KIND == kPaged4 ? WALK : STREAMS * 2 * STAGE;
     static constexpr int RING = FILL > MERGE_BYTES ? FILL : MERGE_BYTES;
     // (4-bit pages, head 64, one row block, as many as LDS has room for, four: 64 sequences of 1024 rows, 4 query rows,
     // 12.2 -> 16.6 us, of 4096 32 -> 37; two row blocks, three: 16 of 300 to 4096 fp16 rows 19 -> 26, by spills)
-    static constexpr int WGS_PER_CU = KIND == kPaged4 ? (RING > 79 * 1024 ? 1 : 2)
+    static constexpr int WGS_PER_CU = KIND == kPaged4 ? 2
         : RING > 72 * 1024 || WAVES > 4 ? 1 : 2;
+    static_assert(KIND != kPaged4 || RING <= 79 * 1024, "room for two workgroups a CU");
     static constexpr int MIN_WAVES = WAVES * WGS_PER_CU / 4;        // of a SIMD
     static __host__ __device__ constexpr int q_swizzle(int r) { return r % (QB / 16 < 16 ? QB / 16 : 16); }
 

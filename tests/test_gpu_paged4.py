@@ -231,6 +231,26 @@ def test_blocks_of_sizes_far_apart(dtype, q_seq, group):
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("head", [64, 128])
+@pytest.mark.parametrize("q_seq,group", [(1, 4), (5, 4), (10, 6)])
+def test_keys_of_sizes_far_apart(dtype, head, q_seq, group):
+    """Keys' powers of two that fp16 has no exponents for, beside usual ones: in one block of 32 values of a sequence, in
+    all blocks of the other."""
+    c = F.Case4(55, dtype, 2, 2, head, 64, [900, 500])
+    g = torch.Generator().manual_seed(56)
+    size = torch.randint(127 - 30, 127 + 15, c.scales[:, 0].shape, generator=g).to(torch.uint8)
+    there = c.there[:, None, :, None].expand(size.shape).clone()
+    for page in set(c.table[0].tolist()) - {-1}:
+        there[page] = False
+    c.scales[:, 0] = torch.where(there, size, c.scales[:, 0])
+    c.scales[int(c.table[0, 3]), 0, 1, 6, 1] = 127 - 17
+    c.device()
+    q = (2.0 ** -7 * torch.randn(4 * group, q_seq, head, generator=g)).to(P.TORCH_DT[dtype])
+    A, lse = _attend(c, q, group, True)
+    _check(c, q, q_seq, group, True, None, A, lse)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("head", [64, 128])
 @pytest.mark.parametrize("byte", [191, 192, 252])
 def test_the_largest_values_of_a_row_without_weight(dtype, head, byte):
     """A row that every query sees, with a score of some -1000 and values of 6 * 2^(byte - 127), among rows of usual ones:
