@@ -379,8 +379,8 @@ class PagedKVCache:
     # where they meet (us over the pages, read back).  bf16, 8 heads of 128, 4 x 2048 rows: 256 queries
     # 31.4, 52.3, 512 40.6, 48.8, 1024 75.5, 56.1; one sequence of 4096: 512 30.3, 36.0, 1024 46.4, 40.0;
     # 8 x 8192: 256 133, 226, 512 261, 219.  fp32, 12 heads of 64, 2 x 2048: 256 54.2, 44.1, 512 91.8,
-    # 49.8.  4 bits, 4 x 2048 and 8 x 8192 rows of bf16: 256 26.8, 49.7 and 110, 216, 512 36.1, 46.5 and
-    # 218, 203, 1024 65.3, 54.2 and 432, 305; of fp16 512 65.0, 46.6 and 424, 217.
+    # 49.8.  4 bits, 4 x 2048 and 8 x 8192 rows of bf16: 256 28.7, 50.2 and 109, 216, 512 36.5, 46.4 and
+    # 214, 203, 1024 65.5, 53.6 and 424, 303; of fp16 512 50.7, 46.9 and 336, 216.
     DENSE_ROWS = 512
 
     def _read_back(self, length, Q, mode, stream):
