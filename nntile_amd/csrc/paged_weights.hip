@@ -196,10 +196,12 @@ void paged_weights_kernel(const PagedWeightsParams p)
     WeightsPlace next = left > 1 ? next_of(place) : place;
     look_up(next, page);
 
-    // Query rows from row0 on into LDS.  True: one of them counts nothing, whatever its scores are.
+    // Query rows from row0 on into LDS, as many as fill blocks of rows.  True: one of them, or the query that fills the rest
+    // up, counts nothing, whatever its scores are.
     auto stage = [&](const WeightsPlace &x, int row0) -> bool
     {
-        const int rows = min(p.rows - row0, ROWS), pieces = (rows + 16 * BLOCKS - 1) / (16 * BLOCKS) * (16 * BLOCKS) * PIECES;
+        const int rows = min(p.rows - row0, ROWS), staged_rows = (rows + 16 * BLOCKS - 1) / (16 * BLOCKS) * (16 * BLOCKS);
+        const int pieces = staged_rows * PIECES;
         // Row r's place in lse (times head: in Q); of a row that is none: the pair's first, whose scores are numbers wherever
         // a row that counts has one (those of a row of zeros are NaN for a key with an infinity).
         auto place_of = [&](int r, int &tok, bool &ok)
@@ -211,8 +213,8 @@ void paged_weights_kernel(const PagedWeightsParams p)
         };
         int my_tok;
         bool my_ok;
-        const int64_t my_row = place_of(min(tid, ROWS - 1), my_tok, my_ok);
-        const float lse = my_ok ? p.lse[my_row] : neg_inf();
+        const int64_t my_row = place_of(min(tid, staged_rows - 1), my_tok, my_ok);
+        const float lse_there = p.lse[my_row], lse = my_ok ? lse_there : neg_inf();
         __syncthreads();        // the rows before these are done with
         // (several loads on their way at a time)
         constexpr int AT_ONCE = 4;
@@ -238,12 +240,12 @@ void paged_weights_kernel(const PagedWeightsParams p)
                 }
             }
         }
-        if(tid < ROWS)
+        if(tid < staged_rows)
         {
             off_of[tid] = lse == neg_inf() ? neg_inf() : -lse * kLog2e;
             last_of[tid] = lse == neg_inf() ? -1 : p.causal ? x.len - x.given + my_tok : x.len - 1;
         }
-        return __syncthreads_or(my_ok && lse == neg_inf());
+        return __syncthreads_or(lse_there == neg_inf());
     };
     bool staged = false;        // the pair's queries lie in LDS, all of them
     bool dead = false;

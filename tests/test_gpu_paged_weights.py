@@ -167,3 +167,23 @@ def test_weights_of_many_sequences(dtype, bits, q_seq, n_batch):
     b = _run(c, q, lse, weights, 2, True, None, 0.25, stream=torch.cuda.Stream())
     assert torch.equal(a.view(torch.int32), b.view(torch.int32))
     _check(c, q, lse, weights, a, q_seq, 2, True, None, 0.25)
+
+
+@pytest.mark.parametrize("dtype,bits", F.KINDS)
+@pytest.mark.parametrize("q_seq,group,given", [(5, 28, 5), (1, 129, 1), (3, 90, 2), (4, 40, 3)])
+@pytest.mark.parametrize("fill", [float("nan"), float("inf")])
+def test_a_first_query_that_counts_nothing(dtype, bits, q_seq, group, given, fill):
+    """More query rows than are staged at a time, some that only fill up a block of 16 or are padding, and a first one
+    whose lse is -inf over a query that is no number: no key receives anything of it."""
+    print("first", dtype, bits, q_seq, group, given, fill, flush=True)
+    lens = [600, 300]               # (more than one block of keys that every query sees)
+    c = F.make(14, dtype, bits, 2, 1, 64, 64, lens).device()
+    g = torch.Generator().manual_seed(15)
+    q = torch.randn(group * 2, q_seq, 64, generator=g).to(P.TORCH_DT[dtype])
+    new_rows = [given, q_seq]
+    lse = torch.from_numpy(P.attend(c, q, q_seq, group, True, new_rows)[1]).float()
+    q.view(group, 2, q_seq, 64)[0, 0, 0] = fill
+    lse.view(group, 2, q_seq)[0, 0, 0] = float("-inf")
+    weights = torch.rand(2, c.max_pages * 64, generator=g)
+    after = _run(c, q, lse, weights, group, True, new_rows, 0.5)
+    _check(c, q, lse, weights, after, q_seq, group, True, new_rows, 0.5)
