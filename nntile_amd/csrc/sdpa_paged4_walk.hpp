@@ -34,15 +34,22 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
     constexpr int RB = Shape::RB, SB = Shape::SB, CPR = Shape::CPR, KEYS = Shape::KEYS, GROUPS = Shape::GROUPS;
     constexpr int LOADS = Shape::LOADS, K_BYTES = Shape::K_BYTES, STREAMS = Shape::STREAMS, QROWS = Shape::QROWS, QB = Shape::QB;
     constexpr int DBLOCKS = HEAD / 16, QREGS = HEAD / 32;
-    // Keys become numbers of the tile type exactly; where a step has powers of two below 2^-13 or above 2^13, for which
-    // fp16 has no exponents, bf16 numbers, and an fp16 query is the sum of two of them then (11 bits in 8 and 3, exactly).
-    // (64 sequences of 2048 rows, 8 heads of 128, 32, 64 and 256 query rows 69, 132 and 512 us with sums of two always, 59,
-    // 110 and 414 now; 8 of 8192, 32 query rows, 39.7 and 43.9, the registers now being those of two workgroups a CU.)
+    // Keys become numbers of the tile type exactly; where a query sees powers of two below 2^-13 or above 2^13 in a step, for
+    // which fp16 has no exponents, bf16 numbers, and an fp16 query is the sum of two of them then (11 bits in 8 and 3, exactly).
+    // Rows that it does not see have no say in that: they leave every bit of its result as it is.
+    // (64 sequences of 2048 rows, 8 heads of 128, 32, 64 and 256 query rows 69, 132 and 512 us with sums of two always, 58,
+    // 102 and 361 now; 8 of 8192, 32 query rows, 39.7 and 38.6.)
     // Probabilities of fp16 tiles are always the sum of two bf16 numbers (16 bits), with products of their own each.
     constexpr bool TWO = __is_same(T, Fp16);
     // Rows that another workgroup reads, too, may stay in the caches: 8 sequences of 8192 rows, 8 heads of 128, bf16, 32 and
-    // 64 query rows 33.1 -> 31.6 and 42.4 -> 40.8 us (fp16 38.8 -> 40.3 and 62.2 -> 63.3: not there).
+    // 64 query rows 33.1 -> 31.6 and 42.4 -> 40.8 us (fp16, while it kept its addresses, 38.8 -> 40.3 and 62.2 -> 63.3:
+    // not there).
     constexpr bool PAST_CACHES = NR == 1 || TWO;
+    // With two row blocks of fp16 tiles addresses that follow from one by an exclusive or are formed where they are used: kept,
+    // they are nine registers more than there are, and a reload waits for the loads on their way, too (64 sequences of 2048
+    // rows, 8 heads of 128, 32 and 256 query rows 65 and 457 us kept, 53 and 367 formed; one row block or bf16, which have the
+    // registers: 1 to 2 % slower formed).
+    constexpr bool FORMED = TWO && NR == 2;
     constexpr int SLANES = GROUPS * SB;         // lanes that have the scale bytes of a step's keys, 16 each
     constexpr int STEP_LOADS = 2 * LOADS + 1;   // load instructions of a step
     const int tid = fresh(threadIdx.x), lane = tid & 63, wave = uniform(tid >> 6);
@@ -94,28 +101,33 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
         return mine;
     };
     // the lane's place in every load: row in its group, chunk
-    uint32_t off[LOADS];
+    uint32_t off[FORMED ? 1 : LOADS];
 #pragma unroll
-    for(int i = 0; i < LOADS; ++i)
+    for(int i = 0; i < (FORMED ? 1 : LOADS); ++i)
     {
         const int r = i * Shape::RPG + lane % 16 / CPR;
         off[i] = (uint32_t)(r * RB + ((lane ^ i ^ quad) & (CPR - 1)) * 16);
     }
+    auto load_off = [&](uint32_t first, int i)
+    {
+        return FORMED ? (first ^ (uint32_t)((i & (CPR - 1)) * 16)) + (uint32_t)(i * Shape::RPG * RB) : off[FORMED ? 0 : i];
+    };
     const uint8_t *const scales_of_lane = (lane < SLANES ? p.c.k_scales : p.c.v_scales) + 16 * (lane % SB);
     auto fetch = [&](int i, const int (&page)[GROUPS])
     {
         const int64_t from = group_page(page, quad) * p.c.page_stride + group_row(i, quad) * RB;
         const char *const k_from = p.c.k_pages + from, *const v_from = p.c.v_pages + from;
         char *const slot = slots + (i & 1) * Shape::STAGE;
+        const uint32_t first = FORMED ? (uint32_t)fresh((int)off[0]) : 0;
 #pragma unroll
         for(int ld = 0; ld < LOADS; ++ld)
         {
-            load_to_lds16<0, PAST_CACHES>(k_from + off[ld], slot + ld * 1024);
+            load_to_lds16<0, PAST_CACHES>(k_from + load_off(first, ld), slot + ld * 1024);
         }
 #pragma unroll
         for(int ld = 0; ld < LOADS; ++ld)
         {
-            load_to_lds16<0, PAST_CACHES>(v_from + off[ld], slot + K_BYTES + ld * 1024);
+            load_to_lds16<0, PAST_CACHES>(v_from + load_off(first, ld), slot + K_BYTES + ld * 1024);
         }
         const int g = lane % SLANES / SB;
         const uint8_t *const scale_from = scales_of_lane + group_page(page, g) * p.c.scale_stride + group_row(i, g) * SB;
@@ -156,15 +168,15 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
     };
 
     // the lane's addresses of a step's operands
-    uint32_t k_at[GROUPS], v_at[CPR];
+    uint32_t k_at[FORMED ? 1 : GROUPS], v_at[FORMED ? 1 : CPR];
 #pragma unroll
-    for(int g = 0; g < GROUPS; ++g)
+    for(int g = 0; g < (FORMED ? 1 : GROUPS); ++g)
     {
         k_at[g] = RB < 64 ? (uint32_t)(Shape::place4(16 * g + col, quad >> 1) + 8 * (quad & 1))
             : (uint32_t)Shape::place4(16 * g + col, quad);
     }
 #pragma unroll
-    for(int c = 0; c < CPR; ++c)
+    for(int c = 0; c < (FORMED ? 1 : CPR); ++c)
     {
         // lane i of a quad gives the address of row i, sixteen values; rows 4g .. 4g + 3 are the 16-key group g's
         v_at[c] = (uint32_t)Shape::place4(16 * (col >> 2) + 4 * quad + (col & 3), c);
@@ -212,6 +224,10 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
         f32x4 s[NR][GROUPS];
         uint32_t codes[GROUPS][QREGS];
         float scale[GROUPS];
+        const uint32_t k_first = FORMED ? (uint32_t)fresh((int)k_at[0]) : 0;
+        // The first key of the step that bf16 numbers are taken for, among those that some query sees (where all queries see
+        // all keys: 0 if there is one).
+        int first_far = KEYS;
         bool far = false;
 #pragma unroll
         for(int g = 0; g < GROUPS; ++g)
@@ -219,11 +235,12 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
             // the power of two of the lane's fourth of its key row
             const uint32_t byte = *reinterpret_cast<const uint8_t *>(k_scales + (16 * g + col) * SB + quad * SB / 4);
             scale[g] = __uint_as_float(byte << 23);
+            const uint32_t k_at_g = FORMED ? (k_first ^ (uint32_t)((g & (CPR - 1)) * 16)) + 256u * g : k_at[FORMED ? 0 : g];
             far = far || (TWO && byte - (127u - 13u) > 26u);
 #pragma unroll
             for(int i = 0; i < QREGS; ++i)
             {
-                codes[g][i] = *reinterpret_cast<const uint32_t *>(k_slot + k_at[g] + 4 * i);
+                codes[g][i] = *reinterpret_cast<const uint32_t *>(k_slot + k_at_g + 4 * i);
             }
 #pragma unroll
             for(int nr = 0; nr < NR; ++nr)
@@ -231,8 +248,24 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
                 s[nr][g] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
         }
+        if(TWO && __any(far))
+        {
+            first_far = PARTLY ? KEYS : 0;
+            if constexpr(PARTLY)
+            {
+#pragma unroll
+                for(int g = GROUPS - 1; g >= 0; --g)
+                {
+                    // (a key in each of 16 lanes, a fourth of it in each 16)
+                    const bool there = key0 + 16 * g + col < seg.len && ((hidden >> g) & 1) == 0;
+                    const unsigned long long lanes = __ballot(there && (__float_as_uint(scale[g]) >> 23) - (127u - 13u) > 26u);
+                    const uint32_t half = (uint32_t)lanes | (uint32_t)(lanes >> 32), keys = (half | half >> 16) & 0xffffu;
+                    first_far = keys != 0 ? 16 * g + __builtin_ctz(keys) : first_far;
+                }
+            }
+        }
         // (the groups' sums side by side: a sum's products wait for each other)
-        if(!TWO || !__any(far))
+        if(!TWO || first_far == KEYS)
         {
 #pragma unroll
             for(int i = 0; i < QREGS; ++i)
@@ -276,6 +309,34 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
                     {
                         s[nr][g] = mfma32<Bf16>(wide[g], q, s[nr][g]);
                         s[nr][g] = mfma32<Bf16>(wide[g], rest, s[nr][g]);
+                    }
+                }
+            }
+            if constexpr(PARTLY)
+            {
+                // Queries that see only keys in front of it have the scores that they have without it.
+#pragma unroll
+                for(int nr = 0; nr < NR; ++nr)
+                {
+                    const bool sees = last[nr] - key0 >= first_far;
+                    if(__all(sees))
+                    {
+                        continue;
+                    }
+#pragma unroll
+                    for(int g = 0; g < GROUPS; ++g)
+                    {
+                        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for(int i = 0; i < QREGS; ++i)
+                        {
+                            x = mfma32<T>(widen8_of_4<T>((uint32_t)fresh((int)codes[g][i]), scale[g]), q_operand(nr, i), x);
+                        }
+#pragma unroll
+                        for(int e = 0; e < 4; ++e)
+                        {
+                            s[nr][g][e] = sees ? s[nr][g][e] : x[e];
+                        }
                     }
                 }
             }
@@ -330,12 +391,14 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
         // ---- output --------------------------------------------------------------------------
         // the lane's column of every 16: codes of sixteen keys
         u32x2 v[DBLOCKS];
+        const uint32_t v_first = FORMED ? (uint32_t)fresh((int)v_at[0]) : 0;
 #pragma unroll
         for(int db = 0; db < DBLOCKS; ++db)
         {
             typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+            const uint32_t v_at_c = FORMED ? v_first ^ (uint32_t)(db / 2 * 16) : v_at[FORMED ? 0 : db / 2];
             v[db] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-                        (lds_i32x2 *)(v_slot + v_at[db / 2] + 8 * (db & 1))));
+                        (lds_i32x2 *)(v_slot + v_at_c + 8 * (db & 1))));
         }
         // scale bytes of the lane's four value rows of each group
         uint32_t vs[GROUPS][SB];

@@ -380,7 +380,7 @@ class PagedKVCache:
     # 31.4, 52.3, 512 40.6, 48.8, 1024 75.5, 56.1; one sequence of 4096: 512 30.3, 36.0, 1024 46.4, 40.0;
     # 8 x 8192: 256 133, 226, 512 261, 219.  fp32, 12 heads of 64, 2 x 2048: 256 54.2, 44.1, 512 91.8,
     # 49.8.  4 bits, 4 x 2048 and 8 x 8192 rows of bf16: 256 28.7, 50.2 and 109, 216, 512 36.5, 46.4 and
-    # 214, 203, 1024 65.5, 53.6 and 424, 303; of fp16 512 50.7, 46.9 and 336, 216.
+    # 214, 203, 1024 65.5, 53.6 and 424, 303; of fp16 512 50.4, 48.1 and 306, 219.
     DENSE_ROWS = 512
 
     def _read_back(self, length, Q, mode, stream):

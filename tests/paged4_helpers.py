@@ -73,6 +73,23 @@ class Case4(P.Case):
                        (self.scales if scales is None else scales)[:, which].numpy())
 
 
+def free_first_page(case):
+    """Page 0, which entries of the table that are no pages are read as, belongs to no sequence any more: it changes
+    places with a page that belongs to none."""
+    spare = next(p for p in range(case.n_pages) if not bool(case.there[p].any()))
+    swap = torch.arange(case.n_pages)
+    swap[0], swap[spare] = spare, 0
+    case.pool, case.scales, case.there = case.pool[swap], case.scales[swap], case.there[swap]
+    real = (case.table >= 0) & (case.table < case.n_pages)
+    case.table = torch.where(real, swap[case.table.clamp(0, case.n_pages - 1).long()].to(torch.int32), case.table)
+
+
+def in_the_rest(case, byte):
+    """`byte` as the power of two of every row that no sequence has."""
+    case.scales[~case.there[:, None, None].expand(case.scales.shape[:4])] = byte
+    return case
+
+
 def make(seed, dtype, bits, n_batch, heads, head, page_rows, lens, **kw):
     """A case whose pages hold `bits` bits (4, 8, or the tile type's)."""
     if bits == 4:

@@ -410,3 +410,41 @@ def test_the_largest_values_stay_finite(dtype):
     h.paged_kv_read(c.k, c.v, c.dtable, c.dlens, y, z, k_scales=c.ks, v_scales=c.vs)
     want = 6.0 * 2.0 ** 125 if dtype == "bf16" else 65504.0
     assert y.double().unique().tolist() == [want] and z.double().unique().tolist() == [-want]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("head", [64, 128])
+@pytest.mark.parametrize("q_seq,group,causal", [(1, 4, True), (1, 32, True), (8, 4, True), (5, 28, False)])
+def test_rows_that_are_none_do_not_choose_the_arithmetic(dtype, head, q_seq, group, causal):
+    """The same bits whatever lies behind the last rows, in pages that no sequence has and in a page that a bad entry of the
+    table is read as."""
+    c = F.Case4(111, dtype, 2, 2, head, 16, [700, 77])
+    c.table[0, 3], c.table[1, 2] = -1, c.n_pages
+    F.free_first_page(c)
+    q = torch.randn(4 * group, q_seq, head, generator=torch.Generator().manual_seed(112)).to(P.TORCH_DT[dtype])
+    runs = [_attend(F.in_the_rest(c, byte).device(), q, group, causal) for byte in (127, 1, 252, 255)]
+    for A, lse in runs[1:]:
+        assert torch.equal(_bits(A), _bits(runs[0][0])) and torch.equal(_bits(lse), _bits(runs[0][1]))
+    _check(c, q, q_seq, group, causal, None, *runs[0])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("head", [64, 128])
+@pytest.mark.parametrize("q_seq,group", [(4, 1), (8, 4), (16, 4), (40, 2)])
+def test_newer_tokens_do_not_choose_the_arithmetic(dtype, head, q_seq, group):
+    """The same bits of every token whatever powers of two the keys and values of the newer ones have."""
+    lens = [700, 77]
+    c = F.Case4(113, dtype, 2, 1, head, 64, lens)
+    q = torch.randn(2 * group, q_seq, head, generator=torch.Generator().manual_seed(114)).to(P.TORCH_DT[dtype])
+    want = [t.cpu() for t in _attend(c.device(), q, group, True)]
+    _check(c, q, q_seq, group, True, None, *want)
+    # (from the newest token on backwards: what has been changed stays)
+    for token in range(q_seq - 1, 0, -max(1, q_seq // 4)):
+        for n, length in enumerate(lens):
+            row = length - q_seq + token
+            c.scales[int(c.table[n, row // 64]), :, 0, row % 64] = 127 - 17
+        got = [t.cpu() for t in _attend(c.device(), q, group, True)]
+        _check(c, q, q_seq, group, True, None, *got)
+        for a, b in zip(got, want):
+            a, b = (t.view(group, 2, q_seq, -1)[:, :, :token] for t in (a, b))
+            assert torch.equal(_bits(a.contiguous()), _bits(b.contiguous()))
