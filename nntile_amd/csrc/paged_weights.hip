@@ -264,10 +264,12 @@ void paged_weights_kernel(const PagedWeightsParams p)
         bool far = false;
         if constexpr(NARROW)
         {
+            // (what lies in rows that are none has no say)
+            const int rows_there = place.len - place.block * BLOCK - wave * KEYS;
 #pragma unroll
             for(int g = 0; g < GK; ++g)
             {
-                far = far || byte[g] - (127u - 13u) > 26u;
+                far = far || (16 * g + col < ((hidden >> g) & 1 ? 0 : rows_there) && byte[g] - (127u - 13u) > 26u);
             }
             far = __any(far);
         }

@@ -187,3 +187,22 @@ def test_a_first_query_that_counts_nothing(dtype, bits, q_seq, group, given, fil
     weights = torch.rand(2, c.max_pages * 64, generator=g)
     after = _run(c, q, lse, weights, group, True, new_rows, 0.5)
     _check(c, q, lse, weights, after, q_seq, group, True, new_rows, 0.5)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("head", [64, 128])
+@pytest.mark.parametrize("q_seq,group", [(1, 4), (2, 16), (5, 28)])
+def test_four_bit_rows_that_are_none_do_not_choose_the_arithmetic(dtype, head, q_seq, group):
+    """The same bits whatever lies behind the last rows, in pages that no sequence has and in a page that a bad entry of the
+    table is read as."""
+    c = F.Case4(16, dtype, 2, 2, head, 16, [300, 77])
+    c.table[0, 3], c.table[1, 2] = -1, c.n_pages
+    F.free_first_page(c)
+    g = torch.Generator().manual_seed(17)
+    q = torch.randn(4 * group, q_seq, head, generator=g).to(P.TORCH_DT[dtype])
+    lse = torch.from_numpy(P.attend(c, q, q_seq, group, True, None)[1]).float()
+    runs = [_run(F.in_the_rest(c, byte).device(), q, lse, torch.zeros(4, c.max_pages * 16), group, True)
+            for byte in (127, 1, 252, 255)]
+    for other in runs[1:]:
+        assert torch.equal(runs[0].view(torch.int32), other.view(torch.int32))
+    _check(c, q, lse, torch.zeros(4, c.max_pages * 16), runs[0], q_seq, group, True, None, 1.0)
