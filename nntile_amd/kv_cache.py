@@ -243,6 +243,13 @@ class PagedKVCache:
         packed = bool(packed) or bits is not None
         if packed and dtype == torch.float32:
             raise TypeError("8-bit pages hold bf16 and fp16 tiles" if bits != 4 else "4-bit pages hold bf16 and fp16 tiles")
+        # (sizes that the attention over 4-bit pages, the weights or the eviction would refuse of a cache that is filled)
+        rows, entries = -(-max_rows // page_rows) * page_rows, n_batch * n_head_kv
+        if (bits == 4 or weighted) and rows > 1 << 30:
+            raise ValueError("a sequence in 4-bit pages, or with weights, has at most 2^30 rows")
+        row_bytes = head // 2 if bits == 4 else head * (1 if packed else dtype.itemsize)
+        if weighted and (entries * -(-rows // 64) > 0x7fffffff or entries * 2 * max(1, row_bytes // 64) > 0x7fffffff):
+            raise ValueError("sequences times heads, times 64 rows or 64 bytes of keys and values, are below 2^31 with weights")
         self.dtype, self.packed = dtype, packed
         self.bits = 4 if bits == 4 else 8 if packed else 8 * dtype.itemsize
         self.n_batch, self.n_head_kv, self.head = n_batch, n_head_kv, head

@@ -90,3 +90,28 @@ def test_a_new_sequence_begins_without_weights(monkeypatch):
     c.release(1)
     of = c.weights.view(2, 2, -1)
     assert float(of[:, 1].abs().max()) == 0 and float(of[:, 0].min()) == 3
+
+
+@pytest.mark.parametrize("kw", [dict(bits=4, weighted=False), dict(bits=8), dict(bits=None), dict(bits=4)])
+@pytest.mark.parametrize("max_rows,page_rows", [((1 << 30) + 1, 65536), ((1 << 30) + 1, 16), ((1 << 31) - 65536, 65536)])
+def test_more_rows_than_attention_weights_or_eviction_take(kw, max_rows, page_rows):
+    """Refused where the cache is made, not when it is filled."""
+    with pytest.raises(ValueError, match="2\\^30 rows"):
+        _cache([0], **dict(dict(n_pages=1, n_head_kv=1, max_rows=max_rows, page_rows=page_rows), **kw))
+
+
+@pytest.mark.parametrize("n_batch,n_head_kv,max_rows,page_rows,head,bits,dtype", [
+    (1 << 16, 1 << 10, 33 * 64, 16, 64, 4, torch.bfloat16),        # 2^26 entries of 33 blocks
+    (1 << 20, 1 << 10, 16, 16, 64, 4, torch.bfloat16),             # 2^30 entries, K and V
+    (1 << 20, 1 << 8, 16, 16, 128, None, torch.float32)])          # 2^28 entries, K and V, 8 times 64 bytes
+def test_more_entries_than_weights_or_eviction_take(n_batch, n_head_kv, max_rows, page_rows, head, bits, dtype):
+    with pytest.raises(ValueError, match="2\\^31"):
+        PagedKVCache(1, page_rows, n_batch, max_rows, n_head_kv, head, dtype=dtype, bits=bits, weighted=True, device="cpu")
+
+
+def test_as_many_rows_as_they_take():
+    c = PagedKVCache(1, 65536, 1, 1 << 30, 1, 64, bits=4, device="cpu")
+    assert c.max_pages * c.page_rows == 1 << 30
+    # (rows as they are, without weights: up to 2^31)
+    c = PagedKVCache(1, 65536, 1, (1 << 31) - 65536, 1, 64, device="cpu")
+    assert c.max_pages * c.page_rows == (1 << 31) - 65536
