@@ -274,10 +274,10 @@ __device__ __forceinline__ void paged_join(const PagedAttendParams &p, int n, in
 }
 
 template<typename T, int KIND, int HEAD, int NR, int HALVES>
-__global__ __launch_bounds__((PagedShape<T, KIND, HEAD, NR, HALVES>::THREADS), (PagedShape<T, KIND, HEAD, NR, HALVES>::MIN_WAVES))
+__global__ __launch_bounds__((PagedShape<KIND, HEAD, NR, HALVES>::THREADS), (PagedShape<KIND, HEAD, NR, HALVES>::MIN_WAVES))
 void sdpa_paged_kernel(const PagedAttendParams p)
 {
-    typedef PagedShape<T, KIND, HEAD, NR, HALVES> Shape;
+    typedef PagedShape<KIND, HEAD, NR, HALVES> Shape;
     constexpr int RB = Shape::RB, CPR = Shape::CPR, KEYS = Shape::KEYS, GROUPS = Shape::GROUPS;
     constexpr int LOADS = Shape::LOADS, K_BYTES = Shape::K_BYTES, STAGE = Shape::STAGE;
     constexpr int WAVES = Shape::WAVES, STREAMS = Shape::STREAMS, THREADS = Shape::THREADS;
@@ -1368,7 +1368,7 @@ static void place_workspace(PagedAttendParams &p, int head, void *workspace)
 template<typename T, int KIND, int HEAD, int NR, int HALVES>
 static int launch_form(hipStream_t stream, PagedAttendParams &p)
 {
-    typedef PagedShape<T, KIND, HEAD, NR, HALVES> Shape;
+    typedef PagedShape<KIND, HEAD, NR, HALVES> Shape;
     p.row_groups = (p.rows + Shape::QROWS - 1) / Shape::QROWS;
     p.units = p.c.n_head_kv * p.row_groups;
     // at most as many shares as there can be blocks

@@ -30,7 +30,7 @@ __device__ __forceinline__ void paged4_walk(const PagedAttendParams &p, const Pa
         int my_first, int n_mine, int all_see, const int (&last)[NR], char *ring,
         f32x4 (&o)[NR][HEAD / 16], float (&m_run)[NR], float (&l_run)[NR])
 {
-    typedef PagedShape<T, kPaged4, HEAD, NR, 1> Shape;
+    typedef PagedShape<kPaged4, HEAD, NR, 1> Shape;
     constexpr int RB = Shape::RB, SB = Shape::SB, CPR = Shape::CPR, KEYS = Shape::KEYS, GROUPS = Shape::GROUPS;
     constexpr int LOADS = Shape::LOADS, K_BYTES = Shape::K_BYTES, STREAMS = Shape::STREAMS, QROWS = Shape::QROWS, QB = Shape::QB;
     constexpr int DBLOCKS = HEAD / 16, QREGS = HEAD / 32;

@@ -22,7 +22,7 @@ constexpr unsigned long long kPagedNone = 0x9e3779b97f4a7000ull;
 constexpr int kPagedCountStride = 8;
 static_assert(kPagedShares < (int)kPagedCountMask, "counts stay below the word");
 
-template<typename T, int KIND, int HEAD, int NR, int HALVES>
+template<int KIND, int HEAD, int NR, int HALVES>
 struct PagedShape
 {
     static constexpr int STREAMS = 4;                       // wavefronts that take different keys
