@@ -811,8 +811,9 @@ int nntile_hip_paged4_attn_weights_fp16(void *stream, const nntile_hip_paged_wei
  *                keep) on
  *   weights      as above; weights_out: the same array, or another of the same size, whose
  *                columns below lens are written: the weights of the rows that stayed, then zeros
- * max_pages * page_rows and keep are at most 2^30.  A row without a page moves as zeros, and none is written where the new place has no page.  No page
- * belongs to two sequences.  cache.new_rows is not looked at. */
+ * max_pages * page_rows and keep are at most 2^30.  A row without a page moves as zeros, and none is
+ * written where the new place has no page.  No page belongs to two sequences.  cache.new_rows is
+ * not looked at. */
 typedef struct nntile_hip_paged_evict_args
 {
     nntile_hip_paged_cache cache;

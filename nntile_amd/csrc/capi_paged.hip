@@ -174,8 +174,8 @@ int attend_call(int dtype, bool four, void *stream, const nntile_hip_sdpa_paged_
         return rc;
     }
     const int64_t rows = query_rows(a->cache, a->q_seq, a->kv_group);
-    if((four && p.c.max_rows > kLongest) || rows < 0 || a->Q == nullptr || a->lse == nullptr || a->A == nullptr || !on16(a->Q) || !on16(a->A)
-            || (reinterpret_cast<uintptr_t>(a->lse) & 3u) != 0
+    if((four && p.c.max_rows > kLongest) || rows < 0 || a->Q == nullptr || a->lse == nullptr || a->A == nullptr
+            || !on16(a->Q) || !on16(a->A) || (reinterpret_cast<uintptr_t>(a->lse) & 3u) != 0
             || (a->flags & ~NNTILE_HIP_SDPA_OVERWRITE) != 0)
     {
         return NNTILE_HIP_EINVAL;
@@ -222,7 +222,8 @@ int weights_call(int dtype, bool four, void *stream, const nntile_hip_paged_weig
     const int64_t rows = query_rows(a->cache, a->q_seq, a->kv_group);
     if(rows < 0 || a->Q == nullptr || a->lse == nullptr || a->weights == nullptr || !on16(a->Q)
             || (reinterpret_cast<uintptr_t>(a->lse) & 3u) != 0 || (reinterpret_cast<uintptr_t>(a->weights) & 3u) != 0
-            || view.max_rows > kLongest || a->columns < view.max_rows || a->columns > kMost || !(a->decay >= 0.0f && a->decay <= 1.0f))
+            || view.max_rows > kLongest || a->columns < view.max_rows || a->columns > kMost
+            || !(a->decay >= 0.0f && a->decay <= 1.0f))
     {
         return NNTILE_HIP_EINVAL;
     }
@@ -249,8 +250,8 @@ int evict_call(int dtype, bool four, void *stream, const nntile_hip_paged_evict_
     {
         return rc;
     }
-    if(p.c.max_rows > kLongest || a->keep <= 0 || a->keep > kLongest || a->recent < 0 || a->recent > a->keep || a->weights == nullptr
-            || a->weights_out == nullptr || a->kept == nullptr || (reinterpret_cast<uintptr_t>(a->weights) & 3u) != 0
+    if(p.c.max_rows > kLongest || a->keep <= 0 || a->keep > kLongest || a->recent < 0 || a->recent > a->keep
+            || a->weights == nullptr || a->weights_out == nullptr || a->kept == nullptr || (reinterpret_cast<uintptr_t>(a->weights) & 3u) != 0
             || (reinterpret_cast<uintptr_t>(a->weights_out) & 3u) != 0
             || (reinterpret_cast<uintptr_t>(a->kept) & 3u) != 0 || a->columns < p.c.max_rows || a->columns > kMost)
     {
